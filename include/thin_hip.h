@@ -362,6 +362,102 @@ thin_status thin_channel_select(const thin_desc* x, int64_t groups, int64_t begi
 thin_status thin_attention(const thin_desc* qkv, int64_t heads, int64_t key_dim, int64_t head_dim, float scale,
                            int32_t prescale, const thin_desc* out, hipStream_t stream);
 
+/* ------------------------------------------------------------------ */
+/* Group norm                                                          */
+/* ------------------------------------------------------------------ */
+
+/* Bytes of workspace thin_group_norm needs (0: none).  x, channels and groups
+ * as there.  No reference counterpart: the reference folds batch norm into the
+ * affine of its convolutions (model_optimization.py:20-31). */
+size_t thin_group_norm_workspace(const thin_desc* x, int32_t blocked, int64_t channels, int64_t groups);
+
+/* y = (x - mean) / sqrt(var + eps) * weight + bias with the mean and the
+ * (biased) variance of each sample's groups of channels / groups adjacent
+ * channels over all rows, then y * sigmoid(y) if silu != 0; fp32 statistics
+ * and arithmetic, one rounding.  fp16, bf16 or fp32 x and out (equal sizes);
+ * weight and bias: NULL, or [channels] of x's type or fp32.
+ *   blocked == 0: x [N, ..., C], channels == C adjacent; the row dimensions
+ *     may need at most two strides (a channel range of a wider tensor, a crop);
+ *   blocked != 0: x [N, C1, H, W, 16] with C1 = ceil(channels / 16); channels
+ *     past the last take no part and are written as zeros.
+ * out may be x itself.  A NaN or infinity makes its group NaN.  The statistic
+ * that the per-channel affine + SiLU chain of the reference's convolutions
+ * (ops.cpp:464-512) cannot fold, followed by that chain, as one operator. */
+thin_status thin_group_norm(const thin_desc* x, int32_t blocked, int64_t channels, int64_t groups,
+                            const thin_desc* weight, const thin_desc* bias, double eps, int32_t silu,
+                            const thin_desc* out, void* workspace, size_t workspace_bytes, hipStream_t stream);
+
+/* ------------------------------------------------------------------ */
+/* Expert blocks                                                       */
+/* ------------------------------------------------------------------ */
+
+/* Routing: weights fp32 and experts int32 [T, k] from logits [T, E] (fp16,
+ * bf16 or fp32, a token's logits adjacent; E <= 1024, k <= 32).
+ *   s = softmax(logits) over E (softmax != 0) or sigmoid(logits);
+ *   c = s + bias (bias fp32 [E]), or without a bias (NULL) the logits, whose
+ *     order is that of s;
+ *   of `groups` equal runs of experts (<= 64) the top_groups best stay, by
+ *     their highest c, with a bias by the sum of their two highest;
+ *   experts = the k with the highest c among those, highest first;
+ *   weights = s of the chosen, divided by their sum if renormalize != 0, times
+ *     scale.
+ * NaN stands before every value and the lower index before its equals; the
+ * order of c is that of 64-bit arithmetic.  The row softmax and the top-K of
+ * the reference (softmax_host.cpp:51-89, selection_flow.cpp:429-499) applied to
+ * experts. */
+thin_status thin_expert_route(const thin_desc* logits, const thin_desc* bias, int32_t softmax, int64_t groups,
+                              int64_t top_groups, int32_t renormalize, float scale, const thin_desc* weights,
+                              const thin_desc* experts, hipStream_t stream);
+
+/* Bytes of workspace thin_expert_dispatch needs (0: none).  No reference
+ * counterpart (its concat copies at fixed places, ops.cpp:419-462). */
+size_t thin_expert_dispatch_workspace(int64_t tokens, int64_t top_k, int64_t num_experts);
+
+/* Rows to their experts.  The T * k assignments of experts int32 [T, k] are put
+ * in the order (expert, token, place): slots int32 [T, k] gets each one's
+ * place, offsets int32 [num_experts + 1] each expert's first, and rows
+ * [T * k, width] x's row of each slot (x [T, width], fp16, bf16 or fp32, moved
+ * bit for bit, a row's elements adjacent).  An expert outside
+ * [0, num_experts) is no assignment: its slot is -1, and the rows from
+ * offsets[num_experts] on are left as they were.  num_experts <= 1024, k <= 32.
+ * The data movement of the reference's concat (ops.cpp:419-462) with places
+ * that depend on the data. */
+thin_status thin_expert_dispatch(const thin_desc* x, const thin_desc* experts, int64_t num_experts,
+                                 const thin_desc* rows, const thin_desc* offsets, const thin_desc* slots,
+                                 void* workspace, size_t workspace_bytes, hipStream_t stream);
+
+/* Rows back from their experts: out[t] = sum over j of weights[t, j] *
+ * y[slots[t, j]], in the order of j, fp32 with one rounding.  y [rows, width]
+ * and out [T, width] fp16, bf16 or fp32, weights fp32 and slots int32 [T, k];
+ * slots outside y contribute nothing.  The mul and add chain of the reference
+ * (ops.cpp:464-497) over gathered rows. */
+thin_status thin_expert_combine(const thin_desc* y, const thin_desc* weights, const thin_desc* slots,
+                                const thin_desc* out, hipStream_t stream);
+
+/* ------------------------------------------------------------------ */
+/* Token log probabilities                                             */
+/* ------------------------------------------------------------------ */
+
+/* Bytes of workspace thin_token_logprobs needs (0: none).  No reference
+ * counterpart (its softmax works in place of its output,
+ * softmax_host.cpp:51-89). */
+size_t thin_token_logprobs_workspace(int64_t rows, int64_t width, int64_t top);
+
+/* For each row of logits [R, V] (fp16, bf16 or fp32, a row's logits adjacent,
+ * V <= 8388608), with p = softmax(row):
+ *   logprobs[r] = log p[tokens[r]] (int64 tokens [R]; NaN for a token outside
+ *     [0, V)), entropy[r] = -sum p log p (0 log 0 = 0);
+ *   top_logprobs, top_ids [R, top] (top <= 32, top <= V): the highest logits,
+ *     highest first, NaN before every value and the lower index before its
+ *     equals.
+ * fp32 outputs (ids int64).  A row with a NaN, a +inf or nothing but -inf has
+ * NaN log probabilities and entropy; its ids follow the order above.  The
+ * reference's row softmax and top-K (softmax_host.cpp:51-89,
+ * selection_flow.cpp:429-499) without the probabilities in between. */
+thin_status thin_token_logprobs(const thin_desc* logits, const thin_desc* tokens, const thin_desc* logprobs,
+                                const thin_desc* entropy, const thin_desc* top_logprobs, const thin_desc* top_ids,
+                                void* workspace, size_t workspace_bytes, hipStream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -104,6 +104,11 @@ def lib() -> ctypes.CDLL:
             "thin_channel_select_shape": [P, i64, i64, i64, ctypes.POINTER(i64)],
             "thin_channel_select": [P, i64, i64, i64, P, vp],
             "thin_attention": [P, i64, i64, i64, ctypes.c_float, i32, P, vp],
+            "thin_group_norm": [P, i32, i64, i64, P, P, f64, i32, P, vp, ctypes.c_size_t, vp],
+            "thin_expert_route": [P, P, i32, i64, i64, i32, f32, P, P, vp],
+            "thin_expert_dispatch": [P, P, i64, P, P, P, vp, ctypes.c_size_t, vp],
+            "thin_expert_combine": [P, P, P, P, vp],
+            "thin_token_logprobs": [P, P, P, P, P, P, vp, ctypes.c_size_t, vp],
         }
         for name, argtypes in sigs.items():
             fn = getattr(L, name, None)
@@ -116,6 +121,14 @@ def lib() -> ctypes.CDLL:
         if hasattr(L, "thin_detection_select_workspace"):
             L.thin_detection_select_workspace.argtypes = [i64, i64, i64, i64, i32]
             L.thin_detection_select_workspace.restype = ctypes.c_size_t
+        for name, argtypes in {"thin_group_norm_workspace": [P, i32, i64, i64],
+                               "thin_expert_dispatch_workspace": [i64, i64, i64],
+                               "thin_token_logprobs_workspace": [i64, i64, i64]}.items():
+            fn = getattr(L, name, None)
+            if fn is None:
+                continue
+            fn.argtypes = argtypes
+            fn.restype = ctypes.c_size_t
         _lib = L
     return _lib
 
@@ -433,4 +446,127 @@ def attention(qkv, heads: int, key_dim: int, head_dim: int, scale: float, presca
         out = torch.empty((1, heads * head_dim // 16, tokens, 16), dtype=torch.float16, device=qkv.device)
     _call("thin_attention", _ref(desc(qkv)), heads, key_dim, head_dim, float(scale), int(bool(prescale)),
           _ref(desc(out)), _stream(stream))
+    return out
+
+
+# The operators below check where their tensors live: a call launches on the
+# current device, whose memory every operand has to be.
+
+def _here(*tensors) -> None:
+    device = tensors[0].device
+    if device.type != "cuda" or device.index != torch._C._cuda_getDevice():
+        raise ValueError(f"the operands must be on the current HIP device, not on {device}")
+    for t in tensors[1:]:
+        if t is not None and t.device != device:
+            raise ValueError(f"operands on {device} and {t.device}")
+
+
+def _workspace(nbytes: int, given, device, stream):
+    """(address, bytes) of a call's workspace: the given tensor, or one of
+    torch's allocator, which gets it back at the end of the wrapper and hands
+    it out again in the order of the stream that it was allocated on; a call on
+    another stream is recorded so that it is not handed out before that ends."""
+    if given is not None:
+        if not given.is_contiguous():
+            raise ValueError("the workspace must be contiguous")
+        return given.data_ptr(), given.numel() * given.element_size()
+    if nbytes == 0:
+        return None, 0
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
+    if stream is not None:
+        ws.record_stream(stream if isinstance(stream, torch.cuda.Stream) else torch.cuda.ExternalStream(stream))
+    return ws.data_ptr(), nbytes
+
+
+def _group_norm(x, blocked, channels, groups, weight, bias, eps, silu, out, workspace, stream):
+    out = torch.empty(x.shape, dtype=x.dtype, device=x.device) if out is None else out
+    _here(x, weight, bias, out, workspace)
+    xd = desc(x)
+    need = lib().thin_group_norm_workspace(_ref(xd), blocked, channels, groups)
+    address, nbytes = _workspace(need, workspace, x.device, stream)
+    _call("thin_group_norm", _ref(xd), blocked, channels, groups, None if weight is None else _ref(desc(weight)),
+          None if bias is None else _ref(desc(bias)), float(eps), int(bool(silu)), _ref(desc(out)), address, nbytes,
+          _stream(stream))
+    return out
+
+
+def group_norm(x, groups: int, weight=None, bias=None, eps: float = 1e-5, silu: bool = False, out=None,
+               workspace=None, stream=None):
+    """Group norm of channels-last x [N, ..., C] (fp16, bf16, fp32), with SiLU
+    after it if silu; weight and bias [C] of x's type or fp32.  out may be x."""
+    if x.dim() < 2:
+        raise ValueError("group_norm takes x [N, ..., C]")
+    return _group_norm(x, 0, x.shape[-1], groups, weight, bias, eps, silu, out, workspace, stream)
+
+
+def group_norm_nc1hwc0(x, groups: int, weight=None, bias=None, eps: float = 1e-5, silu: bool = False,
+                       channels: int | None = None, out=None, workspace=None, stream=None):
+    """Group norm of blocked x [N, C1, H, W, 16]; `channels` (default 16 * C1)
+    take part, the padding behind them is written as zeros."""
+    if x.dim() != 5:
+        raise ValueError("group_norm_nc1hwc0 takes x [N, C1, H, W, 16]")
+    channels = x.shape[1] * 16 if channels is None else channels
+    return _group_norm(x, 1, channels, groups, weight, bias, eps, silu, out, workspace, stream)
+
+
+def expert_route(logits, top_k: int, bias=None, scores: str = "softmax", groups: int = 1, top_groups: int = 1,
+                 renormalize: bool = True, scale: float = 1.0, out=None, stream=None):
+    """(weights fp32, experts int32) [T, top_k] of router logits [T, E]: the
+    top_k highest of softmax or sigmoid scores + bias among the top_groups best
+    of `groups` runs of experts, weighted by their scores without the bias."""
+    if scores not in ("softmax", "sigmoid"):
+        raise ValueError(f"scores are softmax or sigmoid, not {scores!r}")
+    if out is None:
+        t = logits.shape[0]
+        out = (torch.empty((t, top_k), dtype=torch.float32, device=logits.device),
+               torch.empty((t, top_k), dtype=torch.int32, device=logits.device))
+    weights, experts = out
+    _here(logits, bias, weights, experts)
+    _call("thin_expert_route", _ref(desc(logits)), None if bias is None else _ref(desc(bias)),
+          int(scores == "softmax"), groups, top_groups, int(bool(renormalize)), float(scale), _ref(desc(weights)),
+          _ref(desc(experts)), _stream(stream))
+    return weights, experts
+
+
+def expert_dispatch(x, experts, num_experts: int, out=None, workspace=None, stream=None):
+    """(rows [T * k, width], offsets int32 [num_experts + 1], slots int32 [T, k]):
+    x's rows in the order (expert, token), where each expert's begin, and where
+    each assignment went (-1: no expert)."""
+    if out is None:
+        t, k = experts.shape
+        out = (torch.empty((t * k, x.shape[1]), dtype=x.dtype, device=x.device),
+               torch.empty(num_experts + 1, dtype=torch.int32, device=x.device),
+               torch.empty((t, k), dtype=torch.int32, device=x.device))
+    rows, offsets, slots = out
+    _here(x, experts, rows, offsets, slots, workspace)
+    need = lib().thin_expert_dispatch_workspace(experts.shape[0], experts.shape[1], num_experts)
+    address, nbytes = _workspace(need, workspace, x.device, stream)
+    _call("thin_expert_dispatch", _ref(desc(x)), _ref(desc(experts)), num_experts, _ref(desc(rows)),
+          _ref(desc(offsets)), _ref(desc(slots)), address, nbytes, _stream(stream))
+    return rows, offsets, slots
+
+
+def expert_combine(y, weights, slots, out=None, stream=None):
+    """out[t] = sum_j weights[t, j] * y[slots[t, j]] (fp32, one rounding)."""
+    out = torch.empty((slots.shape[0], y.shape[1]), dtype=y.dtype, device=y.device) if out is None else out
+    _here(y, weights, slots, out)
+    _call("thin_expert_combine", _ref(desc(y)), _ref(desc(weights)), _ref(desc(slots)), _ref(desc(out)),
+          _stream(stream))
+    return out
+
+
+def token_logprobs(logits, tokens, top: int = 0, out=None, workspace=None, stream=None):
+    """(logprobs [R], entropy [R], top_logprobs [R, top], top_ids int64 [R, top])
+    of logits [R, V] and int64 tokens [R]; a token outside [0, V) gives NaN."""
+    if out is None:
+        r, dev = logits.shape[0], logits.device
+        out = (torch.empty(r, dtype=torch.float32, device=dev), torch.empty(r, dtype=torch.float32, device=dev),
+               torch.empty((r, top), dtype=torch.float32, device=dev),
+               torch.empty((r, top), dtype=torch.int64, device=dev))
+    logprobs, entropy, top_logprobs, top_ids = out
+    _here(logits, tokens, *out, workspace)
+    need = lib().thin_token_logprobs_workspace(logits.shape[0], logits.shape[1], top_ids.shape[1])
+    address, nbytes = _workspace(need, workspace, logits.device, stream)
+    _call("thin_token_logprobs", _ref(desc(logits)), _ref(desc(tokens)), _ref(desc(logprobs)), _ref(desc(entropy)),
+          _ref(desc(top_logprobs)), _ref(desc(top_ids)), address, nbytes, _stream(stream))
     return out

@@ -1,0 +1,148 @@
+// Rows of scores: element types read as fp32, vectors at element alignment,
+// and the order in which scores are ranked (NaN before everything, then from
+// the highest down, +0 and -0 equal, the lower index first among equals).
+// Shared by the expert routing and the token log probabilities.
+#pragma once
+
+#include "common.h"
+
+namespace thin {
+
+// y = f(T()) for the descriptor's floating type.
+template <typename F>
+thin_status with_float_type(int32_t dtype, F&& f) {
+  switch (dtype) {
+    case THIN_F16: return f((_Float16)0);
+    case THIN_BF16: return f((__bf16)0);
+    default: return f(0.0f);
+  }
+}
+inline bool float_type(int32_t dtype) { return dtype == THIN_F16 || dtype == THIN_BF16 || dtype == THIN_F32; }
+
+// Elements [first, last) that a descriptor's sizes and strides reach from its
+// data pointer.
+inline int64_t extent(const thin_desc* d) {
+  int64_t last = 0;
+  for (int i = 0; i < d->rank; ++i) {
+    if (d->sizes[i] == 0) return 0;
+    last += (d->sizes[i] - 1) * d->strides[i];
+  }
+  return last + 1;
+}
+// True if the bytes two descriptors reach have some in common.
+inline bool overlap(const thin_desc* a, const thin_desc* b) {
+  const char* a0 = static_cast<const char*>(a->data);
+  const char* b0 = static_cast<const char*>(b->data);
+  const int64_t an = extent(a) * dtype_size(a->dtype), bn = extent(b) * dtype_size(b->dtype);
+  return an && bn && a0 < b0 + bn && b0 < a0 + an;
+}
+
+}  // namespace thin
+
+#if defined(__HIPCC__)
+namespace thin {
+namespace dev {
+
+// N elements at element alignment: one wide load or store where the hardware
+// takes unaligned addresses (global memory does).
+template <typename T, int N>
+struct Pack {
+  typedef T type __attribute__((ext_vector_type(N), aligned(sizeof(T))));
+};
+template <typename T, int N>
+__device__ __forceinline__ void load_pack(const T* p, float (&v)[N]) {
+  const typename Pack<T, N>::type w = *reinterpret_cast<const typename Pack<T, N>::type*>(p);
+#pragma unroll
+  for (int j = 0; j < N; ++j) v[j] = (float)w[j];
+}
+template <typename T, int N>
+__device__ __forceinline__ void store_pack(T* p, const float (&v)[N]) {
+  typename Pack<T, N>::type w;
+#pragma unroll
+  for (int j = 0; j < N; ++j) w[j] = (T)v[j];
+  *reinterpret_cast<typename Pack<T, N>::type*>(p) = w;
+}
+
+// Whole numbers in the order of the scores; 0 stands below every score.
+__device__ __forceinline__ uint32_t score_key(float x) {
+  const uint32_t b = __builtin_bit_cast(uint32_t, x + 0.0f);
+  return x != x ? 0xFFFFFFFFu : b ^ ((uint32_t)((int32_t)b >> 31) | 0x80000000u);
+}
+__device__ __forceinline__ uint64_t score_key(double x) {
+  const uint64_t b = __builtin_bit_cast(uint64_t, x + 0.0);
+  return x != x ? ~0ull : b ^ ((uint64_t)((int64_t)b >> 63) | 0x8000000000000000ull);
+}
+__device__ __forceinline__ float key_score(uint32_t k) {
+  return __builtin_bit_cast(float, k & 0x80000000u ? k ^ 0x80000000u : ~k);
+}
+__device__ __forceinline__ double key_score(uint64_t k) {
+  return __builtin_bit_cast(double, k >> 63 ? k ^ 0x8000000000000000ull : ~k);
+}
+
+template <int O>
+__device__ __forceinline__ uint32_t lane_xor_key(uint32_t k) { return lane_xor_bits<O>(k); }
+template <int O>
+__device__ __forceinline__ uint64_t lane_xor_key(uint64_t k) {
+  return (uint64_t)lane_xor_bits<O>((uint32_t)(k >> 32)) << 32 | lane_xor_bits<O>((uint32_t)k);
+}
+template <int G, int O = G / 2, typename K>
+__device__ __forceinline__ K group_max_key(K k) {
+  if constexpr (O == 0) {
+    return k;
+  } else {
+    const K other = lane_xor_key<O>(k);
+    return group_max_key<G, O / 2>(k > other ? k : other);
+  }
+}
+
+// Lanes of this lane's group of G whose predicate holds, bit 0 the group's first.
+template <int G>
+__device__ __forceinline__ uint64_t group_ballot(bool p) {
+  const uint64_t all = __ballot(p);
+  if constexpr (G == 64) return all;
+  return (all >> (threadIdx.x & 63u & ~(uint32_t)(G - 1))) & ((1ull << G) - 1);
+}
+
+// Orders the LDS writes of a wavefront before the LDS reads that follow: the
+// LDS executes a wave's instructions in order, so only the compiler has to.
+__device__ __forceinline__ void wave_lds_fence() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+}
+
+// The n best of the G * PER keys of a group, lane g holding elements
+// g * PER + j: emit(i, element, key) runs on the lane that holds the i-th
+// best.  Keys taken become 0.  Every lane of the group takes part.
+template <int G, int PER, typename K, typename Emit>
+__device__ __forceinline__ void take_best(K (&key)[PER], int n, uint32_t g, Emit emit) {
+  K best = 0;
+  int at = 0;
+#pragma unroll
+  for (int j = 0; j < PER; ++j)
+    if (key[j] > best) {
+      best = key[j];
+      at = j;
+    }
+  for (int i = 0; i < n; ++i) {
+    const K top = group_max_key<G>(best);
+    const uint64_t holders = group_ballot<G>(best == top);
+    if (g == (uint32_t)__builtin_ctzll(holders)) {
+      emit(i, g * PER + at, top);
+      best = 0;
+      int next = 0;
+#pragma unroll
+      for (int j = 0; j < PER; ++j) {
+        if (j == at) key[j] = 0;
+        if (key[j] > best) {
+          best = key[j];
+          next = j;
+        }
+      }
+      at = next;
+    }
+  }
+}
+
+}  // namespace dev
+}  // namespace thin
+#endif

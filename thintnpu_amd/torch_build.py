@@ -16,7 +16,7 @@ OUT = ROOT / "thin_backend"
 
 # library -> sources (relative to csrc/torch); libthin_backend.so first
 LIBS = {
-    "libthin_backend.so": ["runtime.cpp", "ops.cpp"],
+    "libthin_backend.so": ["runtime.cpp", "ops.cpp", "score_ops.cpp"],
     "libflow_ops.so": ["flow_ops.cpp"],
     "libconv_flow.so": ["conv_flow.cpp"],
     "libselection_flow.so": ["selection.cpp"],

@@ -198,10 +198,10 @@ def test_logprobs_refusals():
     logprobs(INVALID, logits=logits, lp=desc((3,), capi.F32, data=logits.data + 4))
     lp = desc((3,), capi.F32)
     logprobs(INVALID, lp=lp, ent=desc((3,), capi.F32, data=lp.data + 8))
-    need = capi.lib().thin_token_logprobs_workspace(3, 5000, 4)
+    need = capi.lib().thin_token_logprobs_workspace(3, 600000, 4)
     assert need > 0 and capi.lib().thin_token_logprobs_workspace(3, 1024, 4) == 0
-    logprobs(WORKSPACE, v=5000)
-    logprobs(WORKSPACE, v=5000, ws=1 << 30, nbytes=need - 1)
+    logprobs(WORKSPACE, v=600000)
+    logprobs(WORKSPACE, v=600000, ws=1 << 30, nbytes=need - 1)
 
 
 def test_wrappers_refuse_host_tensors():

@@ -104,11 +104,12 @@ def lib() -> ctypes.CDLL:
             "thin_channel_select_shape": [P, i64, i64, i64, ctypes.POINTER(i64)],
             "thin_channel_select": [P, i64, i64, i64, P, vp],
             "thin_attention": [P, i64, i64, i64, ctypes.c_float, i32, P, vp],
-            "thin_group_norm": [P, i32, i64, i64, P, P, f64, i32, P, vp, ctypes.c_size_t, vp],
-            "thin_expert_route": [P, P, i32, i64, i64, i32, f32, P, P, vp],
-            "thin_expert_dispatch": [P, P, i64, P, P, P, vp, ctypes.c_size_t, vp],
-            "thin_expert_combine": [P, P, P, P, vp],
-            "thin_token_logprobs": [P, P, P, P, P, P, vp, ctypes.c_size_t, vp],
+            # descriptors as the bytes of _packed(), by address
+            "thin_group_norm": [vp, i32, i64, i64, vp, vp, f64, i32, vp, vp, ctypes.c_size_t, vp],
+            "thin_expert_route": [vp, vp, i32, i64, i64, i32, f32, vp, vp, vp],
+            "thin_expert_dispatch": [vp, vp, i64, vp, vp, vp, vp, ctypes.c_size_t, vp],
+            "thin_expert_combine": [vp, vp, vp, vp, vp],
+            "thin_token_logprobs": [vp, vp, vp, vp, vp, vp, vp, ctypes.c_size_t, vp],
         }
         for name, argtypes in sigs.items():
             fn = getattr(L, name, None)
@@ -121,7 +122,7 @@ def lib() -> ctypes.CDLL:
         if hasattr(L, "thin_detection_select_workspace"):
             L.thin_detection_select_workspace.argtypes = [i64, i64, i64, i64, i32]
             L.thin_detection_select_workspace.restype = ctypes.c_size_t
-        for name, argtypes in {"thin_group_norm_workspace": [P, i32, i64, i64],
+        for name, argtypes in {"thin_group_norm_workspace": [vp, i32, i64, i64],
                                "thin_expert_dispatch_workspace": [i64, i64, i64],
                                "thin_token_logprobs_workspace": [i64, i64, i64]}.items():
             fn = getattr(L, name, None)
@@ -450,43 +451,67 @@ def attention(qkv, heads: int, key_dim: int, head_dim: int, scale: float, presca
 
 
 # The operators below check where their tensors live: a call launches on the
-# current device, whose memory every operand has to be.
+# current device, whose memory every operand has to be.  Half of a small call is
+# the host's (3.6 of it the launch itself): descriptors go as packed bytes (0.5
+# us each, the structure 0.7) and outputs come from empty_strided (1.3 us, empty
+# 1.7).
 
-def _here(*tensors) -> None:
-    device = tensors[0].device
-    if device.type != "cuda" or device.index != torch._C._cuda_getDevice():
-        raise ValueError(f"the operands must be on the current HIP device, not on {device}")
-    for t in tensors[1:]:
-        if t is not None and t.device != device:
-            raise ValueError(f"operands on {device} and {t.device}")
+def _packed(t: torch.Tensor) -> bytes:
+    """The bytes of desc(t)."""
+    shape = t.shape
+    rank = len(shape)
+    if rank > MAX_DIMS:
+        raise ValueError(f"rank {rank} exceeds {MAX_DIMS}")
+    return _PACK[rank].pack(t.data_ptr(), _DTYPES[t.dtype], rank, *shape, *t.stride())
 
 
-def _workspace(nbytes: int, given, device, stream):
-    """(address, bytes) of a call's workspace: the given tensor, or one of
-    torch's allocator, which gets it back at the end of the wrapper and hands
+def _current_device(x: torch.Tensor) -> int:
+    device = x.get_device()
+    if device < 0 or not x.is_cuda or device != torch._C._cuda_getDevice():
+        raise ValueError(f"the operands must be on the current HIP device, not on {x.device}")
+    return device
+
+
+def _on(device: int, t: torch.Tensor) -> bytes:
+    """_packed(t) of an operand that has to be on `device`."""
+    if t.get_device() != device or not t.is_cuda:
+        raise ValueError(f"operands on cuda:{device} and {t.device}")
+    return _packed(t)
+
+
+def _rows(like: torch.Tensor, rows: int, width: int, dtype):
+    return torch.empty_strided((rows, width), (max(width, 1), 1), dtype=dtype, device=like.device)
+
+
+def _workspace(nbytes: int, given, device: int, stream):
+    """(tensor, address, bytes) of a call's workspace: the given tensor, or one
+    of torch's allocator, which gets it back at the end of the wrapper and hands
     it out again in the order of the stream that it was allocated on; a call on
     another stream is recorded so that it is not handed out before that ends."""
     if given is not None:
-        if not given.is_contiguous():
-            raise ValueError("the workspace must be contiguous")
-        return given.data_ptr(), given.numel() * given.element_size()
+        if given.get_device() != device or not given.is_contiguous():
+            raise ValueError("the workspace must be contiguous and on the operands' device")
+        return given, given.data_ptr(), given.numel() * given.element_size()
     if nbytes == 0:
-        return None, 0
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
+        return None, None, 0
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=torch.device("cuda", device))
     if stream is not None:
         ws.record_stream(stream if isinstance(stream, torch.cuda.Stream) else torch.cuda.ExternalStream(stream))
-    return ws.data_ptr(), nbytes
+    return ws, ws.data_ptr(), nbytes
 
 
 def _group_norm(x, blocked, channels, groups, weight, bias, eps, silu, out, workspace, stream):
-    out = torch.empty(x.shape, dtype=x.dtype, device=x.device) if out is None else out
-    _here(x, weight, bias, out, workspace)
-    xd = desc(x)
-    need = lib().thin_group_norm_workspace(_ref(xd), blocked, channels, groups)
-    address, nbytes = _workspace(need, workspace, x.device, stream)
-    _call("thin_group_norm", _ref(xd), blocked, channels, groups, None if weight is None else _ref(desc(weight)),
-          None if bias is None else _ref(desc(bias)), float(eps), int(bool(silu)), _ref(desc(out)), address, nbytes,
-          _stream(stream))
+    device = _current_device(x)
+    if out is None:
+        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    L = lib()
+    xd = _packed(x)
+    need = L.thin_group_norm_workspace(xd, blocked, channels, groups)
+    ws, address, nbytes = _workspace(need, workspace, device, stream)
+    _check("thin_group_norm", L.thin_group_norm(
+        xd, blocked, channels, groups, None if weight is None else _on(device, weight),
+        None if bias is None else _on(device, bias), eps, 1 if silu else 0, _on(device, out), address, nbytes,
+        _stream(stream)))
     return out
 
 
@@ -516,15 +541,14 @@ def expert_route(logits, top_k: int, bias=None, scores: str = "softmax", groups:
     of `groups` runs of experts, weighted by their scores without the bias."""
     if scores not in ("softmax", "sigmoid"):
         raise ValueError(f"scores are softmax or sigmoid, not {scores!r}")
+    device = _current_device(logits)
     if out is None:
         t = logits.shape[0]
-        out = (torch.empty((t, top_k), dtype=torch.float32, device=logits.device),
-               torch.empty((t, top_k), dtype=torch.int32, device=logits.device))
+        out = _rows(logits, t, top_k, torch.float32), _rows(logits, t, top_k, torch.int32)
     weights, experts = out
-    _here(logits, bias, weights, experts)
-    _call("thin_expert_route", _ref(desc(logits)), None if bias is None else _ref(desc(bias)),
-          int(scores == "softmax"), groups, top_groups, int(bool(renormalize)), float(scale), _ref(desc(weights)),
-          _ref(desc(experts)), _stream(stream))
+    _check("thin_expert_route", lib().thin_expert_route(
+        _packed(logits), None if bias is None else _on(device, bias), 1 if scores == "softmax" else 0, groups,
+        top_groups, 1 if renormalize else 0, scale, _on(device, weights), _on(device, experts), _stream(stream)))
     return weights, experts
 
 
@@ -532,41 +556,46 @@ def expert_dispatch(x, experts, num_experts: int, out=None, workspace=None, stre
     """(rows [T * k, width], offsets int32 [num_experts + 1], slots int32 [T, k]):
     x's rows in the order (expert, token), where each expert's begin, and where
     each assignment went (-1: no expert)."""
+    device = _current_device(x)
+    t, k = experts.shape
     if out is None:
-        t, k = experts.shape
-        out = (torch.empty((t * k, x.shape[1]), dtype=x.dtype, device=x.device),
-               torch.empty(num_experts + 1, dtype=torch.int32, device=x.device),
-               torch.empty((t, k), dtype=torch.int32, device=x.device))
+        out = (_rows(x, t * k, x.shape[1], x.dtype),
+               torch.empty_strided((num_experts + 1,), (1,), dtype=torch.int32, device=x.device),
+               _rows(x, t, k, torch.int32))
     rows, offsets, slots = out
-    _here(x, experts, rows, offsets, slots, workspace)
-    need = lib().thin_expert_dispatch_workspace(experts.shape[0], experts.shape[1], num_experts)
-    address, nbytes = _workspace(need, workspace, x.device, stream)
-    _call("thin_expert_dispatch", _ref(desc(x)), _ref(desc(experts)), num_experts, _ref(desc(rows)),
-          _ref(desc(offsets)), _ref(desc(slots)), address, nbytes, _stream(stream))
+    L = lib()
+    ws, address, nbytes = _workspace(L.thin_expert_dispatch_workspace(t, k, num_experts), workspace, device, stream)
+    _check("thin_expert_dispatch", L.thin_expert_dispatch(
+        _packed(x), _on(device, experts), num_experts, _on(device, rows), _on(device, offsets), _on(device, slots),
+        address, nbytes, _stream(stream)))
     return rows, offsets, slots
 
 
 def expert_combine(y, weights, slots, out=None, stream=None):
     """out[t] = sum_j weights[t, j] * y[slots[t, j]] (fp32, one rounding)."""
-    out = torch.empty((slots.shape[0], y.shape[1]), dtype=y.dtype, device=y.device) if out is None else out
-    _here(y, weights, slots, out)
-    _call("thin_expert_combine", _ref(desc(y)), _ref(desc(weights)), _ref(desc(slots)), _ref(desc(out)),
-          _stream(stream))
+    device = _current_device(y)
+    if out is None:
+        out = _rows(y, slots.shape[0], y.shape[1], y.dtype)
+    _check("thin_expert_combine", lib().thin_expert_combine(
+        _packed(y), _on(device, weights), _on(device, slots), _on(device, out), _stream(stream)))
     return out
 
 
 def token_logprobs(logits, tokens, top: int = 0, out=None, workspace=None, stream=None):
     """(logprobs [R], entropy [R], top_logprobs [R, top], top_ids int64 [R, top])
     of logits [R, V] and int64 tokens [R]; a token outside [0, V) gives NaN."""
+    device = _current_device(logits)
+    r, width = logits.shape
     if out is None:
-        r, dev = logits.shape[0], logits.device
-        out = (torch.empty(r, dtype=torch.float32, device=dev), torch.empty(r, dtype=torch.float32, device=dev),
-               torch.empty((r, top), dtype=torch.float32, device=dev),
-               torch.empty((r, top), dtype=torch.int64, device=dev))
+        dev = logits.device
+        out = (torch.empty_strided((r,), (1,), dtype=torch.float32, device=dev),
+               torch.empty_strided((r,), (1,), dtype=torch.float32, device=dev),
+               _rows(logits, r, top, torch.float32), _rows(logits, r, top, torch.int64))
     logprobs, entropy, top_logprobs, top_ids = out
-    _here(logits, tokens, *out, workspace)
-    need = lib().thin_token_logprobs_workspace(logits.shape[0], logits.shape[1], top_ids.shape[1])
-    address, nbytes = _workspace(need, workspace, logits.device, stream)
-    _call("thin_token_logprobs", _ref(desc(logits)), _ref(desc(tokens)), _ref(desc(logprobs)), _ref(desc(entropy)),
-          _ref(desc(top_logprobs)), _ref(desc(top_ids)), address, nbytes, _stream(stream))
+    L = lib()
+    ws, address, nbytes = _workspace(L.thin_token_logprobs_workspace(r, width, top_ids.shape[1]), workspace, device,
+                                     stream)
+    _check("thin_token_logprobs", L.thin_token_logprobs(
+        _packed(logits), _on(device, tokens), _on(device, logprobs), _on(device, entropy), _on(device, top_logprobs),
+        _on(device, top_ids), address, nbytes, _stream(stream)))
     return out

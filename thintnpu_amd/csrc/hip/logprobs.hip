@@ -23,7 +23,8 @@ constexpr int64_t kMaxTop = 32;
 constexpr int64_t kShortRow = 1024;   // longest row that one group of lanes holds
 constexpr uint32_t kRun = 64;         // elements whose maximum is kept
 constexpr uint32_t kTile = kRun * 64;  // elements of a wavefront
-constexpr int64_t kMaxTiles = 64 * kMaxTop;
+constexpr int64_t kMaxWidth = 8388608;
+constexpr int64_t kManyRows = 1024;    // rows from which a wavefront finishes each
 
 struct LogprobsPlan {
   const void* logits;
@@ -48,20 +49,22 @@ struct RowSums {
 // s and u of the elements against their maximum m.  The plain form needs
 // finite logits (-inf weighs nothing but would leave 0 * -inf in u) whose
 // products with L are finite too; the careful one takes every value.
-template <bool CAREFUL, int N, int V>
-__device__ __forceinline__ RowSums sums_of(const float (&v)[N][V], float m) {
+template <bool CAREFUL>
+__device__ __forceinline__ void add_element(RowSums& r, float x, float top, float base) {
+  const float y = CAREFUL ? (x - top) * kLog2e : __builtin_fmaf(x, kLog2e, -base);
+  const float e = __builtin_amdgcn_exp2f(y);
+  r.s += e;
+  r.u = CAREFUL && e == 0.f ? r.u : __builtin_fmaf(e, y, r.u);
+}
+template <bool CAREFUL, typename L, int N>
+__device__ __forceinline__ RowSums sums_of(const L (&v)[N], float m) {
   RowSums r{m, 0.f, 0.f};
   const float top = CAREFUL && m == -__builtin_inff() ? 0.f : m;
   const float base = top * kLog2e;
 #pragma unroll
   for (int l = 0; l < N; ++l)
 #pragma unroll
-    for (int j = 0; j < V; ++j) {
-      const float y = CAREFUL ? (v[l][j] - top) * kLog2e : __builtin_fmaf(v[l][j], kLog2e, -base);
-      const float e = __builtin_amdgcn_exp2f(y);
-      r.s += e;
-      r.u = CAREFUL ? (e == 0.f ? r.u : __builtin_fmaf(e, y, r.u)) : __builtin_fmaf(e, y, r.u);
-    }
+    for (int j = 0; j < L::V; ++j) add_element<CAREFUL>(r, v[l].at(j), top, base);
   return r;
 }
 // The plain form's sums against m itself.
@@ -73,12 +76,19 @@ __device__ __forceinline__ void take_back_rounding(RowSums& r) {
 __device__ __forceinline__ bool plain_range(float m) { return fabsf(m) < 1e38f; }
 
 __device__ __forceinline__ float rest_of(const RowSums& r) { return __builtin_log2f(r.s) * kLn2; }
+// The given token's logit, loaded ahead of what store_row() waits for.
+struct Given {
+  float x;
+  bool known;
+};
 template <typename T>
-__device__ __forceinline__ void store_row(const LogprobsPlan& p, uint32_t row, const T* x, const RowSums& r) {
-  const float rest = rest_of(r);
+__device__ __forceinline__ Given given_of(const LogprobsPlan& p, uint32_t row, const T* x) {
   const int64_t token = p.tokens[(int64_t)row * p.token_step];
   const bool known = (uint64_t)token < (uint64_t)p.width;
-  p.logprob[(int64_t)row * p.lp_step] = known ? ((float)x[token] - r.m) - rest : __builtin_nanf("");
+  return {(float)x[known ? token : 0], known};
+}
+__device__ __forceinline__ void store_row(const LogprobsPlan& p, uint32_t row, const Given& given, const RowSums& r) {
+  p.logprob[(int64_t)row * p.lp_step] = given.known ? (given.x - r.m) - rest_of(r) : __builtin_nanf("");
   p.entropy[(int64_t)row * p.h_step] = (__builtin_log2f(r.s) - r.u / r.s) * kLn2;
 }
 __device__ __forceinline__ void store_alternative(const LogprobsPlan& p, uint32_t row, int i, uint32_t id, float x,
@@ -96,212 +106,569 @@ __global__ __launch_bounds__(256) void short_rows_kernel(LogprobsPlan p) {
   const bool live = row < p.rows;
   const T* x = static_cast<const T*>(p.logits) + (int64_t)min(row, p.rows - 1) * p.row;
   const uint32_t first = g * PER;
-  float v[1][PER];
+  const Given given = given_of(p, min(row, p.rows - 1), x);
+  float v[PER];
   if (first + PER <= p.width) {
-    dev::load_pack<T, PER>(x + first, v[0]);
+    dev::load_pack<T, PER>(x + first, v);
   } else {
 #pragma unroll
-    for (int j = 0; j < PER; ++j) v[0][j] = first + j < p.width ? (float)x[first + j] : -__builtin_inff();
+    for (int j = 0; j < PER; ++j) v[j] = first + j < p.width ? (float)x[first + j] : -__builtin_inff();
   }
   float m = -__builtin_inff();
 #pragma unroll
-  for (int j = 0; j < PER; ++j) m = fmaxf(m, v[0][j]);
-  RowSums r = sums_of<true>(v, dev::group_max<G>(m));
+  for (int j = 0; j < PER; ++j) m = fmaxf(m, v[j]);
+  RowSums r{dev::group_max<G>(m), 0.f, 0.f};
+  const float top = r.m == -__builtin_inff() ? 0.f : r.m;
+#pragma unroll
+  for (int j = 0; j < PER; ++j) add_element<true>(r, v[j], top, 0.f);
   r.s = dev::group_sum<G>(r.s);
   r.u = dev::group_sum<G>(r.u);
-  if (live && g == 0) store_row(p, row, x, r);
+  if (live && g == 0) store_row(p, row, given, r);
   if (p.top == 0) return;
   const float rest = rest_of(r);
   uint32_t key[PER];
 #pragma unroll
-  for (int j = 0; j < PER; ++j) key[j] = first + j < p.width ? dev::score_key(v[0][j]) : 0u;
+  for (int j = 0; j < PER; ++j) key[j] = first + j < p.width ? dev::score_key(v[j]) : 0u;
   dev::take_best<G, PER>(key, p.top, g, [&](int i, uint32_t id, uint32_t k) {
     if (live) store_alternative(p, row, i, id, dev::key_score(k), r.m, rest);
   });
 }
 
 // ---------------------------------------------------------------- long rows
-// A wavefront takes a tile of 4096 elements of a row: its sums, and the
-// maximum of each run of 64, whose order is all that the second launch needs
-// to find the alternatives.
+// NaN before everything.
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  __asm__("v_maximum3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+  return r;
+}
+// Sixteen bytes of a row as loaded.  (Maxima of pairs of halves, which leave the
+// conversion to a mixed-precision fma, measured slower: 71.6 against 67.6 us for
+// 4001 rows of 50001 halves.)
 template <typename T>
-__global__ __launch_bounds__(256) void tiles_kernel(LogprobsPlan p) {
-  constexpr uint32_t V = 16 / sizeof(T);     // elements of a load
-  constexpr uint32_t kLoads = kRun / V;      // loads of a lane
-  constexpr uint32_t kLanes = kRun / V;      // lanes that hold a run
-  const uint32_t lane = threadIdx.x & 63u;
-  const uint32_t wave = blockIdx.x * 4 + (threadIdx.x >> 6);
-  const uint32_t row = p.by_tiles.div(wave);
-  if (row >= p.rows) return;
-  const uint32_t tile = wave - row * p.tiles;
-  const T* x = static_cast<const T*>(p.logits) + (int64_t)row * p.row;
-  float v[kLoads][V];
+struct Lane16 {
+  static constexpr int V = 16 / sizeof(T);
+  typename dev::Pack<T, V>::type raw;
+  __device__ __forceinline__ void load(const T* p) { raw = *reinterpret_cast<const typename dev::Pack<T, V>::type*>(p); }
+  __device__ __forceinline__ void set(int j, T x) { raw[j] = x; }
+  __device__ __forceinline__ void fill(T x) {
 #pragma unroll
-  for (uint32_t l = 0; l < kLoads; ++l) {
-    const uint32_t at = tile * kTile + l * 64 * V + lane * V;
-    if (at + V <= p.width) {
-      dev::load_pack<T, V>(x + at, v[l]);
+    for (int j = 0; j < V; ++j) raw[j] = x;
+  }
+  __device__ __forceinline__ float at(int j) const { return (float)raw[j]; }
+  __device__ __forceinline__ float maximum() const {
+    if constexpr (V == 8) {
+      return max3(max3(max3(at(0), at(1), at(2)), at(3), at(4)), max3(at(5), at(6), at(7)), at(7));
     } else {
-#pragma unroll
-      for (uint32_t j = 0; j < V; ++j) v[l][j] = at + j < p.width ? (float)x[at + j] : -__builtin_inff();
+      return max3(max3(at(0), at(1), at(2)), at(3), at(3));
     }
   }
-  float m = -__builtin_inff();
-  uint32_t run_key = 0;
+};
+
+// Maxima over runs of N lanes of N values each lane: lane i of a run ends with
+// the maximum of value i.  Each step halves the values: a lane keeps one of a
+// pair, and hands the other to the lane across.
+template <int O>
+__device__ __forceinline__ float lane_xor_max(float keep, float send) {
+  const float got = dev::lane_xor<O>(send);
+  return max3(keep, got, got);
+}
+template <int N>
+__device__ __forceinline__ float run_maximum(const float (&v)[N]) {
+  if constexpr (N == 1) {
+    return v[0];
+  } else {
+    constexpr int H = N / 2;
+    const bool up = threadIdx.x & H;
+    float half[H];
 #pragma unroll
-  for (uint32_t l = 0; l < kLoads; ++l) {
-    float top = v[l][0];
-#pragma unroll
-    for (uint32_t j = 1; j < V; ++j) top = __builtin_elementwise_maximum(top, v[l][j]);
-#pragma unroll
-    for (uint32_t o = 1; o < kLanes; o <<= 1) top = __builtin_elementwise_maximum(top, __shfl_xor(top, o, 64));
-    // the lanes of a run keep one load's maximum each
-    const uint32_t at = tile * kTile + l * 64 * V + (lane & ~(kLanes - 1)) * V;
-    if (lane % kLanes == l) run_key = at < p.width ? dev::score_key(top) : 0u;
-    m = __builtin_elementwise_maximum(m, top);
+    for (int i = 0; i < H; ++i) half[i] = lane_xor_max<H>(up ? v[i + H] : v[i], up ? v[i] : v[i + H]);
+    return run_maximum<H>(half);
   }
+}
+
+// A wavefront's tile of 4096 elements: sums and maximum (the same in every
+// lane), and in lane l the maximum of run run_of(l).
+template <typename T>
+__device__ __forceinline__ uint32_t run_of() {
+  constexpr uint32_t kLoads = kRun / Lane16<T>::V;
+  const uint32_t lane = threadIdx.x & 63u;
+  return lane % kLoads * (64 / kLoads) + lane / kLoads;
+}
+// What stands in the place of elements that a row does not have: finite, and of
+// weight 0 next to any maximum above kLowest (an -inf would leave 0 * -inf).
+template <typename T> constexpr float kAbsent = -1e30f;
+template <> constexpr float kAbsent<_Float16> = -65504.f;
+template <typename T> constexpr float kLowest = -1e29f;
+template <> constexpr float kLowest<_Float16> = -65000.f;
+
+// The tile whose 16-byte aligned first position is at x; the row has positions
+// [lo, hi) of it.
+template <typename T>
+__device__ __forceinline__ RowSums tile_sums(const T* x, int32_t lo, int32_t hi, float& run_top) {
+  constexpr int V = Lane16<T>::V;   // elements of a load
+  constexpr int kLoads = kRun / V;  // loads of a lane, and lanes that hold a run
+  typedef typename dev::Pack<T, V>::type P;
+  const int32_t lane = (int32_t)(threadIdx.x & 63u);
+  const bool whole = lo <= 0 && hi >= (int32_t)kTile;  // the same for the whole wave
+  Lane16<T> v[kLoads];
+  if (whole) {
 #pragma unroll
-  for (uint32_t o = kLanes; o < 64; o <<= 1) m = __builtin_elementwise_maximum(m, __shfl_xor(m, o, 64));
-  // wave-uniform: every lane holds m and the sums
+    for (int l = 0; l < kLoads; ++l) {
+      typedef T aligned __attribute__((ext_vector_type(V)));
+      v[l].raw = __builtin_bit_cast(P, *reinterpret_cast<const aligned*>(x + (l * 64 + lane) * V));
+    }
+  } else {
+#pragma unroll
+    for (int l = 0; l < kLoads; ++l) {
+      const int32_t at = (l * 64 + lane) * V;
+      v[l].fill((T)kAbsent<T>);
+      if (at >= lo && at + V <= hi) v[l].load(x + at);
+    }
+    // the vectors in which the row begins and ends, element by element
+#pragma unroll 1
+    for (int e = 0; e < 2; ++e) {
+      const int32_t edge = e ? hi : lo;
+      if (edge <= 0 || edge >= (int32_t)kTile || edge % V == 0 || (e && lo > 0 && lo / V == hi / V)) continue;
+      const int32_t vec = edge / V;
+      if (lane != vec % 64) continue;
+      Lane16<T> part;
+#pragma unroll
+      for (int j = 0; j < V; ++j) part.set(j, vec * V + j >= lo && vec * V + j < hi ? x[vec * V + j] : (T)kAbsent<T>);
+#pragma unroll
+      for (int l = 0; l < kLoads; ++l)
+        if (l == vec / 64) v[l] = part;
+    }
+  }
+  float m;
+  const auto maxima = [&]() {
+    float part[kLoads];
+#pragma unroll
+    for (int l = 0; l < kLoads; ++l) part[l] = v[l].maximum();
+    run_top = run_maximum<kLoads>(part);
+    m = lane_xor_max<32>(run_top, run_top);
+    m = lane_xor_max<16>(m, m);
+    m = lane_xor_max<8>(m, m);
+    m = lane_xor_max<4>(m, m);
+    m = lane_xor_max<2>(m, m);
+    m = lane_xor_max<1>(m, m);
+  };
+  maxima();
   RowSums r{m, 0.f, __builtin_nanf("")};
-  if ((tile + 1) * kTile <= p.width && plain_range(m)) {
+  if (m > kLowest<T> && plain_range(m)) {
     r = sums_of<false>(v, m);
     r.s = dev::group_sum<64>(r.s);
     r.u = dev::group_sum<64>(r.u);
     take_back_rounding(r);
   }
   if (r.u != r.u) {
+    if (!whole) {
+#pragma unroll
+      for (int l = 0; l < kLoads; ++l)
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          const int32_t at = (l * 64 + lane) * V + j;
+          if (at < lo || at >= hi) v[l].set(j, (T)-__builtin_inff());
+        }
+      maxima();
+    }
     r = sums_of<true>(v, m);
     r.s = dev::group_sum<64>(r.s);
     r.u = dev::group_sum<64>(r.u);
   }
-  const uint64_t at = (uint64_t)row * p.tiles + tile;
-  if (lane == 0) {
-    p.tile_keys[at] = dev::score_key(m);
-    p.tile_sums[2 * at] = r.s;
-    p.tile_sums[2 * at + 1] = r.u;
-  }
-  if (p.top) p.run_keys[at * 64 + lane % kLanes * (64 / kLanes) + lane / kLanes] = run_key;
+  return r;
+}
+// The order of the maximum of this lane's run, 0 if the row has none of it.
+template <typename T>
+__device__ __forceinline__ uint32_t run_key(float run_top, int32_t lo, int32_t hi) {
+  const int32_t at = (int32_t)(run_of<T>() * kRun);
+  return at + (int32_t)kRun > lo && at < hi ? dev::score_key(run_top) : 0u;
 }
 
-// The K best of the keys of a wavefront, item i of lane l standing for index
-// base[i] * 64 + l, base ascending.  At least K lanes hold a key as high as the
-// K-th best of the lanes' maxima: what lies above it, and of its equals the
-// first K in the order of the index, contains the K best.  `list` then holds
-// them (at most (K - 1) items of each of the K - 1 lanes above, and K), and
-// ranks by counting put them in order.  Returns how many there are.
-struct Found {
-  uint32_t key, index;
+// A row in 16-byte aligned positions: x[at - skew] is at position `at`.
+template <typename T>
+struct Row {
+  const T* x;
+  int32_t skew;
+  __device__ __forceinline__ Row(const LogprobsPlan& p, uint32_t row)
+      : x(static_cast<const T*>(p.logits) + (int64_t)row * p.row),
+        skew((int32_t)((reinterpret_cast<uintptr_t>(x) & 15u) / sizeof(T))) {}
+  __device__ __forceinline__ RowSums tile(const LogprobsPlan& p, uint32_t t, uint32_t& key) const {
+    const int32_t from = (int32_t)(t * kTile) - skew, lo = -from, hi = (int32_t)p.width - from;
+    float run_top;
+    const RowSums r = tile_sums(x + from, lo, hi, run_top);
+    key = run_key<T>(run_top, lo, hi);
+    return r;
+  }
+  // the order of the element at a position, 0 if the row has none there
+  __device__ __forceinline__ uint32_t key(const LogprobsPlan& p, uint32_t at) const {
+    const uint32_t i = at - (uint32_t)skew;
+    const uint32_t key = dev::score_key((float)x[min(i, p.width - 1)]);
+    return i < p.width ? key : 0u;
+  }
 };
-constexpr int kListed = (int)((kMaxTop - 1) * kMaxTop + kMaxTop);
 
-__device__ int best_of(const uint32_t (&key)[kMaxTop], int items, const uint32_t* base, int K, Found* list,
-                       uint32_t* lane_keys, Found* best) {
+// Adds a tile's sums to the row's, whose maximum r.m is known.
+__device__ __forceinline__ void join(RowSums& r, float m, float s, float u) {
+  if (s == 0.f) return;
+  const float shift = (m - r.m) * kLog2e;
+  const float f = __builtin_amdgcn_exp2f(shift);
+  r.s = __builtin_fmaf(f, s, r.s);
+  if (f != 0.f) r.u = __builtin_fmaf(f, __builtin_fmaf(shift, s, u), r.u);
+}
+
+// The K best of `items` x 64 keys by one wavefront, key(i) being item i of this
+// lane and standing for index(i): entry r of best[], r < n, becomes the r-th
+// best as key << 32 | ~index.  Where K lanes hold a key as high as some bound,
+// the K best are among the keys not below it; those are listed and ranked by
+// counting.  Where equal keys make the list too long, the best are taken one by
+// one.  Keys in LDS and rolled loops: a row runs this twice, and
+// fetching the instructions took longer than running them (unrolled over 32
+// keys a lane in registers, 25 KB of code, three of these took 17 us).
+constexpr int kListed = 256;
+__device__ __forceinline__ uint32_t index_of(uint64_t entry) { return ~(uint32_t)entry; }
+__device__ __forceinline__ uint32_t key_of(uint64_t entry) { return (uint32_t)(entry >> 32); }
+__device__ __forceinline__ uint64_t lane_value(uint64_t v, int lane) {
+  return (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), lane) << 32 |
+         (uint32_t)__builtin_amdgcn_readlane((int)v, lane);
+}
+struct Lists {
+  uint64_t list[kListed];
+  uint64_t best[kMaxTop];
+};
+
+template <typename Key, typename Index>
+__device__ __forceinline__ int best_of(Key key, Index index, int items, int K, Lists& lds) {
   const uint32_t lane = threadIdx.x & 63u;
   uint32_t top = 0;
-#pragma unroll
-  for (int i = 0; i < (int)kMaxTop; ++i)
-    if (i < items) top = max(top, key[i]);
-  lane_keys[lane] = top;
-  dev::wave_lds_fence();
-  int rank = 0;
-  for (int o = 0; o < 64; ++o) {
-    const uint32_t other = lane_keys[o];
-    rank += other > top || (other == top && o < (int)lane);
+#pragma unroll 4
+  for (int i = 0; i < items; ++i) top = max(top, key(i));
+  // the ceil(K / 4)-th best maximum of each 16 lanes (or less, where maxima are
+  // equal): the lowest of the four
+  uint32_t bound = dev::group_max_key<16>(top);
+#pragma unroll 1
+  for (int k = 4; k < K; k += 4) {
+    if (top >= bound) top = 0;
+    bound = dev::group_max_key<16>(top);
   }
-  const uint64_t last = __ballot(rank == K - 1);
-  const uint32_t bound = max(1u, (uint32_t)__builtin_amdgcn_readlane((int)top, __builtin_ctzll(last)));
-  int above = 0, equal = 0;
+  bound = min(bound, dev::lane_xor_bits<16>(bound));
+  bound = max(1u, min(bound, dev::lane_xor_bits<32>(bound)));
+  int listed = 0;
+  const auto entry = [&](int i, uint32_t k) { return (uint64_t)k << 32 | (uint32_t)~index(i); };
+#pragma unroll 1
+  for (int i = 0; i < items; i += 4) {
+    uint32_t k[4];
 #pragma unroll
-  for (int i = 0; i < (int)kMaxTop; ++i) {
-    if (i >= items) continue;
-    const uint64_t over = __ballot(key[i] > bound), same = __ballot(key[i] == bound);
-    const uint64_t below = (1ull << lane) - 1;
-    if (key[i] > bound) list[kMaxTop + above + __builtin_popcountll(over & below)] = Found{key[i], base[i] * 64 + lane};
-    const int place = equal + __builtin_popcountll(same & below);
-    if (key[i] == bound && place < K) list[place] = Found{key[i], base[i] * 64 + lane};
-    above += __builtin_popcountll(over);
-    equal = min(K, equal + (int)__builtin_popcountll(same));
-  }
-  dev::wave_lds_fence();
-  const int n = min(K, above + equal);
-  for (int i = (int)lane; i < above + equal; i += 64) {
-    const Found mine = i < equal ? list[i] : list[kMaxTop + i - equal];
-    int before = 0;
-    for (int o = 0; o < above + equal; ++o) {
-      const Found other = o < equal ? list[o] : list[kMaxTop + o - equal];
-      before += other.key > mine.key || (other.key == mine.key && other.index < mine.index);
+    for (int u = 0; u < 4; ++u) k[u] = key(min(i + u, items - 1));
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const bool hit = k[u] >= bound && i + u < items;
+      const uint64_t here = __ballot(hit);
+      if (here == 0) continue;
+      const int at = listed + (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(here >> 32),
+                                                             __builtin_amdgcn_mbcnt_lo((uint32_t)here, 0));
+      if (hit && at < kListed) lds.list[at] = entry(i + u, k[u]);
+      listed += __builtin_popcountll(here);
     }
-    if (before < K) best[before] = mine;
+  }
+  dev::wave_lds_fence();
+  const int n = min(K, listed);
+  if (listed <= 64) {
+    const uint64_t own = (int)lane < listed ? lds.list[lane] : 0;
+    int before = 0;
+    for (int o = 0; o < listed; ++o) before += lane_value(own, o) > own;
+    if ((int)lane < listed && before < K) lds.best[before] = own;
+  } else if (listed <= kListed) {
+    for (int i = (int)lane; i < listed; i += 64) {
+      const uint64_t own = lds.list[i];
+      int before = 0;
+#pragma unroll 4
+      for (int o = 0; o < listed; ++o) before += lds.list[o] > own;
+      if (before < K) lds.best[before] = own;
+    }
+  } else {
+    uint64_t last = 0;
+#pragma unroll 1
+    for (int k = 0; k < n; ++k) {
+      uint64_t next = 0;
+#pragma unroll 1
+      for (int i = 0; i < items; ++i) {
+        const uint64_t own = entry(i, key(i));
+        if ((k == 0 || own < last) && own > next) next = own;
+      }
+      last = dev::group_max_key<64>(next);
+      if (lane == 0) lds.best[k] = last;
+    }
   }
   dev::wave_lds_fence();
   return n;
 }
 
-// Indices of `best` in ascending order.
-__device__ void ascending(const Found* best, int n, uint32_t* index) {
-  const int lane = (int)(threadIdx.x & 63u);
-  if (lane < n) {
-    const uint32_t mine = best[lane].index;
-    int before = 0;
-    for (int o = 0; o < n; ++o) before += best[o].index < mine;
-    index[before] = mine;
-  }
-  dev::wave_lds_fence();
-}
-
-// A wavefront a row: joins the tiles' sums, then descends from the K tiles
-// with the best maxima to their K best runs and the K best elements of those
-// (any element outside has K better ones before it).
+// The row's K best elements by one wavefront, from `items` x 64 staged keys of
+// its runs or of its tiles (any element outside has K better ones before it).
+// The K best items of a level become the next level's, 64 adjacent keys of each.
 template <typename T>
-__global__ __launch_bounds__(64) void finish_kernel(LogprobsPlan p) {
-  __shared__ Found list[kListed];
-  __shared__ Found best[kMaxTop];
-  __shared__ uint32_t lane_keys[64];
-  __shared__ uint32_t base[kMaxTop];
-  const uint32_t lane = threadIdx.x, row = blockIdx.x;
-  const T* x = static_cast<const T*>(p.logits) + (int64_t)row * p.row;
-  const uint32_t* tile_keys = p.tile_keys + (uint64_t)row * p.tiles;
-  const float* tile_sums = p.tile_sums + 2 * (uint64_t)row * p.tiles;
-  uint32_t top = 0;
-  for (uint32_t t = lane; t < p.tiles; t += 64) top = max(top, tile_keys[t]);
-  top = dev::group_max_key<64>(top);
-  RowSums r{dev::key_score(top), 0.f, 0.f};
-  for (uint32_t t = lane; t < p.tiles; t += 64) {
-    const float s = tile_sums[2 * t], u = tile_sums[2 * t + 1];
-    if (s == 0.f) continue;
-    const float shift = (dev::key_score(tile_keys[t]) - r.m) * kLog2e;
-    const float f = __builtin_amdgcn_exp2f(shift);
-    r.s = __builtin_fmaf(f, s, r.s);
-    if (f != 0.f) r.u = __builtin_fmaf(f, __builtin_fmaf(shift, s, u), r.u);
-  }
-  r.s = dev::group_sum<64>(r.s);
-  r.u = dev::group_sum<64>(r.u);
-  if (lane == 0) store_row(p, row, x, r);
-  if (p.top == 0) return;
-  const float rest = rest_of(r);
-
-  uint32_t key[kMaxTop];
-  if (lane < (uint32_t)kMaxTop) base[lane] = lane;
-  dev::wave_lds_fence();
-  const int items = (int)((p.tiles + 63) / 64);
-#pragma unroll
-  for (int i = 0; i < (int)kMaxTop; ++i) key[i] = i < items && i * 64 + lane < p.tiles ? tile_keys[i * 64 + lane] : 0u;
-  int n = best_of(key, items, base, p.top, list, lane_keys, best);
-  ascending(best, n, base);
+__device__ __forceinline__ void alternatives(const LogprobsPlan& p, uint32_t row, const Row<T>& x, uint32_t* staged,
+                                             int items, bool runs, float m, float rest, Lists& lds) {
+  const uint32_t lane = threadIdx.x & 63u;
   const uint32_t* run_keys = p.run_keys + (uint64_t)row * p.tiles * 64;
+  uint32_t chosen = lane;  // in lane i: what item i stands for
+  const auto item = [&](int i) { return (uint32_t)__builtin_amdgcn_readlane((int)chosen, i) * 64 + lane; };
+  int n = items;
+#pragma unroll 1
+  for (int level = runs ? 1 : 0;; ++level) {  // tiles, runs, elements
+    n = best_of([&](int i) { return staged[i * 64 + lane]; }, item, n, p.top, lds);
+    chosen = (int)lane < n ? index_of(lds.best[lane]) : 0u;
+    if (level == 2) break;
+#pragma unroll 1
+    for (int i = 0; i < n; i += 8) {  // eight loads in flight
+      uint32_t key[8];
+      if (level) {
 #pragma unroll
-  for (int i = 0; i < (int)kMaxTop; ++i) key[i] = i < n ? run_keys[base[i] * 64 + lane] : 0u;
-  n = best_of(key, n, base, p.top, list, lane_keys, best);
-  ascending(best, n, base);
+        for (int u = 0; u < 8; ++u) key[u] = x.key(p, item(min(i + u, n - 1)));
+      } else {
 #pragma unroll
-  for (int i = 0; i < (int)kMaxTop; ++i)
-    key[i] = i < n && base[i] * 64 + lane < p.width ? dev::score_key((float)x[base[i] * 64 + lane]) : 0u;
-  n = best_of(key, n, base, p.top, list, lane_keys, best);
-  if ((int)lane < n) store_alternative(p, row, (int)lane, best[lane].index, dev::key_score(best[lane].key), r.m, rest);
+        for (int u = 0; u < 8; ++u) key[u] = run_keys[item(min(i + u, n - 1))];
+      }
+#pragma unroll
+      for (int u = 0; u < 8; ++u)
+        if (i + u < n) staged[(i + u) * 64 + lane] = key[u];
+    }
+    dev::wave_lds_fence();
+  }
+  if ((int)lane < n)
+    store_alternative(p, row, (int)lane, chosen - (uint32_t)x.skew, dev::key_score(key_of(lds.best[lane])), m, rest);
 }
 
-uint32_t tiles_of(int64_t width) { return (uint32_t)((width + kTile - 1) / kTile); }
+// The sums of all tiles, in every lane.  The first 64 tiles' are loaded before
+// anything else of a row's end, whose loads would otherwise wait for each other.
+struct TileSums {
+  const uint32_t* keys;
+  const float* sums;
+  uint32_t tiles, key;
+  float s, u;
+  __device__ __forceinline__ TileSums(const LogprobsPlan& p, uint32_t row)
+      : keys(p.tile_keys + (uint64_t)row * p.tiles), sums(p.tile_sums + 2 * (uint64_t)row * p.tiles), tiles(p.tiles) {
+    const uint32_t lane = threadIdx.x & 63u, t = min(lane, tiles - 1);
+    key = keys[t];
+    s = sums[2 * t];
+    u = sums[2 * t + 1];
+    if (lane >= tiles) s = 0.f;
+  }
+  __device__ __forceinline__ RowSums row() const {
+    const uint32_t lane = threadIdx.x & 63u;
+    uint32_t top = key;
+    for (uint32_t t = lane + 64; t < tiles; t += 64) top = max(top, keys[t]);
+    RowSums r{dev::key_score(dev::group_max_key<64>(top)), 0.f, 0.f};
+    join(r, dev::key_score(key), s, u);
+    for (uint32_t t = lane + 64; t < tiles; t += 64) join(r, dev::key_score(keys[t]), sums[2 * t], sums[2 * t + 1]);
+    r.s = dev::group_sum<64>(r.s);
+    r.u = dev::group_sum<64>(r.u);
+    return r;
+  }
+};
+
+// Rows of one tile, a wavefront each, in one launch.
+template <typename T>
+__global__ __launch_bounds__(64) void tile_rows_kernel(LogprobsPlan p) {
+  __shared__ Lists lds;
+  __shared__ uint32_t staged[kMaxTop * 64];
+  const uint32_t row = blockIdx.x;
+  const Row<T> x(p, row);
+  const Given given = given_of(p, row, x.x);
+  uint32_t key;
+  const RowSums r = x.tile(p, 0, key);
+  if (threadIdx.x == 0) store_row(p, row, given, r);
+  if (p.top == 0) return;
+  staged[run_of<T>()] = key;
+  dev::wave_lds_fence();
+  alternatives(p, row, x, staged, 1, true, r.m, rest_of(r), lds);
+}
+
+// Longer rows, two launches: tiles anywhere on the device, then the joins.
+template <typename T>
+__global__ __launch_bounds__(256) void tiles_kernel(LogprobsPlan p) {
+  const uint32_t wave = blockIdx.x * 4 + (threadIdx.x >> 6);
+  const uint32_t row = p.by_tiles.div(wave);
+  if (row >= p.rows) return;
+  uint32_t key;
+  const RowSums r = Row<T>(p, row).tile(p, wave - row * p.tiles, key);
+  if ((threadIdx.x & 63u) == 0) {
+    p.tile_keys[wave] = dev::score_key(r.m);
+    p.tile_sums[2 * (uint64_t)wave] = r.s;
+    p.tile_sums[2 * (uint64_t)wave + 1] = r.u;
+  }
+  if (p.top) p.run_keys[(uint64_t)wave * 64 + run_of<T>()] = key;
+}
+
+// Many rows: a wavefront each, which the others on the device hide (as much LDS
+// as the row needs, so that more of them fit).
+constexpr uint32_t kStaged = 33;  // items of 64: the tiles of the longest row, the runs of 33 tiles
+uint32_t staged_items(uint32_t tiles, int64_t top) {
+  return top ? std::max<uint32_t>(tiles <= kStaged ? tiles : (tiles + 63) / 64, (uint32_t)top) : 0u;
+}
+template <typename T>
+__global__ __launch_bounds__(64) void finish_many_kernel(LogprobsPlan p) {
+  __shared__ Lists lds;
+  extern __shared__ uint32_t staged[];  // staged_items() x 64
+  const uint32_t lane = threadIdx.x, row = blockIdx.x;
+  const Row<T> x(p, row);
+  const Given given = given_of(p, row, x.x);
+  const TileSums sums(p, row);
+  const bool runs = p.tiles <= kStaged;
+  const int items = runs ? (int)p.tiles : (int)((p.tiles + 63) / 64);
+  if (p.top) {
+    const uint32_t* keys = runs ? p.run_keys + (uint64_t)row * p.tiles * 64 : sums.keys;
+    const uint32_t count = runs ? p.tiles * 64 : p.tiles;
+#pragma unroll 1
+    for (int i = 0; i < items; i += 16) {  // 16 loads in flight
+      uint32_t key[16];
+#pragma unroll
+      for (int u = 0; u < 16; ++u) key[u] = keys[min((i + u) * 64 + lane, count - 1)];
+#pragma unroll
+      for (int u = 0; u < 16; ++u)
+        if (i + u < items) staged[(i + u) * 64 + lane] = (i + u) * 64 + lane < count ? key[u] : 0u;
+    }
+  }
+  const RowSums r = sums.row();
+  if (lane == 0) store_row(p, row, given, r);
+  dev::wave_lds_fence();
+  if (p.top) alternatives(p, row, x, staged, items, runs, r.m, rest_of(r), lds);
+}
+
+// Few rows: 16 wavefronts each, for the latency.
+// best_of() by a workgroup of 16 wavefronts, item i of a thread standing for
+// index(i): the same bound from the maxima of the 64 lane columns, its counts
+// and ranks shared out over the waves (in one wave each of their steps waits
+// for the last: 11400 cycles for 20 of 2048 keys, a tenth of that here).
+constexpr int kFinishThreads = 1024;
+constexpr int kHeld = 8;  // keys of a thread
+struct WideLists {
+  uint64_t list[kListed];
+  uint64_t best[kMaxTop];
+  uint64_t wave_best[kFinishThreads / 64];
+  uint32_t rank[kListed];
+  uint32_t column[64];
+  uint32_t higher[64];
+  uint32_t count;
+};
+template <typename Index>
+__device__ __forceinline__ int wide_best_of(const uint32_t (&key)[kHeld], Index index, int K, WideLists& lds) {
+  constexpr uint32_t W = kFinishThreads / 64;
+  const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
+  if (threadIdx.x < 64) {
+    lds.column[threadIdx.x] = 0;
+    lds.higher[threadIdx.x] = 0;
+  }
+  if (threadIdx.x < (uint32_t)kListed) lds.rank[threadIdx.x] = 0;
+  if (threadIdx.x == 0) lds.count = 0;
+  __syncthreads();
+  uint32_t top = 0;
+#pragma unroll
+  for (int i = 0; i < kHeld; ++i) top = max(top, key[i]);
+  if (top) atomicMax(&lds.column[lane], top);
+  __syncthreads();
+  const uint32_t mine = lds.column[lane];
+  uint32_t higher = 0;
+#pragma unroll
+  for (uint32_t o = 0; o < 64 / W; ++o) higher += lds.column[wave * (64 / W) + o] > mine;
+  if (higher) atomicAdd(&lds.higher[lane], higher);
+  __syncthreads();
+  // the lowest maximum that fewer than K others pass
+  const uint32_t bound = max(1u, ~dev::group_max_key<64>(lds.higher[lane] < (uint32_t)K ? ~mine : 0u));
+  if (top >= bound) {
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i)
+      if (key[i] >= bound) {
+        const uint32_t at = atomicAdd(&lds.count, 1u);
+        if (at < (uint32_t)kListed) lds.list[at] = (uint64_t)key[i] << 32 | (uint32_t)~index(i);
+      }
+  }
+  __syncthreads();
+  const int listed = (int)lds.count, n = min(K, listed);
+  if (listed <= kListed) {
+    for (int e = (int)lane; e < listed; e += 64) {
+      const uint64_t own = lds.list[e];
+      uint32_t before = 0;
+      for (int o = (int)wave; o < listed; o += W) before += lds.list[o] > own;
+      if (before) atomicAdd(&lds.rank[e], before);
+    }
+    __syncthreads();
+    if ((int)threadIdx.x < listed && lds.rank[threadIdx.x] < (uint32_t)K)
+      lds.best[lds.rank[threadIdx.x]] = lds.list[threadIdx.x];
+  } else {
+    uint64_t last = 0;
+#pragma unroll 1
+    for (int k = 0; k < n; ++k) {
+      uint64_t next = 0;
+#pragma unroll
+      for (int i = 0; i < kHeld; ++i) {
+        const uint64_t own = (uint64_t)key[i] << 32 | (uint32_t)~index(i);
+        if (key[i] && (k == 0 || own < last) && own > next) next = own;
+      }
+      next = dev::group_max_key<64>(next);
+      if (lane == 0) lds.wave_best[wave] = next;
+      __syncthreads();
+      last = 0;
+#pragma unroll 1
+      for (uint32_t w = 0; w < W; ++w) last = lds.wave_best[w] > last ? lds.wave_best[w] : last;
+      __syncthreads();
+      if (threadIdx.x == 0) lds.best[k] = last;
+    }
+  }
+  __syncthreads();
+  return n;
+}
+
+template <typename T>
+__global__ __launch_bounds__(kFinishThreads) void finish_few_kernel(LogprobsPlan p) {
+  constexpr uint32_t W = kFinishThreads / 64;
+  __shared__ WideLists lds;
+  const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, row = blockIdx.x;
+  const Row<T> x(p, row);
+  const Given given = given_of(p, row, x.x);
+  const TileSums sums(p, row);
+  const uint32_t* run_keys = p.run_keys + (uint64_t)row * p.tiles * 64;
+  // the runs of all tiles at once, or first the tiles
+  int level = p.tiles <= kHeld * W ? 1 : 0, n = 0;
+  uint32_t key[kHeld];
+  if (p.top) {
+    const uint32_t* keys = level ? run_keys : sums.keys;
+    const uint32_t count = level ? p.tiles * 64 : p.tiles;
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i) {
+      const uint32_t at = i * kFinishThreads + threadIdx.x, k = keys[min(at, count - 1)];
+      key[i] = at < count ? k : 0u;
+    }
+  }
+  const RowSums r = sums.row();
+  if (threadIdx.x == blockDim.x - 64) store_row(p, row, given, r);
+  if (p.top == 0) return;
+  uint32_t first[kMaxTop / W] = {};  // this wave's items of a level after the first: 64 indices each
+#pragma unroll 1
+  for (int step = 0;; ++step, ++level) {  // tiles, runs, elements
+    n = wide_best_of(key, [&](int i) { return step ? (first[i & 1] + lane) : i * kFinishThreads + threadIdx.x; }, p.top, lds);
+    if (level == 2) break;
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i) {
+      const int item = (int)wave + i * (int)W;
+      key[i] = 0;
+      if (i < (int)(kMaxTop / W) && item < n) {
+        first[i & 1] = index_of(lds.best[item]) * 64;
+        const uint32_t at = first[i & 1] + lane;
+        key[i] = level == 0 ? run_keys[at] : x.key(p, at);
+      }
+    }
+    __syncthreads();
+  }
+  if ((int)threadIdx.x < n) {
+    const uint64_t found = lds.best[threadIdx.x];
+    store_alternative(p, row, (int)threadIdx.x, index_of(found) - (uint32_t)x.skew, dev::key_score(key_of(found)), r.m,
+                      rest_of(r));
+  }
+}
+
+// Tiles of a row, wherever in 16 bytes it begins.
+uint32_t tiles_of(int64_t width, int elem) { return (uint32_t)((width + 16 / elem - 1 + kTile - 1) / kTile); }
 
 template <typename T, int G, int PER>
 thin_status launch_short(const LogprobsPlan& p, hipStream_t stream) {
@@ -317,8 +684,10 @@ thin_status launch_short(const LogprobsPlan& p, hipStream_t stream) {
 using namespace thin;
 
 extern "C" size_t thin_token_logprobs_workspace(int64_t rows, int64_t width, int64_t top) {
-  if (rows <= 0 || width <= kShortRow || width > kMaxTiles * (int64_t)kTile) return 0;
-  return (size_t)rows * tiles_of(width) * (top > 0 ? 64 + 3 : 3) * 4;
+  // (as for 16-bit rows, which may begin further into their first 16 bytes)
+  if (rows <= 0 || width <= kShortRow || width > kMaxWidth) return 0;
+  const int64_t tiles = tiles_of(width, 2);
+  return tiles == 1 ? 0 : (size_t)rows * tiles * (top > 0 ? 64 + 3 : 3) * 4;
 }
 
 extern "C" thin_status thin_token_logprobs(const thin_desc* logits, const thin_desc* tokens, const thin_desc* logprobs,
@@ -344,7 +713,7 @@ extern "C" thin_status thin_token_logprobs(const thin_desc* logits, const thin_d
   THIN_REQUIRE(V >= 1 && K <= V && K <= kMaxTop, THIN_ERR_INVALID,
                "token_logprobs gives up to %lld alternatives of the row's %lld, not %lld", (long long)kMaxTop,
                (long long)V, (long long)K);
-  THIN_REQUIRE(V <= kMaxTiles * (int64_t)kTile && R < (1ll << 31) && R * tiles_of(V) < (1ll << 31),
+  THIN_REQUIRE(V <= kMaxWidth && R < (1ll << 31) && R * tiles_of(V, 2) < (1ll << 31),
                THIN_ERR_UNSUPPORTED, "token_logprobs: tensor too large");
   THIN_REQUIRE(V == 1 || logits->strides[1] == 1, THIN_ERR_UNSUPPORTED,
                "token_logprobs: the logits of a row must be adjacent");
@@ -385,7 +754,12 @@ extern "C" thin_status thin_token_logprobs(const thin_desc* logits, const thin_d
     if (V <= 256) return launch_short<T, 16, 16>(p, stream);
     if (V <= 512) return launch_short<T, 32, 16>(p, stream);
     if (V <= kShortRow) return launch_short<T, 64, 16>(p, stream);
-    p.tiles = tiles_of(V);
+    p.tiles = tiles_of(V, 2);
+    if (p.tiles == 1) {
+      hipLaunchKernelGGL((tile_rows_kernel<T>), dim3(p.rows), dim3(64), 0, stream, p);
+      THIN_LAUNCH_CHECK("token_logprobs_rows");
+      return THIN_OK;
+    }
     p.by_tiles = FastDiv::make(p.tiles);
     const uint64_t waves = (uint64_t)p.rows * p.tiles;
     p.tile_sums = static_cast<float*>(workspace);
@@ -393,7 +767,8 @@ extern "C" thin_status thin_token_logprobs(const thin_desc* logits, const thin_d
     p.run_keys = p.tile_keys + waves;
     hipLaunchKernelGGL((tiles_kernel<T>), dim3((uint32_t)((waves + 3) / 4)), dim3(256), 0, stream, p);
     THIN_LAUNCH_CHECK("token_logprobs_tiles");
-    hipLaunchKernelGGL((finish_kernel<T>), dim3(p.rows), dim3(64), 0, stream, p);
+    if (R < kManyRows) hipLaunchKernelGGL((finish_few_kernel<T>), dim3(p.rows), dim3(p.top ? kFinishThreads : 64), 0, stream, p);
+    else hipLaunchKernelGGL((finish_many_kernel<T>), dim3(p.rows), dim3(64), staged_items(p.tiles, K) * 256, stream, p);
     THIN_LAUNCH_CHECK("token_logprobs_finish");
     return THIN_OK;
   });

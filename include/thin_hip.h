@@ -366,10 +366,11 @@ thin_status thin_attention(const thin_desc* qkv, int64_t heads, int64_t key_dim,
 /* Group norm                                                          */
 /* ------------------------------------------------------------------ */
 
-/* Bytes of workspace thin_group_norm needs (0: none).  x, channels and groups
- * as there.  No reference counterpart: the reference folds batch norm into the
+/* Bytes of workspace thin_group_norm needs (0: none) for its operands of the
+ * same names.  No reference counterpart: the reference folds batch norm into the
  * affine of its convolutions (model_optimization.py:20-31). */
-size_t thin_group_norm_workspace(const thin_desc* x, int32_t blocked, int64_t channels, int64_t groups);
+size_t thin_group_norm_workspace(const thin_desc* x, const thin_desc* out, int32_t blocked, int64_t channels,
+                                 int64_t groups);
 
 /* y = (x - mean) / sqrt(var + eps) * weight + bias with the mean and the
  * (biased) variance of each sample's groups of channels / groups adjacent

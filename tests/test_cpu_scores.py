@@ -69,12 +69,12 @@ def test_group_norm_refusals():
     norm(INVALID, x=x, out=desc((2, 4, 4, 64), data=x.data + 2))  # overlaps without being x
     norm(INVALID, x=x, weight=desc((64,), data=1 << 30), out=desc((2, 4, 4, 64), data=(1 << 30) + 64))
     big = desc((1, 200, 200, 64))
-    need = capi.lib().thin_group_norm_workspace(P(big), 0, 64, 8)
+    need = capi.lib().thin_group_norm_workspace(P(big), P(big), 0, 64, 8)
     assert need > 0
     norm(WORKSPACE, x=big)
     norm(WORKSPACE, x=big, ws=1 << 30, nbytes=need - 1)
-    assert capi.lib().thin_group_norm_workspace(P(big), 0, 64, 7) == 0
-    assert capi.lib().thin_group_norm_workspace(None, 0, 64, 8) == 0
+    assert capi.lib().thin_group_norm_workspace(P(big), P(big), 0, 64, 7) == 0
+    assert capi.lib().thin_group_norm_workspace(None, P(big), 0, 64, 8) == 0
 
 
 def route(code, logits=None, bias=None, groups=1, top=1, weights=None, experts=None, k=2):

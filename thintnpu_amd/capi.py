@@ -122,7 +122,7 @@ def lib() -> ctypes.CDLL:
         if hasattr(L, "thin_detection_select_workspace"):
             L.thin_detection_select_workspace.argtypes = [i64, i64, i64, i64, i32]
             L.thin_detection_select_workspace.restype = ctypes.c_size_t
-        for name, argtypes in {"thin_group_norm_workspace": [vp, i32, i64, i64],
+        for name, argtypes in {"thin_group_norm_workspace": [vp, vp, i32, i64, i64],
                                "thin_expert_dispatch_workspace": [i64, i64, i64],
                                "thin_token_logprobs_workspace": [i64, i64, i64]}.items():
             fn = getattr(L, name, None)
@@ -505,12 +505,12 @@ def _group_norm(x, blocked, channels, groups, weight, bias, eps, silu, out, work
     if out is None:
         out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
     L = lib()
-    xd = _packed(x)
-    need = L.thin_group_norm_workspace(xd, blocked, channels, groups)
+    xd, od = _packed(x), _on(device, out)
+    need = L.thin_group_norm_workspace(xd, od, blocked, channels, groups)
     ws, address, nbytes = _workspace(need, workspace, device, stream)
     _check("thin_group_norm", L.thin_group_norm(
         xd, blocked, channels, groups, None if weight is None else _on(device, weight),
-        None if bias is None else _on(device, bias), eps, 1 if silu else 0, _on(device, out), address, nbytes,
+        None if bias is None else _on(device, bias), eps, 1 if silu else 0, od, address, nbytes,
         _stream(stream)))
     return out
 

@@ -13,6 +13,7 @@ constexpr uint32_t kThreads = 256;
 constexpr int64_t kMaxExperts = 1024;
 constexpr int64_t kMaxChosen = 32;
 constexpr int64_t kMaxGroups = 64;
+constexpr int64_t kFewTokens = 1024;  // tokens up to which each has a whole wavefront
 
 // ---------------------------------------------------------------- routing
 struct RoutePlan {
@@ -24,6 +25,7 @@ struct RoutePlan {
   int64_t wt, wk, et, ek;            // strides of weights and experts
   uint32_t tokens, count;            // tokens, experts
   int32_t k, groups, top, size;      // chosen, groups, kept groups, experts a group
+  int32_t group_lanes;               // lanes of a group that is whole lanes, a power of two; else 0
   int32_t softmax, renormalize;
   FastDiv by_size;
   float scale;
@@ -49,42 +51,13 @@ __device__ __forceinline__ void scores32(const float (&x)[PER], uint32_t first, 
     }
     total = dev::group_sum<G>(total);
 #pragma unroll
-    for (int j = 0; j < PER; ++j) s[j] /= total;
+    for (int j = 0; j < PER; ++j) s[j] *= 1.0f / total;
   } else {
     total = 1.f;
 #pragma unroll
     for (int j = 0; j < PER; ++j) s[j] = dev::sigmoid_fast(x[j]);
   }
 }
-template <int G>
-__device__ double group_sum64(double v) {
-#pragma unroll
-  for (int o = G / 2; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
-  return v;
-}
-template <int G, int PER>
-__device__ void scores64(const float (&x)[PER], uint32_t first, uint32_t count, bool softmax, double (&s)[PER]) {
-  if (softmax) {
-    float m = -__builtin_inff();
-#pragma unroll
-    for (int j = 0; j < PER; ++j)
-      if (first + j < count) m = fmaxf(m, x[j]);
-    m = dev::group_max<G>(m);
-    double total = 0.0;
-#pragma unroll
-    for (int j = 0; j < PER; ++j) {
-      s[j] = first + j < count ? exp((double)x[j] - (double)m) : 0.0;
-      total += s[j];
-    }
-    total = group_sum64<G>(total);
-#pragma unroll
-    for (int j = 0; j < PER; ++j) s[j] /= total;
-  } else {
-#pragma unroll
-    for (int j = 0; j < PER; ++j) s[j] = 1.0 / (1.0 + exp(-(double)x[j]));
-  }
-}
-
 // How near two 32-bit choice scores may be before their order is settled in
 // 64 bits.  A score s <= 1 is off by less than 2^-22 (softmax: s |x - m| 2^-23
 // <= 0.37 * 2^-23 from the exponent's argument, 2^-23 from exp2 and the sum
@@ -94,50 +67,170 @@ __device__ __forceinline__ bool near_tie(float above, float below, float terms) 
   return above - below <= terms * (0x1p-20f + 0x1p-22f * fabsf(above));
 }
 
-// Drops the keys of groups that are not among the `top` best.  `near`: the
-// last kept and the first dropped group are too near for 32 bits.
-template <int G, int PER, bool BIAS, typename K>
-__device__ __forceinline__ bool keep_groups(const RoutePlan& p, K (&key)[PER], uint32_t g, K* staged, K* group_key,
-                                            uint8_t* kept, K* border) {
+// The best two keys of two sets.
+template <typename K>
+__device__ __forceinline__ void join_best(K& best, K& second, K b, K s) {
+  second = max(min(best, b), max(second, s));
+  best = max(best, b);
+}
+template <int O>
+__device__ __forceinline__ void join_lane(uint32_t& best, uint32_t& second) {
+  join_best(best, second, dev::lane_xor_bits<O>(best), dev::lane_xor_bits<O>(second));
+}
+template <bool BIAS, typename K>
+__device__ __forceinline__ K group_score(K best, K second, int size) {
+  return BIAS && size > 1 ? dev::score_key(dev::key_score(best) + dev::key_score(second)) : best;
+}
+
+// Drops the keys of groups that are not among the `top` best, in 32 bits;
+// true if the last kept and the first dropped group are too near for that.
+// Where a group is a power of two of whole lanes, its score comes from
+// registers; any other size goes through LDS.
+struct GroupLds {
+  uint32_t key[kMaxGroups];
+  uint32_t border[2];
+};
+template <int G, int PER, bool BIAS>
+__device__ __forceinline__ bool keep_groups(const RoutePlan& p, uint32_t (&key)[PER], uint32_t g, uint32_t* staged,
+                                            GroupLds& lds) {
   const uint32_t first = g * PER;
+  const bool whole = p.group_lanes != 0;
+  uint32_t own = 0;  // whole: the score of this lane's group
+  if (whole) {
+    uint32_t best = 0, second = 0;
 #pragma unroll
-  for (int j = 0; j < PER; ++j)
-    if (first + j < p.count) staged[first + j] = key[j];
-  dev::wave_lds_fence();
-  for (int q = (int)g; q < p.groups; q += G) {
-    K best = 0, second = 0;
-    int i = q % p.size;  // lanes start at different banks
-    for (int n = 0; n < p.size; ++n) {
-      const K v = staged[q * p.size + i];
-      second = v > best ? best : v > second ? v : second;
-      best = v > best ? v : best;
-      i = i + 1 == p.size ? 0 : i + 1;
+    for (int j = 0; j < PER; ++j) join_best(best, second, key[j], 0u);
+    if (p.group_lanes > 1) join_lane<1>(best, second);
+    if (p.group_lanes > 2) join_lane<2>(best, second);
+    if constexpr (G > 4) {
+      if (p.group_lanes > 4) join_lane<4>(best, second);
     }
-    if (BIAS && p.size > 1) best = dev::score_key(dev::key_score(best) + dev::key_score(second));
-    group_key[q] = best;
+    if constexpr (G > 8) {
+      if (p.group_lanes > 8) join_lane<8>(best, second);
+    }
+    if constexpr (G > 16) {
+      if (p.group_lanes > 16) join_lane<16>(best, second);
+    }
+    if constexpr (G > 32) {
+      if (p.group_lanes > 32) join_lane<32>(best, second);
+    }
+    own = group_score<BIAS>(best, second, p.size);
+    if (first < p.count) lds.key[p.by_size.div(first)] = own;
+  } else {
+#pragma unroll
+    for (int j = 0; j < PER; ++j)
+      if (first + j < p.count) staged[first + j] = key[j];
+    dev::wave_lds_fence();
+    for (int q = (int)g; q < p.groups; q += G) {
+      uint32_t best = 0, second = 0;
+      int i = q % p.size;  // lanes start at different banks
+      for (int n = 0; n < p.size; ++n) {
+        join_best(best, second, staged[q * p.size + i], 0u);
+        i = i + 1 == p.size ? 0 : i + 1;
+      }
+      lds.key[q] = group_score<BIAS>(best, second, p.size);
+    }
   }
   dev::wave_lds_fence();
-  for (int q = (int)g; q < p.groups; q += G) {
-    const K mine = group_key[q];
+  const auto rank_of = [&](int q, uint32_t mine) {
     int rank = 0;
+#pragma unroll 4
     for (int o = 0; o < p.groups; ++o) {
-      const K other = group_key[o];
+      const uint32_t other = lds.key[o];
       rank += other > mine || (other == mine && o < q);
     }
-    kept[q] = rank < p.top;
-    if (rank == p.top - 1) border[0] = mine;
-    if (rank == p.top) border[1] = mine;
+    if (rank == p.top - 1) lds.border[0] = mine;
+    if (rank == p.top) lds.border[1] = mine;
+    return rank;
+  };
+  if (whole) {
+    if (first < p.count && rank_of((int)p.by_size.div(first), own) >= p.top) {
+#pragma unroll
+      for (int j = 0; j < PER; ++j) key[j] = 0;
+    }
+  } else {
+    uint32_t kept[(kMaxGroups + G - 1) / G];
+#pragma unroll
+    for (int i = 0; i < (int)((kMaxGroups + G - 1) / G); ++i) {
+      const int q = (int)g + i * G;
+      kept[i] = q < p.groups && rank_of(q, lds.key[min(q, p.groups - 1)]) < p.top;
+    }
+    dev::wave_lds_fence();
+#pragma unroll
+    for (int i = 0; i < (int)((kMaxGroups + G - 1) / G); ++i)
+      if ((int)g + i * G < p.groups) lds.key[g + i * G] = kept[i];
+    dev::wave_lds_fence();
+#pragma unroll
+    for (int j = 0; j < PER; ++j)
+      if (!lds.key[p.by_size.div(min(first + j, p.count - 1))]) key[j] = 0;
   }
   dev::wave_lds_fence();
-#pragma unroll
-  for (int j = 0; j < PER; ++j) {
-    const uint32_t e = min(first + j, p.count - 1);
-    if (!kept[p.by_size.div(e)]) key[j] = 0;
+  return BIAS && near_tie(dev::key_score(lds.border[0]), dev::key_score(lds.border[1]), 2.f);
+}
+
+// The choice of one token in 64 bits by a whole wavefront; rolled loops, as it
+// is rare (a few tokens in a thousand of 256 experts).
+struct WideLds {
+  uint64_t group_key[kMaxGroups];
+  uint32_t kept[kMaxGroups];
+};
+template <typename T>
+__device__ __forceinline__ void choose64(const RoutePlan& p, const T* row, uint64_t* staged, WideLds& lds, int32_t* chosen) {
+  const uint32_t lane = threadIdx.x & 63u;
+  double top = 0.0, total = 1.0;
+  if (p.softmax) {
+    float m = -__builtin_inff();
+    for (uint32_t e = lane; e < p.count; e += 64) m = fmaxf(m, (float)row[e]);
+    top = (double)dev::group_max<64>(m);
+    total = 0.0;
+#pragma unroll 1
+    for (uint32_t e = lane; e < p.count; e += 64) total += exp((double)(float)row[e] - top);
+#pragma unroll 1
+    for (int o = 32; o > 0; o >>= 1) total += __shfl_xor(total, o, 64);
   }
-  if constexpr (sizeof(K) == 4 && BIAS) {
-    return near_tie(dev::key_score((uint32_t)border[0]), dev::key_score((uint32_t)border[1]), 2.f);
-  } else {
-    return false;
+#pragma unroll 1
+  for (uint32_t e = lane; e < p.count; e += 64) {
+    const double x = (double)(float)row[e], v = exp(p.softmax ? x - top : -x);
+    staged[e] = dev::score_key((p.softmax ? v / total : 1.0 / (1.0 + v)) + (double)p.bias[e * p.bias_step]);
+  }
+  dev::wave_lds_fence();
+  if (p.top < p.groups) {
+    for (int q = (int)lane; q < p.groups; q += 64) {
+      uint64_t best = 0, second = 0;
+#pragma unroll 1
+      for (int i = 0; i < p.size; ++i) join_best(best, second, staged[q * p.size + i], (uint64_t)0);
+      lds.group_key[q] = group_score<true>(best, second, p.size);
+    }
+    dev::wave_lds_fence();
+    for (int q = (int)lane; q < p.groups; q += 64) {
+      int rank = 0;
+#pragma unroll 1
+      for (int o = 0; o < p.groups; ++o)
+        rank += lds.group_key[o] > lds.group_key[q] || (lds.group_key[o] == lds.group_key[q] && o < q);
+      lds.kept[q] = rank < p.top;
+    }
+    dev::wave_lds_fence();
+    for (uint32_t e = lane; e < p.count; e += 64)
+      if (!lds.kept[p.by_size.div(e)]) staged[e] = 0;
+    dev::wave_lds_fence();
+  }
+#pragma unroll 1
+  for (int i = 0; i < p.k; ++i) {
+    uint64_t best = 0;
+    uint32_t at = 0xFFFFFFFFu;
+#pragma unroll 1
+    for (uint32_t e = lane; e < p.count; e += 64)
+      if (staged[e] > best) {
+        best = staged[e];
+        at = e;
+      }
+    const uint64_t most = dev::group_max_key<64>(best);
+    const uint32_t first = ~dev::group_max_key<64>(best == most ? ~at : 0u);  // the lowest of the equals
+    if (lane == 0) {
+      chosen[i] = (int32_t)first;
+      staged[first] = 0;
+    }
+    dev::wave_lds_fence();
   }
 }
 
@@ -152,10 +245,9 @@ __global__ __launch_bounds__(kThreads) void route_kernel(RoutePlan p) {
   constexpr int kTokens = kThreads / G;
   __shared__ int32_t chosen[kTokens][kMaxChosen + 1];
   __shared__ float choice[BIAS ? kTokens : 1][kMaxChosen + 1];
-  __shared__ uint64_t group_key[GROUPED ? kTokens : 1][kMaxGroups];
-  __shared__ uint64_t border[GROUPED ? kTokens : 1][2];
-  __shared__ uint8_t kept[GROUPED ? kTokens : 1][kMaxGroups];
-  extern __shared__ uint64_t staged_lds[];  // GROUPED: a key for each expert of each token
+  __shared__ GroupLds groups[GROUPED ? kTokens : 1];
+  __shared__ WideLds wide[BIAS ? kThreads / 64 : 1];
+  extern __shared__ uint64_t staged_lds[];  // keys: 64-bit ones of a wave's token, 32-bit ones of every token
 
   const uint32_t g = threadIdx.x % G, slot = threadIdx.x / G;
   const uint32_t token = blockIdx.x * kTokens + slot;
@@ -173,22 +265,24 @@ __global__ __launch_bounds__(kThreads) void route_kernel(RoutePlan p) {
   uint32_t key[PER];
   float total = 1.f;
   if constexpr (BIAS) {
+    float b[PER];
+    if (p.bias_step == 1 && first + PER <= p.count) {
+      dev::load_pack<float, PER>(p.bias + first, b);
+    } else {
+#pragma unroll
+      for (int j = 0; j < PER; ++j) b[j] = p.bias[min(first + j, p.count - 1) * p.bias_step];
+    }
     float s[PER];
     scores32<G, PER>(x, first, p.count, p.softmax, s, total);
 #pragma unroll
-    for (int j = 0; j < PER; ++j)
-      key[j] = first + j < p.count ? dev::score_key(s[j] + p.bias[(first + j) * p.bias_step]) : 0u;
+    for (int j = 0; j < PER; ++j) key[j] = first + j < p.count ? dev::score_key(s[j] + b[j]) : 0u;
   } else {
 #pragma unroll
     for (int j = 0; j < PER; ++j) key[j] = first + j < p.count ? dev::score_key(x[j]) : 0u;
   }
-  constexpr size_t kKey = BIAS ? 8 : 4;
-  char* staged = reinterpret_cast<char*>(staged_lds) + slot * (size_t)p.count * kKey;
   bool close = false;
   if constexpr (GROUPED)
-    close = keep_groups<G, PER, BIAS, uint32_t>(p, key, g, reinterpret_cast<uint32_t*>(staged),
-                                                reinterpret_cast<uint32_t*>(group_key[slot]), kept[slot],
-                                                reinterpret_cast<uint32_t*>(border[slot]));
+    close = keep_groups<G, PER, BIAS>(p, key, g, reinterpret_cast<uint32_t*>(staged_lds) + slot * p.count, groups[slot]);
   const int open = GROUPED ? p.top * p.size : (int)p.count;
   const int n = BIAS && p.k < open ? p.k + 1 : p.k;
   dev::take_best<G, PER>(key, n, g, [&](int i, uint32_t e, uint32_t k) {
@@ -202,18 +296,16 @@ __global__ __launch_bounds__(kThreads) void route_kernel(RoutePlan p) {
       const int32_t a = chosen[slot][i], b = chosen[slot][i + 1];
       close = close || (float)row[a] != (float)row[b] || p.bias[a * p.bias_step] != p.bias[b * p.bias_step];
     }
-    if (dev::group_ballot<G>(close)) {
-      double s[PER];
-      scores64<G, PER>(x, first, p.count, p.softmax, s);
-      uint64_t key64[PER];
-#pragma unroll
-      for (int j = 0; j < PER; ++j)
-        key64[j] = first + j < p.count ? dev::score_key(s[j] + (double)p.bias[(first + j) * p.bias_step]) : 0u;
-      if constexpr (GROUPED)
-        keep_groups<G, PER, BIAS, uint64_t>(p, key64, g, reinterpret_cast<uint64_t*>(staged), group_key[slot],
-                                            kept[slot], border[slot]);
-      dev::take_best<G, PER>(key64, p.k, g, [&](int i, uint32_t e, uint64_t) { chosen[slot][i] = (int32_t)e; });
-      dev::wave_lds_fence();
+    uint64_t again = __ballot(close && live);
+    if (again) {
+      const uint32_t wave = threadIdx.x >> 6;
+      while (again) {
+        const uint32_t in_wave = (uint32_t)__builtin_ctzll(again) / G;  // token of the wave
+        again &= ~((G == 64 ? ~0ull : (1ull << G) - 1) << (in_wave * G));
+        const uint32_t s = wave * (64 / G) + in_wave;
+        choose64(p, static_cast<const T*>(p.logits) + (int64_t)(blockIdx.x * kTokens + s) * p.row,
+                 staged_lds + wave * p.count, wide[wave], chosen[s]);
+      }
     }
   }
 
@@ -229,12 +321,14 @@ __global__ __launch_bounds__(kThreads) void route_kernel(RoutePlan p) {
     }
     top = dev::group_max<G>(top);
   }
-  float sum = 0.f;
+  const auto score = [&](float v) { return p.softmax ? expf(v - top) : 1.0f / (1.0f + expf(-v)); };
+  // (one weight a lane in most calls: kept for the second use)
+  float mine = 0.f, sum = 0.f;
+  if ((int)g < p.k) mine = score((float)row[chosen[slot][g]]);
   if (p.renormalize) {
-    for (int i = (int)g; i < p.k; i += G) {
-      const float v = (float)row[chosen[slot][i]];
-      sum += p.softmax ? expf(v - top) : 1.0f / (1.0f + expf(-v));
-    }
+    sum = mine;
+#pragma unroll 1
+    for (int i = (int)g + G; i < p.k; i += G) sum += score((float)row[chosen[slot][i]]);
     sum = dev::group_sum<G>(sum);
     if (BIAS && p.softmax && total != total) sum = total;  // a NaN anywhere is in every score of the row
   } else if (p.softmax) {
@@ -246,24 +340,27 @@ __global__ __launch_bounds__(kThreads) void route_kernel(RoutePlan p) {
     sum = 1.f;
   }
   if (!live) return;
+#pragma unroll 1
   for (int i = (int)g; i < p.k; i += G) {
     const int32_t e = chosen[slot][i];
-    const float v = (float)row[e];
-    const float s = p.softmax ? expf(v - top) : 1.0f / (1.0f + expf(-v));
-    p.weights[(int64_t)token * p.wt + i * p.wk] = s / sum * p.scale;
+    if (i != (int)g) mine = score((float)row[e]);
+    p.weights[(int64_t)token * p.wt + i * p.wk] = mine / sum * p.scale;
     p.experts[(int64_t)token * p.et + i * p.ek] = e;
   }
 }
 
 template <typename T, int G, int PER>
-thin_status launch_route(const RoutePlan& p, hipStream_t stream) {
+thin_status launch_route(RoutePlan p, hipStream_t stream) {
   const uint32_t tokens = kThreads / G;
   const dim3 grid((p.tokens + tokens - 1) / tokens), block(kThreads);
   const bool grouped = p.top < p.groups;
-  const uint32_t lds = grouped ? (uint32_t)(tokens * p.count * (p.bias ? 8 : 4)) : 0u;
+  const uint32_t lanes = (uint32_t)p.size / PER;
+  p.group_lanes = (uint32_t)p.size % PER == 0 && (lanes & (lanes - 1)) == 0 ? (int32_t)lanes : 0;
+  const uint32_t lds = std::max<uint32_t>(p.bias ? kThreads / 64 * p.count * 8 : 0u,
+                                          grouped && !p.group_lanes ? tokens * p.count * 4 : 0u);
   if (p.bias) {
     if (grouped) hipLaunchKernelGGL((route_kernel<T, G, PER, true, true>), grid, block, lds, stream, p);
-    else hipLaunchKernelGGL((route_kernel<T, G, PER, true, false>), grid, block, 0, stream, p);
+    else hipLaunchKernelGGL((route_kernel<T, G, PER, true, false>), grid, block, lds, stream, p);
   } else {
     if (grouped) hipLaunchKernelGGL((route_kernel<T, G, PER, false, true>), grid, block, lds, stream, p);
     else hipLaunchKernelGGL((route_kernel<T, G, PER, false, false>), grid, block, 0, stream, p);
@@ -301,8 +398,10 @@ __device__ __forceinline__ int32_t expert_of(const RowsPlan& p, uint32_t a) {
   return (uint32_t)e < (uint32_t)p.count ? e : -1;
 }
 
-// Vector v of token t's row, copied to the rows its slots name.
-template <typename Slot>
+// Vector v of token t's row, copied to the rows its slots name.  NT: streaming
+// stores, for rows that leave the caches anyway (604 MB: 104 us against 109
+// without and 117 with the loads streaming too).
+template <bool NT, typename Slot>
 __device__ __forceinline__ void copy_row(const RowsPlan& p, uint32_t t, uint32_t v, Slot slot) {
   const char* src = p.x + (int64_t)t * p.xs;
   if (p.bytes >= 16) {
@@ -310,7 +409,10 @@ __device__ __forceinline__ void copy_row(const RowsPlan& p, uint32_t t, uint32_t
     const u4u w = *reinterpret_cast<const u4u*>(src + at);
     for (int j = 0; j < p.k; ++j) {
       const int32_t s = slot(j);
-      if (s >= 0) *reinterpret_cast<u4u*>(p.rows + (int64_t)s * p.rs + at) = w;
+      if (s < 0) continue;
+      u4u* to = reinterpret_cast<u4u*>(p.rows + (int64_t)s * p.rs + at);
+      if constexpr (NT) __builtin_nontemporal_store(w, to);
+      else *to = w;
     }
   } else {
     for (int j = 0; j < p.k; ++j) {
@@ -378,108 +480,125 @@ __global__ __launch_bounds__(kThreads) void dispatch_small_kernel(RowsPlan p) {
   }
   __syncthreads();
   const uint32_t v = blockIdx.y * kThreads + threadIdx.x;
-  if (v * 16 < p.bytes) copy_row(p, t, v, [&](int j) { return part[0][j]; });
+  if (v * 16 < p.bytes) copy_row<false>(p, t, v, [&](int j) { return part[0][j]; });
 }
 
 // Many assignments, in three launches: counts of each block's assignments by
-// expert, slots from them, the copy.  A block's four waves take runs of
-// `chunk` assignments each, in order.
-__global__ __launch_bounds__(kThreads) void dispatch_count_kernel(RowsPlan p) {
-  __shared__ int32_t counts[kMaxExperts];
-  for (int e = threadIdx.x; e < p.count; e += kThreads) counts[e] = 0;
-  __syncthreads();
-  const uint32_t begin = blockIdx.x * p.chunk * (kThreads / 64);
-  const uint32_t end = min(begin + p.chunk * (kThreads / 64), p.assigned);
-  for (uint32_t a = begin + threadIdx.x; a < end; a += kThreads) {
-    const int32_t e = expert_of(p, a);
-    if (e >= 0) atomicAdd(&counts[e], 1);
+// expert, slots from them, the copy.  A block's 16 waves take runs of `chunk`
+// assignments each, in order.  Loads go eight or more at a time: one after
+// another they cost a memory latency each (counts of 64 blocks: 25 us, now 4).
+constexpr uint32_t kPlanThreads = 1024, kPlanWaves = kPlanThreads / 64;
+
+// f(assignment, expert) of the assignments in [begin, end) of a thread that
+// takes every step-th from begin + first on.
+template <typename F>
+__device__ __forceinline__ void each_assignment(const RowsPlan& p, uint32_t first, uint32_t end, uint32_t step, F f) {
+  constexpr int U = 4;
+#pragma unroll 1
+  for (uint32_t a = first; a < end; a += U * step) {
+    int32_t e[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) e[u] = expert_of(p, min(a + u * step, p.assigned - 1));
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (a + u * step < end) f(a + u * step, e[u]);
   }
-  __syncthreads();
-  for (int e = threadIdx.x; e < p.count; e += kThreads) p.counts[(int64_t)blockIdx.x * p.count + e] = counts[e];
 }
 
-__global__ __launch_bounds__(kThreads) void dispatch_slots_kernel(RowsPlan p) {
-  constexpr uint32_t kWaves = kThreads / 64;
-  __shared__ int32_t next[kWaves][kMaxExperts];  // next slot of each expert in each wave's run
-  __shared__ int32_t sums[kThreads];
+__global__ __launch_bounds__(kPlanThreads) void dispatch_count_kernel(RowsPlan p) {
+  __shared__ int32_t counts[kMaxExperts];
+  for (int e = threadIdx.x; e < p.count; e += kPlanThreads) counts[e] = 0;
+  __syncthreads();
+  const uint32_t begin = blockIdx.x * p.chunk * kPlanWaves, end = min(begin + p.chunk * kPlanWaves, p.assigned);
+  each_assignment(p, begin + threadIdx.x, end, kPlanThreads, [&](uint32_t, int32_t e) {
+    if (e >= 0) atomicAdd(&counts[e], 1);
+  });
+  __syncthreads();
+  for (int e = threadIdx.x; e < p.count; e += kPlanThreads) p.counts[(int64_t)blockIdx.x * p.count + e] = counts[e];
+}
+
+__global__ __launch_bounds__(kPlanThreads) void dispatch_slots_kernel(RowsPlan p) {
+  static_assert(kMaxExperts <= kPlanThreads, "a thread an expert");
+  extern __shared__ int32_t next[];  // [waves][count]: next slot of each expert in each wave's run
+  __shared__ int32_t sums[kPlanWaves];
   const uint32_t wave = threadIdx.x >> 6, lane = threadIdx.x & 63u;
-  // each thread owns a run of experts: total of all blocks and of those before this one
-  const int per = (p.count + (int)kThreads - 1) / (int)kThreads;
-  const int e0 = (int)threadIdx.x * per;
-  int32_t total[kMaxExperts / kThreads], before[kMaxExperts / kThreads];
-  int32_t own = 0;
+  const uint32_t begin = (blockIdx.x * kPlanWaves + wave) * p.chunk, end = min(begin + p.chunk, p.assigned);
+  // counts of each wave's run, for the waves behind it
+  for (int i = threadIdx.x; i < (int)kPlanWaves * p.count; i += kPlanThreads) next[i] = 0;
+  __syncthreads();
+  if (wave + 1 < kPlanWaves)
+    each_assignment(p, begin + lane, end, 64, [&](uint32_t, int32_t e) {
+      if (e >= 0) atomicAdd(&next[(wave + 1) * p.count + e], 1);
+    });
+  // a thread an expert: its assignments in all blocks, and in those before this one
+  const int mine = (int)threadIdx.x;
+  int32_t total = 0, before = 0;
+  if (mine < p.count) {
+    constexpr uint32_t U = 16;
+    for (uint32_t b0 = 0; b0 < gridDim.x; b0 += U) {
+      int32_t c[U];
 #pragma unroll
-  for (int i = 0; i < (int)(kMaxExperts / kThreads); ++i) {
-    total[i] = before[i] = 0;
-    if (i < per && e0 + i < p.count) {
-      for (uint32_t b = 0; b < gridDim.x; ++b) {
-        const int32_t c = p.counts[(int64_t)b * p.count + e0 + i];
-        total[i] += c;
-        if (b < blockIdx.x) before[i] += c;
+      for (uint32_t u = 0; u < U; ++u) c[u] = p.counts[(int64_t)min(b0 + u, gridDim.x - 1) * p.count + mine];
+#pragma unroll
+      for (uint32_t u = 0; u < U; ++u) {
+        if (b0 + u < gridDim.x) total += c[u];
+        if (b0 + u < blockIdx.x) before += c[u];
       }
-      own += total[i];
     }
   }
-  sums[threadIdx.x] = own;
-  __syncthreads();
-  for (uint32_t o = 1; o < kThreads; o <<= 1) {
-    const int32_t add = threadIdx.x >= o ? sums[threadIdx.x - o] : 0;
-    __syncthreads();
-    sums[threadIdx.x] += add;
-    __syncthreads();
-  }
-  int32_t start = sums[threadIdx.x] - own;
+  int32_t upto = total;  // sum of the experts' totals up to this one
 #pragma unroll
-  for (int i = 0; i < (int)(kMaxExperts / kThreads); ++i) {
-    if (i < per && e0 + i < p.count) {
-      if (blockIdx.x == 0) p.offsets[(int64_t)(e0 + i) * p.os] = start;
-      next[0][e0 + i] = start + before[i];
-      for (uint32_t w = 1; w < kWaves; ++w) next[w][e0 + i] = 0;
-      start += total[i];
+  for (int o = 1; o < 64; o <<= 1) {
+    const int32_t add = __shfl_up(upto, o, 64);
+    if ((int)lane >= o) upto += add;
+  }
+  if (lane == 63) sums[wave] = upto;
+  __syncthreads();
+  for (uint32_t w = 0; w < wave; ++w) upto += sums[w];
+  if (mine < p.count) {
+    if (blockIdx.x == 0) {
+      p.offsets[(int64_t)mine * p.os] = upto - total;
+      if (mine == p.count - 1) p.offsets[(int64_t)p.count * p.os] = upto;
+    }
+    int32_t at = upto - total + before;
+    for (uint32_t w = 0; w < kPlanWaves; ++w) {
+      const int32_t in_wave = next[w * p.count + mine];  // of the wave before
+      at += in_wave;
+      next[w * p.count + mine] = at;
     }
   }
-  if (blockIdx.x == 0 && threadIdx.x == kThreads - 1) p.offsets[(int64_t)p.count * p.os] = sums[kThreads - 1];
-  __syncthreads();
-  const uint32_t begin = (blockIdx.x * kWaves + wave) * p.chunk;
-  const uint32_t end = min(begin + p.chunk, p.assigned);
-  if (wave + 1 < kWaves)
-    for (uint32_t a = begin + lane; a < end; a += 64) {
-      const int32_t e = expert_of(p, a);
-      if (e >= 0) atomicAdd(&next[wave + 1][e], 1);
-    }
-  __syncthreads();
-  for (int e = threadIdx.x; e < p.count; e += kThreads)
-    for (uint32_t w = 1; w < kWaves; ++w) next[w][e] += next[w - 1][e];
   __syncthreads();
   // 64 assignments at a time: the lanes of one expert take consecutive slots
+  int32_t ahead = begin + lane < end ? expert_of(p, begin + lane) : -1;
   for (uint32_t a0 = begin; a0 < end; a0 += 64) {
     const uint32_t a = a0 + lane;
-    const int32_t e = a < end ? expert_of(p, a) : -1;
+    const int32_t e = ahead;
+    ahead = a + 64 < end ? expert_of(p, a + 64) : -1;
     uint64_t same = __ballot(e >= 0);
     for (int bit = 0; (1 << bit) < p.count; ++bit) {
       const uint64_t set = __ballot((e >> bit) & 1);
       same &= (e >> bit) & 1 ? set : ~set;
     }
+    int32_t slot = -1;
     if (e >= 0) {
       const int leader = __builtin_ctzll(same);
       int32_t base = 0;
-      if ((int)lane == leader) base = atomicAdd(&next[wave][e], __builtin_popcountll(same));
-      base = __shfl(base, leader, 64);
+      if ((int)lane == leader) base = atomicAdd(&next[wave * p.count + e], __builtin_popcountll(same));
+      slot = __shfl(base, leader, 64) + __builtin_popcountll(same & ((1ull << lane) - 1));
+    }
+    if (a < end) {
       const uint32_t t = p.by_k.div(a);
-      p.slots[(int64_t)t * p.st + (int64_t)(a - t * p.k) * p.sk] =
-          base + __builtin_popcountll(same & ((1ull << lane) - 1));
-    } else if (a < end) {
-      const uint32_t t = p.by_k.div(a);
-      p.slots[(int64_t)t * p.st + (int64_t)(a - t * p.k) * p.sk] = -1;
+      p.slots[(int64_t)t * p.st + (int64_t)(a - t * p.k) * p.sk] = slot;
     }
   }
 }
 
+template <bool NT>
 __global__ __launch_bounds__(kThreads) void dispatch_copy_kernel(RowsPlan p) {
   const uint32_t t = blockIdx.x * (kThreads / p.lanes) + threadIdx.x / p.lanes;
   const uint32_t v = blockIdx.y * p.lanes + threadIdx.x % p.lanes;
   if (t >= p.tokens || v * 16 >= p.bytes) return;
-  copy_row(p, t, v, [&](int j) { return p.slots[(int64_t)t * p.st + j * p.sk]; });
+  copy_row<NT>(p, t, v, [&](int j) { return p.slots[(int64_t)t * p.st + j * p.sk]; });
 }
 
 // ---------------------------------------------------------------- sums
@@ -495,38 +614,57 @@ struct CombinePlan {
 };
 
 // out[t] = sum_j weights[t, j] * y[slots[t, j]], in the order of j, in fp32
-// with one rounding; slots outside y contribute nothing.
+// with one rounding; slots outside y contribute nothing.  Eight rows are loaded
+// at a time (one after another 125 us for 604 MB, now 117 us, 5.2 TB/s;
+// streaming loads changed nothing).
+template <typename T, int N>
+__device__ __forceinline__ void add_rows(const CombinePlan& p, uint32_t t, uint32_t at, float (&sum)[N]) {
+  constexpr int U = 8;
+  typedef typename dev::Pack<T, N>::type P;
+  const T* y = static_cast<const T*>(p.y) + at;
+  const float* w = p.weights + (int64_t)t * p.wt;
+  const int32_t* slot = p.slots + (int64_t)t * p.st;
+#pragma unroll 1
+  for (int j = 0; j < p.k; j += U) {
+    uint32_t s[U];
+    float f[U];
+    P r[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int i = min(j + u, p.k - 1);
+      s[u] = (uint32_t)slot[i * p.sk];
+      f[u] = w[i * p.wk];
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const P* from = reinterpret_cast<const P*>(y + (int64_t)min(s[u], p.rows - 1) * p.ys);
+      r[u] = *from;
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (s[u] >= p.rows || j + u >= p.k) continue;
+#pragma unroll
+      for (int i = 0; i < N; ++i) sum[i] = __builtin_fmaf(f[u], (float)r[u][i], sum[i]);
+    }
+  }
+}
 template <typename T>
 __global__ __launch_bounds__(kThreads) void combine_kernel(CombinePlan p) {
   constexpr uint32_t V = 16 / sizeof(T);
-  const uint32_t t = blockIdx.x * (kThreads / p.lanes) + threadIdx.x / p.lanes;
+  const uint32_t t = p.lanes == kThreads ? blockIdx.x : blockIdx.x * (kThreads / p.lanes) + threadIdx.x / p.lanes;
   const uint32_t v = blockIdx.y * p.lanes + threadIdx.x % p.lanes;
   if (t >= p.tokens || v * V >= p.width) return;
-  const T* y = static_cast<const T*>(p.y);
   T* out = static_cast<T*>(p.out) + (int64_t)t * p.os;
-  const float* w = p.weights + (int64_t)t * p.wt;
-  const int32_t* slot = p.slots + (int64_t)t * p.st;
   if (p.width >= V) {
     const uint32_t at = min(v * V, p.width - V);
     float sum[V] = {};
-    for (int j = 0; j < p.k; ++j) {
-      const uint32_t s = (uint32_t)slot[j * p.sk];
-      if (s >= p.rows) continue;
-      float r[V];
-      dev::load_pack<T, V>(y + (int64_t)s * p.ys + at, r);
-      const float f = w[j * p.wk];
-#pragma unroll
-      for (uint32_t i = 0; i < V; ++i) sum[i] = __builtin_fmaf(f, r[i], sum[i]);
-    }
+    if (p.rows) add_rows<T, V>(p, t, at, sum);
     dev::store_pack<T, V>(out + at, sum);
   } else {
     for (uint32_t i = 0; i < p.width; ++i) {
-      float sum = 0.f;
-      for (int j = 0; j < p.k; ++j) {
-        const uint32_t s = (uint32_t)slot[j * p.sk];
-        if (s < p.rows) sum = __builtin_fmaf(w[j * p.wk], (float)y[(int64_t)s * p.ys + i], sum);
-      }
-      out[i] = (T)sum;
+      float sum[1] = {};
+      if (p.rows) add_rows<T, 1>(p, t, i, sum);
+      out[i] = (T)sum[0];
     }
   }
 }
@@ -538,12 +676,12 @@ uint32_t row_lanes(uint64_t vectors) {
   return lanes;
 }
 
-// Blocks of the counting kernels and assignments a wave of them takes: at
-// least 512 a wave, at most 256 blocks (each block reads the counts of all).
-uint32_t count_blocks(int64_t assigned, uint32_t* chunk) {
-  const int64_t wave = std::max<int64_t>(512, (assigned + 1023) / 1024);
+// Blocks of the planning kernels and assignments a wave of them takes: at least
+// 256 a wave, at most 256 blocks (each block reads the counts of all).
+uint32_t plan_blocks(int64_t assigned, uint32_t* chunk) {
+  const int64_t wave = std::max<int64_t>(256, (assigned + 256 * kPlanWaves - 1) / (256 * kPlanWaves));
   *chunk = (uint32_t)((wave + 63) / 64 * 64);
-  return (uint32_t)((assigned + (int64_t)*chunk * 4 - 1) / ((int64_t)*chunk * 4));
+  return (uint32_t)((assigned + (int64_t)*chunk * kPlanWaves - 1) / ((int64_t)*chunk * kPlanWaves));
 }
 
 }  // namespace
@@ -602,6 +740,12 @@ extern "C" thin_status thin_expert_route(const thin_desc* logits, const thin_des
   p.scale = scale;
   return with_float_type(logits->dtype, [&](auto zero) {
     using T_ = decltype(zero);
+    if (T <= kFewTokens) {
+      if (E <= 64) return launch_route<T_, 64, 1>(p, stream);
+      if (E <= 128) return launch_route<T_, 64, 2>(p, stream);
+      if (E <= 256) return launch_route<T_, 64, 4>(p, stream);
+      if (E <= 512) return launch_route<T_, 64, 8>(p, stream);
+    }
     if (E <= 16) return launch_route<T_, 4, 4>(p, stream);
     if (E <= 32) return launch_route<T_, 8, 4>(p, stream);
     if (E <= 64) return launch_route<T_, 16, 4>(p, stream);
@@ -616,7 +760,7 @@ extern "C" size_t thin_expert_dispatch_workspace(int64_t tokens, int64_t top_k, 
   if (tokens <= 0 || top_k <= 0 || num_experts <= 0 || tokens > (1ll << 31) / top_k) return 0;
   if (tokens * top_k <= kCountedAssignments) return 0;
   uint32_t chunk;
-  return (size_t)count_blocks(tokens * top_k, &chunk) * (size_t)num_experts * sizeof(int32_t);
+  return (size_t)plan_blocks(tokens * top_k, &chunk) * (size_t)num_experts * sizeof(int32_t);
 }
 
 extern "C" thin_status thin_expert_dispatch(const thin_desc* x, const thin_desc* experts, int64_t num_experts,
@@ -678,18 +822,22 @@ extern "C" thin_status thin_expert_dispatch(const thin_desc* x, const thin_desc*
     THIN_LAUNCH_CHECK("expert_dispatch");
     return THIN_OK;
   }
-  const uint32_t blocks = count_blocks(p.assigned, &p.chunk);
-  hipLaunchKernelGGL(dispatch_count_kernel, dim3(blocks), dim3(kThreads), 0, stream, p);
+  const uint32_t blocks = plan_blocks(p.assigned, &p.chunk);
+  hipLaunchKernelGGL(dispatch_count_kernel, dim3(blocks), dim3(kPlanThreads), 0, stream, p);
   THIN_LAUNCH_CHECK("expert_dispatch_count");
-  hipLaunchKernelGGL(dispatch_slots_kernel, dim3(blocks), dim3(kThreads), 0, stream, p);
+  hipLaunchKernelGGL(dispatch_slots_kernel, dim3(blocks), dim3(kPlanThreads),
+                     kPlanWaves * (uint32_t)p.count * sizeof(int32_t), stream, p);
   THIN_LAUNCH_CHECK("expert_dispatch_slots");
   if (H == 0) return THIN_OK;
   p.lanes = row_lanes(vectors);
   const uint32_t per = kThreads / p.lanes;
   const uint64_t columns = (vectors + p.lanes - 1) / p.lanes;
   THIN_REQUIRE(columns < 65536, THIN_ERR_UNSUPPORTED, "expert_dispatch: rows too long");
-  hipLaunchKernelGGL(dispatch_copy_kernel, dim3((p.tokens + per - 1) / per, (uint32_t)columns), dim3(kThreads), 0,
-                     stream, p);
+  const dim3 grid((p.tokens + per - 1) / per, (uint32_t)columns);
+  if ((int64_t)p.assigned * p.bytes >= kStreamingBytes)
+    hipLaunchKernelGGL((dispatch_copy_kernel<true>), grid, dim3(kThreads), 0, stream, p);
+  else
+    hipLaunchKernelGGL((dispatch_copy_kernel<false>), grid, dim3(kThreads), 0, stream, p);
   THIN_LAUNCH_CHECK("expert_dispatch_copy");
   return THIN_OK;
 }

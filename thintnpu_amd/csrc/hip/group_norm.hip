@@ -3,22 +3,22 @@
 //   mean, var over the rows and channels of a group, y = (x - mean) /
 //   sqrt(var + eps) * weight + bias, then y * sigmoid(y).
 //
-// Statistics are fp32: a thread sums x - K and its square, K being the first
-// element that it reads of the group, so that a mean far from zero cancels
-// before the squares are formed; partial (count, mean, sum of squared
-// deviations) are joined by Chan, Golub and LeVeque's pairwise rule.
+// Statistics are fp32.
 #include "rows.h"
 
 #include <string.h>
 
 #include <algorithm>
 #include <numeric>
+#include <type_traits>
 
 namespace thin {
 namespace {
 
 constexpr uint32_t kThreads = 256;
-constexpr uint32_t kMaxSlots = 1536;  // group segments of a tile that LDS holds
+constexpr int64_t kFillingTiles = 128;  // workgroups below which one launch needs few vectors in each
+constexpr int64_t kFewVectors = 2048;
+constexpr int64_t kHeldVectors = 16384;  // 16-byte vectors that 1024 threads hold, 16 each
 constexpr int64_t kBlocks = 1024;     // workgroups that fill the device
 
 struct NormPlan {
@@ -38,27 +38,11 @@ struct NormPlan {
   uint32_t vectors, lanes, lines;    // vectors of a tile; threads across (lanes) and down (lines)
   uint32_t slots_per_group;
   uint32_t chunks, chunk_rows;
-  FastDiv by_inner, by_lanes, by_chunks, by_tiles, by_group;
+  uint32_t spans;                    // whole runs of 8 samples
+  FastDiv by_inner, by_lanes, by_chunks, by_tiles, by_group, by_slots, by_span;
   int32_t blocked, silu, weight32, bias32;
   float eps;
 };
-
-struct Moments {
-  float n, mean, m2;
-};
-__device__ __forceinline__ Moments join(const Moments& a, const Moments& b) {
-  if (b.n == 0.f) return a;
-  if (a.n == 0.f) return b;
-  const float n = a.n + b.n, d = b.mean - a.mean, part = b.n / n;
-  return {n, __builtin_fmaf(d, part, a.mean), a.m2 + b.m2 + d * d * a.n * part};
-}
-template <int G>
-__device__ __forceinline__ Moments join_lanes(Moments m) {
-#pragma unroll
-  for (int o = 1; o < G; o <<= 1)
-    m = join(m, Moments{__shfl_xor(m.n, o, 64), __shfl_xor(m.mean, o, 64), __shfl_xor(m.m2, o, 64)});
-  return m;
-}
 
 // Address of row r, channel c (a vector does not cross a block of 16).
 __device__ __forceinline__ int64_t offset_of(const NormPlan& p, int64_t b, int64_t h, int64_t w, uint32_t r,
@@ -68,16 +52,17 @@ __device__ __forceinline__ int64_t offset_of(const NormPlan& p, int64_t b, int64
   return p.blocked ? at + (int64_t)(c >> 4) * b + (c & 15u) : at + c;
 }
 
-// V channels from c on; those past the last are zero.  Blocked memory holds
-// whole blocks, so only channels-last rows end inside a vector.
-template <typename T, int V>
-__device__ __forceinline__ void load_channels(const NormPlan& p, const T* x, uint32_t c, float (&v)[V]) {
-  if (p.blocked || c + V <= p.channels) {
-    dev::load_pack<T, V>(x, v);
-  } else {
+// A vector at c of a row; past the channels of a channels-last row are zeros
+// (EDGE: the vector ends behind them.  Kept out of the other rows' loop, where
+// the choice made every load wait).
+template <typename T, bool EDGE>
+__device__ __forceinline__ typename dev::Pack<T, 16 / sizeof(T)>::type load_vector(const NormPlan& p, const T* x, uint32_t c) {
+  typedef typename dev::Pack<T, 16 / sizeof(T)>::type P;
+  if constexpr (!EDGE) return *reinterpret_cast<const P*>(x);
+  P v;
 #pragma unroll
-    for (int j = 0; j < V; ++j) v[j] = c + j < p.channels ? (float)x[j] : 0.f;
-  }
+  for (int j = 0; j < (int)(16 / sizeof(T)); ++j) v[j] = c + j < p.channels ? x[j] : (T)0.f;
+  return v;
 }
 
 // Where a workgroup works: its groups hold channels [c0, c1), which it walks in
@@ -87,10 +72,10 @@ struct Place {
   uint32_t first, count;  // groups
   uint32_t from, c0, c1;
 };
-__device__ __forceinline__ Place place_of(const NormPlan& p) {
+__device__ __forceinline__ Place place_of(const NormPlan& p, uint32_t block) {
   Place at;
-  const uint32_t q = p.by_chunks.div(blockIdx.x);
-  at.chunk = blockIdx.x - q * p.chunks;
+  const uint32_t q = p.by_chunks.div(block);
+  at.chunk = block - q * p.chunks;
   at.sample = p.by_tiles.div(q);
   at.tile = q - at.sample * p.tiles;
   at.first = at.tile * p.tile_groups;
@@ -101,217 +86,431 @@ __device__ __forceinline__ Place place_of(const NormPlan& p) {
   return at;
 }
 
-// Moments of the tile's groups over rows [begin, end), into group[].
-template <typename T, int SEG>
-__device__ void tile_moments(const NormPlan& p, const Place& at, uint32_t begin, uint32_t end, Moments* lines,
-                             Moments* slots, Moments* group) {
-  constexpr int V = 16 / sizeof(T), W = V / SEG;  // channels of a vector, of a segment
-  constexpr int U = 4;                            // rows in flight
-  const uint32_t ty = p.by_lanes.div(threadIdx.x), tx = threadIdx.x - ty * p.lanes;
-  const T* x = static_cast<const T*>(p.x) + (int64_t)at.sample * p.xn;
-  for (uint32_t v0 = 0; v0 < p.vectors; v0 += p.lanes) {
-    const uint32_t vec = v0 + tx, c = at.from + vec * V;
-    const bool live = ty < p.lines && vec < p.vectors && c < at.c1;
-    Moments m[SEG];
-#pragma unroll
-    for (int s = 0; s < SEG; ++s) m[s] = {0.f, 0.f, 0.f};
-    if (live && begin + ty < end) {
-      float k[SEG], s1[SEG] = {}, s2[SEG] = {};
-      uint32_t n = 0;
-      for (uint32_t r = begin + ty; r < end; r += U * p.lines) {
-        float v[U][V];
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-          const uint32_t row = min(r + u * p.lines, end - 1);
-          load_channels<T, V>(p, x + offset_of(p, p.xb, p.xh, p.xw, row, c), c, v[u]);
-        }
-        if (n == 0) {
-#pragma unroll
-          for (int s = 0; s < SEG; ++s) k[s] = v[0][s * W];
-        }
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-          if (r + u * p.lines >= end) continue;
-          ++n;
-#pragma unroll
-          for (int j = 0; j < V; ++j) {
-            const float d = c + j >= at.c0 && c + j < at.c1 ? v[u][j] - k[j / W] : 0.f;
-            s1[j / W] += d;
-            s2[j / W] = __builtin_fmaf(d, d, s2[j / W]);
-          }
-        }
-      }
-#pragma unroll
-      for (int s = 0; s < SEG; ++s) {
-        const uint32_t lo = max(c + s * W, at.c0), hi = min(c + s * W + W, at.c1);
-        if (lo >= hi) continue;
-        const float count = (float)(n * (hi - lo)), mean = s1[s] / count;
-        const float m2 = s2[s] - s1[s] * mean;
-        m[s] = {count, k[s] + mean, m2 < 0.f ? 0.f : m2};
-      }
-    }
-    // down the lines of the workgroup, a tree
-    for (uint32_t left = p.lines; left > 1;) {
-      const uint32_t half = (left + 1) / 2;
-      if (live && ty >= half && ty < left) {
-#pragma unroll
-        for (int s = 0; s < SEG; ++s) lines[((ty - half) * p.lanes + tx) * SEG + s] = m[s];
-      }
-      __syncthreads();
-      if (live && ty + half < left) {
-#pragma unroll
-        for (int s = 0; s < SEG; ++s) m[s] = join(m[s], lines[(ty * p.lanes + tx) * SEG + s]);
-      }
-      __syncthreads();
-      left = half;
-    }
-    if (ty == 0 && vec < p.vectors) {
-#pragma unroll
-      for (int s = 0; s < SEG; ++s) slots[vec * SEG + s] = m[s];
-    }
-  }
-  __syncthreads();
-  // across the segments of a group: 8 lanes each
-  for (uint32_t g0 = 0; g0 < at.count; g0 += kThreads / 8) {
-    const uint32_t g = g0 + threadIdx.x / 8;
-    Moments m = {0.f, 0.f, 0.f};
-    if (g < at.count)
-      for (uint32_t s = threadIdx.x % 8; s < p.slots_per_group; s += 8) m = join(m, slots[g * p.slots_per_group + s]);
-    m = join_lanes<8>(m);
-    if (g < at.count && threadIdx.x % 8 == 0) group[g] = m;
-  }
-  __syncthreads();
-}
-
 template <typename T>
 __device__ __forceinline__ float param(const void* w, int32_t is32, int64_t at) {
   return is32 ? static_cast<const float*>(w)[at] : (float)static_cast<const T*>(w)[at];
 }
+template <typename T, bool SILU>
+__device__ __forceinline__ float activate(float y) {
+  if constexpr (!SILU) return y;
+  else return sizeof(T) == 2 ? y * dev::sigmoid_fast(y) : y / (1.0f + expf(-y));
+}
 
-// y of rows [begin, end) from the group's moments (m2 already 1 / sqrt).
+// (x - mean) * scale + shift as x * scale + (shift - mean * scale) where that
+// loses nothing next to a 16-bit result: the products are below 32, so that
+// their rounding stays under 2^-18.
 template <typename T>
-__device__ void apply_rows(const NormPlan& p, const Place& at, uint32_t begin, uint32_t end, const Moments* group) {
-  constexpr int V = 16 / sizeof(T), U = 4;
-  const uint32_t ty = p.by_lanes.div(threadIdx.x), tx = threadIdx.x - ty * p.lanes;
-  if (ty >= p.lines) return;
+__device__ __forceinline__ bool folds(float mean, float scale) {
+  return sizeof(T) == 2 && fabsf(mean * scale) < 32.f;
+}
+
+// One launch, where tiles and channels end at whole vectors: a workgroup holds
+// all rows of its groups in registers, H vectors a thread, so that x is read once.
+__device__ __forceinline__ void add_lines(float& v, uint32_t lanes) {  // over the lines of a wavefront
+  if (lanes <= 32) v += dev::lane_xor<32>(v);
+  if (lanes <= 16) v += dev::lane_xor<16>(v);
+  if (lanes <= 8) v += dev::lane_xor<8>(v);
+  if (lanes <= 4) v += dev::lane_xor<4>(v);
+  if (lanes <= 2) v += dev::lane_xor<2>(v);
+  if (lanes <= 1) v += dev::lane_xor<1>(v);
+}
+// Sums of a value a segment over the workgroup's lines and each group's
+// segments, into group[].  part: [waves][lanes * SEG].
+template <int SEG, int THREADS>
+__device__ __forceinline__ void add_up(const NormPlan& p, const Place& at, float (&v)[SEG], float* part, float* group) {
+  constexpr uint32_t W = THREADS / 64;
+  const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, width = p.lanes * SEG;
+#pragma unroll
+  for (int s = 0; s < SEG; ++s) {
+    add_lines(v[s], p.lanes);
+    if (lane < p.lanes) part[wave * width + lane * SEG + s] = v[s];
+  }
+  __syncthreads();
+  const uint32_t entries = W * p.slots_per_group;
+  for (uint32_t g0 = 0; g0 < at.count; g0 += THREADS / 16) {
+    const uint32_t g = g0 + threadIdx.x / 16;
+    float sum = 0.f;
+    if (g < at.count)
+      for (uint32_t k = threadIdx.x % 16; k < entries; k += 16) {
+        const uint32_t w = p.by_slots.div(k);
+        sum += part[w * width + g * p.slots_per_group + (k - w * p.slots_per_group)];
+      }
+    sum = dev::group_sum<16>(sum);
+    if (g < at.count && threadIdx.x % 16 == 0) group[g] = sum;
+  }
+  __syncthreads();
+}
+
+// A thread's sums of x - k and its square over n elements of each segment, k
+// being the first element that it reads, so that a mean far from zero cancels
+// before the squares are formed.
+template <int SEG>
+struct Sums {
+  float k[SEG], s1[SEG], s2[SEG], n[SEG];
+};
+// Sums of the workgroup's `count` elements of each group: off[g] = sum of x -
+// reference (the group's first element in the workgroup's first row), and
+// dev2[g] = sum of squared deviations from the mean that gives.  Each thread's
+// mean goes against the reference, then its squares with their distance from
+// the mean of all.  Sums alone: joined pair by pair with a division each, this
+// took longer than reading the rows (15.6 us for 33 MB).
+// lds: part of add_up(), then off, dev2 and the references, one a group each.
+struct Reference {
+  float first, second;  // of groups threadIdx.x and threadIdx.x + THREADS (a tile has at most 512)
+};
+template <typename T, int THREADS>
+__device__ __forceinline__ Reference reference_of(const NormPlan& p, const Place& at, const T* x, uint32_t r) {
+  const auto element = [&](uint32_t g) {
+    return g < at.count ? (float)x[offset_of(p, p.xb, p.xh, p.xw, r, at.c0 + g * p.per_group)] : 0.f;
+  };
+  return {element(threadIdx.x), element(threadIdx.x + THREADS)};
+}
+struct Joined {
+  const float* off;
+  const float* dev2;
+  const float* reference;
+};
+template <int SEG, int W, int THREADS>
+__device__ __forceinline__ Joined join_threads(const NormPlan& p, const Place& at, const uint32_t (&of)[SEG],
+                                               const Reference& reference, float inverse, const Sums<SEG>& t,
+                                               float* lds) {
+  float* off = lds + THREADS / 64 * p.lanes * SEG;
+  float* dev2 = off + p.tile_groups;
+  float* against = dev2 + p.tile_groups;
+  if (threadIdx.x < at.count) against[threadIdx.x] = reference.first;
+  if (threadIdx.x + THREADS < at.count) against[threadIdx.x + THREADS] = reference.second;
+  __syncthreads();
+  float mean[SEG], m2[SEG], sum[SEG];
+#pragma unroll
+  for (int s = 0; s < SEG; ++s) {
+    const float d = t.n[s] != 0.f ? t.s1[s] * (1.0f / t.n[s]) : 0.f, m = t.s2[s] - t.s1[s] * d;
+    mean[s] = t.k[s] - against[of[s]] + d;
+    m2[s] = m < 0.f ? 0.f : m;
+    sum[s] = t.n[s] != 0.f ? mean[s] * t.n[s] : 0.f;
+  }
+  add_up<SEG, THREADS>(p, at, sum, lds, off);
+#pragma unroll
+  for (int s = 0; s < SEG; ++s) {
+    const float d = mean[s] - off[of[s]] * inverse;
+    sum[s] = t.n[s] != 0.f ? __builtin_fmaf(d * d, t.n[s], m2[s]) : 0.f;
+  }
+  add_up<SEG, THREADS>(p, at, sum, lds, dev2);
+  return {off, dev2, against};
+}
+template <typename T, int SEG, int THREADS, int H>
+__global__ __launch_bounds__(THREADS) void norm_held_kernel(NormPlan p) {
+  constexpr int V = 16 / sizeof(T), W = V / SEG;
+  typedef typename dev::Pack<T, V>::type P;
+  typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+  extern __shared__ float lds[];
+  // the tiles of a sample on one XCD, whose L2 then holds the lines they share
+  uint32_t block = blockIdx.x;
+  const uint32_t span = 8 * p.tiles, q = p.by_span.div(block);
+  if (q < p.spans) {
+    const uint32_t r = block - q * span;
+    block = q * span + (r & 7u) * p.tiles + (r >> 3);
+  }
+  const Place at = place_of(p, block);
+  const uint32_t tx = threadIdx.x & (p.lanes - 1), ty = p.by_lanes.div(threadIdx.x);
+  const uint32_t c = min(at.c0 + tx * V, at.c1 - V);
+  const bool live = tx < p.vectors;
   const T* x = static_cast<const T*>(p.x) + (int64_t)at.sample * p.xn;
   T* out = static_cast<T*>(p.out) + (int64_t)at.sample * p.on;
-  // the last tile of a blocked tensor also writes the padding channels (zeros)
-  const uint32_t last = at.c1 == p.channels ? p.padded : at.c1;
-  for (uint32_t c = at.from + tx * V; c < last; c += p.lanes * V) {
-    float mean[V], scale[V], shift[V];
+  // what the ends need first, so that the rows can be added as they arrive
+  float scale[V], shift[V];
+  const Reference reference = reference_of<T, THREADS>(p, at, x, 0);
+  uint32_t of[SEG];  // group of a segment
 #pragma unroll
-    for (int j = 0; j < V; ++j) {
-      const uint32_t ch = min(max(c + j, at.c0), at.c1 - 1);
-      const Moments g = group[p.by_group.div(ch) - at.first];
-      mean[j] = g.mean;
-      scale[j] = p.weight ? g.m2 * param<T>(p.weight, p.weight32, ch * p.ws) : g.m2;
-      shift[j] = p.bias ? param<T>(p.bias, p.bias32, ch * p.bs) : 0.f;
-    }
-    for (uint32_t r = begin + ty; r < end; r += U * p.lines) {
-      float v[U][V];
+  for (int j = 0; j < V; ++j) {
+    scale[j] = p.weight ? param<T>(p.weight, p.weight32, (c + j) * p.ws) : 1.f;
+    shift[j] = p.bias ? param<T>(p.bias, p.bias32, (c + j) * p.bs) : 0.f;
+  }
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const uint32_t row = min(r + u * p.lines, end - 1);
-        load_channels<T, V>(p, x + offset_of(p, p.xb, p.xh, p.xw, row, c), c, v[u]);
-      }
+  for (int s = 0; s < SEG; ++s) of[s] = p.by_group.div(c + s * W) - at.first;
+  // as integers, so that no pass keeps the fp32 values of another alive; rows
+  // past the last load the last (a load under a condition makes the wait for
+  // any of them a wait for all)
+  u4 v[H];
+  const auto at_hand = [&](int h, int j) { return (float)__builtin_bit_cast(P, v[h])[j]; };
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const uint32_t row = r + u * p.lines;
-        if (row >= end) continue;
-        float y[V];
+  for (int h = 0; h < H; ++h)
+    v[h] = __builtin_bit_cast(
+        u4, *reinterpret_cast<const P*>(x + offset_of(p, p.xb, 0, p.xw, min(ty + h * p.lines, p.rows - 1), c)));
+  Sums<SEG> t = {};
 #pragma unroll
-        for (int j = 0; j < V; ++j) {
-          y[j] = __builtin_fmaf(v[u][j] - mean[j], scale[j], shift[j]);
-          if (p.silu) y[j] = sizeof(T) == 2 ? y[j] * dev::sigmoid_fast(y[j]) : y[j] / (1.0f + expf(-y[j]));
-        }
-        T* o = out + offset_of(p, p.ob, p.oh, p.ow, row, c);
-        if (c >= at.c0 && c + V <= at.c1) {
-          dev::store_pack<T, V>(o, y);
-        } else {
+  for (int s = 0; s < SEG; ++s) t.k[s] = at_hand(0, s * W);
+  uint32_t mine = 0;  // rows of this thread
 #pragma unroll
-          for (int j = 0; j < V; ++j)
-            if (c + j >= at.c0 && c + j < last) o[j] = c + j < p.channels ? (T)y[j] : (T)0.f;
-        }
+  for (int h = 0; h < H; ++h) {
+    if (ty + h * p.lines < p.rows) {
+      ++mine;
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        const float d = at_hand(h, j) - t.k[j / W];
+        t.s1[j / W] += d;
+        t.s2[j / W] = __builtin_fmaf(d, d, t.s2[j / W]);
       }
     }
   }
-}
-
-__device__ __forceinline__ float inverse_deviation(const NormPlan& p, const Moments& m) {
-  return 1.0f / __builtin_sqrtf(m.m2 / m.n + p.eps);
-}
-
-// One launch: a workgroup takes all rows of its groups, twice.
-template <typename T, int SEG>
-__global__ __launch_bounds__(kThreads) void norm_whole_kernel(NormPlan p) {
-  extern __shared__ float lds[];
-  Moments* lines = reinterpret_cast<Moments*>(lds);
-  Moments* slots = lines + kThreads * SEG;
-  Moments* group = slots + p.vectors * SEG;
-  const Place at = place_of(p);
-  tile_moments<T, SEG>(p, at, 0, p.rows, lines, slots, group);
-  for (uint32_t g = threadIdx.x; g < at.count; g += kThreads) group[g].m2 = inverse_deviation(p, group[g]);
-  __syncthreads();
-  apply_rows<T>(p, at, 0, p.rows, group);
+#pragma unroll
+  for (int s = 0; s < SEG; ++s) t.n[s] = live ? (float)(mine * W) : 0.f;
+  const float inverse = 1.0f / (float)(p.rows * p.per_group);
+  const Joined joined = join_threads<SEG, W, THREADS>(p, at, of, reference, inverse, t, lds);
+  float mean[SEG];
+#pragma unroll
+  for (int s = 0; s < SEG; ++s) {
+    mean[s] = __builtin_fmaf(joined.off[of[s]], inverse, joined.reference[of[s]]);
+    const float inv = 1.0f / __builtin_sqrtf(__builtin_fmaf(joined.dev2[of[s]], inverse, p.eps));
+#pragma unroll
+    for (int j = 0; j < W; ++j) scale[s * W + j] *= inv;
+  }
+  if (!live) return;
+  bool fold = true;
+#pragma unroll
+  for (int j = 0; j < V; ++j) fold = fold && folds<T>(mean[j / W], scale[j]);
+  if (fold) {
+#pragma unroll
+    for (int j = 0; j < V; ++j) shift[j] = __builtin_fmaf(-mean[j / W], scale[j], shift[j]);
+  }
+  const auto rows = [&](auto silu, auto folded) {
+    T* to = out + offset_of(p, p.ob, 0, p.ow, ty, c);
+#pragma unroll
+    for (int h = 0; h < H; ++h) {
+      __asm__ volatile("" : "+v"(v[h]));
+      if (ty + h * p.lines < p.rows) {
+        P y;
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          const float d = decltype(folded)::value ? at_hand(h, j) : at_hand(h, j) - mean[j / W];
+          y[j] = (T)activate<T, decltype(silu)::value>(__builtin_fmaf(d, scale[j], shift[j]));
+        }
+        *reinterpret_cast<P*>(to) = y;
+      }
+      to += p.lines * p.ow;
+    }
+  };
+  const auto with_silu = [&](auto folded) {
+    if (p.silu) rows(std::true_type{}, folded);
+    else rows(std::false_type{}, folded);
+  };
+  if constexpr (sizeof(T) == 2) {
+    if (fold) return with_silu(std::true_type{});
+  }
+  with_silu(std::false_type{});
 }
 
 // Two launches: moments of a chunk of rows, then the rows with the moments of
 // all chunks joined.
 template <typename T, int SEG>
 __global__ __launch_bounds__(kThreads) void norm_moments_kernel(NormPlan p) {
+  constexpr int V = 16 / sizeof(T), W = V / SEG, U = 4;  // rows at hand; as many are on their way
+  typedef typename dev::Pack<T, V>::type P;
   extern __shared__ float lds[];
-  Moments* lines = reinterpret_cast<Moments*>(lds);
-  Moments* slots = lines + kThreads * SEG;
-  Moments* group = slots + p.vectors * SEG;
-  const Place at = place_of(p);
+  const Place at = place_of(p, blockIdx.x);
   const uint32_t begin = at.chunk * p.chunk_rows, end = min(begin + p.chunk_rows, p.rows);
-  tile_moments<T, SEG>(p, at, begin, end, lines, slots, group);
+  const uint32_t ty = p.by_lanes.div(threadIdx.x), tx = threadIdx.x & (p.lanes - 1);
+  const T* x = static_cast<const T*>(p.x) + (int64_t)at.sample * p.xn;
+  const Reference reference = reference_of<T, kThreads>(p, at, x, begin);
+  uint32_t of[SEG];  // group of a segment
+#pragma unroll
+  for (int s = 0; s < SEG; ++s) of[s] = p.by_group.div(min(max(at.from + tx * V + s * W, at.c0), at.c1 - 1)) - at.first;
+  Sums<SEG> t = {};
+  bool fresh = true;
+  // (one turn, or several over the vectors of a single wide group)
+  for (uint32_t c = at.from + tx * V; c < at.c1 && begin + ty < end; c += p.lanes * V) {
+    const bool whole = c >= at.c0 && c + V <= at.c1;
+    uint32_t seen = 0;
+    const auto row_loop = [&](auto edge) {
+      P ahead[U];
+      const auto load = [&](uint32_t r) {
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+          ahead[u] = load_vector<T, decltype(edge)::value>(
+              p, x + offset_of(p, p.xb, p.xh, p.xw, min(r + u * p.lines, end - 1), c), c);
+      };
+      load(begin + ty);
+      for (uint32_t r = begin + ty; r < end; r += U * p.lines) {
+        P v[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) v[u] = ahead[u];
+        if (r + U * p.lines < end) load(r + U * p.lines);
+        if (fresh) {
+#pragma unroll
+          for (int s = 0; s < SEG; ++s) t.k[s] = (float)v[0][s * W];
+          fresh = false;
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          if (r + u * p.lines >= end) continue;
+          ++seen;
+#pragma unroll
+          for (int j = 0; j < V; ++j) {
+            float d = (float)v[u][j] - t.k[j / W];
+            if constexpr (decltype(edge)::value) d = c + j >= at.c0 && c + j < at.c1 ? d : 0.f;
+            t.s1[j / W] += d;
+            t.s2[j / W] = __builtin_fmaf(d, d, t.s2[j / W]);
+          }
+        }
+      }
+    };
+    if (whole) row_loop(std::false_type{});
+    else row_loop(std::true_type{});
+#pragma unroll
+    for (int s = 0; s < SEG; ++s) {
+      const uint32_t lo = max(c + s * W, at.c0), hi = min(c + s * W + W, at.c1);
+      t.n[s] += lo < hi ? (float)(seen * (hi - lo)) : 0.f;
+    }
+  }
+  const float inverse = 1.0f / (float)((end - begin) * p.per_group);
+  const Joined joined = join_threads<SEG, W, kThreads>(p, at, of, reference, inverse, t, lds);
   for (uint32_t g = threadIdx.x; g < at.count; g += kThreads) {
     float* o = p.partial + (((uint64_t)at.sample * p.groups + at.first + g) * p.chunks + at.chunk) * 2;
-    o[0] = group[g].mean;
-    o[1] = group[g].m2;
+    o[0] = __builtin_fmaf(joined.off[g], inverse, joined.reference[g]);
+    o[1] = joined.dev2[g];
   }
 }
 
-template <typename T>
-__global__ __launch_bounds__(kThreads) void norm_apply_kernel(NormPlan p) {
-  extern __shared__ float lds[];
-  Moments* group = reinterpret_cast<Moments*>(lds);
-  const Place at = place_of(p);
-  for (uint32_t g0 = 0; g0 < at.count; g0 += kThreads / 8) {
-    const uint32_t g = g0 + threadIdx.x / 8;
-    Moments m = {0.f, 0.f, 0.f};
-    if (g < at.count) {
-      const float* part = p.partial + ((uint64_t)at.sample * p.groups + at.first + g) * p.chunks * 2;
-      for (uint32_t k = threadIdx.x % 8; k < p.chunks; k += 8) {
-        const uint32_t rows = min(p.chunk_rows, p.rows - k * p.chunk_rows);
-        m = join(m, Moments{(float)(rows * p.per_group), part[2 * k], part[2 * k + 1]});
-      }
+// Mean and 1 / sqrt(var + eps) of the tile's groups from the chunks' moments:
+// the mean from the chunks' means (against the first, so that a common offset
+// cancels), then the squares' sum with each chunk's distance from it.
+constexpr int kChunkLanes = 16, kHeldChunks = 8;  // lanes of a group, chunks of a lane
+__device__ __forceinline__ void join_chunks(const NormPlan& p, const Place& at, float* group) {
+  for (uint32_t g0 = 0; g0 < at.count; g0 += kThreads / kChunkLanes) {
+    const uint32_t g = min(g0 + threadIdx.x / kChunkLanes, at.count - 1);
+    const float* part = p.partial + ((uint64_t)at.sample * p.groups + at.first + g) * p.chunks * 2;
+    float mean[kHeldChunks], m2[kHeldChunks], n[kHeldChunks];
+#pragma unroll
+    for (int i = 0; i < kHeldChunks; ++i) {
+      const uint32_t k = threadIdx.x % kChunkLanes + i * kChunkLanes, held = min(k, p.chunks - 1);
+      mean[i] = part[2 * held];
+      m2[i] = part[2 * held + 1];
+      n[i] = k < p.chunks ? (float)(min(p.chunk_rows, p.rows - k * p.chunk_rows) * p.per_group) : 0.f;
     }
-    m = join_lanes<8>(m);
-    if (g < at.count && threadIdx.x % 8 == 0) group[g] = {m.n, m.mean, inverse_deviation(p, m)};
+    const float first = part[0], total = (float)(p.rows * p.per_group);
+    float sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < kHeldChunks; ++i)
+      if (n[i] != 0.f) sum = __builtin_fmaf(mean[i] - first, n[i], sum);
+    const float mu = first + dev::group_sum<kChunkLanes>(sum) / total;
+    float squares = 0.f;
+#pragma unroll
+    for (int i = 0; i < kHeldChunks; ++i)
+      if (n[i] != 0.f) squares += __builtin_fmaf((mean[i] - mu) * (mean[i] - mu), n[i], m2[i]);
+    squares = dev::group_sum<kChunkLanes>(squares);
+    if (g0 + threadIdx.x / kChunkLanes < at.count && threadIdx.x % kChunkLanes == 0) {
+      group[2 * g] = mu;
+      group[2 * g + 1] = 1.0f / __builtin_sqrtf(squares / total + p.eps);
+    }
   }
   __syncthreads();
-  const uint32_t begin = at.chunk * p.chunk_rows;
-  apply_rows<T>(p, at, begin, min(begin + p.chunk_rows, p.rows), group);
+}
+
+template <typename T, bool SILU>
+__global__ __launch_bounds__(kThreads) void norm_apply_kernel(NormPlan p) {
+  constexpr int V = 16 / sizeof(T), U = 4;
+  extern __shared__ float lds[];
+  const Place at = place_of(p, blockIdx.x);
+  const uint32_t begin = at.chunk * p.chunk_rows, end = min(begin + p.chunk_rows, p.rows);
+  const uint32_t ty = p.by_lanes.div(threadIdx.x), tx = threadIdx.x & (p.lanes - 1);
+  const T* x = static_cast<const T*>(p.x) + (int64_t)at.sample * p.xn;
+  T* out = static_cast<T*>(p.out) + (int64_t)at.sample * p.on;
+  // the last tile of a blocked tensor also writes the padding channels (zeros)
+  const uint32_t last = at.c1 == p.channels ? p.padded : at.c1;
+  uint32_t c = at.from + tx * V;
+  const bool busy = c < last && begin + ty < end;
+  typedef typename dev::Pack<T, V>::type P;
+  // U rows from r on; the first ones are on their way while the moments are joined
+  const auto load = [&](uint32_t r, P (&v)[U], auto edge) {
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      v[u] = load_vector<T, decltype(edge)::value>(
+          p, x + offset_of(p, p.xb, p.xh, p.xw, min(r + u * p.lines, end - 1), c), c);
+  };
+  // memory past the channels of a row is not this tensor's, in the blocked layout its padding
+  const auto inside = [&]() { return p.blocked || c + V <= p.channels; };
+  float scale[V], shift[V];
+  const auto params = [&]() {
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      const uint32_t ch = min(max(c + j, at.c0), at.c1 - 1);
+      scale[j] = p.weight ? param<T>(p.weight, p.weight32, ch * p.ws) : 1.f;
+      shift[j] = p.bias ? param<T>(p.bias, p.bias32, ch * p.bs) : 0.f;
+    }
+  };
+  P v[U];
+  if (busy) {
+    params();
+    if (inside()) load(begin + ty, v, std::false_type{});
+  }
+  join_chunks(p, at, lds);
+  if (!busy) return;
+  for (; c < last; c += p.lanes * V) {
+    if (c != at.from + tx * V) {
+      params();
+      if (inside()) load(begin + ty, v, std::false_type{});
+    }
+    if (!inside()) load(begin + ty, v, std::true_type{});
+    float mean[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      const uint32_t g = p.by_group.div(min(max(c + j, at.c0), at.c1 - 1)) - at.first;
+      mean[j] = lds[2 * g];
+      scale[j] *= lds[2 * g + 1];
+    }
+    bool fold = true;
+#pragma unroll
+    for (int j = 0; j < V; ++j) fold = fold && folds<T>(mean[j], scale[j]);
+    const bool inner = c >= at.c0 && c + V <= at.c1;
+    if (fold && inner) {
+#pragma unroll
+      for (int j = 0; j < V; ++j) shift[j] = __builtin_fmaf(-mean[j], scale[j], shift[j]);
+    }
+    const auto row_loop = [&](auto folded, auto edge) {
+    for (uint32_t r = begin + ty; r < end;) {
+      P y[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) y[u] = v[u];
+      const uint32_t now = r;
+      r += U * p.lines;
+      if (r < end) load(r, v, edge);
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const uint32_t row = now + u * p.lines;
+        if (row >= end) continue;
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          const float d = decltype(folded)::value ? (float)y[u][j] : (float)y[u][j] - mean[j];
+          y[u][j] = (T)activate<T, SILU>(__builtin_fmaf(d, scale[j], shift[j]));
+        }
+        T* to = out + offset_of(p, p.ob, p.oh, p.ow, row, c);
+        if constexpr (!decltype(edge)::value) {
+          *reinterpret_cast<P*>(to) = y[u];
+        } else {
+#pragma unroll
+          for (int j = 0; j < V; ++j)
+            if (c + j >= at.c0 && c + j < last) to[j] = c + j < p.channels ? y[u][j] : (T)0.f;
+        }
+      }
+    }
+    };
+    if (!inner) row_loop(std::false_type{}, std::true_type{});
+    else if (sizeof(T) == 2 && fold) row_loop(std::true_type{}, std::false_type{});
+    else row_loop(std::false_type{}, std::false_type{});
+  }
 }
 
 // How the work is cut, from sizes alone (the workspace's size follows it).
 struct Cut {
   uint32_t tile_groups, tiles, vectors, lanes, lines, segments, slots_per_group, chunks, chunk_rows;
-  bool ok;
+  uint32_t threads, held;  // one launch: threads of a workgroup and vectors of a thread; else 0
 };
-Cut cut_of(int64_t samples, int64_t rows, int64_t channels, int64_t groups, int elem, bool blocked) {
-  Cut c;
-  memset(&c, 0, sizeof c);
-  const int64_t V = 16 / elem, per = channels / groups;
-  // a tile holds whole groups, where few enough so many that it starts and ends
-  // at a whole vector (a whole block of 16), else one
-  const int64_t whole = blocked ? 16 : V, most_channels = blocked ? 512 : 1024;
-  const int64_t unit = whole / std::gcd(per, whole);
-  int64_t tg = 1;
-  if (unit * per <= most_channels) tg = blocked ? unit : most_channels / (unit * per) * unit;
+uint32_t power_of_two(uint32_t n) {
+  uint32_t p = 1;
+  while (p < n) p *= 2;
+  return p;
+}
+// The parts that follow from tg groups a tile.
+void cut_tile(Cut& c, int64_t tg, int64_t groups, int64_t per, int64_t V, bool blocked) {
   tg = std::min(tg, groups);
   c.tile_groups = (uint32_t)tg;
   c.tiles = (uint32_t)((groups + tg - 1) / tg);
@@ -325,14 +524,57 @@ Cut cut_of(int64_t samples, int64_t rows, int64_t channels, int64_t groups, int 
     c.slots_per_group = c.vectors;
   }
   c.segments = (uint32_t)(V / width);
-  c.ok = (int64_t)c.vectors * c.segments <= kMaxSlots;
-  c.lanes = std::min(c.vectors, kThreads);
+}
+Cut cut_of(int64_t samples, int64_t rows, bool flat, int64_t channels, int64_t groups, int elem, bool blocked) {
+  Cut c;
+  memset(&c, 0, sizeof c);
+  const int64_t V = 16 / elem, per = channels / groups;
+  // a tile holds whole groups, where few enough so many that it starts and ends
+  // at a whole vector (a whole block of 16), else one
+  const int64_t unit = V / std::gcd(per, V), most_channels = 64 * V;  // a wavefront across
+  const bool aligned = unit * per <= most_channels;
+  // one launch: the widest tile whose rows registers hold, narrower (down to 32
+  // bytes) while there are too few of them for the device
+  int64_t tg = aligned ? std::min(unit, groups) : 1;
+  cut_tile(c, tg, groups, per, V, blocked);
+  const auto fits = [&](const Cut& k) {
+    const int64_t lanes = power_of_two(k.vectors);
+    if (!flat || channels % (blocked ? 16 : V) || k.tile_groups * per % V) return false;
+    return lanes <= 32 && lanes * k.segments <= 256 && lanes * rows <= kHeldVectors;
+  };
+  if (fits(c) && (samples * c.tiles >= kFillingTiles || (int64_t)c.vectors * rows <= kFewVectors)) {
+    while (aligned) {
+      Cut wider = c;
+      cut_tile(wider, tg * 2, groups, per, V, blocked);
+      if (wider.tiles >= c.tiles || !fits(wider)) break;
+      if (samples * wider.tiles < 256 && (c.vectors >= 2 || samples * wider.tiles < kFillingTiles)) break;
+      c = wider;
+      tg *= 2;
+    }
+    c.lanes = power_of_two(c.vectors);
+    const int64_t vectors = c.lanes * rows;
+    c.threads = vectors <= 1024 ? 256 : 1024;
+    c.held = vectors <= 4096 ? 4 : vectors <= 8192 ? 8 : 16;
+    c.lines = c.threads / c.lanes;
+    c.chunks = 1;
+    c.chunk_rows = (uint32_t)rows;
+    return c;
+  }
+  // two launches: tiles of at least 256 bytes a row where whole vectors allow
+  // (a whole block of 16 in the blocked layout, which is one run of memory)
+  const int64_t least = blocked ? 16 : 256 / elem;
+  cut_tile(c, aligned ? std::min((least + unit * per - 1) / (unit * per), most_channels / (unit * per)) * unit : 1,
+           groups, per, V, blocked);
+  c.lanes = std::min<uint32_t>(power_of_two(c.vectors), 64);
   c.lines = kThreads / c.lanes;
-  const int64_t blocks = samples * c.tiles;
-  const int64_t most = (rows + c.lines * 8 - 1) / (c.lines * 8);
-  int64_t chunks = std::max<int64_t>(1, std::min((kBlocks + blocks - 1) / blocks, most));
-  c.chunk_rows = (uint32_t)((rows + chunks - 1) / chunks);
-  c.chunks = (uint32_t)((rows + c.chunk_rows - 1) / c.chunk_rows);
+  if (c.tile_groups == 1) c.slots_per_group = c.lanes;
+  // rows a thread: few while that gives the device enough workgroups, and the
+  // second launch not more chunks than it joins
+  int64_t each = 2;
+  const auto chunks = [&](int64_t m) { return (rows + c.lines * m - 1) / (c.lines * m); };
+  while (chunks(each) > kChunkLanes * kHeldChunks || (chunks(each) > 1 && samples * c.tiles * chunks(each) > kBlocks)) each *= 2;
+  c.chunk_rows = (uint32_t)std::min<int64_t>(rows, c.lines * each);
+  c.chunks = (uint32_t)chunks(each);
   return c;
 }
 
@@ -374,17 +616,27 @@ Shape shape_of(const thin_desc* x, const thin_desc* out, bool blocked) {
 }
 
 template <typename T, int SEG>
-thin_status launch_norm(const NormPlan& p, hipStream_t stream) {
+thin_status launch_norm(const NormPlan& p, const Cut& c, hipStream_t stream) {
   const uint32_t blocks = p.samples * p.tiles * p.chunks;
-  const size_t lds = sizeof(Moments) * ((size_t)kThreads * SEG + p.vectors * SEG + p.tile_groups);
-  if (p.chunks == 1) {
-    hipLaunchKernelGGL((norm_whole_kernel<T, SEG>), dim3(blocks), dim3(kThreads), lds, stream, p);
+  if (c.held) {
+    const size_t lds = sizeof(float) * (c.threads / 64 * p.lanes * SEG + 3 * p.tile_groups);
+    if (c.threads == 256)
+      hipLaunchKernelGGL((norm_held_kernel<T, SEG, 256, 4>), dim3(blocks), dim3(256), lds, stream, p);
+    else if (c.held == 4)
+      hipLaunchKernelGGL((norm_held_kernel<T, SEG, 1024, 4>), dim3(blocks), dim3(1024), lds, stream, p);
+    else if (c.held == 8)
+      hipLaunchKernelGGL((norm_held_kernel<T, SEG, 1024, 8>), dim3(blocks), dim3(1024), lds, stream, p);
+    else
+      hipLaunchKernelGGL((norm_held_kernel<T, SEG, 1024, 16>), dim3(blocks), dim3(1024), lds, stream, p);
     THIN_LAUNCH_CHECK("group_norm");
     return THIN_OK;
   }
+  const size_t lds = sizeof(float) * (kThreads / 64 * p.lanes * SEG + 3 * p.tile_groups);
   hipLaunchKernelGGL((norm_moments_kernel<T, SEG>), dim3(blocks), dim3(kThreads), lds, stream, p);
   THIN_LAUNCH_CHECK("group_norm_moments");
-  hipLaunchKernelGGL((norm_apply_kernel<T>), dim3(blocks), dim3(kThreads), sizeof(Moments) * p.tile_groups, stream, p);
+  const size_t group = sizeof(float) * 2 * p.tile_groups;
+  if (p.silu) hipLaunchKernelGGL((norm_apply_kernel<T, true>), dim3(blocks), dim3(kThreads), group, stream, p);
+  else hipLaunchKernelGGL((norm_apply_kernel<T, false>), dim3(blocks), dim3(kThreads), group, stream, p);
   THIN_LAUNCH_CHECK("group_norm_apply");
   return THIN_OK;
 }
@@ -394,14 +646,16 @@ thin_status launch_norm(const NormPlan& p, hipStream_t stream) {
 
 using namespace thin;
 
-extern "C" size_t thin_group_norm_workspace(const thin_desc* x, int32_t blocked, int64_t channels, int64_t groups) {
-  if (!desc_valid(x) || !float_type(x->dtype) || x->rank < (blocked ? 5 : 2) || groups < 1 || channels < groups ||
+extern "C" size_t thin_group_norm_workspace(const thin_desc* x, const thin_desc* out, int32_t blocked, int64_t channels,
+                                            int64_t groups) {
+  if (!desc_valid(x) || !desc_valid(out) || !same_sizes(x, out) || !float_type(x->dtype) || x->rank < (blocked ? 5 : 2) || groups < 1 || channels < groups ||
       channels % groups || numel(x) == 0)
     return 0;
   int64_t rows = 1;
   for (int d = blocked ? 2 : 1; d < x->rank - 1; ++d) rows *= x->sizes[d];
-  const Cut c = cut_of(x->sizes[0], rows, channels, groups, dtype_size(x->dtype), blocked != 0);
-  return c.ok && c.chunks > 1 ? (size_t)x->sizes[0] * groups * c.chunks * 2 * sizeof(float) : 0;
+  const bool flat = shape_of(x, out, blocked != 0).outer == 1;
+  const Cut c = cut_of(x->sizes[0], rows, flat, channels, groups, dtype_size(x->dtype), blocked != 0);
+  return !c.held ? (size_t)x->sizes[0] * groups * c.chunks * 2 * sizeof(float) : 0;
 }
 
 extern "C" thin_status thin_group_norm(const thin_desc* x, int32_t blocked, int64_t channels, int64_t groups,
@@ -440,11 +694,9 @@ extern "C" thin_status thin_group_norm(const thin_desc* x, int32_t blocked, int6
   THIN_REQUIRE(s.rows < (1ll << 31) && channels < (1ll << 31) && s.samples < (1ll << 31) &&
                    s.rows * (channels / groups) < (1ll << 31),
                THIN_ERR_UNSUPPORTED, "group_norm: tensor too large");
-  const Cut c = cut_of(s.samples, s.rows, channels, groups, elem, blocked != 0);
-  THIN_REQUIRE(c.ok, THIN_ERR_UNSUPPORTED, "group_norm: groups of %lld channels are not supported",
-               (long long)(channels / groups));
+  const Cut c = cut_of(s.samples, s.rows, s.outer == 1, channels, groups, elem, blocked != 0);
   THIN_REQUIRE(s.samples * c.tiles * (int64_t)c.chunks < (1ll << 31), THIN_ERR_UNSUPPORTED, "group_norm: tensor too large");
-  const size_t need = c.chunks > 1 ? (size_t)s.samples * groups * c.chunks * 2 * sizeof(float) : 0;
+  const size_t need = !c.held ? (size_t)s.samples * groups * c.chunks * 2 * sizeof(float) : 0;
   THIN_REQUIRE(workspace_bytes >= need && (need == 0 || workspace), THIN_ERR_WORKSPACE,
                "group_norm needs %zu bytes of workspace, got %zu", need, workspace_bytes);
   NormPlan p;
@@ -481,17 +733,20 @@ extern "C" thin_status thin_group_norm(const thin_desc* x, int32_t blocked, int6
   p.by_chunks = FastDiv::make(p.chunks);
   p.by_tiles = FastDiv::make(p.tiles);
   p.by_group = FastDiv::make(p.per_group);
+  p.by_slots = FastDiv::make(p.slots_per_group);
+  p.by_span = FastDiv::make(8 * p.tiles);
+  p.spans = p.samples / 8;
   p.blocked = blocked ? 1 : 0;
   p.silu = silu ? 1 : 0;
   p.eps = (float)eps;
   return with_float_type(x->dtype, [&](auto zero) {
     using T = decltype(zero);
     switch (c.segments) {
-      case 1: return launch_norm<T, 1>(p, stream);
-      case 2: return launch_norm<T, 2>(p, stream);
-      case 4: return launch_norm<T, 4>(p, stream);
+      case 1: return launch_norm<T, 1>(p, c, stream);
+      case 2: return launch_norm<T, 2>(p, c, stream);
+      case 4: return launch_norm<T, 4>(p, c, stream);
       default:
-        if constexpr (sizeof(T) == 2) return launch_norm<T, 8>(p, stream);
+        if constexpr (sizeof(T) == 2) return launch_norm<T, 8>(p, c, stream);
         else return THIN_ERR_UNSUPPORTED;
     }
   });

@@ -44,7 +44,7 @@ at::Tensor group_norm(const at::Tensor& x, int64_t groups, const Maybe& weight, 
   auto out = at::empty(x.sizes(), x.options().memory_format(c10::MemoryFormat::Contiguous));
   thin_desc xd = desc(x), od = desc(out);
   MaybeDesc w(weight, "thin_fused.group_norm"), b(bias, "thin_fused.group_norm");
-  const size_t bytes = thin_group_norm_workspace(&xd, blocked, c, groups);
+  const size_t bytes = thin_group_norm_workspace(&xd, &od, blocked, c, groups);
   at::Tensor ws;
   if (bytes) ws = empty_bytes((int64_t)bytes);
   check(thin_group_norm(&xd, blocked, c, groups, w.ptr, b.ptr, eps, silu ? 1 : 0, &od, bytes ? ws.data_ptr() : nullptr,

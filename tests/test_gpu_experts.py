@@ -74,6 +74,35 @@ def test_token_counts_and_views(gpu, t):
     assert not room[0][:, 1::2].any()
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("e", [3, 16, 30, 60, 128, 250, 256, 512, 700])
+def test_many_tokens(gpu, e, dtype):
+    """More tokens than get a wavefront each: rows of a few kinds, all over."""
+    from thintnpu_amd import capi
+    g = gen(e)
+    kinds = (torch.randn((11, e), generator=g) * 2).to(TYPES[dtype])
+    kinds[3] = 0
+    kinds[4, e // 2:] = -math.inf
+    kinds[5, 0] = math.nan
+    which = torch.randint(0, 11, (1500,), generator=g)
+    bias = torch.randn(e, generator=g) * 0.1
+    k, groups, top = min(e, 9), 5 if e % 5 == 0 else 4 if e % 4 == 0 else 1, 2
+    for options in ({}, {"bias": bias, "scores": "sigmoid"}, {"bias": bias, "renormalize": False},
+                    {"groups": groups, "top_groups": min(top, groups)},
+                    {"bias": bias, "scores": "sigmoid", "groups": groups, "top_groups": min(top, groups), "scale": 2.5}):
+        if options.get("groups", 1) > 1 and k > e // groups * 2:
+            continue
+        rw, re = ex.route(kinds, k, **options)
+        moved = {**options, "bias": bias.to(gpu)} if "bias" in options else options
+        w, experts = capi.expert_route(kinds[which].to(gpu), k, **moved)
+        assert torch.equal(experts.cpu(), re[which])
+        few = capi.expert_route(kinds.to(gpu), k, **moved)[0].cpu()
+        # the two differ in the order of a sum of positive terms: 16 in a lane at most and 6 joins, so 22 u on
+        # either side, and 2 u each for the quotient and the product
+        torch.testing.assert_close(w.cpu(), few[which], rtol=48 * U, atol=0, equal_nan=True)
+        torch.testing.assert_close(few.double(), rw, rtol=(2 * 20 + 2 * k + 24) * 2 * U, atol=1e-37, equal_nan=True)
+
+
 def test_ties_go_to_the_lower_index(gpu):
     logits = torch.zeros((5, 96))
     logits[1, 50:] = 1

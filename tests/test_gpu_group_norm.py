@@ -97,6 +97,23 @@ def test_blocked(gpu, n, c, h, w, groups, dtype):
         assert torch.equal(rest, torch.zeros_like(rest))
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("shape,groups", [
+    ((17, 12, 12, 64), 8),     # one launch, samples dealt to the XCDs with some left over
+    ((2, 70, 70, 32), 4), ((9, 50, 60, 64), 16),  # 4, 8 and 16 vectors a thread
+    ((2, 110, 100, 128), 32),  # two launches, streaming stores
+    ((1, 160, 150, 72), 9), ((1, 90, 120, 328), 41), ((1, 64, 65, 520), 65)])
+def test_larger(gpu, shape, groups, dtype):
+    from thintnpu_amd import capi
+    x, w, b = inputs(shape, TYPES[dtype], 31, "same")
+    check(capi.group_norm(x.to(gpu), groups, w.to(gpu), b.to(gpu), silu=True), x, groups, w, b, 1e-5, True)
+    n, h, w_, c = shape
+    if c % 16 == 0:
+        blocked = x.view(n, h, w_, c // 16, 16).permute(0, 3, 1, 2, 4).contiguous()
+        got = capi.group_norm_nc1hwc0(blocked.to(gpu), groups, w.to(gpu), b.to(gpu), silu=True)
+        check(norm.blocked(got.cpu(), c), x, groups, w, b, 1e-5, True)
+
+
 def test_whole_blocks_need_no_channel_count(gpu):
     from thintnpu_amd import capi
     x = torch.randn((1, 2, 3, 4, 16), generator=gen(1)).half()

@@ -64,6 +64,27 @@ def test_row_counts(gpu, r):
         check(gpu, x, tokens, 3)
 
 
+@pytest.mark.parametrize("v", [4090, 4097, 20000, 140001])
+def test_many_rows(gpu, v):
+    """Rows enough that a wavefront ends each: a few kinds of them, all over."""
+    from thintnpu_amd import capi
+    kinds = (torch.randn((7, v), generator=gen(v)) * 2).half()
+    kinds[1] = -math.inf
+    kinds[1, v // 2: v // 2 + 9] = 1.0
+    kinds[2] = 0.5
+    kinds[3] = torch.randint(0, 3, (v,), generator=gen(v + 1)).half()
+    kinds[4, 7] = kinds[4, v - 2] = math.nan
+    kinds[5, 9] = math.inf
+    kinds[6] = -math.inf
+    which = torch.randint(0, 7, (900,), generator=gen(v + 2))
+    tokens = torch.randint(0, v, (7,), generator=gen(v + 3))
+    for top in (0, 1, 5, 32):
+        few = check(gpu, kinds, tokens, top)
+        many = capi.token_logprobs(kinds.to(gpu)[which.to(gpu)], tokens[which].to(gpu), top)
+        for a, b in zip(many, few):
+            torch.testing.assert_close(a, b[which.to(gpu)], rtol=0, atol=0 if a.dtype == torch.int64 else 64 * U, equal_nan=True)
+
+
 def test_wide_row(gpu):
     x, tokens = rows(2, 200003, torch.float32, 1)
     check(gpu, x, tokens, 32)

@@ -16,8 +16,12 @@ namespace thin {
 namespace {
 
 constexpr uint32_t kThreads = 256;
-constexpr int64_t kFillingTiles = 128;  // workgroups below which one launch needs few vectors in each
-constexpr int64_t kFewVectors = 2048;
+// One launch with fewer than kFillingTiles workgroups only where each holds few
+// vectors: in the blocked layout, whose tiles are runs of memory, 8192 (one
+// [128,80,80] frame 11.4 us a call against 13.9 in two launches), else 2048 (the
+// same frame channels last 19.2 against 14.1).
+constexpr int64_t kFillingTiles = 128;
+constexpr int64_t kFewVectors = 2048, kFewBlockedVectors = 8192;
 constexpr int64_t kHeldVectors = 16384;  // 16-byte vectors that 1024 threads hold, 16 each
 constexpr int64_t kBlocks = 1024;     // workgroups that fill the device
 
@@ -405,7 +409,11 @@ __device__ __forceinline__ void join_chunks(const NormPlan& p, const Place& at, 
   __syncthreads();
 }
 
-template <typename T, bool SILU>
+// NT: streaming stores, where a tile's rows are whole lines of a large output.
+// They leave the caches to the next x (moments of 210 MB after such a pass 46
+// us, after plain stores 64); in parts of lines they cost more than the whole
+// (52 MB in 32-byte parts by the one launch: 71 against 27 us).
+template <typename T, bool SILU, bool NT>
 __global__ __launch_bounds__(kThreads) void norm_apply_kernel(NormPlan p) {
   constexpr int V = 16 / sizeof(T), U = 4;
   extern __shared__ float lds[];
@@ -484,7 +492,8 @@ __global__ __launch_bounds__(kThreads) void norm_apply_kernel(NormPlan p) {
         }
         T* to = out + offset_of(p, p.ob, p.oh, p.ow, row, c);
         if constexpr (!decltype(edge)::value) {
-          *reinterpret_cast<P*>(to) = y[u];
+          if constexpr (NT) __builtin_nontemporal_store(y[u], reinterpret_cast<P*>(to));
+          else *reinterpret_cast<P*>(to) = y[u];
         } else {
 #pragma unroll
           for (int j = 0; j < V; ++j)
@@ -542,7 +551,7 @@ Cut cut_of(int64_t samples, int64_t rows, bool flat, int64_t channels, int64_t g
     if (!flat || channels % (blocked ? 16 : V) || k.tile_groups * per % V) return false;
     return lanes <= 32 && lanes * k.segments <= 256 && lanes * rows <= kHeldVectors;
   };
-  if (fits(c) && (samples * c.tiles >= kFillingTiles || (int64_t)c.vectors * rows <= kFewVectors)) {
+  if (fits(c) && (samples * c.tiles >= kFillingTiles || (int64_t)c.vectors * rows <= (blocked ? kFewBlockedVectors : kFewVectors))) {
     while (aligned) {
       Cut wider = c;
       cut_tile(wider, tg * 2, groups, per, V, blocked);
@@ -616,7 +625,7 @@ Shape shape_of(const thin_desc* x, const thin_desc* out, bool blocked) {
 }
 
 template <typename T, int SEG>
-thin_status launch_norm(const NormPlan& p, const Cut& c, hipStream_t stream) {
+thin_status launch_norm(const NormPlan& p, const Cut& c, bool streaming, hipStream_t stream) {
   const uint32_t blocks = p.samples * p.tiles * p.chunks;
   if (c.held) {
     const size_t lds = sizeof(float) * (c.threads / 64 * p.lanes * SEG + 3 * p.tile_groups);
@@ -635,8 +644,11 @@ thin_status launch_norm(const NormPlan& p, const Cut& c, hipStream_t stream) {
   hipLaunchKernelGGL((norm_moments_kernel<T, SEG>), dim3(blocks), dim3(kThreads), lds, stream, p);
   THIN_LAUNCH_CHECK("group_norm_moments");
   const size_t group = sizeof(float) * 2 * p.tile_groups;
-  if (p.silu) hipLaunchKernelGGL((norm_apply_kernel<T, true>), dim3(blocks), dim3(kThreads), group, stream, p);
-  else hipLaunchKernelGGL((norm_apply_kernel<T, false>), dim3(blocks), dim3(kThreads), group, stream, p);
+  const dim3 grid(blocks), block(kThreads);
+  if (p.silu && streaming) hipLaunchKernelGGL((norm_apply_kernel<T, true, true>), grid, block, group, stream, p);
+  else if (p.silu) hipLaunchKernelGGL((norm_apply_kernel<T, true, false>), grid, block, group, stream, p);
+  else if (streaming) hipLaunchKernelGGL((norm_apply_kernel<T, false, true>), grid, block, group, stream, p);
+  else hipLaunchKernelGGL((norm_apply_kernel<T, false, false>), grid, block, group, stream, p);
   THIN_LAUNCH_CHECK("group_norm_apply");
   return THIN_OK;
 }
@@ -739,14 +751,16 @@ extern "C" thin_status thin_group_norm(const thin_desc* x, int32_t blocked, int6
   p.blocked = blocked ? 1 : 0;
   p.silu = silu ? 1 : 0;
   p.eps = (float)eps;
+  const bool streaming = numel(x) * elem >= kStreamingBytes &&
+                         (blocked ? p.ow == 16 : c.vectors % 8 == 0 && s.strides[1][3] * elem % 128 == 0);
   return with_float_type(x->dtype, [&](auto zero) {
     using T = decltype(zero);
     switch (c.segments) {
-      case 1: return launch_norm<T, 1>(p, c, stream);
-      case 2: return launch_norm<T, 2>(p, c, stream);
-      case 4: return launch_norm<T, 4>(p, c, stream);
+      case 1: return launch_norm<T, 1>(p, c, streaming, stream);
+      case 2: return launch_norm<T, 2>(p, c, streaming, stream);
+      case 4: return launch_norm<T, 4>(p, c, streaming, stream);
       default:
-        if constexpr (sizeof(T) == 2) return launch_norm<T, 8>(p, c, stream);
+        if constexpr (sizeof(T) == 2) return launch_norm<T, 8>(p, c, streaming, stream);
         else return THIN_ERR_UNSUPPORTED;
     }
   });

@@ -111,8 +111,8 @@ __device__ __forceinline__ void wave_lds_fence() {
 }
 
 // The n best of the G * PER keys of a group, lane g holding elements
-// g * PER + j: emit(i, element, key) runs on the lane that holds the i-th
-// best.  Keys taken become 0.  Every lane of the group takes part.
+// g * PER + j, one after another: emit(i, element, key) runs on the lane that
+// holds the i-th best.  Keys taken become 0.  Every lane of the group takes part.
 template <int G, int PER, typename K, typename Emit>
 __device__ __forceinline__ void take_best(K (&key)[PER], int n, uint32_t g, Emit emit) {
   K best = 0;

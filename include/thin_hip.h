@@ -381,7 +381,8 @@ size_t thin_group_norm_workspace(const thin_desc* x, const thin_desc* out, int32
  *     may need at most two strides (a channel range of a wider tensor, a crop);
  *   blocked != 0: x [N, C1, H, W, 16] with C1 = ceil(channels / 16); channels
  *     past the last take no part and are written as zeros.
- * out may be x itself.  A NaN or infinity makes its group NaN.  The statistic
+ * out may be x itself; the workspace is 4-byte aligned and overlaps no operand.
+ * A NaN or infinity makes its group NaN.  The statistic
  * that the per-channel affine + SiLU chain of the reference's convolutions
  * (ops.cpp:464-512) cannot fold, followed by that chain, as one operator. */
 thin_status thin_group_norm(const thin_desc* x, int32_t blocked, int64_t channels, int64_t groups,
@@ -421,6 +422,7 @@ size_t thin_expert_dispatch_workspace(int64_t tokens, int64_t top_k, int64_t num
  * bit for bit, a row's elements adjacent).  An expert outside
  * [0, num_experts) is no assignment: its slot is -1, and the rows from
  * offsets[num_experts] on are left as they were.  num_experts <= 1024, k <= 32.
+ * The workspace is 4-byte aligned and overlaps no operand.
  * The data movement of the reference's concat (ops.cpp:419-462) with places
  * that depend on the data. */
 thin_status thin_expert_dispatch(const thin_desc* x, const thin_desc* experts, int64_t num_experts,
@@ -451,7 +453,8 @@ size_t thin_token_logprobs_workspace(int64_t rows, int64_t width, int64_t top);
  *   top_logprobs, top_ids [R, top] (top <= 32, top <= V): the highest logits,
  *     highest first, NaN before every value and the lower index before its
  *     equals.
- * fp32 outputs (ids int64).  A row with a NaN, a +inf or nothing but -inf has
+ * fp32 outputs (ids int64); the workspace is 4-byte aligned and overlaps no
+ * operand.  A row with a NaN, a +inf or nothing but -inf has
  * NaN log probabilities and entropy; its ids follow the order above.  The
  * reference's row softmax and top-K (softmax_host.cpp:51-89,
  * selection_flow.cpp:429-499) without the probabilities in between. */

@@ -47,6 +47,7 @@ def norm(code, x=None, out=None, blocked=0, channels=64, groups=8, weight=None, 
 
 def test_group_norm_refusals():
     norm(INVALID, channels=60)
+    norm(UNSUPPORTED, x=desc((2 ** 24, 64)))  # 2^32 threads
     norm(INVALID, groups=7)
     norm(INVALID, groups=0)
     norm(INVALID, groups=-8)
@@ -73,6 +74,7 @@ def test_group_norm_refusals():
     assert need > 0
     norm(WORKSPACE, x=big)
     norm(WORKSPACE, x=big, ws=1 << 30, nbytes=need - 1)
+    norm(WORKSPACE, x=big, ws=(1 << 30) + 2, nbytes=need)
     assert capi.lib().thin_group_norm_workspace(P(big), P(big), 0, 64, 7) == 0
     assert capi.lib().thin_group_norm_workspace(None, P(big), 0, 64, 8) == 0
 
@@ -103,6 +105,9 @@ def test_route_refusals():
     route(INVALID, bias=desc((16,)))
     route(INVALID, weights=desc((4, 2), capi.F32))
     route(INVALID, weights=desc((5, 2)))
+    t = 2 ** 30  # 2^32 threads
+    route(UNSUPPORTED, logits=desc((t, 16), strides=(0, 1)), weights=desc((t, 2), capi.F32),
+          experts=desc((t, 2), capi.I32))
     route(INVALID, experts=desc((5, 2), capi.I64))
     route(INVALID, experts=desc((5, 3), capi.I32))
     logits = desc((5, 16), capi.F32)
@@ -144,6 +149,10 @@ def test_dispatch_refusals():
     need = capi.lib().thin_expert_dispatch_workspace(5000, 2, 4)
     assert need > 0 and capi.lib().thin_expert_dispatch_workspace(6, 2, 4) == 0
     dispatch(WORKSPACE, t=5000)
+    dispatch(WORKSPACE, t=5000, ws=(1 << 30) + 2, nbytes=need)
+    t = 2 ** 24  # 2^32 threads
+    dispatch(UNSUPPORTED, t=t, k=1, x=desc((t, 2048)), rows=desc((t, 2048)), ws=1 << 30, nbytes=1 << 30)
+    dispatch(UNSUPPORTED, x=desc((6, 1 << 28)), rows=desc((12, 1 << 28)))
     dispatch(WORKSPACE, t=5000, ws=1 << 30, nbytes=need - 1)
 
 
@@ -165,6 +174,9 @@ def test_combine_refusals():
     combine(INVALID, out=desc((5, 8)))
     combine(UNSUPPORTED, y=desc((9, 8), strides=(1, 9)))
     combine(UNSUPPORTED, out=desc((4, 8), strides=(16, 2)))
+    t = 2 ** 24  # 2^32 threads
+    combine(UNSUPPORTED, y=desc((9, 2048)), weights=desc((t, 2), capi.F32), slots=desc((t, 2), capi.I32),
+            out=desc((t, 2048)))
     y = desc((9, 8))
     combine(INVALID, y=y, out=desc((4, 8), data=y.data))
 
@@ -194,6 +206,8 @@ def test_logprobs_refusals():
     logprobs(UNSUPPORTED, logits=desc((3, 50), strides=(1, 3)))
     logprobs(UNSUPPORTED, r=1, v=8388609)
     logprobs(UNSUPPORTED, r=2 ** 27, v=80000)
+    logprobs(UNSUPPORTED, r=2 ** 26, v=1000)  # 2^32 threads
+    logprobs(UNSUPPORTED, r=2 ** 25, v=5000)
     logits = desc((3, 50))
     logprobs(INVALID, logits=logits, lp=desc((3,), capi.F32, data=logits.data + 4))
     lp = desc((3,), capi.F32)
@@ -201,6 +215,7 @@ def test_logprobs_refusals():
     need = capi.lib().thin_token_logprobs_workspace(3, 600000, 4)
     assert need > 0 and capi.lib().thin_token_logprobs_workspace(3, 1024, 4) == 0
     logprobs(WORKSPACE, v=600000)
+    logprobs(WORKSPACE, v=600000, ws=(1 << 30) + 2, nbytes=need)
     logprobs(WORKSPACE, v=600000, ws=1 << 30, nbytes=need - 1)
 
 

@@ -136,6 +136,26 @@ def test_borders_that_32_bits_cannot_tell(gpu):
     check_route(gpu, x, 32, bias=bias, scores="sigmoid", groups=4, top_groups=3)
 
 
+@pytest.mark.parametrize("e,groups,top,k", [(60, 5, 2, 8), (120, 8, 3, 6), (250, 5, 2, 9), (500, 20, 7, 8), (1000, 8, 3, 8)])
+def test_close_choices_in_groups_of_any_size(gpu, e, groups, top, k):
+    """Every other row's choice scores are equal but for the bias's rounding, so
+    that waves choose again in 64 bits while others rank groups whose sizes are
+    not powers of two; few tokens and many."""
+    from thintnpu_amd import capi
+    g = gen(e)
+    x = torch.randn((12, e), generator=g)
+    s = 1.0 / (1.0 + torch.exp(-x[0].double()))
+    bias = (0.9 - s).float()
+    x[::2] = x[0]
+    x[4] = x[0].flip(0)
+    options = {"scores": "sigmoid", "groups": groups, "top_groups": top}
+    want = ex.route(x, k, bias, **options)[1]
+    for tokens in (333, 2100):
+        which = torch.randint(0, 12, (tokens,), generator=g)
+        got = capi.expert_route(x[which].to(gpu), k, bias=bias.to(gpu), **options)[1]
+        assert torch.equal(got.cpu(), want[which])
+
+
 def test_route_special_values(gpu):
     nan, inf = math.nan, math.inf
     logits = torch.randn((6, 40), generator=gen(8))
@@ -190,7 +210,7 @@ def check_dispatch(gpu, x, experts, count, xv=None, ev=None):
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("t,k,e,width", [(1, 1, 1, 1), (1, 8, 16, 64), (3, 2, 5, 7), (48, 8, 256, 520), (33, 3, 1024, 2049),
                                          (100, 1, 7, 16), (5, 32, 40, 3), (512, 8, 64, 40), (513, 8, 64, 33),
-                                         (700, 6, 1000, 9), (1500, 4, 3, 300), (4097, 1, 600, 24)])
+                                         (700, 6, 1000, 9), (1500, 4, 3, 300), (4097, 1, 600, 24), (1200, 4, 1024, 8)])
 def test_dispatch(gpu, t, k, e, width, dtype):
     g = gen(t * k)
     x = torch.randn((t, width), generator=g).to(TYPES[dtype])

@@ -26,6 +26,7 @@ struct RoutePlan {
   uint32_t tokens, count;            // tokens, experts
   int32_t k, groups, top, size;      // chosen, groups, kept groups, experts a group
   int32_t group_lanes;               // lanes of a group that is whole lanes, a power of two; else 0
+  uint32_t staged;                   // 64-bit words of LDS that a wave stages keys in
   int32_t softmax, renormalize;
   FastDiv by_size;
   float scale;
@@ -247,11 +248,13 @@ __global__ __launch_bounds__(kThreads) void route_kernel(RoutePlan p) {
   __shared__ float choice[BIAS ? kTokens : 1][kMaxChosen + 1];
   __shared__ GroupLds groups[GROUPED ? kTokens : 1];
   __shared__ WideLds wide[BIAS ? kThreads / 64 : 1];
-  extern __shared__ uint64_t staged_lds[];  // keys: 64-bit ones of a wave's token, 32-bit ones of every token
+  extern __shared__ uint64_t staged_lds[];
 
   const uint32_t g = threadIdx.x % G, slot = threadIdx.x / G;
   const uint32_t token = blockIdx.x * kTokens + slot;
   const bool live = token < p.tokens;  // every lane joins the group's exchanges
+  // this wave's own, as waves do not wait for each other: 32-bit keys of all its tokens, then 64-bit ones of one
+  uint64_t* staged = staged_lds + (threadIdx.x >> 6) * p.staged;
   const T* row = static_cast<const T*>(p.logits) + (int64_t)min(token, p.tokens - 1) * p.row;
   const uint32_t first = g * PER;
   float x[PER];
@@ -282,7 +285,7 @@ __global__ __launch_bounds__(kThreads) void route_kernel(RoutePlan p) {
   }
   bool close = false;
   if constexpr (GROUPED)
-    close = keep_groups<G, PER, BIAS>(p, key, g, reinterpret_cast<uint32_t*>(staged_lds) + slot * p.count, groups[slot]);
+    close = keep_groups<G, PER, BIAS>(p, key, g, reinterpret_cast<uint32_t*>(staged) + slot % (64 / G) * p.count, groups[slot]);
   const int open = GROUPED ? p.top * p.size : (int)p.count;
   const int n = BIAS && p.k < open ? p.k + 1 : p.k;
   dev::take_best<G, PER>(key, n, g, [&](int i, uint32_t e, uint32_t k) {
@@ -304,7 +307,7 @@ __global__ __launch_bounds__(kThreads) void route_kernel(RoutePlan p) {
         again &= ~((G == 64 ? ~0ull : (1ull << G) - 1) << (in_wave * G));
         const uint32_t s = wave * (64 / G) + in_wave;
         choose64(p, static_cast<const T*>(p.logits) + (int64_t)(blockIdx.x * kTokens + s) * p.row,
-                 staged_lds + wave * p.count, wide[wave], chosen[s]);
+                 staged, wide[wave], chosen[s]);
       }
     }
   }
@@ -353,17 +356,18 @@ template <typename T, int G, int PER>
 thin_status launch_route(RoutePlan p, hipStream_t stream) {
   const uint32_t tokens = kThreads / G;
   const dim3 grid((p.tokens + tokens - 1) / tokens), block(kThreads);
+  THIN_REQUIRE(launchable(grid.x, kThreads), THIN_ERR_UNSUPPORTED, "expert_route: too many tokens");
   const bool grouped = p.top < p.groups;
   const uint32_t lanes = (uint32_t)p.size / PER;
   p.group_lanes = (uint32_t)p.size % PER == 0 && (lanes & (lanes - 1)) == 0 ? (int32_t)lanes : 0;
-  const uint32_t lds = std::max<uint32_t>(p.bias ? kThreads / 64 * p.count * 8 : 0u,
-                                          grouped && !p.group_lanes ? tokens * p.count * 4 : 0u);
+  p.staged = std::max<uint32_t>(p.bias ? p.count : 0u, grouped && !p.group_lanes ? (64 / G * p.count + 1) / 2 : 0u);
+  const uint32_t lds = kThreads / 64 * p.staged * 8;
   if (p.bias) {
     if (grouped) hipLaunchKernelGGL((route_kernel<T, G, PER, true, true>), grid, block, lds, stream, p);
     else hipLaunchKernelGGL((route_kernel<T, G, PER, true, false>), grid, block, lds, stream, p);
   } else {
     if (grouped) hipLaunchKernelGGL((route_kernel<T, G, PER, false, true>), grid, block, lds, stream, p);
-    else hipLaunchKernelGGL((route_kernel<T, G, PER, false, false>), grid, block, 0, stream, p);
+    else hipLaunchKernelGGL((route_kernel<T, G, PER, false, false>), grid, block, lds, stream, p);
   }
   THIN_LAUNCH_CHECK("expert_route");
   return THIN_OK;
@@ -384,7 +388,7 @@ struct RowsPlan {
   int64_t st, sk;                    // element strides of slots
   uint32_t tokens, assigned;         // assigned = tokens * k
   int32_t k, count;                  // experts a token, experts
-  uint32_t bytes, elem;              // bytes of a row, of an element
+  uint32_t bytes;                    // of a row
   uint32_t lanes;                    // threads that copy one row (a power of two)
   uint32_t chunk;                    // assignments a wave of the counting kernels
   FastDiv by_k;
@@ -790,10 +794,17 @@ extern "C" thin_status thin_expert_dispatch(const thin_desc* x, const thin_desc*
                    !overlap(slots, x) && !overlap(offsets, x) && !overlap(slots, rows) && !overlap(offsets, rows) &&
                    !overlap(offsets, slots),
                THIN_ERR_INVALID, "expert_dispatch: an output overlaps another operand");
+  const uint32_t elem = (uint32_t)dtype_size(x->dtype);
+  const int64_t vectors = (H * elem + 15) / 16;
+  const bool small = T * k <= kCountedAssignments;
+  const int64_t lanes = small ? kThreads : row_lanes(vectors), per = kThreads / lanes;
+  const dim3 grid((uint32_t)(small ? T + 1 : (T + per - 1) / per), (uint32_t)std::max<int64_t>(1, (vectors + lanes - 1) / lanes));
+  THIN_REQUIRE(launchable(grid.x, kThreads) && grid.y < 65536, THIN_ERR_UNSUPPORTED, "expert_dispatch: tensors too large");
   const size_t need = thin_expert_dispatch_workspace(T, k, num_experts);
   THIN_REQUIRE(workspace_bytes >= need && (need == 0 || workspace), THIN_ERR_WORKSPACE,
                "expert_dispatch needs %zu bytes of workspace, got %zu", need, workspace_bytes);
-  const uint32_t elem = (uint32_t)dtype_size(x->dtype);
+  THIN_REQUIRE(need == 0 || workspace_aligned(workspace), THIN_ERR_WORKSPACE,
+               "expert_dispatch: the workspace must be 4-byte aligned");
   RowsPlan p;
   memset(&p, 0, sizeof p);
   p.x = static_cast<const char*>(x->data);
@@ -812,13 +823,10 @@ extern "C" thin_status thin_expert_dispatch(const thin_desc* x, const thin_desc*
   p.k = (int32_t)k;
   p.count = (int32_t)num_experts;
   p.bytes = (uint32_t)(H * elem);
-  p.elem = elem;
   p.by_k = FastDiv::make((uint32_t)k);
-  const uint64_t vectors = (p.bytes + 15) / 16;
-  if (p.assigned <= kCountedAssignments) {
-    const uint64_t columns = std::max<uint64_t>(1, (vectors + kThreads - 1) / kThreads);
-    THIN_REQUIRE(columns < 65536, THIN_ERR_UNSUPPORTED, "expert_dispatch: rows too long");
-    hipLaunchKernelGGL(dispatch_small_kernel, dim3(p.tokens + 1, (uint32_t)columns), dim3(kThreads), 0, stream, p);
+  p.lanes = (uint32_t)lanes;
+  if (small) {
+    hipLaunchKernelGGL(dispatch_small_kernel, grid, dim3(kThreads), 0, stream, p);
     THIN_LAUNCH_CHECK("expert_dispatch");
     return THIN_OK;
   }
@@ -829,11 +837,6 @@ extern "C" thin_status thin_expert_dispatch(const thin_desc* x, const thin_desc*
                      kPlanWaves * (uint32_t)p.count * sizeof(int32_t), stream, p);
   THIN_LAUNCH_CHECK("expert_dispatch_slots");
   if (H == 0) return THIN_OK;
-  p.lanes = row_lanes(vectors);
-  const uint32_t per = kThreads / p.lanes;
-  const uint64_t columns = (vectors + p.lanes - 1) / p.lanes;
-  THIN_REQUIRE(columns < 65536, THIN_ERR_UNSUPPORTED, "expert_dispatch: rows too long");
-  const dim3 grid((p.tokens + per - 1) / per, (uint32_t)columns);
   if ((int64_t)p.assigned * p.bytes >= kStreamingBytes)
     hipLaunchKernelGGL((dispatch_copy_kernel<true>), grid, dim3(kThreads), 0, stream, p);
   else
@@ -880,8 +883,8 @@ extern "C" thin_status thin_expert_combine(const thin_desc* y, const thin_desc* 
   p.lanes = row_lanes(vectors);
   const uint32_t per = kThreads / p.lanes;
   const uint64_t columns = (vectors + p.lanes - 1) / p.lanes;
-  THIN_REQUIRE(columns < 65536, THIN_ERR_UNSUPPORTED, "expert_combine: rows too long");
   const dim3 grid((p.tokens + per - 1) / per, (uint32_t)columns), block(kThreads);
+  THIN_REQUIRE(columns < 65536 && launchable(grid.x, kThreads), THIN_ERR_UNSUPPORTED, "expert_combine: tensors too large");
   return with_float_type(y->dtype, [&](auto zero) {
     hipLaunchKernelGGL((combine_kernel<decltype(zero)>), grid, block, 0, stream, p);
     THIN_LAUNCH_CHECK("expert_combine");

@@ -707,10 +707,13 @@ extern "C" thin_status thin_group_norm(const thin_desc* x, int32_t blocked, int6
                    s.rows * (channels / groups) < (1ll << 31),
                THIN_ERR_UNSUPPORTED, "group_norm: tensor too large");
   const Cut c = cut_of(s.samples, s.rows, s.outer == 1, channels, groups, elem, blocked != 0);
-  THIN_REQUIRE(s.samples * c.tiles * (int64_t)c.chunks < (1ll << 31), THIN_ERR_UNSUPPORTED, "group_norm: tensor too large");
+  THIN_REQUIRE(launchable(s.samples * c.tiles * (int64_t)c.chunks, c.held ? c.threads : kThreads), THIN_ERR_UNSUPPORTED,
+               "group_norm: tensor too large");
   const size_t need = !c.held ? (size_t)s.samples * groups * c.chunks * 2 * sizeof(float) : 0;
   THIN_REQUIRE(workspace_bytes >= need && (need == 0 || workspace), THIN_ERR_WORKSPACE,
                "group_norm needs %zu bytes of workspace, got %zu", need, workspace_bytes);
+  THIN_REQUIRE(need == 0 || workspace_aligned(workspace), THIN_ERR_WORKSPACE,
+               "group_norm: the workspace must be 4-byte aligned");
   NormPlan p;
   memset(&p, 0, sizeof p);
   p.x = x->data;

@@ -676,6 +676,7 @@ uint32_t tiles_of(int64_t width, int elem) { return (uint32_t)((width + 16 / ele
 template <typename T, int G, int PER>
 thin_status launch_short(const LogprobsPlan& p, hipStream_t stream) {
   const uint32_t rows = 256 / G;
+  THIN_REQUIRE(launchable((p.rows + rows - 1) / rows, 256), THIN_ERR_UNSUPPORTED, "token_logprobs: tensor too large");
   hipLaunchKernelGGL((short_rows_kernel<T, G, PER>), dim3((p.rows + rows - 1) / rows), dim3(256), 0, stream, p);
   THIN_LAUNCH_CHECK("token_logprobs");
   return THIN_OK;
@@ -716,7 +717,7 @@ extern "C" thin_status thin_token_logprobs(const thin_desc* logits, const thin_d
   THIN_REQUIRE(V >= 1 && K <= V && K <= kMaxTop, THIN_ERR_INVALID,
                "token_logprobs gives up to %lld alternatives of the row's %lld, not %lld", (long long)kMaxTop,
                (long long)V, (long long)K);
-  THIN_REQUIRE(V <= kMaxWidth && R < (1ll << 31) && R * tiles_of(V, 2) < (1ll << 31),
+  THIN_REQUIRE(V <= kMaxWidth && R < (1ll << 31) && (V <= kShortRow || launchable(R * tiles_of(V, 2) + 3, 64)),
                THIN_ERR_UNSUPPORTED, "token_logprobs: tensor too large");
   THIN_REQUIRE(V == 1 || logits->strides[1] == 1, THIN_ERR_UNSUPPORTED,
                "token_logprobs: the logits of a row must be adjacent");
@@ -731,6 +732,8 @@ extern "C" thin_status thin_token_logprobs(const thin_desc* logits, const thin_d
   const size_t need = thin_token_logprobs_workspace(R, V, K);
   THIN_REQUIRE(workspace_bytes >= need && (need == 0 || workspace), THIN_ERR_WORKSPACE,
                "token_logprobs needs %zu bytes of workspace, got %zu", need, workspace_bytes);
+  THIN_REQUIRE(need == 0 || workspace_aligned(workspace), THIN_ERR_WORKSPACE,
+               "token_logprobs: the workspace must be 4-byte aligned");
   LogprobsPlan p;
   memset(&p, 0, sizeof p);
   p.logits = logits->data;

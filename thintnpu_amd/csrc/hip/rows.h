@@ -37,6 +37,11 @@ inline bool overlap(const thin_desc* a, const thin_desc* b) {
   return an && bn && a0 < b0 + bn && b0 < a0 + an;
 }
 
+// HIP launches below 2^32 threads along a dimension.
+inline bool launchable(int64_t blocks, int64_t threads) { return blocks * threads < (1ll << 32); }
+// Workspaces hold 32-bit values.
+inline bool workspace_aligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 3u) == 0; }
+
 }  // namespace thin
 
 #if defined(__HIPCC__)

@@ -68,6 +68,18 @@ def test_group_norm_refusals():
     norm(UNSUPPORTED, x=desc((1, 2 ** 16, 2 ** 16, 64)))
     x = desc((2, 4, 4, 64))
     norm(INVALID, x=x, out=desc((2, 4, 4, 64), data=x.data + 2))  # overlaps without being x
+    row = (4 * 4 * 96, 4 * 96, 96, 1)  # channel ranges of one tensor that share some channels
+    x = desc((2, 4, 4, 64), strides=row)
+    norm(INVALID, x=x, out=desc((2, 4, 4, 64), data=x.data + 2 * 32, strides=row))
+    norm(INVALID, x=x, out=desc((2, 4, 4, 64), data=x.data + 2 * 63, strides=row))
+    norm(INVALID, x=x, out=desc((2, 4, 4, 64), data=x.data + 2 * 64, strides=row))  # the next row's
+    row = (4 * 4 * 128, 4 * 128, 128, 1)
+    x = desc((2, 4, 4, 64), strides=row)
+    norm(INVALID, x=x, out=desc((2, 4, 4, 64), data=x.data + 2 * 60, strides=row))
+    norm(INVALID, x=x, out=desc((2, 4, 4, 64), data=x.data + 2 * (128 * 5 + 68), strides=row))
+    norm(INVALID, out=desc((2, 4, 4, 64), strides=(0, 256, 64, 1)))
+    norm(INVALID, x=desc((2, 4, 4, 64), data=1 << 30, strides=(0, 256, 64, 1)),
+         out=desc((2, 4, 4, 64), data=1 << 30, strides=(0, 256, 64, 1)))
     norm(INVALID, x=x, weight=desc((64,), data=1 << 30), out=desc((2, 4, 4, 64), data=(1 << 30) + 64))
     big = desc((1, 200, 200, 64))
     need = capi.lib().thin_group_norm_workspace(P(big), P(big), 0, 64, 8)
@@ -105,6 +117,7 @@ def test_route_refusals():
     route(INVALID, bias=desc((16,)))
     route(INVALID, weights=desc((4, 2), capi.F32))
     route(INVALID, weights=desc((5, 2)))
+    route(INVALID, weights=desc((5, 2), capi.F32, strides=(0, 1)))
     t = 2 ** 30  # 2^32 threads
     route(UNSUPPORTED, logits=desc((t, 16), strides=(0, 1)), weights=desc((t, 2), capi.F32),
           experts=desc((t, 2), capi.I32))
@@ -135,6 +148,8 @@ def test_dispatch_refusals():
     dispatch(INVALID, offsets=desc((4,), capi.I32))
     dispatch(INVALID, offsets=desc((5,), capi.I64))
     dispatch(INVALID, slots=desc((6, 3), capi.I32))
+    dispatch(INVALID, slots=desc((6, 2), capi.I32, strides=(0, 1)))
+    dispatch(INVALID, rows=desc((12, 8), strides=(0, 1)))
     dispatch(UNSUPPORTED, count=1025)
     dispatch(UNSUPPORTED, count=0, offsets=desc((1,), capi.I32))
     dispatch(UNSUPPORTED, k=33)
@@ -172,6 +187,7 @@ def test_combine_refusals():
     combine(INVALID, weights=desc((4, 3), capi.F32))
     combine(INVALID, slots=desc((4, 2), capi.I64))
     combine(INVALID, out=desc((5, 8)))
+    combine(INVALID, out=desc((4, 8), strides=(0, 1)))
     combine(UNSUPPORTED, y=desc((9, 8), strides=(1, 9)))
     combine(UNSUPPORTED, out=desc((4, 8), strides=(16, 2)))
     t = 2 ** 24  # 2^32 threads
@@ -201,6 +217,7 @@ def test_logprobs_refusals():
     logprobs(INVALID, tl=desc((3, 5), capi.F32))
     logprobs(INVALID, ti=desc((3, 4), capi.I32))
     logprobs(INVALID, top=33)
+    logprobs(INVALID, lp=desc((3,), capi.F32, strides=(0,)))
     logprobs(INVALID, v=3)
     logprobs(INVALID, v=0, top=0)
     logprobs(UNSUPPORTED, logits=desc((3, 50), strides=(1, 3)))

@@ -141,6 +141,22 @@ def test_views(gpu, dtype):
     check(norm.blocked(got.cpu(), 64), norm.blocked(x[:, 4:], 64), 16, None, None, 1e-5, True)
 
 
+@pytest.mark.parametrize("h", [8, 150])
+def test_between_channel_ranges(gpu, h):
+    """From one channel range of a tensor to another, and between blocks of one."""
+    from thintnpu_amd import capi
+    base = torch.randn((2, h, h, 160), generator=gen(h)).half()
+    dev = base.to(gpu)
+    capi.group_norm(dev[..., :64], 8, silu=True, out=dev[..., 96:])
+    check(dev[..., 96:], base[..., :64], 8, None, None, 1e-5, True)
+    assert torch.equal(dev[..., :96].cpu(), base[..., :96])
+    base = torch.randn((2, 8, h, h, 16), generator=gen(h + 1)).half()
+    dev = base.to(gpu)
+    capi.group_norm_nc1hwc0(dev[:, 4:], 8, silu=True, out=dev[:, :4])
+    check(norm.blocked(dev[:, :4].cpu(), 64), norm.blocked(base[:, 4:], 64), 8, None, None, 1e-5, True)
+    assert torch.equal(dev[:, 4:].cpu(), base[:, 4:])
+
+
 @pytest.mark.parametrize("shape,groups", [((2, 8, 8, 64), 8), ((1, 150, 150, 64), 16)])
 def test_in_place(gpu, shape, groups):
     from thintnpu_amd import capi

@@ -722,6 +722,7 @@ extern "C" thin_status thin_expert_route(const thin_desc* logits, const thin_des
   THIN_REQUIRE(!overlap(weights, logits) && !overlap(experts, logits) && !overlap(weights, experts) &&
                    (!bias || (!overlap(weights, bias) && !overlap(experts, bias))), THIN_ERR_INVALID,
                "expert_route: an output overlaps another operand");
+  THIN_REQUIRE(!repeats(weights) && !repeats(experts), THIN_ERR_INVALID, "expert_route: an output has a stride of 0");
   RoutePlan p;
   memset(&p, 0, sizeof p);
   p.logits = logits->data;
@@ -794,6 +795,8 @@ extern "C" thin_status thin_expert_dispatch(const thin_desc* x, const thin_desc*
                    !overlap(slots, x) && !overlap(offsets, x) && !overlap(slots, rows) && !overlap(offsets, rows) &&
                    !overlap(offsets, slots),
                THIN_ERR_INVALID, "expert_dispatch: an output overlaps another operand");
+  THIN_REQUIRE(!repeats(rows) && !repeats(offsets) && !repeats(slots), THIN_ERR_INVALID,
+               "expert_dispatch: an output has a stride of 0");
   const uint32_t elem = (uint32_t)dtype_size(x->dtype);
   const int64_t vectors = (H * elem + 15) / 16;
   const bool small = T * k <= kCountedAssignments;
@@ -865,6 +868,7 @@ extern "C" thin_status thin_expert_combine(const thin_desc* y, const thin_desc* 
   if (T == 0 || H == 0) return THIN_OK;
   THIN_REQUIRE(!overlap(out, y) && !overlap(out, weights) && !overlap(out, slots), THIN_ERR_INVALID,
                "expert_combine: the output overlaps an input");
+  THIN_REQUIRE(!repeats(out), THIN_ERR_INVALID, "expert_combine: the output has a stride of 0");
   CombinePlan p;
   memset(&p, 0, sizeof p);
   p.y = y->data;

@@ -699,6 +699,7 @@ extern "C" thin_status thin_group_norm(const thin_desc* x, int32_t blocked, int6
   THIN_REQUIRE(s.ok, THIN_ERR_UNSUPPORTED, "group_norm: the rows of a sample need more than two strides");
   bool same = x->data == out->data;
   for (int d = 0; d < x->rank; ++d) same = same && (x->sizes[d] == 1 || x->strides[d] == out->strides[d]);
+  THIN_REQUIRE(!repeats(out), THIN_ERR_INVALID, "group_norm: the output has a stride of 0");
   THIN_REQUIRE(same || !overlap(out, x), THIN_ERR_INVALID, "group_norm: the output overlaps x without being x");
   for (int i = 0; i < 2; ++i)
     THIN_REQUIRE(!params[i] || !overlap(out, params[i]), THIN_ERR_INVALID, "group_norm: the output overlaps a parameter");

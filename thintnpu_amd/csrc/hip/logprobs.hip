@@ -724,6 +724,7 @@ extern "C" thin_status thin_token_logprobs(const thin_desc* logits, const thin_d
   if (R == 0) return THIN_OK;
   const thin_desc* outs[4] = {logprobs, entropy, top_logprobs, top_ids};
   for (int i = 0; i < 4; ++i) {
+    THIN_REQUIRE(!repeats(outs[i]), THIN_ERR_INVALID, "token_logprobs: an output has a stride of 0");
     THIN_REQUIRE(!overlap(outs[i], logits) && !overlap(outs[i], tokens), THIN_ERR_INVALID,
                  "token_logprobs: an output overlaps an input");
     for (int j = 0; j < i; ++j)

@@ -29,14 +29,33 @@ inline int64_t extent(const thin_desc* d) {
   }
   return last + 1;
 }
-// True if the bytes two descriptors reach have some in common.
+// True if the bytes two descriptors reach may have some in common.  Ranges that
+// interleave (channel ranges of one wider tensor) have none where, modulo a
+// stride that the outer dimensions are multiples of, the inner parts are apart.
 inline bool overlap(const thin_desc* a, const thin_desc* b) {
-  const char* a0 = static_cast<const char*>(a->data);
-  const char* b0 = static_cast<const char*>(b->data);
-  const int64_t an = extent(a) * dtype_size(a->dtype), bn = extent(b) * dtype_size(b->dtype);
-  return an && bn && a0 < b0 + bn && b0 < a0 + an;
+  const int64_t delta = static_cast<const char*>(b->data) - static_cast<const char*>(a->data);
+  const int64_t ea = dtype_size(a->dtype), eb = dtype_size(b->dtype), an = extent(a) * ea, bn = extent(b) * eb;
+  if (!an || !bn || delta >= an || -delta >= bn) return false;
+  for (int i = 0; i < a->rank; ++i) {
+    const int64_t period = a->strides[i] * ea;
+    if (period <= 0) continue;
+    const auto inner = [&](const thin_desc* d, int64_t elem) {
+      int64_t bytes = elem;
+      for (int k = 0; k < d->rank; ++k)
+        if (d->strides[k] * elem % period) bytes += (d->sizes[k] - 1) * d->strides[k] * elem;
+      return bytes;
+    };
+    const int64_t ia = inner(a, ea), ib = inner(b, eb), at = ((delta % period) + period) % period;
+    if (at >= ia && at + ib <= period) return false;
+  }
+  return true;
 }
-
+// True if elements of an output share memory by a stride of 0.
+inline bool repeats(const thin_desc* d) {
+  for (int i = 0; i < d->rank; ++i)
+    if (d->sizes[i] > 1 && d->strides[i] == 0) return true;
+  return false;
+}
 // HIP launches below 2^32 threads along a dimension.
 inline bool launchable(int64_t blocks, int64_t threads) { return blocks * threads < (1ll << 32); }
 // Workspaces hold 32-bit values.

@@ -13,7 +13,9 @@ constexpr uint32_t kThreads = 256;
 constexpr int64_t kMaxExperts = 1024;
 constexpr int64_t kMaxChosen = 32;
 constexpr int64_t kMaxGroups = 64;
-constexpr int64_t kFewTokens = 1024;  // tokens up to which each has a whole wavefront
+// Tokens up to which each has a whole wavefront: with few of them the latency of
+// one counts (48 tokens of 256 experts: 5.7 us, by 16 lanes a token 13).
+constexpr int64_t kFewTokens = 1024;
 
 // ---------------------------------------------------------------- routing
 struct RoutePlan {
@@ -36,18 +38,18 @@ constexpr float kLog2e = 1.4426950408889634f;
 
 // Scores s of a row held by G lanes: softmax or sigmoid of x in V.
 template <int G, int PER>
-__device__ __forceinline__ void scores32(const float (&x)[PER], uint32_t first, uint32_t count, bool softmax,
+__device__ __forceinline__ void scores32(const float (&x)[PER], const dev::Part<PER, false>& part, bool softmax,
                                          float (&s)[PER], float& total) {
   if (softmax) {
     float m = -__builtin_inff();
 #pragma unroll
     for (int j = 0; j < PER; ++j)
-      if (first + j < count) m = fmaxf(m, x[j]);
+      if (part.own(j)) m = fmaxf(m, x[j]);
     m = dev::group_max<G>(m);
     total = 0.f;
 #pragma unroll
     for (int j = 0; j < PER; ++j) {
-      s[j] = first + j < count ? __builtin_amdgcn_exp2f((x[j] - m) * kLog2e) : 0.f;
+      s[j] = part.own(j) ? __builtin_amdgcn_exp2f((x[j] - m) * kLog2e) : 0.f;
       total += s[j];
     }
     total = dev::group_sum<G>(total);
@@ -92,8 +94,8 @@ struct GroupLds {
   uint32_t border[2];
 };
 template <int G, int PER, bool BIAS>
-__device__ __forceinline__ bool keep_groups(const RoutePlan& p, uint32_t (&key)[PER], uint32_t g, uint32_t* staged,
-                                            GroupLds& lds) {
+__device__ __forceinline__ bool keep_groups(const RoutePlan& p, uint32_t (&key)[PER], const dev::Part<PER, false>& part,
+                                            uint32_t g, uint32_t* staged, GroupLds& lds) {
   const uint32_t first = g * PER;
   const bool whole = p.group_lanes != 0;
   uint32_t own = 0;  // whole: the score of this lane's group
@@ -120,7 +122,7 @@ __device__ __forceinline__ bool keep_groups(const RoutePlan& p, uint32_t (&key)[
   } else {
 #pragma unroll
     for (int j = 0; j < PER; ++j)
-      if (first + j < p.count) staged[first + j] = key[j];
+      if (part.own(j)) staged[part.from + j] = key[j];
     dev::wave_lds_fence();
     for (int q = (int)g; q < p.groups; q += G) {
       uint32_t best = 0, second = 0;
@@ -163,7 +165,7 @@ __device__ __forceinline__ bool keep_groups(const RoutePlan& p, uint32_t (&key)[
     dev::wave_lds_fence();
 #pragma unroll
     for (int j = 0; j < PER; ++j)
-      if (!lds.key[p.by_size.div(min(first + j, p.count - 1))]) key[j] = 0;
+      if (!lds.key[p.by_size.div(min(part.from + j, p.count - 1))]) key[j] = 0;
   }
   dev::wave_lds_fence();
   return BIAS && near_tie(dev::key_score(lds.border[0]), dev::key_score(lds.border[1]), 2.f);
@@ -241,9 +243,19 @@ __device__ __forceinline__ void choose64(const RoutePlan& p, const T* row, uint6
 // the border of the groups) are nearer than that arithmetic can tell apart the
 // token is chosen again in 64 bits; equal logits with equal biases are equal
 // in either.
+//
+// The logits are read once, at the start; what bounds the kernel is the issue of
+// instructions, not their bytes.  16384 tokens of 256 fp32 logits, 8 of them out
+// of 4 of 8 groups: 21 us (0.85 TB/s; 1400 VALU instructions a wave of 4 tokens;
+// of 25k cycles the loads take 3.5k, the scores 5.5k, the groups 3.4k and the
+// selection 10.7k).  51200 tokens of 60 fp16 logits, 4 of them: 7.8 us.  Hence the
+// shape: as few lanes a token as hold its logits 4 to 16 each, so that a wave's
+// reductions serve several tokens, and keys that are whole numbers, so that a
+// maximum is one instruction and needs no second one for its place.
 template <typename T, int G, int PER, bool BIAS, bool GROUPED>
 __global__ __launch_bounds__(kThreads) void route_kernel(RoutePlan p) {
   constexpr int kTokens = kThreads / G;
+  constexpr bool kPlaces = !BIAS && sizeof(T) == 2;  // a 16-bit logit and its place in one key
   __shared__ int32_t chosen[kTokens][kMaxChosen + 1];
   __shared__ float choice[BIAS ? kTokens : 1][kMaxChosen + 1];
   __shared__ GroupLds groups[GROUPED ? kTokens : 1];
@@ -256,42 +268,44 @@ __global__ __launch_bounds__(kThreads) void route_kernel(RoutePlan p) {
   // this wave's own, as waves do not wait for each other: 32-bit keys of all its tokens, then 64-bit ones of one
   uint64_t* staged = staged_lds + (threadIdx.x >> 6) * p.staged;
   const T* row = static_cast<const T*>(p.logits) + (int64_t)min(token, p.tokens - 1) * p.row;
-  const uint32_t first = g * PER;
+  const dev::Part<PER, false> part(g, p.count);
   float x[PER];
-  if (first + PER <= p.count) {
-    dev::load_pack<T, PER>(row + first, x);
-  } else {
-#pragma unroll
-    for (int j = 0; j < PER; ++j) x[j] = first + j < p.count ? (float)row[first + j] : 0.f;
-  }
+  part.load(row, x);
 
   uint32_t key[PER];
   float total = 1.f;
   if constexpr (BIAS) {
     float b[PER];
-    if (p.bias_step == 1 && first + PER <= p.count) {
-      dev::load_pack<float, PER>(p.bias + first, b);
+    if (p.bias_step == 1) {
+      part.load(p.bias, b);
     } else {
 #pragma unroll
-      for (int j = 0; j < PER; ++j) b[j] = p.bias[min(first + j, p.count - 1) * p.bias_step];
+      for (int j = 0; j < PER; ++j) b[j] = p.bias[min(part.from + j, p.count - 1) * p.bias_step];
     }
     float s[PER];
-    scores32<G, PER>(x, first, p.count, p.softmax, s, total);
+    scores32<G, PER>(x, part, p.softmax, s, total);
 #pragma unroll
-    for (int j = 0; j < PER; ++j) key[j] = first + j < p.count ? dev::score_key(s[j] + b[j]) : 0u;
+    for (int j = 0; j < PER; ++j) key[j] = part.own(j) ? dev::score_key(s[j] + b[j]) : 0u;
   } else {
 #pragma unroll
-    for (int j = 0; j < PER; ++j) key[j] = first + j < p.count ? dev::score_key(x[j]) : 0u;
+    for (int j = 0; j < PER; ++j) {
+      if constexpr (kPlaces) key[j] = part.own(j) ? dev::place_key<T>(x[j], part.from + j) : 0u;
+      else key[j] = part.own(j) ? dev::score_key(x[j]) : 0u;
+    }
   }
   bool close = false;
   if constexpr (GROUPED)
-    close = keep_groups<G, PER, BIAS>(p, key, g, reinterpret_cast<uint32_t*>(staged) + slot % (64 / G) * p.count, groups[slot]);
+    close = keep_groups<G, PER, BIAS>(p, key, part, g, reinterpret_cast<uint32_t*>(staged) + slot % (64 / G) * p.count, groups[slot]);
   const int open = GROUPED ? p.top * p.size : (int)p.count;
   const int n = BIAS && p.k < open ? p.k + 1 : p.k;
-  dev::take_best<G, PER>(key, n, g, [&](int i, uint32_t e, uint32_t k) {
-    chosen[slot][i] = (int32_t)e;
-    if constexpr (BIAS) choice[slot][i] = dev::key_score(k);
-  });
+  if constexpr (kPlaces) {
+    dev::take_places<G, PER>(key, n, g, [&](int i, uint32_t k) { chosen[slot][i] = (int32_t)dev::place_index(k); });
+  } else {
+    dev::take_best<G, PER>(key, n, g, [&](int i, uint32_t e, uint32_t k) {
+      chosen[slot][i] = (int32_t)(e - part.skip);
+      if constexpr (BIAS) choice[slot][i] = dev::key_score(k);
+    });
+  }
   dev::wave_lds_fence();
   if constexpr (BIAS) {
     for (int i = (int)g; i < n - 1; i += G) {
@@ -320,7 +334,7 @@ __global__ __launch_bounds__(kThreads) void route_kernel(RoutePlan p) {
     } else {
 #pragma unroll
       for (int j = 0; j < PER; ++j)
-        if (first + j < p.count) top = fmaxf(top, x[j]);
+        if (part.own(j)) top = fmaxf(top, x[j]);
     }
     top = dev::group_max<G>(top);
   }
@@ -337,7 +351,7 @@ __global__ __launch_bounds__(kThreads) void route_kernel(RoutePlan p) {
   } else if (p.softmax) {
 #pragma unroll
     for (int j = 0; j < PER; ++j)
-      if (first + j < p.count) sum += expf(x[j] - top);
+      if (part.own(j)) sum += expf(x[j] - top);
     sum = dev::group_sum<G>(sum);
   } else {
     sum = 1.f;
@@ -430,7 +444,11 @@ __device__ __forceinline__ void copy_row(const RowsPlan& p, uint32_t t, uint32_t
 
 // Few assignments: block (t, y) counts for each of its token's assignments the
 // ones before it in the order (expert, assignment) among all, and copies 256
-// vectors of the row; block (tokens, 0) writes the offsets.  One launch.
+// vectors of the row; block (tokens, 0) writes the offsets.  One launch, bound by
+// latency: the ids' load, a pass over them in LDS and the row's own load and
+// stores one after another (48 tokens of 4096 bf16, 8 experts each: 6.3 us for
+// 3.5 MB, where counting, planning and copying in launches of their own would
+// cost three times the launch alone).
 constexpr uint32_t kCountedAssignments = 4096;
 __global__ __launch_bounds__(kThreads) void dispatch_small_kernel(RowsPlan p) {
   constexpr int kWaves = kThreads / 64, kAtOnce = 8;
@@ -489,8 +507,10 @@ __global__ __launch_bounds__(kThreads) void dispatch_small_kernel(RowsPlan p) {
 
 // Many assignments, in three launches: counts of each block's assignments by
 // expert, slots from them, the copy.  A block's 16 waves take runs of `chunk`
-// assignments each, in order.  Loads go eight or more at a time: one after
-// another they cost a memory latency each (counts of 64 blocks: 25 us, now 4).
+// assignments each, in order, so that no slot depends on the order of atomics.
+// The first two are bound by latency, a load of ids and LDS atomics in turn;
+// loads therefore go four or more at a time (131072 assignments to 256 experts:
+// 4.8 and 8.4 us; with one wave's loads one after another the slots took 25 us).
 constexpr uint32_t kPlanThreads = 1024, kPlanWaves = kPlanThreads / 64;
 
 // f(assignment, expert) of the assignments in [begin, end) of a thread that
@@ -597,6 +617,9 @@ __global__ __launch_bounds__(kPlanThreads) void dispatch_slots_kernel(RowsPlan p
   }
 }
 
+// The copy: HBM alone.  16384 rows of 4 KB to 8 places each: 104 us for 604 MB
+// (5.8 TB/s); the stores by themselves, with no row read, also take 104 us.  A
+// row is read once and written k times from registers.
 template <bool NT>
 __global__ __launch_bounds__(kThreads) void dispatch_copy_kernel(RowsPlan p) {
   const uint32_t t = blockIdx.x * (kThreads / p.lanes) + threadIdx.x / p.lanes;
@@ -618,9 +641,11 @@ struct CombinePlan {
 };
 
 // out[t] = sum_j weights[t, j] * y[slots[t, j]], in the order of j, in fp32
-// with one rounding; slots outside y contribute nothing.  Eight rows are loaded
-// at a time (one after another 125 us for 604 MB, now 117 us, 5.2 TB/s;
-// streaming loads changed nothing).
+// with one rounding; slots outside y contribute nothing.  A thread owns 16 bytes
+// of out[t], so sums need neither LDS nor atomics.  Bound by HBM: 16384 tokens, 8
+// rows of 4 KB each, 604 MB in 117 us (5.2 TB/s; rows of 4 KB at random places
+// stay below a copy's 6.4).  Eight rows are loaded at a time (one after another
+// 125 us; streaming loads changed nothing).
 template <typename T, int N>
 __device__ __forceinline__ void add_rows(const CombinePlan& p, uint32_t t, uint32_t at, float (&sum)[N]) {
   constexpr int U = 8;
@@ -745,6 +770,7 @@ extern "C" thin_status thin_expert_route(const thin_desc* logits, const thin_des
   p.scale = scale;
   return with_float_type(logits->dtype, [&](auto zero) {
     using T_ = decltype(zero);
+    if (E < 4) return launch_route<T_, 64, 1>(p, stream);  // (a lane's part is no longer than the row)
     if (T <= kFewTokens) {
       if (E <= 64) return launch_route<T_, 64, 1>(p, stream);
       if (E <= 128) return launch_route<T_, 64, 2>(p, stream);

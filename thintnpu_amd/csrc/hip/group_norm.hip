@@ -3,7 +3,10 @@
 //   mean, var over the rows and channels of a group, y = (x - mean) /
 //   sqrt(var + eps) * weight + bias, then y * sigmoid(y).
 //
-// Statistics are fp32.
+// Statistics are fp32.  x has to be read before the first of y is known: either
+// a workgroup holds all rows of its groups in registers (one launch, x read
+// once), or the moments take a launch of their own and x is read again, from the
+// Infinity Cache where it fits.
 #include "rows.h"
 
 #include <string.h>
@@ -201,6 +204,11 @@ __device__ __forceinline__ Joined join_threads(const NormPlan& p, const Place& a
   add_up<SEG, THREADS>(p, at, sum, lds, dev2);
   return {off, dev2, against};
 }
+// 32 samples of [80,80,128] fp16 in 32 groups with SiLU, 105 MB: 26.5 us (4 TB/s;
+// blocked 24.5).  One workgroup of 16 waves fills a CU's registers, so that its
+// phases do not overlap: 9.6 us of loads (5.4 TB/s), 2 of joins, 8 of SiLU and
+// stores, the rest of ramps.  A single blocked frame: 11.7 us by 16 workgroups,
+// each bound by its own CU's loads.
 template <typename T, int SEG, int THREADS, int H>
 __global__ __launch_bounds__(THREADS) void norm_held_kernel(NormPlan p) {
   constexpr int V = 16 / sizeof(T), W = V / SEG;
@@ -304,7 +312,10 @@ __global__ __launch_bounds__(THREADS) void norm_held_kernel(NormPlan p) {
 }
 
 // Two launches: moments of a chunk of rows, then the rows with the moments of
-// all chunks joined.
+// all chunks joined.  Both are bound by memory and by what comes before a
+// workgroup's first load and after its last: 5 samples of [61,83,648] bf16 (half
+// the channels of 1296), 33 MB, moments 13.7 us and rows 15.6 us; of 210 MB 46 us
+// (4.6 TB/s).
 template <typename T, int SEG>
 __global__ __launch_bounds__(kThreads) void norm_moments_kernel(NormPlan p) {
   constexpr int V = 16 / sizeof(T), W = V / SEG, U = 4;  // rows at hand; as many are on their way

@@ -100,41 +100,75 @@ __device__ __forceinline__ void store_alternative(const LogprobsPlan& p, uint32_
   p.top_ids[(int64_t)row * p.ir + i * p.ik] = (int64_t)id;
 }
 
+// What stands in the place of elements that a row does not have: finite, and of
+// weight 0 next to any maximum above kLowest (an -inf would leave 0 * -inf).
+template <typename T> constexpr float kAbsent = -1e30f;
+template <> constexpr float kAbsent<_Float16> = -65504.f;
+template <typename T> constexpr float kLowest = -1e29f;
+template <> constexpr float kLowest<_Float16> = -65000.f;
+
 // ---------------------------------------------------------------- short rows
-// G lanes a row, lane g holding elements g * PER + j.
+// G lanes a row, lane g holding elements g * PER + j, so that a row is read once
+// and everything after it is registers.  Bound by the issue of instructions, above
+// all those of the alternatives, taken one after another: 200000 rows of 1000
+// bf16, 400 MB, 94 us with none (4.3 TB/s), 216 with 5 and 390 with 20 (fp32 129,
+// 265 and 660: its keys leave no room for the index, so that the one taken has to
+// be found and removed).
 template <typename T, int G, int PER>
 __global__ __launch_bounds__(256) void short_rows_kernel(LogprobsPlan p) {
   const uint32_t g = threadIdx.x % G;
   const uint32_t row = blockIdx.x * (256 / G) + threadIdx.x / G;
   const bool live = row < p.rows;
   const T* x = static_cast<const T*>(p.logits) + (int64_t)min(row, p.rows - 1) * p.row;
-  const uint32_t first = g * PER;
   const Given given = given_of(p, min(row, p.rows - 1), x);
+  const dev::Part<PER, true> part(g, p.width);
   float v[PER];
-  if (first + PER <= p.width) {
-    dev::load_pack<T, PER>(x + first, v);
-  } else {
-#pragma unroll
-    for (int j = 0; j < PER; ++j) v[j] = first + j < p.width ? (float)x[first + j] : -__builtin_inff();
-  }
+  part.load(x, v);
   float m = -__builtin_inff();
 #pragma unroll
-  for (int j = 0; j < PER; ++j) m = fmaxf(m, v[j]);
+  for (int j = 0; j < PER; ++j) {
+    v[j] = part.own(j) ? v[j] : kAbsent<float>;
+    m = fmaxf(m, v[j]);
+  }
   RowSums r{dev::group_max<G>(m), 0.f, 0.f};
-  const float top = r.m == -__builtin_inff() ? 0.f : r.m;
+  const bool plain = r.m > kLowest<float> && plain_range(r.m);
+  const float base = r.m * kLog2e;
 #pragma unroll
-  for (int j = 0; j < PER; ++j) add_element<true>(r, v[j], top, 0.f);
+  for (int j = 0; j < PER; ++j) add_element<false>(r, v[j], r.m, base);
   r.s = dev::group_sum<G>(r.s);
   r.u = dev::group_sum<G>(r.u);
+  take_back_rounding(r);
+  if (!plain || r.u != r.u) {  // the same for the lanes of a row
+    m = -__builtin_inff();
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+      v[j] = part.own(j) ? v[j] : -__builtin_inff();
+      m = fmaxf(m, v[j]);
+    }
+    r = {dev::group_max<G>(m), 0.f, 0.f};
+    const float top = r.m == -__builtin_inff() ? 0.f : r.m;
+#pragma unroll
+    for (int j = 0; j < PER; ++j) add_element<true>(r, v[j], top, 0.f);
+    r.s = dev::group_sum<G>(r.s);
+    r.u = dev::group_sum<G>(r.u);
+  }
   if (live && g == 0) store_row(p, row, given, r);
   if (p.top == 0) return;
   const float rest = rest_of(r);
   uint32_t key[PER];
+  if constexpr (sizeof(T) == 2) {
 #pragma unroll
-  for (int j = 0; j < PER; ++j) key[j] = first + j < p.width ? dev::score_key(v[j]) : 0u;
-  dev::take_best<G, PER>(key, p.top, g, [&](int i, uint32_t id, uint32_t k) {
-    if (live) store_alternative(p, row, i, id, dev::key_score(k), r.m, rest);
-  });
+    for (int j = 0; j < PER; ++j) key[j] = part.own(j) ? dev::place_key<T>(v[j], part.from + j) : 0u;
+    dev::take_places<G, PER>(key, p.top, g, [&](int i, uint32_t k) {
+      if (live) store_alternative(p, row, i, dev::place_index(k), dev::place_score<T>(k), r.m, rest);
+    });
+  } else {
+#pragma unroll
+    for (int j = 0; j < PER; ++j) key[j] = part.own(j) ? dev::score_key(v[j]) : 0u;
+    dev::take_best<G, PER>(key, p.top, g, [&](int i, uint32_t id, uint32_t k) {
+      if (live) store_alternative(p, row, i, id - part.skip, dev::key_score(k), r.m, rest);
+    });
+  }
 }
 
 // ---------------------------------------------------------------- long rows
@@ -189,7 +223,10 @@ __device__ __forceinline__ float run_maximum(const float (&v)[N]) {
   }
 }
 
-// A wavefront's tile of 4096 elements: sums and maximum (the same in every
+// A wavefront's tile of 4096 elements, in registers: the maximum first, then the
+// sums against it, so that no running maximum rescales them.  Tiles begin at
+// 16-byte aligned addresses whatever the row's own start, which leaves the odd
+// elements to a row's first and last tile.  Sums and maximum (the same in every
 // lane), and in lane l the maximum of run run_of(l).
 template <typename T>
 __device__ __forceinline__ uint32_t run_of() {
@@ -197,13 +234,6 @@ __device__ __forceinline__ uint32_t run_of() {
   const uint32_t lane = threadIdx.x & 63u;
   return lane % kLoads * (64 / kLoads) + lane / kLoads;
 }
-// What stands in the place of elements that a row does not have: finite, and of
-// weight 0 next to any maximum above kLowest (an -inf would leave 0 * -inf).
-template <typename T> constexpr float kAbsent = -1e30f;
-template <> constexpr float kAbsent<_Float16> = -65504.f;
-template <typename T> constexpr float kLowest = -1e29f;
-template <> constexpr float kLowest<_Float16> = -65000.f;
-
 // The tile whose 16-byte aligned first position is at x; the row has positions
 // [lo, hi) of it.
 template <typename T>
@@ -487,7 +517,11 @@ __global__ __launch_bounds__(64) void tile_rows_kernel(LogprobsPlan p) {
   alternatives(p, row, x, staged, 1, true, r.m, rest_of(r), lds);
 }
 
-// Longer rows, two launches: tiles anywhere on the device, then the joins.
+// Longer rows, two launches: tiles anywhere on the device, however few the rows,
+// then the joins.  The first is bound by HBM and, next to it, by issue (550 VALU
+// instructions a tile, 64 of them exponentials): 4001 rows of 50001, 400 MB, 64 us
+// in bf16 (6.3 TB/s) and 72 us in fp16 (5.5, a conversion an element more); 48
+// rows of 128000 5.8 us.
 template <typename T>
 __global__ __launch_bounds__(256) void tiles_kernel(LogprobsPlan p) {
   const uint32_t wave = blockIdx.x * 4 + (threadIdx.x >> 6);
@@ -504,7 +538,9 @@ __global__ __launch_bounds__(256) void tiles_kernel(LogprobsPlan p) {
 }
 
 // Many rows: a wavefront each, which the others on the device hide (as much LDS
-// as the row needs, so that more of them fit).
+// as the row needs, so that more of them fit).  Bound by the issue of the
+// selection's instructions: 4001 rows of 13 tiles, 5 alternatives, 14 us (740
+// VALU instructions a row for 10 MB of keys).
 constexpr uint32_t kStaged = 33;  // items of 64: the tiles of the longest row, the runs of 33 tiles
 uint32_t staged_items(uint32_t tiles, int64_t top) {
   return top ? std::max<uint32_t>(tiles <= kStaged ? tiles : (tiles + 63) / 64, (uint32_t)top) : 0u;
@@ -538,7 +574,9 @@ __global__ __launch_bounds__(64) void finish_many_kernel(LogprobsPlan p) {
   if (p.top) alternatives(p, row, x, staged, items, runs, r.m, rest_of(r), lds);
 }
 
-// Few rows: 16 wavefronts each, for the latency.
+// Few rows: 16 wavefronts each, for the latency, which is all there is: loads of
+// the keys, two or three rounds of counting and ranking, and between them loads
+// of what was chosen (48 rows of 32 tiles, 20 alternatives: 7.3 us).
 // best_of() by a workgroup of 16 wavefronts, item i of a thread standing for
 // index(i): the same bound from the maxima of the 64 lane columns, its counts
 // and ranks shared out over the waves (in one wave each of their steps waits

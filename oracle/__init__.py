@@ -10,6 +10,9 @@ Modules (each function cites the reference file:line it restates):
   movement   -- cat, upsample, NC1HWC0 pack/unpack, strided copies (numpy)
   reductions -- softmax, DFL softmax and expectation via PyTorch CPU
   selection  -- YOLO26 score keys, half->float bits, stable two-stage top-K
+  norm       -- group norm in 64 bits
+  experts    -- routing, dispatch and combine in 64 bits, token by token
+  logprobs   -- token log probabilities, entropy and alternatives in 64 bits
 
 Pinning status of every function is listed in its module docstring.
 """

@@ -21,8 +21,9 @@ namespace {
 constexpr uint32_t kThreads = 256;
 // One launch with fewer than kFillingTiles workgroups only where each holds few
 // vectors: in the blocked layout, whose tiles are runs of memory, 8192 (one
-// [128,80,80] frame 11.4 us a call against 13.9 in two launches), else 2048 (the
-// same frame channels last 19.2 against 14.1).
+// [128,80,80] frame 10.8 us a call against 13.9 in two launches), else 2048
+// (recorded into a graph, the same frame channels last 12.8 us against 11.3, two
+// of them 17.6 against 11.6).
 constexpr int64_t kFillingTiles = 128;
 constexpr int64_t kFewVectors = 2048, kFewBlockedVectors = 8192;
 constexpr int64_t kHeldVectors = 16384;  // 16-byte vectors that 1024 threads hold, 16 each
@@ -207,7 +208,7 @@ __device__ __forceinline__ Joined join_threads(const NormPlan& p, const Place& a
 // 32 samples of [80,80,128] fp16 in 32 groups with SiLU, 105 MB: 26.5 us (4 TB/s;
 // blocked 24.5).  One workgroup of 16 waves fills a CU's registers, so that its
 // phases do not overlap: 9.6 us of loads (5.4 TB/s), 2 of joins, 8 of SiLU and
-// stores, the rest of ramps.  A single blocked frame: 11.7 us by 16 workgroups,
+// stores, the rest of ramps.  A single blocked frame: 11.4 us by 16 workgroups,
 // each bound by its own CU's loads.
 template <typename T, int SEG, int THREADS, int H>
 __global__ __launch_bounds__(THREADS) void norm_held_kernel(NormPlan p) {
@@ -215,12 +216,17 @@ __global__ __launch_bounds__(THREADS) void norm_held_kernel(NormPlan p) {
   typedef typename dev::Pack<T, V>::type P;
   typedef uint32_t u4 __attribute__((ext_vector_type(4)));
   extern __shared__ float lds[];
-  // the tiles of a sample on one XCD, whose L2 then holds the lines they share
+  // neighbouring tiles on one XCD, whose L2 then holds the lines they share: each
+  // of 8 samples on its own, of fewer samples an eighth each (3 of [40,40,256]
+  // 10.5 us without, 7.0 with)
   uint32_t block = blockIdx.x;
   const uint32_t span = 8 * p.tiles, q = p.by_span.div(block);
   if (q < p.spans) {
     const uint32_t r = block - q * span;
     block = q * span + (r & 7u) * p.tiles + (r >> 3);
+  } else if (p.tiles % 8 == 0) {
+    const uint32_t t = block - p.by_tiles.div(block) * p.tiles;
+    block += (t & 7u) * (p.tiles >> 3) + (t >> 3) - t;
   }
   const Place at = place_of(p, block);
   const uint32_t tx = threadIdx.x & (p.lanes - 1), ty = p.by_lanes.div(threadIdx.x);

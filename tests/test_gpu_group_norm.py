@@ -242,3 +242,28 @@ def test_same_bits_and_captured(gpu, shape):
         torch.cuda.synchronize()
         expect = capi.group_norm(x * (step + 1), 8, w, b, silu=True)
         assert all(torch.equal(o, expect) for o in outs)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("c,groups,h", [(130, 2, 9), (130, 2, 40), (1001, 7, 5), (268, 4, 11), (1044, 4, 4)])
+def test_groups_that_begin_inside_a_vector(gpu, c, groups, h, dtype):
+    """A blocked group that begins between two whole vectors: the channels before
+    it are another group's, whose NaN, infinities and far values are not its own."""
+    from thintnpu_amd import capi
+    base, w, b = inputs((2, h, 7, c), TYPES[dtype], c + h, "same")
+    per = c // groups
+    for value in (math.nan, math.inf, -math.inf, 1000.0, -1e4, 6e4):
+        for odd in (0, 1):
+            x = base.clone().view(2, h, 7, groups, per)
+            x[:, :, :, odd::2] = value if not math.isfinite(value) else (x[:, :, :, odd::2].float() + value).to(x.dtype)
+            x = x.view(2, h, 7, c)
+            full = torch.zeros((2, h, 7, (c + 15) // 16 * 16), dtype=x.dtype)
+            full[..., :c] = x
+            blocked = full.view(2, h, 7, -1, 16).permute(0, 3, 1, 2, 4).contiguous()
+            got = norm.blocked(capi.group_norm_nc1hwc0(blocked.to(gpu), groups, w.to(gpu), b.to(gpu), channels=c).cpu(), c)
+            for i in range(groups):
+                own = slice(i * per, (i + 1) * per)
+                if math.isfinite(value) or i % 2 != odd:
+                    check(got[..., own], x[..., own], 1, w[own], b[own], 1e-5, False)
+                else:
+                    assert torch.isnan(got[..., own]).all()

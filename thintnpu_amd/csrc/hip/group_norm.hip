@@ -150,7 +150,7 @@ __device__ __forceinline__ void add_up(const NormPlan& p, const Place& at, float
 }
 
 // A thread's sums of x - k and its square over n elements of each segment, k
-// being the first element that it reads, so that a mean far from zero cancels
+// being the first of them that it reads, so that a mean far from zero cancels
 // before the squares are formed.
 template <int SEG>
 struct Sums {
@@ -357,7 +357,15 @@ __global__ __launch_bounds__(kThreads) void norm_moments_kernel(NormPlan p) {
         if (r + U * p.lines < end) load(r + U * p.lines);
         if (fresh) {
 #pragma unroll
-          for (int s = 0; s < SEG; ++s) t.k[s] = (float)v[0][s * W];
+          for (int s = 0; s < SEG; ++s) {
+            t.k[s] = (float)v[0][s * W];
+            // a vector that begins before the group: what stands there is another group's
+            if constexpr (decltype(edge)::value) {
+#pragma unroll
+              for (int j = 1; j < W; ++j)
+                if (c + s * W + j <= at.c0) t.k[s] = (float)v[0][s * W + j];
+            }
+          }
           fresh = false;
         }
 #pragma unroll

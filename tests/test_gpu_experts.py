@@ -328,3 +328,57 @@ def test_rows_beyond_32_bits(gpu):
     one = torch.ones((3, 1), device=gpu)
     back = capi.expert_combine(rows, one, slots, out=v)
     assert torch.equal(back.cpu(), x)
+
+
+# ---------------------------------------------------------------- choices and weights that 32 bits lose
+def check_routes(gpu, kinds, k, bias=None, **options):
+    """check_route() of the rows, and of so many of them that 16 lanes take a token."""
+    from thintnpu_amd import capi
+    check_route(gpu, kinds, k, bias=bias, **options)
+    which = torch.randint(0, kinds.shape[0], (1100,), generator=gen(k))
+    moved = None if bias is None else bias.to(gpu)
+    w, e = capi.expert_route(kinds[which].to(gpu), k, bias=moved, **options)
+    few = capi.expert_route(kinds.to(gpu), k, bias=moved, **options)
+    assert torch.equal(e.cpu(), few[1].cpu()[which])
+    # as in test_many_tokens: the order of one sum of positive terms
+    torch.testing.assert_close(w.cpu(), few[0].cpu()[which], rtol=48 * U, atol=1e-37, equal_nan=True)
+
+
+@pytest.mark.parametrize("scores", ["sigmoid", "softmax"])
+@pytest.mark.parametrize("e,groups", [(4, 2), (16, 8), (24, 4), (32, 4), (256, 8), (240, 8), (1024, 4)])
+@pytest.mark.parametrize("size", [1.0, 30.0, 137.0, 5000.0])
+def test_group_borders_of_large_biases(gpu, e, groups, size, scores):
+    """A group's two highest choice scores are near +h and -h, h another number
+    for each group: their sums are alike, and off by the rounding of h in 32 bits."""
+    per = e // groups
+    g = gen(e + int(size))
+    x = torch.randn((60, e), generator=g)
+    s = ex.scores64(x[:1], scores)[0].view(groups, per)
+    h = size * (1 + torch.arange(groups).double() / 7)
+    bias = torch.full((groups, per), -4.0 * size, dtype=torch.float64)
+    bias[:, 0], bias[:, 1] = h - s[:, 0], -h - s[:, 1]
+    bias = bias.float()
+    choice = s + bias.double()
+    sums = choice.sort(1).values[:, -2:].sum(1)
+    gaps = sums.sort().values.diff()
+    assert gaps.max() < size * 2.0 ** -21 and gaps.min() > 1e-12  # within 32-bit rounding, and 64 bits tell them apart
+    # rows whose first group's sum stands a little above or below another's: by the first logit alone
+    for i in range(1, 60):
+        x[i] = x[0]
+        x[i, 0] += (i - 30) * size * 2.0 ** -22
+    for top in sorted({1, groups // 2}):
+        for k in (1, top * min(per, 2)):
+            check_routes(gpu, x, k, bias=bias.view(-1), scores=scores, groups=groups, top_groups=top)
+
+
+def test_group_borders_past_the_range(gpu):
+    """Sums of two finite choice scores that 32 bits do not hold, and masks of
+    -inf and of the lowest value."""
+    low = torch.finfo(torch.float32).min
+    x = torch.randn((9, 4), generator=gen(1))
+    for bias in ([-3.4e38, -3e38, -3.4e38, -1e38], [3.4e38, 1e38, 3.4e38, 3e38], [low, low, low, 0.0], [low, low, low, low],
+                 [low, 0.1, low, 0.2], [-math.inf, 0.0, 0.1, 0.2], [-math.inf, -math.inf, 0.1, 0.2],
+                 [-math.inf, 1.0, -math.inf, 2.0], [math.inf, -1.0, math.inf, -2.0]):
+        for scores in ("softmax", "sigmoid"):
+            for k in (1, 2):
+                check_route(gpu, x, k, bias=torch.tensor(bias), scores=scores, groups=2, top_groups=1, renormalize=False)

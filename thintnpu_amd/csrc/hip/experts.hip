@@ -64,11 +64,19 @@ __device__ __forceinline__ void scores32(const float (&x)[PER], const dev::Part<
 // How near two 32-bit choice scores may be before their order is settled in
 // 64 bits.  A score s <= 1 is off by less than 2^-22 (softmax: s |x - m| 2^-23
 // <= 0.37 * 2^-23 from the exponent's argument, 2^-23 from exp2 and the sum
-// each), the bias adds half a step of c: the two sides together stay below
-// 2^-20 + 2^-22 |c|.  A group's score adds two of them.
-__device__ __forceinline__ bool near_tie(float above, float below, float terms) {
-  return above - below <= terms * (0x1p-20f + 0x1p-22f * fabsf(above));
+// each), two of them by less than kSlack; the bias adds half a step of c on
+// either side, together 2^-23 |c|, which counts twice here.
+constexpr float kSlack = 0x1p-20f;
+__device__ __forceinline__ bool near_tie(float above, float below) {
+  return above - below <= kSlack + 0x1p-22f * fabsf(above);
 }
+// The same for a group's score, the mean of its two highest c, a and b: each
+// side is off by half of kSlack, by the half steps of a and b (2^-24 of their
+// mean size, however near the mean itself is to 0) and by its own (no more).  A
+// group stays clear of the border if it lies further than that from the middle
+// of the last kept and the first dropped score.  Infinities and NaN are exact in
+// either arithmetic, and near nothing.
+__device__ __forceinline__ float group_reach(float size) { return 0.5f * kSlack + 0x1p-22f * size; }
 
 // The best two keys of two sets.
 template <typename K>
@@ -80,15 +88,22 @@ template <int O>
 __device__ __forceinline__ void join_lane(uint32_t& best, uint32_t& second) {
   join_best(best, second, dev::lane_xor_bits<O>(best), dev::lane_xor_bits<O>(second));
 }
+// A group's score: with a bias the mean of its two highest, whose order is that
+// of the sum and which no finite scores take past the range.
 template <bool BIAS, typename K>
 __device__ __forceinline__ K group_score(K best, K second, int size) {
-  return BIAS && size > 1 ? dev::score_key(dev::key_score(best) + dev::key_score(second)) : best;
+  return BIAS && size > 1 ? dev::score_key(0.5f * dev::key_score(best) + 0.5f * dev::key_score(second)) : best;
+}
+// The mean size of what group_score() adds.
+__device__ __forceinline__ float group_size(uint32_t best, uint32_t second, int size) {
+  const float a = fabsf(dev::key_score(best));
+  return size > 1 ? 0.5f * a + 0.5f * fabsf(dev::key_score(second)) : a;
 }
 
 // Drops the keys of groups that are not among the `top` best, in 32 bits;
-// true if the last kept and the first dropped group are too near for that.
-// Where a group is a power of two of whole lanes, its score comes from
-// registers; any other size goes through LDS.
+// true in some lane if a group is too near the border for that.  Where a group
+// is a power of two of whole lanes, its score comes from registers; any other
+// size goes through LDS, where its size then takes the place of its first key.
 struct GroupLds {
   uint32_t key[kMaxGroups];
   uint32_t border[2];
@@ -99,6 +114,8 @@ __device__ __forceinline__ bool keep_groups(const RoutePlan& p, uint32_t (&key)[
   const uint32_t first = g * PER;
   const bool whole = p.group_lanes != 0;
   uint32_t own = 0;  // whole: the score of this lane's group
+  float own_size = 0.f;
+  bool near = false;
   if (whole) {
     uint32_t best = 0, second = 0;
 #pragma unroll
@@ -118,6 +135,7 @@ __device__ __forceinline__ bool keep_groups(const RoutePlan& p, uint32_t (&key)[
       if (p.group_lanes > 32) join_lane<32>(best, second);
     }
     own = group_score<BIAS>(best, second, p.size);
+    if constexpr (BIAS) own_size = group_size(best, second, p.size);
     if (first < p.count) lds.key[p.by_size.div(first)] = own;
   } else {
 #pragma unroll
@@ -132,6 +150,7 @@ __device__ __forceinline__ bool keep_groups(const RoutePlan& p, uint32_t (&key)[
         i = i + 1 == p.size ? 0 : i + 1;
       }
       lds.key[q] = group_score<BIAS>(best, second, p.size);
+      if constexpr (BIAS) staged[q * p.size] = __builtin_bit_cast(uint32_t, group_size(best, second, p.size));
     }
   }
   dev::wave_lds_fence();
@@ -146,11 +165,19 @@ __device__ __forceinline__ bool keep_groups(const RoutePlan& p, uint32_t (&key)[
     if (rank == p.top) lds.border[1] = mine;
     return rank;
   };
+  const auto near_border = [&](bool kept, uint32_t key, float size) {
+    const float middle = 0.5f * dev::key_score(lds.border[0]) + 0.5f * dev::key_score(lds.border[1]);
+    const float score = dev::key_score(key), reach = group_reach(size);
+    return kept ? score - reach < middle : score + reach > middle;
+  };
   if (whole) {
-    if (first < p.count && rank_of((int)p.by_size.div(first), own) >= p.top) {
+    const bool kept = first >= p.count || rank_of((int)p.by_size.div(first), own) < p.top;
+    if (!kept) {
 #pragma unroll
       for (int j = 0; j < PER; ++j) key[j] = 0;
     }
+    dev::wave_lds_fence();
+    if constexpr (BIAS) near = first < p.count && near_border(kept, own, own_size);
   } else {
     uint32_t kept[(kMaxGroups + G - 1) / G];
 #pragma unroll
@@ -160,15 +187,20 @@ __device__ __forceinline__ bool keep_groups(const RoutePlan& p, uint32_t (&key)[
     }
     dev::wave_lds_fence();
 #pragma unroll
-    for (int i = 0; i < (int)((kMaxGroups + G - 1) / G); ++i)
-      if ((int)g + i * G < p.groups) lds.key[g + i * G] = kept[i];
+    for (int i = 0; i < (int)((kMaxGroups + G - 1) / G); ++i) {
+      const int q = (int)g + i * G;
+      if (q >= p.groups) continue;
+      if constexpr (BIAS)
+        near = near || near_border(kept[i], lds.key[q], __builtin_bit_cast(float, staged[q * p.size]));
+      lds.key[q] = kept[i];
+    }
     dev::wave_lds_fence();
 #pragma unroll
     for (int j = 0; j < PER; ++j)
       if (!lds.key[p.by_size.div(min(part.from + j, p.count - 1))]) key[j] = 0;
   }
   dev::wave_lds_fence();
-  return BIAS && near_tie(dev::key_score(lds.border[0]), dev::key_score(lds.border[1]), 2.f);
+  return near;
 }
 
 // The choice of one token in 64 bits by a whole wavefront; rolled loops, as it
@@ -309,7 +341,7 @@ __global__ __launch_bounds__(kThreads) void route_kernel(RoutePlan p) {
   dev::wave_lds_fence();
   if constexpr (BIAS) {
     for (int i = (int)g; i < n - 1; i += G) {
-      if (!near_tie(choice[slot][i], choice[slot][i + 1], 1.f)) continue;
+      if (!near_tie(choice[slot][i], choice[slot][i + 1])) continue;
       const int32_t a = chosen[slot][i], b = chosen[slot][i + 1];
       close = close || (float)row[a] != (float)row[b] || p.bias[a * p.bias_step] != p.bias[b * p.bias_step];
     }

@@ -382,3 +382,22 @@ def test_group_borders_past_the_range(gpu):
         for scores in ("softmax", "sigmoid"):
             for k in (1, 2):
                 check_route(gpu, x, k, bias=torch.tensor(bias), scores=scores, groups=2, top_groups=1, renormalize=False)
+
+
+@pytest.mark.parametrize("e", [256, 300, 512, 1024])
+def test_softmax_sums_that_32_bits_lose(gpu, e):
+    """Terms that are each less than half a step of the sum that they join: the
+    total, and with it the first score, is off by their sum."""
+    x = torch.full((4, e), -200.0)
+    small = list(range(1, 16)) + [16, 32, 64, 128] + ([256] if e > 300 else []) + ([512] if e > 512 else [])
+    x[:, 0] = 0.0
+    x[:, small] = -16.66
+    x[1] = x[1].roll(3)
+    lost = len(small) * math.exp(-16.66)
+    for share in (0.5, 0.9, 0.97, 1.03):
+        bias = torch.full((e,), -5.0)
+        bias[0] = -1.0
+        bias[3] = -1.0
+        bias[200] = -lost * share
+        for k in (1, 2):
+            check_routes(gpu, x, k, bias=bias)

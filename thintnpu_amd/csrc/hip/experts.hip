@@ -62,21 +62,31 @@ __device__ __forceinline__ void scores32(const float (&x)[PER], const dev::Part<
   }
 }
 // How near two 32-bit choice scores may be before their order is settled in
-// 64 bits.  A score s <= 1 is off by less than 2^-22 (softmax: s |x - m| 2^-23
-// <= 0.37 * 2^-23 from the exponent's argument, 2^-23 from exp2 and the sum
-// each), two of them by less than kSlack; the bias adds half a step of c on
-// either side, together 2^-23 |c|, which counts twice here.
-constexpr float kSlack = 0x1p-20f;
-__device__ __forceinline__ bool near_tie(float above, float below) {
-  return above - below <= kSlack + 0x1p-22f * fabsf(above);
+// 64 bits: further apart than the scores' two errors (the slack) and the half
+// steps of c = s + bias on either side (2^-23 |c|, which counts twice here).
+//
+// Slack of two sigmoids: each is off by at most 2 * 2^-23 (0.23 from the
+// exponent's argument, as s (1 - s) |x| <= 0.23, 0.25 from exp2, 0.5 from the
+// sum, 1 from the reciprocal), so 2^-21; taken as 2^-20.
+// Slack of two softmax scores s = e / total, in units of u = 2^-24 and of the
+// row's highest score 1 / total.  With y = m - x, each e is off by (2.25 y + 2) u
+// and its product by u, and s y <= 0.37 / total: 8 for two of them.  What the
+// total is off by moves both alike, and their difference by no more than the
+// highest score times it: 2 for the reciprocal, 2 + 2.25 * 4.5 for the terms
+// (the mean of y, weighted by s, is at most 4.5 for 1024 experts), and 15 sums in
+// a lane and 6 joins, each of which may lose half a step of the whole: 21.  That
+// makes 44; taken as 48.
+__device__ __forceinline__ float slack_of(bool softmax, float total) { return softmax ? 0x1.8p-19f / total : 0x1p-20f; }
+__device__ __forceinline__ bool near_tie(float above, float below, float slack) {
+  return above - below <= slack + 0x1p-22f * fabsf(above);
 }
-// The same for a group's score, the mean of its two highest c, a and b: each
-// side is off by half of kSlack, by the half steps of a and b (2^-24 of their
-// mean size, however near the mean itself is to 0) and by its own (no more).  A
-// group stays clear of the border if it lies further than that from the middle
-// of the last kept and the first dropped score.  Infinities and NaN are exact in
-// either arithmetic, and near nothing.
-__device__ __forceinline__ float group_reach(float size) { return 0.5f * kSlack + 0x1p-22f * size; }
+// The same for a group's score, the mean of its two highest c, a and b: two
+// groups together are off by the slack, each by the half steps of its a and b
+// (2^-24 of their mean size, however near the mean itself is to 0) and of its own
+// (no more; the two count twice here).  A group stays clear of the border if it
+// lies further than that from the middle of the last kept and the first dropped
+// score.  Infinities and NaN are exact in either arithmetic, and near nothing.
+__device__ __forceinline__ float group_reach(float size, float slack) { return 0.5f * slack + 0x1p-22f * size; }
 
 // The best two keys of two sets.
 template <typename K>
@@ -110,7 +120,7 @@ struct GroupLds {
 };
 template <int G, int PER, bool BIAS>
 __device__ __forceinline__ bool keep_groups(const RoutePlan& p, uint32_t (&key)[PER], const dev::Part<PER, false>& part,
-                                            uint32_t g, uint32_t* staged, GroupLds& lds) {
+                                            uint32_t g, float slack, uint32_t* staged, GroupLds& lds) {
   const uint32_t first = g * PER;
   const bool whole = p.group_lanes != 0;
   uint32_t own = 0;  // whole: the score of this lane's group
@@ -167,7 +177,7 @@ __device__ __forceinline__ bool keep_groups(const RoutePlan& p, uint32_t (&key)[
   };
   const auto near_border = [&](bool kept, uint32_t key, float size) {
     const float middle = 0.5f * dev::key_score(lds.border[0]) + 0.5f * dev::key_score(lds.border[1]);
-    const float score = dev::key_score(key), reach = group_reach(size);
+    const float score = dev::key_score(key), reach = group_reach(size, slack);
     return kept ? score - reach < middle : score + reach > middle;
   };
   if (whole) {
@@ -325,9 +335,11 @@ __global__ __launch_bounds__(kThreads) void route_kernel(RoutePlan p) {
       else key[j] = part.own(j) ? dev::score_key(x[j]) : 0u;
     }
   }
+  const float slack = slack_of(p.softmax, total);
   bool close = false;
   if constexpr (GROUPED)
-    close = keep_groups<G, PER, BIAS>(p, key, part, g, reinterpret_cast<uint32_t*>(staged) + slot % (64 / G) * p.count, groups[slot]);
+    close = keep_groups<G, PER, BIAS>(p, key, part, g, slack,
+                                      reinterpret_cast<uint32_t*>(staged) + slot % (64 / G) * p.count, groups[slot]);
   const int open = GROUPED ? p.top * p.size : (int)p.count;
   const int n = BIAS && p.k < open ? p.k + 1 : p.k;
   if constexpr (kPlaces) {
@@ -341,7 +353,7 @@ __global__ __launch_bounds__(kThreads) void route_kernel(RoutePlan p) {
   dev::wave_lds_fence();
   if constexpr (BIAS) {
     for (int i = (int)g; i < n - 1; i += G) {
-      if (!near_tie(choice[slot][i], choice[slot][i + 1])) continue;
+      if (!near_tie(choice[slot][i], choice[slot][i + 1], slack)) continue;
       const int32_t a = chosen[slot][i], b = chosen[slot][i + 1];
       close = close || (float)row[a] != (float)row[b] || p.bias[a * p.bias_step] != p.bias[b * p.bias_step];
     }

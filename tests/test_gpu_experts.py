@@ -401,3 +401,20 @@ def test_softmax_sums_that_32_bits_lose(gpu, e):
         bias[200] = -lost * share
         for k in (1, 2):
             check_routes(gpu, x, k, bias=bias)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("e", [3, 16, 60, 256, 700])
+def test_sigmoid_weights_of_very_negative_logits(gpu, e, dtype):
+    """Sigmoids below the smallest fp32 number, whose quotients are not."""
+    g = gen(e)
+    x = (-85 - 215 * torch.rand((12, e), generator=g)).to(TYPES[dtype])
+    x[1] = (-60 - 60 * torch.rand(e, generator=g)).to(x.dtype)
+    x[2] = -100
+    x[3] = torch.linspace(-95, -1, e).to(x.dtype)
+    x[4, 1:] = -math.inf
+    x[5] = (torch.randn(e, generator=g) - 1.5).to(x.dtype)
+    x[6, 0] = 3.0
+    for k in sorted({1, min(e, 8)}):
+        check_routes(gpu, x, k, scores="sigmoid", scale=2.5)
+        check_routes(gpu, x, k, bias=torch.rand(e, generator=gen(k)) + 0.5, scores="sigmoid")

@@ -382,15 +382,40 @@ __global__ __launch_bounds__(kThreads) void route_kernel(RoutePlan p) {
     }
     top = dev::group_max<G>(top);
   }
-  const auto score = [&](float v) { return p.softmax ? expf(v - top) : 1.0f / (1.0f + expf(-v)); };
+  bool low = false;
+  const auto score = [&](float v) {
+    if (low) return expf(v - top) / (1.0f + expf(v));
+    return p.softmax ? expf(v - top) : 1.0f / (1.0f + expf(-v));
+  };
   // (one weight a lane in most calls: kept for the second use)
   float mine = 0.f, sum = 0.f;
   if ((int)g < p.k) mine = score((float)row[chosen[slot][g]]);
   if (p.renormalize) {
-    sum = mine;
+    const auto add_scores = [&]() {
+      float s = mine;
 #pragma unroll 1
-    for (int i = (int)g + G; i < p.k; i += G) sum += score((float)row[chosen[slot][i]]);
-    sum = dev::group_sum<G>(sum);
+      for (int i = (int)g + G; i < p.k; i += G) s += score((float)row[chosen[slot][i]]);
+      return dev::group_sum<G>(s);
+    };
+    sum = add_scores();
+    // Logits below -86 leave less and less of 1 / (1 + e^-v) in 32 bits, which
+    // matters where no sigmoid reaches 1/2: there the terms are
+    // e^(v - top) / (1 + e^v), top being the highest chosen logit, whose
+    // exponential cancels.
+    if (!p.softmax && __any(sum < 0.5f)) {
+      bool lost = false;
+      for (int i = (int)g; i < p.k; i += G) {
+        const float v = (float)row[chosen[slot][i]];
+        lost = lost || v < -86.f;
+        top = fmaxf(top, v);
+      }
+      low = sum < 0.5f && dev::group_ballot<G>(lost) != 0;  // the same for the lanes of a token
+      if (__any(low)) {
+        top = dev::group_max<G>(top);
+        if ((int)g < p.k) mine = score((float)row[chosen[slot][g]]);
+        sum = add_scores();
+      }
+    }
     if (BIAS && p.softmax && total != total) sum = total;  // a NaN anywhere is in every score of the row
   } else if (p.softmax) {
 #pragma unroll

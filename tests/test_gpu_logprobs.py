@@ -206,3 +206,28 @@ def test_same_bits_and_captured(gpu, v):
         torch.cuda.synchronize()
         for v_, out in zip(xs, outs):
             assert all(torch.equal(a, b) for a, b in zip(out, capi.token_logprobs(v_, tokens, 6)))
+
+
+def _steps_lost(low, high, count, seed):
+    """fp32 numbers m whose m log2(e) is off by low to high in its 32-bit rounding."""
+    m = torch.rand(1 << 20, generator=gen(seed)).add(1.0).mul(2.0 ** 30).float()
+    product = m.double() * float(torch.tensor(1.4426950408889634, dtype=torch.float32))
+    off = product - (m * 1.4426950408889634).double()
+    return m[(off > low) & (off < high)][:count].tolist()
+
+
+@pytest.mark.parametrize("v", [40, 900, 3000, 9000])
+def test_large_maxima(gpu, v):
+    """Maxima far from zero, where m log2(e) loses more than the exponent's range."""
+    lost = _steps_lost(-128, -126, 3, 1) + _steps_lost(126, 128, 3, 2) + _steps_lost(60, 64, 2, 3)
+    assert len(lost) == 8 and min(lost) > 1e9
+    peaks = [1601153152.0, *lost, *(1.3 * 2.0 ** e for e in range(8, 126, 6))]
+    peaks += [-p for p in peaks if p < 1e28]
+    x = torch.empty((len(peaks), v))
+    for i, m in enumerate(peaks):
+        x[i] = m - abs(m) * torch.rand(v, generator=gen(i))
+        x[i, i % v], x[i, (7 * i + 5) % v], x[i, v - 1 - i % 3] = m, m, m
+        x[i, 9] = m * (1 - 2.0 ** -22 if m > 0 else 1 + 2.0 ** -22)
+    tokens = torch.tensor([(i % v, 9, 11)[i % 3] for i in range(len(peaks))])
+    for dtype in (torch.float32, torch.bfloat16):
+        check(gpu, x.to(dtype), tokens, 9)

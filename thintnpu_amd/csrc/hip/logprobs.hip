@@ -7,7 +7,8 @@
 //   log p(x) = (x - m) - log2(s) ln 2,    entropy = (log2 s - u / s) ln 2,
 // in which no term is larger than the result's own range.  y is one fma against
 // M = fl(m L), whose rounding d = m L - M is taken back from the sums:
-// s 2^-d and (u - d s) 2^-d.
+// s 2^-d and (u - d s) 2^-d.  That holds while d is small (plain_range()); larger
+// maxima take x - m first.
 #include "rows.h"
 
 #include <string.h>
@@ -49,9 +50,10 @@ struct RowSums {
   float m, s, u;
 };
 
-// s and u of the elements against their maximum m.  The plain form needs
-// finite logits (-inf weighs nothing but would leave 0 * -inf in u) whose
-// products with L are finite too; the careful one takes every value.
+// s and u of the elements against their maximum m.  The plain form needs a
+// maximum in plain_range() and finite logits (-inf weighs nothing but would leave
+// 0 * -inf in u) whose products with L are finite too; the careful one takes
+// every value.
 template <bool CAREFUL>
 __device__ __forceinline__ void add_element(RowSums& r, float x, float top, float base) {
   const float y = CAREFUL ? (x - top) * kLog2e : __builtin_fmaf(x, kLog2e, -base);
@@ -76,7 +78,9 @@ __device__ __forceinline__ void take_back_rounding(RowSums& r) {
   r.u = __builtin_fmaf(-d, r.s, r.u) * f;
   r.s *= f;
 }
-__device__ __forceinline__ bool plain_range(float m) { return fabsf(m) < 1e38f; }
+// |d| <= 2^-4 (from about 2^30 on it passes the exponent's range, and sums and
+// their factor of 0 and infinity would meet).
+__device__ __forceinline__ bool plain_range(float m) { return fabsf(m) < 0x1p20f; }
 
 __device__ __forceinline__ float rest_of(const RowSums& r) { return __builtin_log2f(r.s) * kLn2; }
 // The given token's logit, loaded ahead of what store_row() waits for.

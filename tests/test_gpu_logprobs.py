@@ -231,3 +231,23 @@ def test_large_maxima(gpu, v):
     tokens = torch.tensor([(i % v, 9, 11)[i % 3] for i in range(len(peaks))])
     for dtype in (torch.float32, torch.bfloat16):
         check(gpu, x.to(dtype), tokens, 9)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("v", [700, 1100, 5000, 9001])
+def test_low_masks(gpu, v, dtype):
+    """Masked logits of any finite size: no run that the row ends in stands above another."""
+    edge = 2.3586574e38  # about the largest whose product with log2(e) is finite
+    base = torch.zeros((12, v + 8), dtype=TYPES[dtype])
+    for i, low in enumerate((-1e28, -9e29, -1e30, -1.01e30, -1e31, -1e35, -2e38, -edge * 0.999, -edge, -edge * 1.001, -3e38, -3.38e38)):
+        base[i] = low
+    tokens = torch.arange(12)
+    dev = base.to(gpu)
+    for skew in (0, 3):
+        x, view = base[:, skew:skew + v], dev[:, skew:skew + v]
+        x[:, 100] = view[:, 100] = 0.5
+        x[:, v - 600] = view[:, v - 600] = -0.25
+        for top in (3, 32):
+            check(gpu, x, tokens, top, view=view)
+        x[:, v // 2] = view[:, v // 2] = -math.inf
+        check(gpu, x, tokens, 5, view=view)

@@ -104,11 +104,15 @@ __device__ __forceinline__ void store_alternative(const LogprobsPlan& p, uint32_
   p.top_ids[(int64_t)row * p.ir + i * p.ik] = (int64_t)id;
 }
 
-// What stands in the place of elements that a row does not have: finite, and of
-// weight 0 next to any maximum above kLowest (an -inf would leave 0 * -inf).
-template <typename T> constexpr float kAbsent = -1e30f;
+// What stands in the place of elements that a row does not have: finite (an -inf
+// would leave 0 * -inf), of weight 0 next to any maximum above kLowest, and the
+// lowest value whose product with L is finite.  A lower element leaves a NaN in
+// u, for which a tile is summed again without what stands in; so where it stays,
+// it raises no run's maximum above that of the run's own elements.
+template <typename T> constexpr float kAbsent = -0x1.62e42ep127f;
+template <> constexpr float kAbsent<__bf16> = -0x1.62p127f;
 template <> constexpr float kAbsent<_Float16> = -65504.f;
-template <typename T> constexpr float kLowest = -1e29f;
+template <typename T> constexpr float kLowest = -0x1p20f;
 template <> constexpr float kLowest<_Float16> = -65000.f;
 
 // ---------------------------------------------------------------- short rows

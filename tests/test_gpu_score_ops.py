@@ -154,3 +154,47 @@ def test_expert_head(gpu):
     assert torch.equal(got[3].cpu(), want[3])
     for a, b in zip(got[:3], want[:3]):
         torch.testing.assert_close(a.cpu().double(), b, rtol=200 * U, atol=400 * U)
+
+
+@pytest.mark.parametrize("raw", [False, True])
+def test_calls_on_another_stream(gpu, raw):
+    """Outputs and workspaces of a call on another stream are not blocks that the
+    caller's stream still writes, and the outputs are not handed out again while
+    it reads them."""
+    from thintnpu_amd import capi
+    g = gen(3)
+    x = torch.randn((1, 160, 160, 64), generator=g).half().to(gpu)
+    logits, rows = torch.randn((3000, 64), generator=g).to(gpu), torch.randn((3000, 40), generator=g).half().to(gpu)
+    ids, weights = torch.randint(0, 64, (3000, 4), generator=g).int().to(gpu), torch.rand((3000, 4), generator=g).to(gpu)
+    wide, tokens = torch.randn((40, 9000), generator=g).to(gpu), torch.randint(0, 9000, (40,), generator=g).to(gpu)
+    moved, _, slots = capi.expert_dispatch(rows, ids, 64)
+    calls = [lambda s: (capi.group_norm(x, 8, silu=True, stream=s),),
+             lambda s: (capi.group_norm_nc1hwc0(x.view(1, 4, 160, 160, 16), 4, stream=s),),
+             lambda s: capi.expert_route(logits, 4, groups=8, top_groups=3, stream=s),
+             lambda s: capi.expert_dispatch(rows, ids, 64, stream=s),
+             lambda s: (capi.expert_combine(moved, weights, slots, stream=s),),
+             lambda s: capi.token_logprobs(wide, tokens, 5, stream=s)]
+    busy = torch.zeros(1 << 28, device=gpu)
+    side = torch.cuda.Stream()
+    stream = side.cuda_stream if raw else side
+    for call in calls:
+        ref = [t.clone() for t in call(None)]
+        torch.cuda.synchronize()
+        for _ in range(20):
+            busy.add_(1)  # the caller's stream is some milliseconds behind
+        blocks = [torch.empty_like(t) for t in ref] + [torch.empty(1 << n, dtype=torch.uint8, device=gpu) for n in range(9, 21)]
+        for b in blocks:
+            b.fill_(77)
+        del b, blocks
+        got = call(stream)
+        side.synchronize()
+        kept = [t.clone() for t in got]
+        del got
+        again = call(stream)
+        torch.cuda.synchronize()
+        for a, b, c in zip(ref, kept, again):
+            assert torch.equal(a, b) and torch.equal(a, c)
+    out = torch.empty_like(x)
+    assert capi.group_norm(x, 8, silu=True, out=out, stream=stream) is out
+    side.synchronize()
+    assert torch.equal(out, calls[0](None)[0])

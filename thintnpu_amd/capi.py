@@ -10,6 +10,7 @@ libamdhip64.so.7).  A missing library raises: there is no CPU fallback.
 from __future__ import annotations
 
 import ctypes
+import functools
 import os
 import struct
 from pathlib import Path
@@ -483,11 +484,10 @@ def _rows(like: torch.Tensor, rows: int, width: int, dtype):
     return torch.empty_strided((rows, width), (max(width, 1), 1), dtype=dtype, device=like.device)
 
 
-def _workspace(nbytes: int, given, device: int, stream):
+def _workspace(nbytes: int, given, device: int):
     """(tensor, address, bytes) of a call's workspace: the given tensor, or one
     of torch's allocator, which gets it back at the end of the wrapper and hands
-    it out again in the order of the stream that it was allocated on; a call on
-    another stream is recorded so that it is not handed out before that ends."""
+    it out again in the order of the current stream."""
     if given is not None:
         if given.get_device() != device or not given.is_contiguous():
             raise ValueError("the workspace must be contiguous and on the operands' device")
@@ -495,23 +495,41 @@ def _workspace(nbytes: int, given, device: int, stream):
     if nbytes == 0:
         return None, None, 0
     ws = torch.empty(nbytes, dtype=torch.uint8, device=torch.device("cuda", device))
-    if stream is not None:
-        ws.record_stream(stream if isinstance(stream, torch.cuda.Stream) else torch.cuda.ExternalStream(stream))
     return ws, ws.data_ptr(), nbytes
 
 
-def _group_norm(x, blocked, channels, groups, weight, bias, eps, silu, out, workspace, stream):
+def _elsewhere(stream, out, call, *args):
+    """call(*args, out=out) with `stream` (a Stream or a raw handle) current, so
+    that what it allocates is memory in the order of that stream: a block of the
+    caller's own may have work of the caller's pending.  New outputs are recorded
+    for the caller's stream, so that they outlive what it does with them."""
+    device = _current_device(args[0])
+    other = stream if isinstance(stream, torch.cuda.Stream) else torch.cuda.ExternalStream(stream)
+    if other.device_index != device:
+        raise ValueError(f"operands on cuda:{device} and a stream of cuda:{other.device_index}")
+    caller = torch.cuda.current_stream()
+    with torch.cuda.stream(other):
+        result = call(*args, out=out)
+    if out is None:
+        for t in (result,) if isinstance(result, torch.Tensor) else result:
+            t.record_stream(caller)
+    return result
+
+
+def _group_norm(x, blocked, channels, groups, weight, bias, eps, silu, workspace, stream=None, out=None):
+    if stream is not None:
+        return _elsewhere(stream, out, _group_norm, x, blocked, channels, groups, weight, bias, eps, silu, workspace)
     device = _current_device(x)
     if out is None:
         out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
     L = lib()
     xd, od = _packed(x), _on(device, out)
     need = L.thin_group_norm_workspace(xd, od, blocked, channels, groups)
-    ws, address, nbytes = _workspace(need, workspace, device, stream)
+    ws, address, nbytes = _workspace(need, workspace, device)
     _check("thin_group_norm", L.thin_group_norm(
         xd, blocked, channels, groups, None if weight is None else _on(device, weight),
         None if bias is None else _on(device, bias), eps, 1 if silu else 0, od, address, nbytes,
-        _stream(stream)))
+        _stream(None)))
     return out
 
 
@@ -521,7 +539,7 @@ def group_norm(x, groups: int, weight=None, bias=None, eps: float = 1e-5, silu: 
     after it if silu; weight and bias [C] of x's type or fp32.  out may be x."""
     if x.dim() < 2:
         raise ValueError("group_norm takes x [N, ..., C]")
-    return _group_norm(x, 0, x.shape[-1], groups, weight, bias, eps, silu, out, workspace, stream)
+    return _group_norm(x, 0, x.shape[-1], groups, weight, bias, eps, silu, workspace, stream, out)
 
 
 def group_norm_nc1hwc0(x, groups: int, weight=None, bias=None, eps: float = 1e-5, silu: bool = False,
@@ -531,7 +549,7 @@ def group_norm_nc1hwc0(x, groups: int, weight=None, bias=None, eps: float = 1e-5
     if x.dim() != 5:
         raise ValueError("group_norm_nc1hwc0 takes x [N, C1, H, W, 16]")
     channels = x.shape[1] * 16 if channels is None else channels
-    return _group_norm(x, 1, channels, groups, weight, bias, eps, silu, out, workspace, stream)
+    return _group_norm(x, 1, channels, groups, weight, bias, eps, silu, workspace, stream, out)
 
 
 def expert_route(logits, top_k: int, bias=None, scores: str = "softmax", groups: int = 1, top_groups: int = 1,
@@ -541,6 +559,8 @@ def expert_route(logits, top_k: int, bias=None, scores: str = "softmax", groups:
     of `groups` runs of experts, weighted by their scores without the bias."""
     if scores not in ("softmax", "sigmoid"):
         raise ValueError(f"scores are softmax or sigmoid, not {scores!r}")
+    if stream is not None:
+        return _elsewhere(stream, out, expert_route, logits, top_k, bias, scores, groups, top_groups, renormalize, scale)
     device = _current_device(logits)
     if out is None:
         t = logits.shape[0]
@@ -548,7 +568,7 @@ def expert_route(logits, top_k: int, bias=None, scores: str = "softmax", groups:
     weights, experts = out
     _check("thin_expert_route", lib().thin_expert_route(
         _packed(logits), None if bias is None else _on(device, bias), 1 if scores == "softmax" else 0, groups,
-        top_groups, 1 if renormalize else 0, scale, _on(device, weights), _on(device, experts), _stream(stream)))
+        top_groups, 1 if renormalize else 0, scale, _on(device, weights), _on(device, experts), _stream(None)))
     return weights, experts
 
 
@@ -556,6 +576,8 @@ def expert_dispatch(x, experts, num_experts: int, out=None, workspace=None, stre
     """(rows [T * k, width], offsets int32 [num_experts + 1], slots int32 [T, k]):
     x's rows in the order (expert, token), where each expert's begin, and where
     each assignment went (-1: no expert)."""
+    if stream is not None:
+        return _elsewhere(stream, out, functools.partial(expert_dispatch, workspace=workspace), x, experts, num_experts)
     device = _current_device(x)
     t, k = experts.shape
     if out is None:
@@ -564,26 +586,30 @@ def expert_dispatch(x, experts, num_experts: int, out=None, workspace=None, stre
                _rows(x, t, k, torch.int32))
     rows, offsets, slots = out
     L = lib()
-    ws, address, nbytes = _workspace(L.thin_expert_dispatch_workspace(t, k, num_experts), workspace, device, stream)
+    ws, address, nbytes = _workspace(L.thin_expert_dispatch_workspace(t, k, num_experts), workspace, device)
     _check("thin_expert_dispatch", L.thin_expert_dispatch(
         _packed(x), _on(device, experts), num_experts, _on(device, rows), _on(device, offsets), _on(device, slots),
-        address, nbytes, _stream(stream)))
+        address, nbytes, _stream(None)))
     return rows, offsets, slots
 
 
 def expert_combine(y, weights, slots, out=None, stream=None):
     """out[t] = sum_j weights[t, j] * y[slots[t, j]] (fp32, one rounding)."""
+    if stream is not None:
+        return _elsewhere(stream, out, expert_combine, y, weights, slots)
     device = _current_device(y)
     if out is None:
         out = _rows(y, slots.shape[0], y.shape[1], y.dtype)
     _check("thin_expert_combine", lib().thin_expert_combine(
-        _packed(y), _on(device, weights), _on(device, slots), _on(device, out), _stream(stream)))
+        _packed(y), _on(device, weights), _on(device, slots), _on(device, out), _stream(None)))
     return out
 
 
 def token_logprobs(logits, tokens, top: int = 0, out=None, workspace=None, stream=None):
     """(logprobs [R], entropy [R], top_logprobs [R, top], top_ids int64 [R, top])
     of logits [R, V] and int64 tokens [R]; a token outside [0, V) gives NaN."""
+    if stream is not None:
+        return _elsewhere(stream, out, functools.partial(token_logprobs, workspace=workspace), logits, tokens, top)
     device = _current_device(logits)
     r, width = logits.shape
     if out is None:
@@ -593,9 +619,8 @@ def token_logprobs(logits, tokens, top: int = 0, out=None, workspace=None, strea
                _rows(logits, r, top, torch.float32), _rows(logits, r, top, torch.int64))
     logprobs, entropy, top_logprobs, top_ids = out
     L = lib()
-    ws, address, nbytes = _workspace(L.thin_token_logprobs_workspace(r, width, top_ids.shape[1]), workspace, device,
-                                     stream)
+    ws, address, nbytes = _workspace(L.thin_token_logprobs_workspace(r, width, top_ids.shape[1]), workspace, device)
     _check("thin_token_logprobs", L.thin_token_logprobs(
         _packed(logits), _on(device, tokens), _on(device, logprobs), _on(device, entropy), _on(device, top_logprobs),
-        _on(device, top_ids), address, nbytes, _stream(stream)))
+        _on(device, top_ids), address, nbytes, _stream(None)))
     return out

@@ -14,7 +14,9 @@ constexpr int64_t kMaxExperts = 1024;
 constexpr int64_t kMaxChosen = 32;
 constexpr int64_t kMaxGroups = 64;
 // Tokens up to which each has a whole wavefront: with few of them the latency of
-// one counts (48 tokens of 256 experts: 5.7 us, by 16 lanes a token 13).
+// one counts (256 bf16 logits, bias and groups: 16 tokens 5.2 us against 7.4 by 16
+// lanes a token, 1024 9.2 against 11.1, 4096 14.8 against 15.0; fp16 without a
+// bias: 1024 3.8 against 4.2, 2048 4.2 against 4.3, 4096 5.4 against 4.3).
 constexpr int64_t kFewTokens = 1024;
 
 // ---------------------------------------------------------------- routing
@@ -214,7 +216,9 @@ __device__ __forceinline__ bool keep_groups(const RoutePlan& p, uint32_t (&key)[
 }
 
 // The choice of one token in 64 bits by a whole wavefront; rolled loops, as it
-// is rare (a few tokens in a thousand of 256 experts).
+// is rare (a few tokens in a thousand of 256 experts).  Rows that all need it cost
+// more: 16384 tokens of 256 experts whose groups tie 64 us, where others take 21,
+// and peaked softmax rows with a bias of zeros 38, where flatter ones take 20.
 struct WideLds {
   uint64_t group_key[kMaxGroups];
   uint32_t kept[kMaxGroups];
@@ -288,12 +292,13 @@ __device__ __forceinline__ void choose64(const RoutePlan& p, const T* row, uint6
 //
 // The logits are read once, at the start; what bounds the kernel is the issue of
 // instructions, not their bytes.  16384 tokens of 256 fp32 logits, 8 of them out
-// of 4 of 8 groups: 21 us (0.85 TB/s; 1400 VALU instructions a wave of 4 tokens;
-// of 25k cycles the loads take 3.5k, the scores 5.5k, the groups 3.4k and the
-// selection 10.7k).  51200 tokens of 60 fp16 logits, 4 of them: 7.8 us.  Hence the
-// shape: as few lanes a token as hold its logits 4 to 16 each, so that a wave's
-// reductions serve several tokens, and keys that are whole numbers, so that a
-// maximum is one instruction and needs no second one for its place.
+// of 4 of 8 groups: 21 us (0.85 TB/s; 1480 VALU instructions a wave of 4 tokens;
+// of 25k cycles the loads take 3.5k, the scores 5.5k, the groups 3.4k, without the
+// 80 instructions of their reach, and the selection 10.7k).  51200 tokens of 60
+// fp16 logits, 4 of them: 7.8 us.  Hence the shape: as few lanes a token as hold
+// its logits 4 to 16 each, so that a wave's reductions serve several tokens, and
+// keys that are whole numbers, so that a maximum is one instruction and needs no
+// second one for its place.
 template <typename T, int G, int PER, bool BIAS, bool GROUPED>
 __global__ __launch_bounds__(kThreads) void route_kernel(RoutePlan p) {
   constexpr int kTokens = kThreads / G;
@@ -517,7 +522,10 @@ __device__ __forceinline__ void copy_row(const RowsPlan& p, uint32_t t, uint32_t
 // latency: the ids' load, a pass over them in LDS and the row's own load and
 // stores one after another (48 tokens of 4096 bf16, 8 experts each: 6.3 us for
 // 3.5 MB, where counting, planning and copying in launches of their own would
-// cost three times the launch alone).
+// cost three times the launch alone).  Up to 4096 assignments: to 256 experts 128
+// of them take 4.9 us against 9.6 in three launches, 2048 10.0 against 12.7, 4096
+// 16.1 against 14.1.  To 1024 experts the offsets, a sum of its own for each, take
+// 24 us of one block whatever the assignments, three launches 11 to 16.
 constexpr uint32_t kCountedAssignments = 4096;
 __global__ __launch_bounds__(kThreads) void dispatch_small_kernel(RowsPlan p) {
   constexpr int kWaves = kThreads / 64, kAtOnce = 8;

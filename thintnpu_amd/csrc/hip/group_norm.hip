@@ -20,10 +20,12 @@ namespace {
 
 constexpr uint32_t kThreads = 256;
 // One launch with fewer than kFillingTiles workgroups only where each holds few
-// vectors: in the blocked layout, whose tiles are runs of memory, 8192 (one
-// [128,80,80] frame 10.8 us a call against 13.9 in two launches), else 2048
-// (recorded into a graph, the same frame channels last 12.8 us against 11.3, two
-// of them 17.6 against 11.6).
+// vectors: in the blocked layout, whose tiles are runs of memory, 8192 (frames of
+// 128 channels in 32 groups, recorded into a graph: [64,64] 8.4 us against 9.9 in
+// two launches, [80,80] 9.9 against 10.0, [100,100] 13.2 against 11.0; a call of
+// its own [80,80] 10.8 against 13.9), else 2048 (channels last: [40,40] 7.2 against
+// 10.6, [64,64] 9.7 against 10.7, [80,80] 12.2 against 11.2, two of them 17.5
+// against 11.6).
 constexpr int64_t kFillingTiles = 128;
 constexpr int64_t kFewVectors = 2048, kFewBlockedVectors = 8192;
 constexpr int64_t kHeldVectors = 16384;  // 16-byte vectors that 1024 threads hold, 16 each
@@ -208,8 +210,8 @@ __device__ __forceinline__ Joined join_threads(const NormPlan& p, const Place& a
 // 32 samples of [80,80,128] fp16 in 32 groups with SiLU, 105 MB: 26.5 us (4 TB/s;
 // blocked 24.5).  One workgroup of 16 waves fills a CU's registers, so that its
 // phases do not overlap: 9.6 us of loads (5.4 TB/s), 2 of joins, 8 of SiLU and
-// stores, the rest of ramps.  A single blocked frame: 11.4 us by 16 workgroups,
-// each bound by its own CU's loads.
+// stores, the rest of ramps.  A single blocked frame: 11.4 us by 16 workgroups, 9.9
+// where launches follow each other, each bound by its own CU's loads.
 template <typename T, int SEG, int THREADS, int H>
 __global__ __launch_bounds__(THREADS) void norm_held_kernel(NormPlan p) {
   constexpr int V = 16 / sizeof(T), W = V / SEG;

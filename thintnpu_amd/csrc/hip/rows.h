@@ -92,7 +92,7 @@ __device__ __forceinline__ void store_pack(T* p, const float (&v)[N]) {
 // Lane g's part of a row of n elements, PER each: the row's [g * PER, (g + 1) *
 // PER), loaded from `from` on.  The last part is moved back to end with the row;
 // its first `skip` elements are another lane's.  So every lane makes one wide
-// load under no condition (200000 rows of 1000 bf16: 94 us, 146 with the ragged
+// load under no condition (200000 rows of 1000 bf16: 97 us, 146 with the ragged
 // lane's elements loaded one by one).
 // SHORT: the row may have fewer than PER elements.
 template <int PER, bool SHORT>

@@ -198,3 +198,34 @@ def test_calls_on_another_stream(gpu, raw):
     assert capi.group_norm(x, 8, silu=True, out=out, stream=stream) is out
     side.synchronize()
     assert torch.equal(out, calls[0](None)[0])
+
+
+def test_streams_of_any_kind(gpu):
+    """The default stream's null handle, a c_void_p, and a stream that a capture
+    takes in, with replays."""
+    import ctypes
+
+    from thintnpu_amd import capi
+    x = torch.randn((1, 160, 160, 64), generator=gen(5)).half().to(gpu)
+    logits = torch.randn((40, 9000), generator=gen(6)).to(gpu)
+    tokens = torch.arange(40, device=gpu)
+    side = torch.cuda.Stream()
+    ref = capi.group_norm(x, 8), *capi.token_logprobs(logits, tokens, 3)
+    torch.cuda.synchronize()
+    for stream in (0, ctypes.c_void_p(None), ctypes.c_void_p(side.cuda_stream), torch.cuda.current_stream(),
+                   torch.cuda.default_stream()):
+        got = capi.group_norm(x, 8, stream=stream), *capi.token_logprobs(logits, tokens, 3, stream=stream)
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, ref))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        side.wait_stream(torch.cuda.current_stream())
+        out = capi.group_norm(x, 8, stream=side), *capi.token_logprobs(logits, tokens, 3, stream=side)
+        torch.cuda.current_stream().wait_stream(side)
+    for step in range(3):
+        x.copy_(torch.randn(x.shape, generator=gen(step)).half())
+        logits.copy_(torch.randn(logits.shape, generator=gen(10 + step)))
+        graph.replay()
+        torch.cuda.synchronize()
+        ref = capi.group_norm(x, 8), *capi.token_logprobs(logits, tokens, 3)
+        assert all(torch.equal(a, b) for a, b in zip(out, ref))

@@ -499,12 +499,14 @@ def _workspace(nbytes: int, given, device: int):
 
 
 def _elsewhere(stream, out, call, *args):
-    """call(*args, out=out) with `stream` (a Stream or a raw handle) current, so
+    """call(*args, out=out) with `stream` (a Stream or a handle) current, so
     that what it allocates is memory in the order of that stream: a block of the
     caller's own may have work of the caller's pending.  New outputs are recorded
     for the caller's stream, so that they outlive what it does with them."""
     device = _current_device(args[0])
-    other = stream if isinstance(stream, torch.cuda.Stream) else torch.cuda.ExternalStream(stream)
+    handle = getattr(stream, "cuda_stream", stream)
+    handle = getattr(handle, "value", handle) or 0  # of a c_void_p; null is the default stream
+    other = stream if isinstance(stream, torch.cuda.Stream) else torch.cuda.ExternalStream(handle)
     if other.device_index != device:
         raise ValueError(f"operands on cuda:{device} and a stream of cuda:{other.device_index}")
     caller = torch.cuda.current_stream()

@@ -462,6 +462,129 @@ thin_status thin_token_logprobs(const thin_desc* logits, const thin_desc* tokens
                                 const thin_desc* entropy, const thin_desc* top_logprobs, const thin_desc* top_ids,
                                 void* workspace, size_t workspace_bytes, hipStream_t stream);
 
+/* ------------------------------------------------------------------ */
+/* Rotary positions                                                    */
+/* ------------------------------------------------------------------ */
+
+/* Turns the pairs of each head of q [B, T, H, D] and, unless both are NULL, of
+ * k [B, T, Hk, D] (fp16, bf16 or fp32, a head's dims adjacent) by
+ *   angle = positions[axes[i], b, t] * freqs[i]:  (x, y) -> (x cos - y sin, y cos + x sin)
+ * positions int32 or int64 [A, B, T] (time, height, width, ...: any A), freqs
+ * fp32 and axes int32 [P]: the frequency and the axis of pair i, 2 P <= D.  Pair
+ * i is dims (i, P + i), with interleaved != 0 dims (2 i, 2 i + 1); dims from 2 P
+ * on are copied.  A pair whose axis is outside [0, A) stays as it is.  inverse
+ * != 0 turns back (which is also the gradient of the turn).  Angles in 64 bits,
+ * one rounding; below 2^28 radians they add no error to that of fp32.  q_out may be q itself and k_out k
+ * itself.  The per-channel mul and add chain of the reference (ops.cpp:464-497)
+ * with factors that depend on the place. */
+thin_status thin_rotary_axes(const thin_desc* q, const thin_desc* k, const thin_desc* positions, const thin_desc* freqs,
+                             const thin_desc* axes, int32_t interleaved, int32_t inverse, const thin_desc* q_out,
+                             const thin_desc* k_out, hipStream_t stream);
+
+/* ------------------------------------------------------------------ */
+/* Cross attention                                                     */
+/* ------------------------------------------------------------------ */
+
+/* Bytes of workspace thin_cross_attention needs (0: none) for its q and k.  No
+ * reference counterpart (its products run one by one, bmm_flow.cpp:276-359). */
+size_t thin_cross_attention_workspace(const thin_desc* q, const thin_desc* k);
+
+/* out[b, t, h] = sum_j p_j v[b, j, h'] with p = softmax over j of
+ * scale * q[b, t, h] . k[b, j, h'], h' = h / (H / Hk): q and out [B, T, H, D], k
+ * and v [B, S, Hk, D], fp16 or bf16 of one type, a head's dims adjacent, D a
+ * multiple of 8 from 8 to 256, other strides free; scale positive.
+ *   lengths: NULL, or int32 [B]: only states j < lengths[b] are seen;
+ *   mask: NULL, or bytes [B, S]: only states whose byte is not 0.
+ * A row that sees no state (or nothing but scores of -inf) is zeros; what is
+ * not seen is not read into the result, NaN and infinities included.  fp32
+ * scores, maxima and sums; the weights are rounded to the operands' type for the product
+ * with v.  The workspace is 4-byte aligned and overlaps no operand.  The
+ * attention chain of the reference (whole_blocked.py:91-103) with keys of
+ * another length. */
+thin_status thin_cross_attention(const thin_desc* q, const thin_desc* k, const thin_desc* v, const thin_desc* lengths,
+                                 const thin_desc* mask, float scale, const thin_desc* out, void* workspace,
+                                 size_t workspace_bytes, hipStream_t stream);
+
+/* ------------------------------------------------------------------ */
+/* A cache of keys and values in 8 bits                                */
+/* ------------------------------------------------------------------ */
+
+/* The cache: k_cache and v_cache, e4m3 codes in bytes [pages, Hk, page, D] (D a
+ * multiple of 16 from 16 to 256, page one from 16 to 1024, a token's codes
+ * adjacent, other strides free), and k_scales and v_scales, fp32 [pages, Hk]: a
+ * value is its code times the scale of its page and head.  table int32
+ * [B, slots]: token j of sequence b is token j % page of page
+ * table[b, j / page].  lengths int32 [B]: the tokens of each sequence, the call's
+ * own among them; counts NULL (T), or int32 [B]: how many of its T rows are
+ * tokens, the sequence's last ones.  Tokens before the first and behind
+ * slots * page do not exist; a page outside [0, pages) is neither written nor
+ * seen.  A page belongs to one sequence of a call that writes it: two that write
+ * it race (copy it first), any number may read it. */
+
+/* New keys and values k and v [B, T, Hk, D] (fp16, bf16 or fp32, a head's dims
+ * adjacent) into the cache at positions lengths[b] - counts[b] on.  For each page
+ * and head that gets tokens:
+ *   s = the least 2^e (e >= -110) with |x| <= 448 * 2^e for its new values, or
+ *       the scale it has if that is larger and earlier tokens of the sequence
+ *       are on the page;
+ *   codes = e4m3(x / s), to the nearest, ties to even; earlier tokens, where the
+ *       scale grew, e4m3(code * old / s).
+ * Infinities become the largest code, NaN stays NaN; neither counts for s.  Codes
+ * behind a sequence's last token stay as they are, so tokens given up by a lower length
+ * may be written anew.  The strided copies of the reference (ops.cpp:32-78) at
+ * places that depend on the data, with another type. */
+thin_status thin_cache_write(const thin_desc* k, const thin_desc* v, const thin_desc* k_cache, const thin_desc* v_cache,
+                             const thin_desc* k_scales, const thin_desc* v_scales, const thin_desc* table,
+                             const thin_desc* lengths, const thin_desc* counts, hipStream_t stream);
+
+/* Bytes of workspace thin_cache_attention needs (0: none) for its operands of
+ * the same names.  No reference counterpart (bmm_flow.cpp:276-359 takes whole
+ * tensors). */
+size_t thin_cache_attention_workspace(const thin_desc* q, const thin_desc* k_cache, const thin_desc* table);
+
+/* Attention of each sequence's last tokens, q and out [B, T, H, D] (fp16 or bf16,
+ * a head's dims adjacent, Hk divides H), over its cached ones: row t < counts[b]
+ * sees the tokens up to and with its own, j <= lengths[b] - counts[b] + t.  Rows
+ * from counts[b] on, and rows that see nothing, are zeros.  fp32 scores, maxima
+ * and sums; a weight times its page's scale is rounded to bf16 for the product with the codes
+ * of v.  What a row does not see has no part in it, NaN included.  The workspace is
+ * 4-byte aligned and overlaps no operand.  The attention chain of the reference
+ * (whole_blocked.py:91-103) over pages. */
+thin_status thin_cache_attention(const thin_desc* q, const thin_desc* k_cache, const thin_desc* v_cache,
+                                 const thin_desc* k_scales, const thin_desc* v_scales, const thin_desc* table,
+                                 const thin_desc* lengths, const thin_desc* counts, float scale, const thin_desc* out,
+                                 void* workspace, size_t workspace_bytes, hipStream_t stream);
+
+/* ------------------------------------------------------------------ */
+/* Verification of drafted tokens                                      */
+/* ------------------------------------------------------------------ */
+
+/* Bytes of workspace thin_verify_drafts needs (0: none).  No reference
+ * counterpart (its selection knows no chance, selection_flow.cpp:429-499). */
+size_t thin_verify_drafts_workspace(int64_t batch, int64_t vocab);
+
+/* Which drafted tokens the target keeps, and the token after them.  target
+ * [B, K + 1, V] and draft [B, K, V] or NULL (drafts that were certain):
+ * probabilities, fp16, bf16 or fp32 of one type, a row's adjacent, V <= 8388608,
+ * K <= 64; tokens int64 [B, K], counts NULL (K) or int32 [B]: drafts of each
+ * sequence; accept fp32 [B, K] and sample fp32 [B]: random numbers in [0, 1).
+ *   draft i stays if all before it do and accept[b, i] * draft[b, i, x] <
+ *     target[b, i, x], x = tokens[b, i] (a token outside [0, V) falls);
+ *   n = taken[b] (int32 [B]) of them stay;
+ *   the next token comes from max(target[b, n] - draft[b, n], 0) if draft n fell
+ *     (without draft: target[b, n] with x left out), from target[b, n] if none did
+ *     or if that leaves nothing: the first token at which the running sum passes
+ *     sample[b] times the total;
+ *   out [B, K + 1] int64: the n drafts, that token, then -1.
+ * Probabilities that are not positive and finite count as 0; if all do, the next
+ * token is -1.  Products and sums in 64 bits.  The workspace is 8-byte aligned and
+ * overlaps no operand.  The selection of the reference (selection_flow.cpp:429-499)
+ * with given chances in place of the order. */
+thin_status thin_verify_drafts(const thin_desc* target, const thin_desc* draft, const thin_desc* tokens,
+                               const thin_desc* counts, const thin_desc* accept, const thin_desc* sample,
+                               const thin_desc* out, const thin_desc* taken, void* workspace, size_t workspace_bytes,
+                               hipStream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

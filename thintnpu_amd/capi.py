@@ -111,6 +111,11 @@ def lib() -> ctypes.CDLL:
             "thin_expert_dispatch": [vp, vp, i64, vp, vp, vp, vp, ctypes.c_size_t, vp],
             "thin_expert_combine": [vp, vp, vp, vp, vp],
             "thin_token_logprobs": [vp, vp, vp, vp, vp, vp, vp, ctypes.c_size_t, vp],
+            "thin_rotary_axes": [vp, vp, vp, vp, vp, i32, i32, vp, vp, vp],
+            "thin_cross_attention": [vp, vp, vp, vp, vp, f32, vp, vp, ctypes.c_size_t, vp],
+            "thin_cache_write": [vp] * 10,
+            "thin_cache_attention": [vp, vp, vp, vp, vp, vp, vp, vp, f32, vp, vp, ctypes.c_size_t, vp],
+            "thin_verify_drafts": [vp, vp, vp, vp, vp, vp, vp, vp, vp, ctypes.c_size_t, vp],
         }
         for name, argtypes in sigs.items():
             fn = getattr(L, name, None)
@@ -125,7 +130,10 @@ def lib() -> ctypes.CDLL:
             L.thin_detection_select_workspace.restype = ctypes.c_size_t
         for name, argtypes in {"thin_group_norm_workspace": [vp, vp, i32, i64, i64],
                                "thin_expert_dispatch_workspace": [i64, i64, i64],
-                               "thin_token_logprobs_workspace": [i64, i64, i64]}.items():
+                               "thin_token_logprobs_workspace": [i64, i64, i64],
+                               "thin_cross_attention_workspace": [vp, vp],
+                               "thin_cache_attention_workspace": [vp, vp, vp],
+                               "thin_verify_drafts_workspace": [i64, i64]}.items():
             fn = getattr(L, name, None)
             if fn is None:
                 continue
@@ -626,3 +634,125 @@ def token_logprobs(logits, tokens, top: int = 0, out=None, workspace=None, strea
         _packed(logits), _on(device, tokens), _on(device, logprobs), _on(device, entropy), _on(device, top_logprobs),
         _on(device, top_ids), address, nbytes, _stream(None)))
     return out
+
+
+def rotary_tables(sections, base: float = 10000.0, per_axis: bool = False, device="cuda"):
+    """(freqs fp32, axes int32) [sum(sections)] for rotary_axes: sections[a] pairs
+    turn with axis a, pair i by base ** -(i / pairs); with per_axis each axis has
+    such a run of its own."""
+    sections = [int(n) for n in sections]
+    pairs = sum(sections)
+    steps = [i / n for n in sections for i in range(n)] if per_axis else [i / pairs for i in range(pairs)]
+    freqs = torch.tensor([float(base) ** -s for s in steps], dtype=torch.float64).float().to(device)
+    return freqs, torch.tensor([a for a, n in enumerate(sections) for _ in range(n)], dtype=torch.int32, device=device)
+
+
+def _contiguous_like(x: torch.Tensor) -> torch.Tensor:
+    return torch.empty(x.shape, dtype=x.dtype, device=x.device)
+
+
+def rotary_axes(q, positions, freqs, axes, k=None, interleaved: bool = False, inverse: bool = False, out=None,
+                stream=None):
+    """q [B, T, H, D] (and k [B, T, Hk, D]) with pair i of each head turned by
+    positions[axes[i], b, t] * freqs[i]; positions int [A, B, T], freqs and axes
+    as rotary_tables gives them.  Returns q's result, or (q's, k's) with k; out:
+    the tensor or the two, which may be q and k themselves."""
+    if stream is not None:
+        return _elsewhere(stream, out, functools.partial(rotary_axes, k=k, interleaved=interleaved, inverse=inverse),
+                          q, positions, freqs, axes)
+    device = _current_device(q)
+    if out is None:
+        out = _contiguous_like(q) if k is None else (_contiguous_like(q), _contiguous_like(k))
+    q_out, k_out = (out, None) if k is None else out
+    _check("thin_rotary_axes", lib().thin_rotary_axes(
+        _packed(q), None if k is None else _on(device, k), _on(device, positions), _on(device, freqs),
+        _on(device, axes), 1 if interleaved else 0, 1 if inverse else 0, _on(device, q_out),
+        None if k is None else _on(device, k_out), _stream(None)))
+    return q_out if k is None else (q_out, k_out)
+
+
+def cross_attention(q, k, v, lengths=None, mask=None, scale: float | None = None, out=None, workspace=None, stream=None):
+    """Attention of q [B, T, H, D] to k and v [B, S, Hk, D] (fp16 or bf16): states
+    below lengths[b] (int32 [B]) whose mask [B, S] (bool) is set; scale defaults to
+    D ** -0.5.  Rows that see no state are zeros."""
+    if stream is not None:
+        return _elsewhere(stream, out, functools.partial(cross_attention, workspace=workspace), q, k, v, lengths, mask, scale)
+    device = _current_device(q)
+    if out is None:
+        out = _contiguous_like(q)
+    L = lib()
+    qd, kd = _packed(q), _on(device, k)
+    ws, address, nbytes = _workspace(L.thin_cross_attention_workspace(qd, kd), workspace, device)
+    _check("thin_cross_attention", L.thin_cross_attention(
+        qd, kd, _on(device, v), None if lengths is None else _on(device, lengths),
+        None if mask is None else _on(device, mask), q.shape[-1] ** -0.5 if scale is None else scale, _on(device, out),
+        address, nbytes, _stream(None)))
+    return out
+
+
+def _codes(device: int, t: torch.Tensor) -> bytes:
+    """_on(device, t) of e4m3 codes, as float8_e4m3fn or as bytes."""
+    if t.dtype != torch.float8_e4m3fn:
+        return _on(device, t)
+    if t.get_device() != device or not t.is_cuda:
+        raise ValueError(f"operands on cuda:{device} and {t.device}")
+    return _PACK[t.dim()].pack(t.data_ptr(), U8, t.dim(), *t.shape, *t.stride())
+
+
+def cache_write(k, v, k_cache, v_cache, k_scales, v_scales, table, lengths, counts=None, stream=None):
+    """k and v [B, T, Hk, D], the last counts[b] (default T) tokens of sequences of
+    lengths[b], into the cache: e4m3 codes [pages, Hk, page, D] (float8_e4m3fn or
+    uint8) with fp32 scales [pages, Hk], where table [B, slots] says."""
+    if stream is not None:
+        _elsewhere(stream, (), lambda *args, out: cache_write(*args), k, v, k_cache, v_cache, k_scales, v_scales, table,
+                   lengths, counts)
+        return
+    device = _current_device(k)
+    _check("thin_cache_write", lib().thin_cache_write(
+        _packed(k), _on(device, v), _codes(device, k_cache), _codes(device, v_cache), _on(device, k_scales),
+        _on(device, v_scales), _on(device, table), _on(device, lengths),
+        None if counts is None else _on(device, counts), _stream(None)))
+
+
+def cache_attention(q, k_cache, v_cache, k_scales, v_scales, table, lengths, counts=None, scale: float | None = None,
+                    out=None, workspace=None, stream=None):
+    """Attention of q [B, T, H, D] (fp16 or bf16), the last counts[b] (default T)
+    tokens of sequences of lengths[b], over the tokens of the cache up to each
+    one's own; scale defaults to D ** -0.5.  Rows from counts[b] on are zeros."""
+    if stream is not None:
+        return _elsewhere(stream, out, functools.partial(cache_attention, workspace=workspace), q, k_cache, v_cache,
+                          k_scales, v_scales, table, lengths, counts, scale)
+    device = _current_device(q)
+    if out is None:
+        out = _contiguous_like(q)
+    L = lib()
+    qd, kd, td = _packed(q), _codes(device, k_cache), _on(device, table)
+    ws, address, nbytes = _workspace(L.thin_cache_attention_workspace(qd, kd, td), workspace, device)
+    _check("thin_cache_attention", L.thin_cache_attention(
+        qd, kd, _codes(device, v_cache), _on(device, k_scales), _on(device, v_scales), td, _on(device, lengths),
+        None if counts is None else _on(device, counts), q.shape[-1] ** -0.5 if scale is None else scale,
+        _on(device, out), address, nbytes, _stream(None)))
+    return out
+
+
+def verify_drafts(target, draft, tokens, accept, sample, counts=None, out=None, workspace=None, stream=None):
+    """(tokens int64 [B, K + 1], taken int32 [B]): of the drafted tokens [B, K] those
+    that the target's probabilities [B, K + 1, V] keep against the draft's [B, K, V]
+    (None: certain drafts) for the random numbers accept [B, K], then the one that
+    sample [B] gives, then -1."""
+    if stream is not None:
+        return _elsewhere(stream, out, functools.partial(verify_drafts, counts=counts, workspace=workspace), target, draft,
+                          tokens, accept, sample)
+    device = _current_device(target)
+    b, rows, vocab = target.shape
+    if out is None:
+        out = (_rows(target, b, rows, torch.int64),
+               torch.empty_strided((b,), (1,), dtype=torch.int32, device=target.device))
+    kept, taken = out
+    L = lib()
+    ws, address, nbytes = _workspace(L.thin_verify_drafts_workspace(b, vocab), workspace, device)
+    _check("thin_verify_drafts", L.thin_verify_drafts(
+        _packed(target), None if draft is None else _on(device, draft), _on(device, tokens),
+        None if counts is None else _on(device, counts), _on(device, accept), _on(device, sample), _on(device, kept),
+        _on(device, taken), address, nbytes, _stream(None)))
+    return kept, taken

@@ -1,0 +1,396 @@
+// Verification of drafted tokens against the target's probabilities.
+//
+//   draft i of a sequence stays while u_i q_i(x_i) < p_i(x_i), all before it
+//   having stayed; then one more token comes from the target: from
+//   max(p_n - q_n, 0) at the first draft n that fell, from p_n if none did, the
+//   first whose distribution function passes r times the total.
+//
+// So the tokens are distributed as the target's own.  Products and sums are
+// taken in 64 bits: u q is exact there, and the order of rounding in a sum over
+// the vocabulary moves a border by 1e-16 of the total, not by 1e-7.
+//
+// Bound by memory: of the target's and the draft's rows only one each is read
+// whole.  Few rows, so each is cut into tiles over the card; a second launch
+// finds the tile that holds the border and scans it again.  A row of one tile
+// takes one launch.
+#include "rows.h"
+
+#include <string.h>
+
+namespace thin {
+namespace {
+
+constexpr int kChunk = 2048;       // elements of a workgroup at a time: 8 a thread
+constexpr int64_t kMaxDrafts = 64; // one lane each
+constexpr int64_t kMaxVocab = 1 << 23;
+constexpr int64_t kWorkgroups = 1024;
+constexpr int64_t kMostChunks = 8;
+
+struct DraftPlan {
+  const void* target;
+  const void* draft;
+  int64_t pb, pk, qb, qk;
+  const int64_t* tokens;
+  int64_t tb, tk;
+  const int32_t* counts;
+  int64_t count_step;
+  const float* accept;
+  int64_t ub, uk;
+  const float* sample;
+  int64_t sample_step;
+  int64_t* out;
+  int64_t ob, ok;
+  int32_t* taken;
+  int64_t taken_step;
+  uint32_t drafts, vocab, tiles, chunks;  // chunks of a tile
+  FastDiv by_tiles;
+  double* sums;     // [batch, tiles, 2]: of what is left, of the target's row
+  int32_t* stayed;  // [batch]
+};
+
+// How many drafts stay; every lane of a wavefront gets it.
+template <typename T>
+__device__ __forceinline__ uint32_t stayed_of(const DraftPlan& p, uint32_t b, uint32_t lane, uint32_t& count) {
+  const int32_t n = p.counts ? p.counts[b * p.count_step] : (int32_t)p.drafts;
+  count = (uint32_t)max(0, min(n, (int32_t)p.drafts));
+  bool stays = false;
+  if (lane < count) {
+    const int64_t x = p.tokens[b * p.tb + lane * p.tk];
+    if (x >= 0 && x < (int64_t)p.vocab) {
+      const double pt = (double)(float)static_cast<const T*>(p.target)[b * p.pb + lane * p.pk + x];
+      const double qt = p.draft ? (double)(float)static_cast<const T*>(p.draft)[b * p.qb + lane * p.qk + x] : 1.0;
+      stays = (double)p.accept[b * p.ub + lane * p.uk] * qt < pt;
+    }
+  }
+  const uint64_t fell = ~__ballot(stays);
+  return fell ? (uint32_t)__builtin_ctzll(fell) : 64u;
+}
+
+__device__ __forceinline__ double positive(double x) { return x > 0.0 && x <= 1.7976931348623157e308 ? x : 0.0; }
+
+// The row that the next token comes from.
+template <typename T>
+struct Rest {
+  const T* p;
+  const T* q;       // null: nothing is taken off but `without`
+  int64_t without;  // a token that has no part, or -1
+  uint32_t vocab;
+  __device__ __forceinline__ Rest(const DraftPlan& a, uint32_t b, uint32_t stayed, uint32_t count)
+      : p(static_cast<const T*>(a.target) + b * a.pb + stayed * a.pk), q(nullptr), without(-1), vocab(a.vocab) {
+    if (stayed < count) {
+      if (a.draft) q = static_cast<const T*>(a.draft) + b * a.qb + stayed * a.qk;
+      else without = a.tokens[b * a.tb + stayed * a.tk];
+    }
+  }
+  // Elements [at, at + 8): what is left of them, and the target's own.
+  __device__ __forceinline__ void load(uint32_t at, double (&left)[8], double (&own)[8]) const {
+    float x[8], y[8];
+    const uint32_t n = at < vocab ? vocab - at : 0u;
+    if (n >= 8) {
+      dev::load_pack<T, 8>(p + at, x);
+      if (q) dev::load_pack<T, 8>(q + at, y);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        x[j] = (uint32_t)j < n ? (float)p[at + j] : 0.f;
+        y[j] = q && (uint32_t)j < n ? (float)q[at + j] : 0.f;
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      own[j] = positive((double)x[j]);
+      left[j] = (int64_t)(at + j) == without ? 0.0 : q ? (own[j] > 0.0 ? positive((double)x[j] - (double)y[j]) : 0.0) : own[j];
+    }
+  }
+};
+
+__device__ __forceinline__ double wave_total(double v) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+  return v;
+}
+// Sum over the lanes up to this one.
+__device__ __forceinline__ double wave_scan(double v, uint32_t lane) {
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const double below = __shfl_up(v, o, 64);
+    if (lane >= (uint32_t)o) v += below;
+  }
+  return v;
+}
+
+struct Shared {
+  double left[4], own[4];
+  uint32_t found, last;
+};
+
+// Sums of a tile's 8 * 256 * chunks elements; every thread gets them.
+template <typename T>
+__device__ __forceinline__ void tile_sums(const Rest<T>& rest, uint32_t first, uint32_t chunks, Shared& lds, double& left, double& own) {
+  const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
+  left = own = 0.0;
+  for (uint32_t c = 0; c < chunks; ++c) {
+    double a[8], o[8];
+    rest.load(first + c * kChunk + threadIdx.x * 8, a, o);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      left += a[j];
+      own += o[j];
+    }
+  }
+  left = wave_total(left);
+  own = wave_total(own);
+  if (lane == 0) {
+    lds.left[wave] = left;
+    lds.own[wave] = own;
+  }
+  __syncthreads();
+  left = ((lds.left[0] + lds.left[1]) + lds.left[2]) + lds.left[3];
+  own = ((lds.own[0] + lds.own[1]) + lds.own[2]) + lds.own[3];
+  __syncthreads();
+}
+
+// The first element of a tile whose sum, with `before` ahead of the tile, passes
+// `edge`; where rounding leaves none, the tile's last that has a part.
+template <typename T>
+__device__ __forceinline__ uint32_t find_in_tile(const Rest<T>& rest, bool whole, uint32_t first, uint32_t chunks, double before,
+                                                 double edge, Shared& lds) {
+  const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
+  if (threadIdx.x == 0) {
+    lds.found = 0xFFFFFFFFu;
+    lds.last = 0;
+  }
+  for (uint32_t c = 0; c < chunks; ++c) {
+    const uint32_t at = first + c * kChunk + threadIdx.x * 8;
+    double a[8], o[8], sum = 0.0;
+    rest.load(at, a, o);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      if (whole) a[j] = o[j];
+      sum += a[j];
+    }
+    const double scan = wave_scan(sum, lane);
+    __syncthreads();
+    if (lane == 63) lds.left[wave] = scan;
+    __syncthreads();
+    double base = before;
+    for (uint32_t i = 0; i < wave; ++i) base += lds.left[i];
+    double run = base + (scan - sum);
+    uint32_t found = 0xFFFFFFFFu, last = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      run += a[j];
+      if (a[j] > 0.0) {
+        last = at + j;
+        if (run > edge && found == 0xFFFFFFFFu) found = at + j;
+      }
+    }
+    if (found != 0xFFFFFFFFu) atomicMin(&lds.found, found);
+    if (last) atomicMax(&lds.last, last);
+    before += ((lds.left[0] + lds.left[1]) + lds.left[2]) + lds.left[3];
+  }
+  __syncthreads();
+  return lds.found != 0xFFFFFFFFu ? lds.found : lds.last;
+}
+
+// The sequence's tokens, the last of them `next`.
+__device__ __forceinline__ void store_tokens(const DraftPlan& p, uint32_t b, uint32_t stayed, int64_t next) {
+  for (uint32_t i = threadIdx.x; i <= p.drafts; i += 256)
+    p.out[b * p.ob + i * p.ok] = i < stayed ? p.tokens[b * p.tb + i * p.tk] : i == stayed ? next : -1;
+  if (threadIdx.x == 0) p.taken[b * p.taken_step] = (int32_t)stayed;
+}
+__device__ __forceinline__ double edge_of(const DraftPlan& p, uint32_t b, double total) {
+  const float r = p.sample[b * p.sample_step];
+  return (double)(r > 0.f ? fminf(r, 1.f) : 0.f) * total;
+}
+
+template <typename T>
+__global__ __launch_bounds__(256) void sums_kernel(DraftPlan p) {
+  __shared__ Shared lds;
+  const uint32_t b = p.by_tiles.div(blockIdx.x), tile = blockIdx.x - b * p.tiles;
+  uint32_t count;
+  const uint32_t stayed = stayed_of<T>(p, b, threadIdx.x & 63u, count);
+  const Rest<T> rest(p, b, stayed, count);
+  double left, own;
+  tile_sums(rest, tile * p.chunks * kChunk, p.chunks, lds, left, own);
+  if (p.tiles == 1) {
+    const bool whole = !(left > 0.0);
+    const double total = whole ? own : left;
+    const uint32_t next = find_in_tile(rest, whole, 0, p.chunks, 0.0, edge_of(p, b, total), lds);
+    store_tokens(p, b, stayed, total > 0.0 ? (int64_t)next : -1);
+  } else if (threadIdx.x == 0) {
+    p.sums[blockIdx.x * 2ull] = left;
+    p.sums[blockIdx.x * 2ull + 1] = own;
+    if (tile == 0) p.stayed[b] = (int32_t)stayed;
+  }
+}
+
+template <typename T>
+__global__ __launch_bounds__(256) void find_kernel(DraftPlan p) {
+  __shared__ Shared lds;
+  __shared__ uint32_t lds_tile;
+  __shared__ double lds_before, lds_edge;
+  __shared__ uint32_t lds_whole;
+  const uint32_t b = blockIdx.x, lane = threadIdx.x & 63u;
+  const double* sums = p.sums + (uint64_t)b * p.tiles * 2;
+  const uint32_t stayed = (uint32_t)p.stayed[b];
+  const int32_t n = p.counts ? p.counts[b * p.count_step] : (int32_t)p.drafts;
+  const uint32_t count = (uint32_t)max(0, min(n, (int32_t)p.drafts));
+  const Rest<T> rest(p, b, stayed, count);
+  if (threadIdx.x < 64) {
+    double left = 0.0, own = 0.0;
+    for (uint32_t i = 0; i < p.tiles; i += 64) {  // in the order of the scan below
+      const uint32_t at = i + lane;
+      double a = 0.0, o = 0.0;
+      if (at < p.tiles) {
+        a = sums[at * 2];
+        o = sums[at * 2 + 1];
+      }
+      left += __shfl(wave_scan(a, lane), 63, 64);
+      own += __shfl(wave_scan(o, lane), 63, 64);
+    }
+    const bool whole = !(left > 0.0);
+    const double total = whole ? own : left, edge = edge_of(p, b, total);
+    double before = 0.0, tile_before = 0.0;
+    uint32_t tile = 0xFFFFFFFFu, last = 0;
+    double last_before = 0.0;
+    for (uint32_t i = 0; i < p.tiles && tile == 0xFFFFFFFFu; i += 64) {
+      const uint32_t at = i + lane;
+      const double v = at < p.tiles ? sums[at * 2 + (whole ? 1 : 0)] : 0.0, scan = wave_scan(v, lane);
+      const uint64_t passed = __ballot(v > 0.0 && before + scan > edge), some = __ballot(v > 0.0);
+      const double ahead = before + (scan - v);
+      if (passed) {
+        const int l = __builtin_ctzll(passed);
+        tile = i + l;
+        tile_before = __shfl(ahead, l, 64);
+      }
+      if (some) {
+        const int l = 63 - __builtin_clzll(some);
+        last = i + l;
+        last_before = __shfl(ahead, l, 64);
+      }
+      before += __shfl(scan, 63, 64);
+    }
+    if (lane == 0) {
+      lds_tile = tile != 0xFFFFFFFFu ? tile : last;
+      lds_before = tile != 0xFFFFFFFFu ? tile_before : last_before;
+      lds_edge = edge;
+      lds_whole = whole | (total > 0.0 ? 2u : 0u);
+    }
+  }
+  __syncthreads();
+  const uint32_t next = find_in_tile(rest, lds_whole & 1u, lds_tile * p.chunks * kChunk, p.chunks, lds_before, lds_edge, lds);
+  store_tokens(p, b, stayed, lds_whole & 2u ? (int64_t)next : -1);
+}
+
+// Chunks of a tile: one, or as many as leave enough workgroups.
+int64_t chunks_of(int64_t batch, int64_t vocab) {
+  const int64_t all = (vocab + kChunk - 1) / kChunk;
+  int64_t n = 1;
+  while (n < kMostChunks && batch * ((all + 2 * n - 1) / (2 * n)) >= kWorkgroups) n *= 2;
+  return n;
+}
+int64_t tiles_of(int64_t batch, int64_t vocab) {
+  const int64_t per = kChunk * chunks_of(batch, vocab);
+  return (vocab + per - 1) / per;
+}
+
+}  // namespace
+}  // namespace thin
+
+using namespace thin;
+
+extern "C" size_t thin_verify_drafts_workspace(int64_t batch, int64_t vocab) {
+  if (batch <= 0 || vocab <= 0 || vocab > kMaxVocab) return 0;
+  const int64_t tiles = tiles_of(batch, vocab);
+  return tiles == 1 ? 0 : (size_t)batch * (tiles * 16 + 8);
+}
+
+extern "C" thin_status thin_verify_drafts(const thin_desc* target, const thin_desc* draft, const thin_desc* tokens,
+                                          const thin_desc* counts, const thin_desc* accept, const thin_desc* sample,
+                                          const thin_desc* out, const thin_desc* taken, void* workspace,
+                                          size_t workspace_bytes, hipStream_t stream) {
+  clear_error();
+  THIN_REQUIRE(desc_valid(target) && desc_valid(tokens) && desc_valid(accept) && desc_valid(sample) && desc_valid(out) &&
+                   desc_valid(taken) && (!draft || desc_valid(draft)) && (!counts || desc_valid(counts)),
+               THIN_ERR_INVALID, "verify_drafts: invalid descriptor");
+  THIN_REQUIRE(float_type(target->dtype) && target->rank == 3 && target->sizes[1] >= 1, THIN_ERR_INVALID,
+               "verify_drafts takes float16, bfloat16 or float32 target probabilities [batch, drafts + 1, vocab]");
+  const int64_t B = target->sizes[0], K = target->sizes[1] - 1, V = target->sizes[2];
+  THIN_REQUIRE(!draft || (draft->dtype == target->dtype && draft->rank == 3 && draft->sizes[0] == B && draft->sizes[1] == K &&
+                          draft->sizes[2] == V),
+               THIN_ERR_INVALID, "verify_drafts takes draft probabilities [batch, drafts, vocab] of the target's type");
+  THIN_REQUIRE(tokens->rank == 2 && tokens->dtype == THIN_I64 && tokens->sizes[0] == B && tokens->sizes[1] == K &&
+                   accept->rank == 2 && accept->dtype == THIN_F32 && accept->sizes[0] == B && accept->sizes[1] == K &&
+                   sample->rank == 1 && sample->dtype == THIN_F32 && sample->sizes[0] == B &&
+                   (!counts || (counts->rank == 1 && counts->dtype == THIN_I32 && counts->sizes[0] == B)),
+               THIN_ERR_INVALID,
+               "verify_drafts takes int64 tokens and float32 accept [batch, drafts], float32 sample and int32 counts [batch]");
+  THIN_REQUIRE(out->rank == 2 && out->dtype == THIN_I64 && out->sizes[0] == B && out->sizes[1] == K + 1 && taken->rank == 1 &&
+                   taken->dtype == THIN_I32 && taken->sizes[0] == B,
+               THIN_ERR_INVALID, "verify_drafts writes int64 tokens [batch, drafts + 1] and int32 taken [batch]");
+  THIN_REQUIRE(V >= 1, THIN_ERR_INVALID, "verify_drafts needs a vocabulary");
+  THIN_REQUIRE(K <= kMaxDrafts && V <= kMaxVocab, THIN_ERR_UNSUPPORTED,
+               "verify_drafts takes up to %lld drafts of up to %lld tokens", (long long)kMaxDrafts, (long long)kMaxVocab);
+  THIN_REQUIRE(V == 1 || (target->strides[2] == 1 && (!draft || draft->strides[2] == 1)), THIN_ERR_UNSUPPORTED,
+               "verify_drafts: the probabilities of a row must be adjacent");
+  if (B == 0) return THIN_OK;
+  THIN_REQUIRE(B < (1ll << 24), THIN_ERR_UNSUPPORTED, "verify_drafts: tensor too large");
+  const int64_t tiles = tiles_of(B, V);
+  THIN_REQUIRE(launchable(B * tiles, 256), THIN_ERR_UNSUPPORTED, "verify_drafts: tensor too large");
+  const thin_desc* outs[2] = {out, taken};
+  for (const thin_desc* o : outs) {
+    THIN_REQUIRE(!repeats(o), THIN_ERR_INVALID, "verify_drafts: an output has a stride of 0");
+    for (const thin_desc* in : {target, draft, tokens, counts, accept, sample})
+      THIN_REQUIRE(!in || !overlap(o, in), THIN_ERR_INVALID, "verify_drafts: an output overlaps an input");
+  }
+  THIN_REQUIRE(!overlap(out, taken), THIN_ERR_INVALID, "verify_drafts: two outputs overlap");
+  const size_t need = thin_verify_drafts_workspace(B, V);
+  THIN_REQUIRE(workspace_bytes >= need && (need == 0 || workspace), THIN_ERR_WORKSPACE,
+               "verify_drafts needs %zu bytes of workspace, got %zu", need, workspace_bytes);
+  THIN_REQUIRE(need == 0 || (reinterpret_cast<uintptr_t>(workspace) & 7u) == 0, THIN_ERR_WORKSPACE,
+               "verify_drafts: the workspace must be 8-byte aligned");
+  DraftPlan p;
+  memset(&p, 0, sizeof p);
+  p.target = target->data;
+  p.pb = target->strides[0];
+  p.pk = target->strides[1];
+  if (draft && K > 0) {
+    p.draft = draft->data;
+    p.qb = draft->strides[0];
+    p.qk = draft->strides[1];
+  }
+  p.tokens = static_cast<const int64_t*>(tokens->data);
+  p.tb = tokens->strides[0]; p.tk = tokens->strides[1];
+  if (counts) {
+    p.counts = static_cast<const int32_t*>(counts->data);
+    p.count_step = counts->strides[0];
+  }
+  p.accept = static_cast<const float*>(accept->data);
+  p.ub = accept->strides[0]; p.uk = accept->strides[1];
+  p.sample = static_cast<const float*>(sample->data);
+  p.sample_step = sample->strides[0];
+  p.out = static_cast<int64_t*>(out->data);
+  p.ob = out->strides[0]; p.ok = out->strides[1];
+  p.taken = static_cast<int32_t*>(taken->data);
+  p.taken_step = taken->strides[0];
+  p.drafts = (uint32_t)K;
+  p.vocab = (uint32_t)V;
+  p.tiles = (uint32_t)tiles;
+  p.chunks = (uint32_t)chunks_of(B, V);
+  p.by_tiles = FastDiv::make(p.tiles);
+  if (tiles > 1) {
+    p.sums = static_cast<double*>(workspace);
+    p.stayed = reinterpret_cast<int32_t*>(p.sums + 2 * B * tiles);
+  }
+  return with_float_type(target->dtype, [&](auto zero) {
+    using T = decltype(zero);
+    hipLaunchKernelGGL((sums_kernel<T>), dim3((uint32_t)(B * tiles)), dim3(256), 0, stream, p);
+    THIN_LAUNCH_CHECK("verify_drafts");
+    if (tiles > 1) {
+      hipLaunchKernelGGL((find_kernel<T>), dim3((uint32_t)B), dim3(256), 0, stream, p);
+      THIN_LAUNCH_CHECK("verify_drafts_find");
+    }
+    return THIN_OK;
+  });
+}

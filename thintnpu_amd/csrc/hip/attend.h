@@ -66,7 +66,7 @@ struct AttendPlan {
   float* stats;
 };
 
-constexpr int kFewRows = 32;    // rows of one matrix tile: keys are split over the wavefronts
+constexpr int kFewRows = 32;    // one or two matrix tiles of 16: keys are split over the wavefronts
 constexpr int kBlockRows = 128; // rows of a workgroup otherwise: 32 a wavefront
 
 // Head widths that kernels exist for.
@@ -76,20 +76,22 @@ inline int padded_dim(int64_t d) {
   return 0;
 }
 
-// Splits of a row's keys: until there are two workgroups a CU, none under
-// kSplitKeys keys (shorter ones cost more to join than they give).
+// Splits of a row's keys: until the card is full (a few rows' workgroups, of
+// which four fit a CU, twice over, as sequences are not of one length), none under kSplitKeys
+// keys (shorter ones cost more to join than they give).
 constexpr int64_t kSplitKeys = 256;
-constexpr int64_t kWorkgroups = 512;
+constexpr int64_t kWorkgroups = 512, kFewWorkgroups = 2048;
 constexpr int64_t kMaxSplits = 128;
-inline int64_t splits_of(int64_t units, int64_t keys) {
-  const int64_t most = (keys + kSplitKeys - 1) / kSplitKeys, want = kWorkgroups / (units > 0 ? units : 1);
+inline int64_t splits_of(int64_t units, int64_t rows, int64_t keys) {
+  const int64_t most = (keys + kSplitKeys - 1) / kSplitKeys;
+  const int64_t want = (rows <= kFewRows ? kFewWorkgroups : kWorkgroups) / (units > 0 ? units : 1);
   const int64_t n = want < most ? want : most;
   return n < 1 ? 1 : n > kMaxSplits ? kMaxSplits : n;
 }
 inline int64_t row_blocks_of(int64_t rows) { return rows <= kFewRows ? 1 : (rows + kBlockRows - 1) / kBlockRows; }
 inline size_t attend_workspace(int64_t batch, int64_t heads, int64_t rows, int64_t keys, int64_t dim) {
   if (batch <= 0 || heads <= 0 || rows <= 0 || keys <= 0 || !padded_dim(dim)) return 0;
-  const int64_t units = batch * heads * row_blocks_of(rows), splits = splits_of(units, keys);
+  const int64_t units = batch * heads * row_blocks_of(rows), splits = splits_of(units, rows, keys);
   if (splits == 1) return 0;
   return (size_t)(units * splits * (rows <= kFewRows ? rows : kBlockRows) * (dim + 2) * 4);
 }
@@ -111,7 +113,7 @@ inline void plan_attend(AttendPlan& p, const thin_desc* q, const thin_desc* out,
   p.keys = (uint32_t)keys;
   p.c = c;
   const int64_t blocks = row_blocks_of(p.rows), units = (int64_t)p.batch * heads * blocks;
-  const int64_t splits = splits_of(units, keys), block_rows = p.rows <= kFewRows ? p.rows : kBlockRows;
+  const int64_t splits = splits_of(units, p.rows, keys), block_rows = p.rows <= kFewRows ? p.rows : kBlockRows;
   p.row_blocks = (uint32_t)blocks;
   p.splits = (uint32_t)splits;
   p.by_group = FastDiv::make(p.group);
@@ -135,6 +137,8 @@ typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u4e __attribute__((ext_vector_type(4), aligned(1)));  // at element alignment
 typedef short s4 __attribute__((ext_vector_type(4)));
 
+// An infinite scale or a NaN code reaches the rows that see it alone: a weight
+// of zero is no protection in a matrix product.
 template <typename T>
 struct Matrix;
 template <>
@@ -144,6 +148,9 @@ struct Matrix<__bf16> {
   static constexpr float kShift = 0.f;
   static __device__ __forceinline__ f16v mul(v8 a, v8 b, f16v c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ f4 mul16(v8 a, v8 b, f4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
   }
   template <bool HI>
   static __device__ __forceinline__ uint32_t of_codes(uint32_t w) {
@@ -159,19 +166,25 @@ struct Matrix<_Float16> {
   static __device__ __forceinline__ f16v mul(v8 a, v8 b, f16v c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
   }
+  static __device__ __forceinline__ f4 mul16(v8 a, v8 b, f4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+  }
   template <bool HI>
   static __device__ __forceinline__ uint32_t of_codes(uint32_t w) {
     return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, HI));
   }
 };
 
-// 16 codes as 16 numbers of 16 bits (exact: e4m3 has 3 bits and exponents -9 to 8).
+// 8 and 16 codes as numbers of 16 bits (exact: e4m3 has 3 bits and exponents -9 to 8).
+template <typename T>
+__device__ __forceinline__ u4 widen8(uint32_t lo, uint32_t hi) {
+  return u4{Matrix<T>::template of_codes<false>(lo), Matrix<T>::template of_codes<true>(lo),
+            Matrix<T>::template of_codes<false>(hi), Matrix<T>::template of_codes<true>(hi)};
+}
 template <typename T>
 __device__ __forceinline__ void widen(u4 w, u4& a, u4& b) {
-  a = u4{Matrix<T>::template of_codes<false>(w[0]), Matrix<T>::template of_codes<true>(w[0]),
-         Matrix<T>::template of_codes<false>(w[1]), Matrix<T>::template of_codes<true>(w[1])};
-  b = u4{Matrix<T>::template of_codes<false>(w[2]), Matrix<T>::template of_codes<true>(w[2]),
-         Matrix<T>::template of_codes<false>(w[3]), Matrix<T>::template of_codes<true>(w[3])};
+  a = widen8<T>(w[0], w[1]);
+  b = widen8<T>(w[2], w[3]);
 }
 // Whether a NaN code (0x7F, 0xFF) is among 16.
 __device__ __forceinline__ bool has_nan(u4 w) {
@@ -180,14 +193,28 @@ __device__ __forceinline__ bool has_nan(u4 w) {
   for (int i = 0; i < 4; ++i) found |= ((w[i] & 0x7F7F7F7Fu) ^ 0x7F7F7F7Fu) - 0x01010101u;
   return found & 0x80808080u;
 }
+// Takes the NaN codes out of 16 of a key's values and notes the key at their dims:
+// lowest[d] is the first key whose value is NaN there.
+__device__ __forceinline__ void take_nan(u4& w, int32_t key, int32_t* lowest) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (((w[i] >> (8 * j)) & 0x7Fu) == 0x7Fu) {
+        atomicMin(lowest + i * 4 + j, key);
+        w[i] &= ~(0xFFu << (8 * j));
+      }
+}
 
 // Row strides of LDS tiles in elements of 16 bits.  K is read in 16-byte pieces
 // of consecutive rows: a stride of an odd number of them meets every bank once.
-// V is read in 32-byte pieces of four rows: an odd number of those does.
+// V is read in pieces of four rows: 64 bytes each for tiles of 32 rows, 32 bytes
+// each for tiles of 16; an odd number of those does.
 template <int DP>
 struct Strides {
   static constexpr int K = DP + 8;
   static constexpr int V = DP + (DP / 32 % 2 ? 0 : 32);
+  static constexpr int V16 = DP + 16;
 };
 
 // A sequence's part of the work.
@@ -373,43 +400,6 @@ __device__ __forceinline__ void mix(State<DP>& st, const f16v (&s)[N], const TV*
         st.o[i] = Matrix<TV>::mul(values8<TV, Strides<DP>::V>(v, n * 32 + kb * 16, i, lane), p, st.o[i]);
     }
 }
-// The same where a value is NaN and not every row sees every key: a key's value
-// reaches the rows that see it alone.  One pass for each token of the wavefront,
-// its keys' values alone, into its rows alone.
-template <typename TV, int DP, int N>
-__device__ __forceinline__ void mix_apart(State<DP>& st, const f16v (&s)[N], const TV* v, uint32_t lane, int32_t limit, int32_t k0) {
-  int32_t done = -1;
-  for (;;) {
-    int32_t next = limit > done ? limit : 0x7FFFFFFF;  // the lowest limit not done
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) next = min(next, __shfl_xor(next, o, 64));
-    if (next == 0x7FFFFFFF) break;
-    done = next;
-#pragma unroll
-    for (int i = 0; i < DP / 32; ++i) {
-      f16v part;
-#pragma unroll
-      for (int j = 0; j < 16; ++j) part[j] = 0.f;
-#pragma unroll
-      for (int n = 0; n < N; ++n)
-#pragma unroll
-        for (int kb = 0; kb < 2; ++kb) {
-          typename Matrix<TV>::v8 a = values8<TV, Strides<DP>::V>(v, n * 32 + kb * 16, i, lane);
-#pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            const int32_t key = k0 + n * 32 + kb * 16 + (int32_t)(lane >> 5) * 4 + (j & 3) + (j >> 2) * 8;
-            if (key >= next) a[j] = (TV)0.f;
-          }
-          part = Matrix<TV>::mul(a, pack8<TV>(s[n], kb), part);
-        }
-      if (limit == next) {
-#pragma unroll
-        for (int j = 0; j < 16; ++j) st.o[i][j] += part[j];
-      }
-    }
-  }
-}
-
 // Scores of unseen keys to -inf: bit k of `bits` is key k of the tile, the row
 // sees keys below `limit`.
 template <int N>
@@ -437,6 +427,15 @@ __device__ __forceinline__ void scale16(f16v (&s)[N], const KeyInfo& info, float
       for (int j = 0; j < 8; ++j) s[n][kb * 8 + j] *= f;
     }
 }
+// The values' scales go into the weights, as multiples of the largest so far (a
+// power of two; what is summed is scaled along): so the weights fit a half.
+// Whether a scale raises that.
+__device__ __forceinline__ bool raises(float vs, float ref) { return vs > ref && vs <= 3.4028235e38f; }
+__device__ __forceinline__ float power_of(float vs) {
+  return __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, vs) & 0x7F800000u);
+}
+__device__ __forceinline__ float inverse_of(float ref) { return ref > 0.f ? 1.f / ref : 0.f; }
+
 // After the scales of the values: infinite ones leave unseen keys at zero.
 template <int N>
 __device__ __forceinline__ void hide_weights(f16v (&s)[N], uint64_t bits, int32_t k0, int32_t limit, uint32_t half) {
@@ -516,12 +515,13 @@ __device__ __forceinline__ Place place_of(const AttendPlan& p) {
 // unseen values become zeros and codes 16-bit numbers.
 template <typename T, int DP, bool PAGED>
 __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void tile_kernel(AttendPlan p) {
-  typedef typename std::conditional<PAGED, __bf16, T>::type TV;
+  typedef T TV;
   constexpr int KT = 64, kPer = PAGED ? DP / 16 : DP / 8;        // pieces of a row
   constexpr int kPieces = KT * kPer, kMine = (kPieces + 255) / 256;
   constexpr int KS = Strides<DP>::K, VS = Strides<DP>::V;
   __shared__ __align__(16) uint16_t lds_k[KT * KS];
   __shared__ __align__(16) uint16_t lds_v[KT * VS];
+  __shared__ int32_t lowest[PAGED ? DP : 1];  // keys with NaN values, where rows see different keys
   const uint32_t tid = threadIdx.x, lane = tid & 63u, half = (tid >> 5) & 1u, wave = tid >> 6;
   const Place w = place_of(p);
   const Sequence seq = sequence_of<PAGED>(p, w.b);
@@ -546,6 +546,9 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void tile_kernel(AttendPlan
   u4 q[DP / 16];
   load_query<T, DP>(p, w.b, w.h, t, g, live, half, q);
   State<DP> st;
+  float ref = PAGED ? 0.f : 1.f, inv_ref = ref;
+  if constexpr (PAGED)
+    for (uint32_t d = tid; d < (uint32_t)DP; d += 256) lowest[d] = 0x7FFFFFFF;
 
   u4 rk[kMine], rv[kMine];
   KeyInfo next;
@@ -575,7 +578,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void tile_kernel(AttendPlan
   if (range.begin < range.end) fetch(range.begin);
   for (int32_t k0 = range.begin; k0 < range.end; k0 += KT) {
     __syncthreads();  // the tile before is read
-    bool nan = false;
+    const bool edge = k0 + KT > least;
 #pragma unroll
     for (int i = 0; i < kMine; ++i) {
       const uint32_t piece = tid + i * 256, r = piece / kPer, col = piece - r * kPer;
@@ -585,10 +588,10 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void tile_kernel(AttendPlan
           widen<T>(rk[i], a, b);
           *reinterpret_cast<u4*>(lds_k + r * KS + col * 16) = a;
           *reinterpret_cast<u4*>(lds_k + r * KS + col * 16 + 8) = b;
+          if (edge && has_nan(rv[i])) take_nan(rv[i], k0 + (int32_t)r, lowest + col * 16);
           widen<TV>(rv[i], a, b);
           *reinterpret_cast<u4*>(lds_v + r * VS + col * 16) = a;
           *reinterpret_cast<u4*>(lds_v + r * VS + col * 16 + 8) = b;
-          nan |= has_nan(rv[i]);
         } else {
           *reinterpret_cast<u4*>(lds_k + r * KS + col * 8) = rk[i];
           *reinterpret_cast<u4*>(lds_v + r * VS + col * 8) = rv[i];
@@ -597,9 +600,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void tile_kernel(AttendPlan
     }
     const KeyInfo info = next;
     const uint64_t bits = __ballot(info.seen);
-    bool apart = false;
-    if (PAGED && k0 + KT > least) apart = __syncthreads_or(nan);
-    else __syncthreads();
+    __syncthreads();
     if (k0 + KT < range.end) fetch(k0 + KT);
     if (idle || k0 >= wave_most) continue;
 
@@ -620,11 +621,33 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void tile_kernel(AttendPlan
     if (!whole) hide<2>(s, bits, k0, limit, half);
     soften<TV, DP, 2>(st, s, p.c);
     if constexpr (PAGED) {
-      scale16<2>(s, info, &KeyInfo::vs);
+      if (__any(raises(info.vs, ref))) {
+        float most_vs = raises(info.vs, ref) ? info.vs : ref;
+        most_vs = power_of(group_max<64>(most_vs));
+        const float a = ref * inverse_of(most_vs);
+#pragma unroll
+        for (int i = 0; i < DP / 32; ++i)
+#pragma unroll
+          for (int j = 0; j < 16; ++j) st.o[i][j] *= a;
+        ref = most_vs;
+        inv_ref = inverse_of(ref);
+      }
+      KeyInfo part = info;
+      part.vs *= inv_ref;
+      scale16<2>(s, part, &KeyInfo::vs);
       if (!whole) hide_weights<2>(s, bits, k0, limit, half);
     }
-    if (PAGED && apart) mix_apart<TV, DP, 2>(st, s, reinterpret_cast<const TV*>(lds_v), lane, limit, k0);
-    else mix<TV, DP, 2>(st, s, reinterpret_cast<const TV*>(lds_v), lane);
+    mix<TV, DP, 2>(st, s, reinterpret_cast<const TV*>(lds_v), lane);
+  }
+  if constexpr (PAGED) {
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < DP / 32; ++i)
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        st.o[i][j] *= ref;
+        if (limit > lowest[i * 32 + j / 4 * 8 + half * 4 + j % 4]) st.o[i][j] = __builtin_nanf("");
+      }
   }
   const float l = st.l + lane_xor<32>(st.l);
   if (mine && (p.splits == 1 || range.begin < range.end)) {
@@ -634,146 +657,317 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void tile_kernel(AttendPlan
 }
 
 // ---------------------------------------------------------------- few rows
-// Up to 32 rows of a head, as a token's or a few drafts' are: four wavefronts
-// take tiles of 32 keys in turn, each on its own, and join at the end.  Keys go
-// from memory to the operand's registers (a lane's 32 bytes, or 16 codes, are of
-// one key), values through the wavefront's own part of LDS.
-template <typename T, int DP, bool PAGED>
-__global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void few_kernel(AttendPlan p) {
-  typedef typename std::conditional<PAGED, __bf16, T>::type TV;
-  constexpr int KT = 32, W = 4, kPer = PAGED ? DP / 16 : DP / 8, kMine = KT * kPer / 64;
-  constexpr int VS = Strides<DP>::V;
+// Up to 16 R rows of a head, as a token's or a few drafts' are: bound by the keys'
+// and values' way from memory.  Four wavefronts take tiles of 32 keys in turn,
+// each on its own (no barrier in the loop), and join at the end.  Matrix tiles of
+// 16 rows: S^T = K Q^T is two of 16 keys, a lane holding one row (lane & 15) and
+// keys 4 (lane / 16) + 0..3 of each, which are the eight of its B operand.  Keys go
+// from memory to the A operand's registers (a lane's bytes are of one key), values
+// through the wavefront's own part of LDS.  A page holds whole groups of 16
+// tokens, so that a matrix tile has one page and one scale, which stay scalar.
+// Registers for the sums are half of what tiles of 32 rows take: 16 wavefronts
+// a CU, each with its next 32 keys in flight.
+
+// Step s of q . k takes dims dim_of() .. + 8 of quarter q of the lanes: 16 codes
+// (32 bytes of 16-bit numbers) in one piece where the head is wide enough.
+template <int DP>
+__device__ __forceinline__ constexpr uint32_t dim_of(uint32_t s, uint32_t quarter) {
+  return DP % 64 == 0 ? (s / 2) * 64 + quarter * 16 + (s % 2) * 8 : s * 32 + quarter * 8;
+}
+
+template <typename T, int DP, bool PAGED, int R>
+__global__ __launch_bounds__(256, DP * R <= 64 ? 4 : DP <= 128 && DP * R <= 128 ? 3 : DP <= 128 || (PAGED && R == 1) ? 2 : 1) void few_kernel(AttendPlan p) {
+  typedef typename Matrix<T>::v8 v8;
+  constexpr int KT = 32, W = 4, kSteps = DP / 32;
+  constexpr int kPer = PAGED ? DP / 16 : DP / 8, kMine = KT * kPer / 64;  // pieces of a value row, of a lane
+  constexpr int VS = Strides<DP>::V16;
   constexpr int kDims = DP % 64 ? 32 : 64;
-  constexpr int kTile = KT * VS * 2, kJoin = 32 * (kDims + 4) * 4;  // bytes of a wavefront's values, of its sums
+  constexpr int kTile = KT * VS * 2, kJoin = 16 * R * (kDims + 4) * 4;  // bytes of a wavefront's values, of its sums
   __shared__ __align__(16) char lds[W * (kTile > kJoin ? kTile : kJoin)];
-  __shared__ float lds_m[W][32], lds_l[W][32], row_m[32], row_l[32];
-  const uint32_t tid = threadIdx.x, lane = tid & 63u, half = (tid >> 5) & 1u, wave = tid >> 6, col = lane & 31u;
+  __shared__ float lds_m[W][16 * R], lds_l[W][16 * R], row_m[16 * R], row_l[16 * R];
+  __shared__ int32_t lowest[PAGED ? DP : 1];
+  const uint32_t tid = threadIdx.x, lane = tid & 63u, col = lane & 15u, quarter = lane >> 4;
+  const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(tid >> 6));
   const Place w = place_of(p);
   const Sequence seq = sequence_of<PAGED>(p, w.b);
-  const uint32_t t = p.by_group.div(col), g = col - t * p.group;
-  const bool mine = col < p.rows, live = mine && (int32_t)t < seq.tokens;
-  const int32_t limit = live ? limit_of<PAGED>(seq, (int32_t)t) : 0x7FFFFFFF;
   const int32_t most = seq.tokens > 0 ? limit_of<PAGED>(seq, seq.tokens - 1) : 0, least = limit_of<PAGED>(seq, 0);
   const Range range = range_of(most, w.split, p.splits, KT);
-  TV* lds_v = reinterpret_cast<TV*>(lds + wave * kTile);
+  T* lds_v = reinterpret_cast<T*>(lds + wave * kTile);
 
-  u4 q[DP / 16];
-  load_query<T, DP>(p, w.b, w.h, t, g, live, half, q);
-  State<DP> st;
-
-  constexpr int kKeys = PAGED ? DP / 32 : DP / 16;  // 16-byte pieces of a lane's key
-  u4 rk[kKeys], rv[kMine];
-  KeyInfo next;
-  const auto fetch_keys = [&](int32_t k0) {
-    const int32_t key = k0 + (int32_t)col;
-    next = key_info<PAGED>(p, w.b, w.h, key, range.end);
+  u4 q[R][kSteps];
+  int32_t limit[R];
 #pragma unroll
-    for (int i = 0; i < kKeys; ++i) {
-      rk[i] = u4{0, 0, 0, 0};
-      if constexpr (PAGED) {
-        const uint32_t d = i * 32 + half * 16;
-        if (next.seen && d < p.dim) {
-          const uint32_t at = (uint32_t)key - p.by_page.div((uint32_t)key) * p.page_size;
-          rk[i] = load16(code_at(p.kp, next.id, w.h, at) + d);
-        }
+  for (int r = 0; r < R; ++r) {
+    const uint32_t row = r * 16 + col, t = p.by_group.div(row), g = row - t * p.group;
+    const bool live = row < p.rows && (int32_t)t < seq.tokens;
+    limit[r] = live ? limit_of<PAGED>(seq, (int32_t)t) : 0;
+    const T* x = static_cast<const T*>(p.q) + w.b * p.q_batch + t * p.q_token + (w.h * p.group + g) * p.q_head;
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s) {
+      q[r][s] = u4{0, 0, 0, 0};
+      if (live && dim_of<DP>(s, quarter) < p.dim) q[r][s] = load16(x + dim_of<DP>(s, quarter));
+    }
+  }
+  f4 o[R][DP / 16];
+  float m[R], l[R];
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    m[r] = -__builtin_inff();
+    l[r] = 0.f;
+#pragma unroll
+    for (int i = 0; i < DP / 16; ++i) o[r][i] = f4{0.f, 0.f, 0.f, 0.f};
+  }
+  float ref = PAGED ? 0.f : 1.f, inv_ref = ref;
+  if constexpr (PAGED) {
+    for (uint32_t d = tid; d < (uint32_t)DP; d += 256) lowest[d] = 0x7FFFFFFF;
+    __syncthreads();
+  }
+
+  // PAGED: lane i knows the 16 keys i of the wavefront's next 32 tiles (i / 2 the tile, i % 2 its half)
+  int32_t page_id = -1;
+  float page_ks = 0.f, page_vs = 0.f;
+  const auto look_up = [&](int32_t k0) {
+    const int32_t key = k0 + (int32_t)(lane >> 1) * (W * KT) + (int32_t)(lane & 1u) * 16;
+    page_id = -1;
+    page_ks = page_vs = 0.f;
+    if (key < range.end) {
+      page_id = p.table[w.b * p.table_batch + p.by_page.div((uint32_t)key) * p.table_slot];
+      if ((uint32_t)page_id >= p.pages) {
+        page_id = -1;
       } else {
-        const uint32_t d = (i / 2) * 32 + half * 16 + (i % 2) * 8;
-        if (next.seen && d < p.dim)
-          rk[i] = load16(static_cast<const T*>(p.k.data) + w.b * p.k.batch + (int64_t)key * p.k.key + w.h * p.k.head + d);
+        page_ks = p.kp.scales[page_id * p.kp.scale_page + w.h * p.kp.scale_head];
+        page_vs = p.vp.scales[page_id * p.vp.scale_page + w.h * p.vp.scale_head];
       }
     }
   };
-  const auto fetch_values = [&](int32_t k0) {
-    const uint64_t bits = __ballot(next.seen);
+
+  // what is loaded of the next tile
+  u4 rk[2][PAGED ? (kSteps + 1) / 2 : kSteps];
+  u4 rv[kMine];
+  int32_t id[2] = {0, 0};
+  float ks[2] = {0.f, 0.f}, vs[2] = {0.f, 0.f};
+  bool seen = true;  // of key lane & 31
+  const auto fetch = [&](int32_t k0, int32_t ahead) {  // `ahead` tiles behind the last look_up()
+    if constexpr (PAGED) {
+      const uint8_t* kb[2];
+      const uint8_t* vb[2];
 #pragma unroll
-    for (int i = 0; i < kMine; ++i) {
-      const uint32_t piece = lane + i * 64, r = piece / kPer, c = piece - r * kPer;
-      const uint32_t key = (uint32_t)k0 + r;
-      rv[i] = u4{0, 0, 0, 0};
-      if constexpr (PAGED) {
-        const int32_t id = __shfl(next.id, (int)r, 64);
-        if (((bits >> r) & 1u) && c * 16 < p.dim) {
-          rv[i] = load16(code_at(p.vp, id, w.h, key - p.by_page.div(key) * p.page_size) + c * 16);
+      for (int n = 0; n < 2; ++n) {
+        id[n] = __builtin_amdgcn_readlane(page_id, ahead * 2 + n);
+        ks[n] = lane_value(page_ks, ahead * 2 + n);
+        vs[n] = lane_value(page_vs, ahead * 2 + n);
+        const uint32_t key = (uint32_t)k0 + n * 16, at = key - p.by_page.div(key) * p.page_size;
+        kb[n] = code_at(p.kp, id[n], w.h, at);
+        vb[n] = code_at(p.vp, id[n], w.h, at);
+      }
+      const uint32_t key_off = col * (uint32_t)p.kp.token;
+#pragma unroll
+      for (int n = 0; n < 2; ++n)
+#pragma unroll
+        for (int i = 0; i < (kSteps + 1) / 2; ++i) {
+          rk[n][i] = u4{0, 0, 0, 0};
+          if (id[n] >= 0) {
+            if constexpr (DP % 64 == 0) {
+              const uint32_t d = i * 64 + quarter * 16;
+              if (d < p.dim) rk[n][i] = load16(kb[n] + key_off + d);
+            } else {
+#pragma unroll
+              for (int e = 0; e < 2; ++e) {
+                const uint32_t d = (2 * i + e) * 32 + quarter * 8;
+                if (2 * i + e < kSteps && d < p.dim) {
+                  typedef uint32_t u2e __attribute__((ext_vector_type(2), aligned(1)));
+                  const u2e x = *reinterpret_cast<const u2e*>(kb[n] + key_off + d);
+                  rk[n][i][2 * e] = x[0];
+                  rk[n][i][2 * e + 1] = x[1];
+                }
+              }
+            }
+          }
         }
-      } else {
-        if (((bits >> r) & 1u) && c * 8 < p.dim)
-          rv[i] = load16(static_cast<const T*>(p.v.data) + w.b * p.v.batch + (int64_t)key * p.v.key + w.h * p.v.head + c * 8);
+#pragma unroll
+      for (int i = 0; i < kMine; ++i) {
+        const uint32_t piece = lane + i * 64, r = piece / kPer, c = (piece - r * kPer) * 16;
+        // the rows of one load are of the first half, of the second, or of both
+        const uint32_t off = (r & 15u) * (uint32_t)p.vp.token + c;
+        rv[i] = u4{0, 0, 0, 0};
+        if (i * 64 + 63 < 16 * kPer) {
+          if (id[0] >= 0 && c < p.dim) rv[i] = load16(vb[0] + off);
+        } else if (i * 64 >= 16 * kPer) {
+          if (id[1] >= 0 && c < p.dim) rv[i] = load16(vb[1] + off);
+        } else {
+          if ((r < 16 ? id[0] : id[1]) >= 0 && c < p.dim) rv[i] = load16((r < 16 ? vb[0] : vb[1]) + off);
+        }
+      }
+    } else {
+      const int32_t mine = k0 + (int32_t)(lane & 31u);
+      seen = mine < range.end;
+      if (p.mask && seen) seen = p.mask[w.b * p.mask_batch + mine * p.mask_key] != 0;
+      const T* kb = static_cast<const T*>(p.k.data) + w.b * p.k.batch + w.h * p.k.head;
+      const T* vb = static_cast<const T*>(p.v.data) + w.b * p.v.batch + w.h * p.v.head;
+      // keys past the last read the last
+#pragma unroll
+      for (int n = 0; n < 2; ++n) {
+        const T* row = kb + (int64_t)min(k0 + n * 16 + (int32_t)col, range.end - 1) * p.k.key;
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s) {
+          const uint32_t d = dim_of<DP>(s, quarter);
+          rk[n][s] = u4{0, 0, 0, 0};
+          if (d < p.dim) rk[n][s] = load16(row + d);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < kMine; ++i) {
+        const uint32_t piece = lane + i * 64, r = piece / kPer, c = (piece - r * kPer) * 8;
+        rv[i] = u4{0, 0, 0, 0};
+        if (c < p.dim) rv[i] = load16(vb + (int64_t)min(k0 + (int32_t)r, range.end - 1) * p.v.key + c);
       }
     }
   };
-  int32_t k0 = range.begin + (int32_t)wave * KT;
+
+  int32_t k0 = range.begin + (int32_t)wave * KT, ahead = 0;
   if (k0 < range.end) {
-    fetch_keys(k0);
-    fetch_values(k0);
+    if (PAGED) look_up(k0);
+    fetch(k0, 0);
   }
   for (; k0 < range.end; k0 += W * KT) {
-    const KeyInfo info = next;
-    const uint64_t bits = __ballot(info.seen);  // the halves alike
-    f16v s[1];
+    // scores
+    f4 s[R][2];
 #pragma unroll
-    for (int j = 0; j < 16; ++j) s[0][j] = 0.f;
+    for (int n = 0; n < 2; ++n) {
 #pragma unroll
-    for (int i = 0; i < DP / 32; ++i) {
-      u4 a, b;
-      if constexpr (PAGED) {
-        widen<T>(rk[i], a, b);
-      } else {
-        a = rk[2 * i];
-        b = rk[2 * i + 1];
+      for (int r = 0; r < R; ++r) s[r][n] = f4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int i = 0; i < kSteps; ++i) {
+        u4 a;
+        if constexpr (PAGED) a = widen8<T>(rk[n][i / 2][i % 2 * 2], rk[n][i / 2][i % 2 * 2 + 1]);
+        else a = rk[n][i];
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+          s[r][n] = Matrix<T>::mul16(__builtin_bit_cast(v8, a), __builtin_bit_cast(v8, q[r][i]), s[r][n]);
       }
-      typedef typename Matrix<T>::v8 v8;
-      s[0] = Matrix<T>::mul(__builtin_bit_cast(v8, a), __builtin_bit_cast(v8, q[2 * i]), s[0]);
-      s[0] = Matrix<T>::mul(__builtin_bit_cast(v8, b), __builtin_bit_cast(v8, q[2 * i + 1]), s[0]);
     }
-    bool nan = false;
+    // which keys every live row sees
+    uint32_t bits;
+    if constexpr (PAGED) bits = (id[0] >= 0 ? 0xFFFFu : 0u) | (id[1] >= 0 ? 0xFFFF0000u : 0u);
+    else bits = (uint32_t)__ballot(seen);
+    const bool whole = bits == ~0u && k0 + KT <= least;
+    // values to LDS
     wave_lds_fence();
 #pragma unroll
     for (int i = 0; i < kMine; ++i) {
       const uint32_t piece = lane + i * 64, r = piece / kPer, c = piece - r * kPer;
       if constexpr (PAGED) {
+        if (!whole && has_nan(rv[i])) take_nan(rv[i], k0 + (int32_t)r, lowest + c * 16);
         u4 a, b;
-        widen<TV>(rv[i], a, b);
+        widen<T>(rv[i], a, b);
         *reinterpret_cast<u4*>(lds_v + r * VS + c * 16) = a;
         *reinterpret_cast<u4*>(lds_v + r * VS + c * 16 + 8) = b;
-        nan |= has_nan(rv[i]);
       } else {
+        if (!whole && !((bits >> r) & 1u)) rv[i] = u4{0, 0, 0, 0};
         *reinterpret_cast<u4*>(lds_v + r * VS + c * 8) = rv[i];
       }
     }
     wave_lds_fence();
+    const float ks0 = ks[0], ks1 = ks[1], vs0 = vs[0], vs1 = vs[1];
     if (k0 + W * KT < range.end) {
-      fetch_keys(k0 + W * KT);
-      fetch_values(k0 + W * KT);
+      if (PAGED && ++ahead == 32) {
+        look_up(k0 + W * KT);
+        ahead = 0;
+      }
+      fetch(k0 + W * KT, ahead);
     }
-    const bool whole = bits == ~0ull && k0 + KT <= least;
-    if constexpr (PAGED) scale16<1>(s, info, &KeyInfo::ks);
-    if (!whole) hide<1>(s, bits, k0, limit, half);
-    soften<TV, DP, 1>(st, s, p.c);
     if constexpr (PAGED) {
-      scale16<1>(s, info, &KeyInfo::vs);
-      if (!whole) hide_weights<1>(s, bits, k0, limit, half);
+      if (raises(vs0, ref) || raises(vs1, ref)) {
+        const float top = power_of(fmaxf(raises(vs0, ref) ? vs0 : ref, raises(vs1, ref) ? vs1 : ref)), a = ref * inverse_of(top);
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+#pragma unroll
+          for (int i = 0; i < DP / 16; ++i) o[r][i] *= a;
+        ref = top;
+        inv_ref = inverse_of(ref);
+      }
     }
-    if (PAGED && k0 + KT > least && __any(nan)) mix_apart<TV, DP, 1>(st, s, lds_v, lane, limit, k0);
-    else mix<TV, DP, 1>(st, s, lds_v, lane);
+    // exponentials
+    v8 pr[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const int32_t left = limit[r] - k0 - (int32_t)quarter * 4;
+      const uint32_t mine = bits >> (quarter * 4);
+      if constexpr (PAGED) {
+        s[r][0] *= ks0;
+        s[r][1] *= ks1;
+      }
+      if (!whole) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (!((mine >> (j / 4 * 16 + j % 4)) & 1u) || j / 4 * 16 + j % 4 >= left) s[r][j / 4][j % 4] = -__builtin_inff();
+      }
+      float top = s[r][0][0];
+#pragma unroll
+      for (int j = 1; j < 8; ++j) top = fmaxf(top, s[r][j / 4][j % 4]);
+      top = fmaxf(top, lane_xor<16>(top));
+      top = fmaxf(top, lane_xor<32>(top));
+      if (__any(top > m[r])) {
+        const float to = fmaxf(m[r], top), a = rescale_of(m[r], to, p.c);
+        l[r] *= a;
+#pragma unroll
+        for (int i = 0; i < DP / 16; ++i) o[r][i] *= a;
+        m[r] = to;
+      }
+      const float off = offset_of(m[r], p.c, 0.f) + Matrix<T>::kShift;
+      float sum = 0.f;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r][j / 4][j % 4], p.c, off));
+        sum += e;
+        if constexpr (PAGED) {
+          e *= (j < 4 ? vs0 : vs1) * inv_ref;
+          if (!whole && (!((mine >> (j / 4 * 16 + j % 4)) & 1u) || j / 4 * 16 + j % 4 >= left)) e = 0.f;
+        }
+        pr[r][j] = (T)e;
+      }
+      l[r] += sum;
+    }
+    // values, 16 dims a time
+#pragma unroll
+    for (int i = 0; i < DP / 16; ++i) {
+      const uint32_t at = (quarter * 4 + (col >> 2)) * VS + i * 16 + (col & 3u) * 4;
+      union {
+        s4 part[2];
+        v8 all;
+      } v;
+      v.part[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4*)(lds_v + at));
+      v.part[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4*)(lds_v + at + 16 * VS));
+#pragma unroll
+      for (int r = 0; r < R; ++r) o[r][i] = Matrix<T>::mul16(v.all, pr[r], o[r][i]);
+    }
   }
 
   // join the wavefronts, kDims dims at a time
-  float l = st.l + lane_xor<32>(st.l);
-  if (half == 0) {
-    lds_m[wave][col] = st.m;
-    lds_l[wave][col] = l;
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    l[r] += lane_xor<16>(l[r]);
+    l[r] += lane_xor<32>(l[r]);
+    if (quarter == 0) {
+      lds_m[wave][r * 16 + col] = m[r];
+      lds_l[wave][r * 16 + col] = l[r];
+    }
   }
   __syncthreads();
-  float m = lds_m[0][col];
+  float a[R];
 #pragma unroll
-  for (int i = 1; i < W; ++i) m = fmaxf(m, lds_m[i][col]);
-  const float a = rescale_of(st.m, m, p.c);
-  l = 0.f;
+  for (int r = 0; r < R; ++r) {
+    const uint32_t row = r * 16 + col;
+    float top = lds_m[0][row], sum = 0.f;
 #pragma unroll
-  for (int i = 0; i < W; ++i) l += lds_l[i][col] * rescale_of(lds_m[i][col], m, p.c);
-  if (wave == 0 && half == 0) {
-    row_m[col] = m;
-    row_l[col] = l;
+    for (int i = 1; i < W; ++i) top = fmaxf(top, lds_m[i][row]);
+#pragma unroll
+    for (int i = 0; i < W; ++i) sum += lds_l[i][row] * rescale_of(lds_m[i][row], top, p.c);
+    a[r] = rescale_of(m[r], top, p.c) * ref;
+    if (wave == 0 && quarter == 0) {
+      row_m[row] = top;
+      row_l[row] = sum;
+    }
   }
   float* sums = reinterpret_cast<float*>(lds);
   const uint64_t unit = (uint64_t)w.b * p.heads + w.h;
@@ -781,13 +975,11 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void few_kernel(AttendPlan 
 #pragma unroll
   for (int part = 0; part < DP / kDims; ++part) {
 #pragma unroll
-    for (int i = 0; i < kDims / 32; ++i)
+    for (int r = 0; r < R; ++r)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        f4 v;
-#pragma unroll
-        for (int k = 0; k < 4; ++k) v[k] = st.o[part * (kDims / 32) + i][j * 4 + k] * a;
-        *reinterpret_cast<f4*>(sums + (wave * 32 + col) * (kDims + 4) + i * 32 + j * 8 + half * 4) = v;
+      for (int i = 0; i < kDims / 16; ++i) {
+        f4 v = o[r][part * (kDims / 16) + i] * a[r];
+        *reinterpret_cast<f4*>(sums + (wave * 16 * R + r * 16 + col) * (kDims + 4) + i * 16 + quarter * 4) = v;
       }
     __syncthreads();
     for (uint32_t at = tid; at < p.rows * (kDims / 4); at += 256) {
@@ -796,14 +988,21 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void few_kernel(AttendPlan 
       float v[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int i = 0; i < W; ++i) {
-        const f4 x = *reinterpret_cast<const f4*>(sums + (i * 32 + r) * (kDims + 4) + c);
+        const f4 x = *reinterpret_cast<const f4*>(sums + (i * 16 * R + r) * (kDims + 4) + c);
 #pragma unroll
         for (int k = 0; k < 4; ++k) v[k] += x[k];
       }
       const uint32_t rt = p.by_group.div(r), rg = r - rt * p.group;
+      const bool live = (int32_t)rt < seq.tokens;
+      if constexpr (PAGED) {
+        const int32_t row_limit = live ? limit_of<PAGED>(seq, (int32_t)rt) : 0;
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          if (row_limit > lowest[d + k]) v[k] = __builtin_nanf("");
+      }
       if (p.splits == 1) {
         const float total = row_l[r];
-        const bool none = (int32_t)rt >= seq.tokens || total == 0.f;
+        const bool none = !live || total == 0.f;
         const float inv = 1.f / total;
 #pragma unroll
         for (int k = 0; k < 4; ++k) v[k] = none ? 0.f : v[k] * inv;
@@ -871,7 +1070,8 @@ template <typename T, int DP, bool PAGED>
 thin_status launch_attend_dim(const AttendPlan& p, hipStream_t stream) {
   const bool few = p.rows <= kFewRows;
   const uint32_t grid = p.batch * p.heads * p.row_blocks * p.splits;
-  if (few) hipLaunchKernelGGL((dev::few_kernel<T, DP, PAGED>), dim3(grid), dim3(256), 0, stream, p);
+  if (p.rows <= 16) hipLaunchKernelGGL((dev::few_kernel<T, DP, PAGED, 1>), dim3(grid), dim3(256), 0, stream, p);
+  else if (few) hipLaunchKernelGGL((dev::few_kernel<T, DP, PAGED, 2>), dim3(grid), dim3(256), 0, stream, p);
   else hipLaunchKernelGGL((dev::tile_kernel<T, DP, PAGED>), dim3(grid), dim3(256), 0, stream, p);
   THIN_LAUNCH_CHECK("attend");
   if (p.splits > 1) {

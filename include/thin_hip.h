@@ -576,8 +576,9 @@ size_t thin_verify_drafts_workspace(int64_t batch, int64_t vocab);
  *     or if that leaves nothing: the first token at which the running sum passes
  *     sample[b] times the total;
  *   out [B, K + 1] int64: the n drafts, that token, then -1.
- * Probabilities that are not positive and finite count as 0; if all do, the next
- * token is -1.  Products and sums in 64 bits.  The workspace is 8-byte aligned and
+ * Target probabilities that are not positive and finite count as 0; a draft whose
+ * own is not finite falls, and so does the part of a token whose draft probability
+ * is not.  If nothing has a part, the next token is -1.  Products and sums in 64 bits.  The workspace is 8-byte aligned and
  * overlaps no operand.  The selection of the reference (selection_flow.cpp:429-499)
  * with given chances in place of the order. */
 thin_status thin_verify_drafts(const thin_desc* target, const thin_desc* draft, const thin_desc* tokens,

@@ -13,6 +13,10 @@ Modules (each function cites the reference file:line it restates):
   norm       -- group norm in 64 bits
   experts    -- routing, dispatch and combine in 64 bits, token by token
   logprobs   -- token log probabilities, entropy and alternatives in 64 bits
+  rotary     -- rotary positions with several axes in 64 bits
+  attend     -- attention to the keys that each row sees, in 64 bits
+  cache      -- e4m3 codes and scales of the paged cache in exact arithmetic
+  drafts     -- verification of drafted tokens with exact fractions
 
 Pinning status of every function is listed in its module docstring.
 """

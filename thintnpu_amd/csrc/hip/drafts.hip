@@ -48,6 +48,9 @@ struct DraftPlan {
   int32_t* stayed;  // [batch]
 };
 
+// A probability; what is none counts as 0.
+__device__ __forceinline__ double positive(double x) { return x > 0.0 && x <= 1.7976931348623157e308 ? x : 0.0; }
+
 // How many drafts stay; every lane of a wavefront gets it.
 template <typename T>
 __device__ __forceinline__ uint32_t stayed_of(const DraftPlan& p, uint32_t b, uint32_t lane, uint32_t& count) {
@@ -57,7 +60,7 @@ __device__ __forceinline__ uint32_t stayed_of(const DraftPlan& p, uint32_t b, ui
   if (lane < count) {
     const int64_t x = p.tokens[b * p.tb + lane * p.tk];
     if (x >= 0 && x < (int64_t)p.vocab) {
-      const double pt = (double)(float)static_cast<const T*>(p.target)[b * p.pb + lane * p.pk + x];
+      const double pt = positive((double)(float)static_cast<const T*>(p.target)[b * p.pb + lane * p.pk + x]);
       const double qt = p.draft ? (double)(float)static_cast<const T*>(p.draft)[b * p.qb + lane * p.qk + x] : 1.0;
       stays = (double)p.accept[b * p.ub + lane * p.uk] * qt < pt;
     }
@@ -65,8 +68,6 @@ __device__ __forceinline__ uint32_t stayed_of(const DraftPlan& p, uint32_t b, ui
   const uint64_t fell = ~__ballot(stays);
   return fell ? (uint32_t)__builtin_ctzll(fell) : 64u;
 }
-
-__device__ __forceinline__ double positive(double x) { return x > 0.0 && x <= 1.7976931348623157e308 ? x : 0.0; }
 
 // The row that the next token comes from.
 template <typename T>

@@ -82,6 +82,7 @@ inline int padded_dim(int64_t d) {
 constexpr int64_t kSplitKeys = 256;
 constexpr int64_t kWorkgroups = 512, kFewWorkgroups = 2048;
 constexpr int64_t kMaxSplits = 128;
+constexpr uint32_t kJoinByWave = 8;  // splits that one wavefront joins; more take a workgroup
 inline int64_t splits_of(int64_t units, int64_t rows, int64_t keys) {
   const int64_t most = (keys + kSplitKeys - 1) / kSplitKeys;
   const int64_t want = (rows <= kFewRows ? kFewWorkgroups : kWorkgroups) / (units > 0 ? units : 1);
@@ -1021,14 +1022,15 @@ __global__ __launch_bounds__(256, DP * R <= 64 ? 4 : DP <= 128 && DP * R <= 128 
 }
 
 // ---------------------------------------------------------------- splits
-// One wavefront a row: its splits' sums at their highest maximum, four dims a
-// lane (a row's dims past 256 do not exist).
-template <typename T, bool PAGED>
+// A row's splits at their highest maximum, by E threads: four dims a thread, and
+// as many splits side by side as that leaves threads for (128 splits of 240 rows
+// took 62 us by one wavefront a row, split after split).
+template <typename T, bool PAGED, int E>
 __global__ __launch_bounds__(256) void join_kernel(AttendPlan p, uint32_t few) {
-  const uint32_t lane = threadIdx.x & 63u, block_rows = few ? p.rows : kBlockRows;
-  const uint64_t at = (uint64_t)blockIdx.x * 4 + (threadIdx.x >> 6);  // (b, h, row)
-  const uint64_t units = (uint64_t)p.batch * p.heads;
-  if (at >= units * p.rows) return;
+  __shared__ f4 part[256];
+  const uint32_t lane = threadIdx.x & 63u, mine = threadIdx.x % E, block_rows = few ? p.rows : kBlockRows;
+  const uint64_t at = (uint64_t)blockIdx.x * (256 / E) + threadIdx.x / E;  // (b, h, row)
+  if (E < 256 && at >= (uint64_t)p.batch * p.heads * p.rows) return;
   const uint32_t unit = (uint32_t)(at / p.rows), row = (uint32_t)(at - (uint64_t)unit * p.rows);
   const uint32_t b = p.by_heads.div(unit), h = unit - b * p.heads;
   const uint32_t t = p.by_group.div(row), g = row - t * p.group;
@@ -1039,27 +1041,38 @@ __global__ __launch_bounds__(256) void join_kernel(AttendPlan p, uint32_t few) {
   const int32_t most = t_last < t_first ? 0 : limit_of<PAGED>(seq, t_last);
   const int32_t n = (int32_t)t < seq.tokens ? active_splits(most, p.splits, few ? 32 : 64) : 0;
   const uint64_t first = ((uint64_t)unit * p.row_blocks + block) * p.splits * block_rows + (row - block * block_rows);
-  float m = -__builtin_inff();
+  // every wavefront knows the maximum and the total
+  float m = -__builtin_inff(), l = 0.f;
   for (int32_t i = (int32_t)lane; i < n; i += 64) m = fmaxf(m, p.stats[(first + (uint64_t)i * block_rows) * 2]);
   m = group_max<64>(m);
-  float l = 0.f, v[4] = {0.f, 0.f, 0.f, 0.f};
-  const uint32_t d = lane * 4;
-  for (int32_t i = 0; i < n; ++i) {
-    const uint64_t slot = first + (uint64_t)i * block_rows;
-    const float f = rescale_of(p.stats[slot * 2], m, p.c);
-    l += p.stats[slot * 2 + 1] * f;
-    if (d < p.dim) {
+  for (int32_t i = (int32_t)lane; i < n; i += 64) {
+    const float* stats = p.stats + (first + (uint64_t)i * block_rows) * 2;
+    l += stats[1] * rescale_of(stats[0], m, p.c);
+  }
+  l = group_sum<64>(l);
+  const uint32_t quads = p.dim / 4, sides = E / quads, side = mine / quads, d = (mine - side * quads) * 4;
+  f4 v = {0.f, 0.f, 0.f, 0.f};
+  if (side < sides) {
+#pragma unroll 4
+    for (int32_t i = (int32_t)side; i < n; i += (int32_t)sides) {
+      const uint64_t slot = first + (uint64_t)i * block_rows;
       float x[4];
       load_pack<float, 4>(p.sums + slot * p.dim + d, x);
+      const float f = rescale_of(p.stats[slot * 2], m, p.c);
 #pragma unroll
       for (int k = 0; k < 4; ++k) v[k] += x[k] * f;
     }
   }
-  if (d < p.dim) {
+  part[threadIdx.x] = v;
+  if (E == 256) __syncthreads();
+  else wave_lds_fence();
+  if (side == 0) {
+    for (uint32_t i = 1; i < sides; ++i) v += part[threadIdx.x + i * quads];
     const float r = 1.f / l;
+    float o[4];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) v[k] = n == 0 || l == 0.f ? 0.f : v[k] * r;
-    store_pack<T, 4>(static_cast<T*>(p.out) + b * p.o_batch + t * p.o_token + (h * p.group + g) * p.o_head + d, v);
+    for (int k = 0; k < 4; ++k) o[k] = n == 0 || l == 0.f ? 0.f : v[k] * r;
+    store_pack<T, 4>(static_cast<T*>(p.out) + b * p.o_batch + t * p.o_token + (h * p.group + g) * p.o_head + d, o);
   }
 }
 
@@ -1076,7 +1089,10 @@ thin_status launch_attend_dim(const AttendPlan& p, hipStream_t stream) {
   THIN_LAUNCH_CHECK("attend");
   if (p.splits > 1) {
     const uint64_t rows = (uint64_t)p.batch * p.heads * p.rows;
-    hipLaunchKernelGGL((dev::join_kernel<T, PAGED>), dim3((uint32_t)((rows + 3) / 4)), dim3(256), 0, stream, p, few ? 1u : 0u);
+    if (p.splits <= kJoinByWave)
+      hipLaunchKernelGGL((dev::join_kernel<T, PAGED, 64>), dim3((uint32_t)((rows + 3) / 4)), dim3(256), 0, stream, p, few ? 1u : 0u);
+    else
+      hipLaunchKernelGGL((dev::join_kernel<T, PAGED, 256>), dim3((uint32_t)rows), dim3(256), 0, stream, p, few ? 1u : 0u);
     THIN_LAUNCH_CHECK("attend_join");
   }
   return THIN_OK;

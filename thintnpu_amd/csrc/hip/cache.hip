@@ -269,7 +269,7 @@ extern "C" thin_status thin_cache_attention(const thin_desc* q, const thin_desc*
   if (numel(q) == 0) return THIN_OK;
   const int64_t rows = T * (H / Hk), blocks = row_blocks_of(rows);
   THIN_REQUIRE(rows < (1ll << 30) && B < (1ll << 30) && launchable(B * Hk * blocks, 256) &&
-                   launchable((B * Hk * rows + 3) / 4, 256),
+                   launchable(B * Hk * rows, 256),
                THIN_ERR_UNSUPPORTED, "cache_attention: tensor too large");
   THIN_REQUIRE(!repeats(out), THIN_ERR_INVALID, "cache_attention: out has a stride of 0");
   for (const thin_desc* in : {q, k_cache, v_cache, k_scales, v_scales, table, lengths, counts})

@@ -45,7 +45,7 @@ extern "C" thin_status thin_cross_attention(const thin_desc* q, const thin_desc*
   if (numel(q) == 0) return THIN_OK;
   const int64_t rows = T * (H / Hk), blocks = row_blocks_of(rows);
   THIN_REQUIRE(rows < (1ll << 30) && S < (1ll << 30) && B < (1ll << 30) && launchable(B * Hk * blocks, 256) &&
-                   launchable((B * Hk * rows + 3) / 4, 256),
+                   launchable(B * Hk * rows, 256),
                THIN_ERR_UNSUPPORTED, "cross_attention: tensor too large");
   THIN_REQUIRE(!repeats(out), THIN_ERR_INVALID, "cross_attention: out has a stride of 0");
   for (const thin_desc* in : {q, k, v, lengths, mask})

@@ -24,7 +24,7 @@ constexpr int kChunk = 2048;       // elements of a workgroup at a time: 8 a thr
 constexpr int64_t kMaxDrafts = 64; // one lane each
 constexpr int64_t kMaxVocab = 1 << 23;
 constexpr int64_t kWorkgroups = 1024;
-constexpr int64_t kMostChunks = 8;
+constexpr int64_t kMostChunks = 4;
 
 struct DraftPlan {
   const void* target;
@@ -42,7 +42,7 @@ struct DraftPlan {
   int64_t ob, ok;
   int32_t* taken;
   int64_t taken_step;
-  uint32_t drafts, vocab, tiles, chunks;  // chunks of a tile
+  uint32_t drafts, vocab, tiles;
   FastDiv by_tiles;
   double* sums;     // [batch, tiles, 2]: of what is left, of the target's row
   int32_t* stayed;  // [batch]
@@ -125,12 +125,13 @@ struct Shared {
   uint32_t found, last;
 };
 
-// Sums of a tile's 8 * 256 * chunks elements; every thread gets them.
-template <typename T>
-__device__ __forceinline__ void tile_sums(const Rest<T>& rest, uint32_t first, uint32_t chunks, Shared& lds, double& left, double& own) {
+// Sums of a tile's 8 * 256 * CHUNKS elements; every thread gets them.
+template <typename T, int CHUNKS>
+__device__ __forceinline__ void tile_sums(const Rest<T>& rest, uint32_t first, Shared& lds, double& left, double& own) {
   const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
   left = own = 0.0;
-  for (uint32_t c = 0; c < chunks; ++c) {
+#pragma unroll 2
+  for (int c = 0; c < CHUNKS; ++c) {
     double a[8], o[8];
     rest.load(first + c * kChunk + threadIdx.x * 8, a, o);
 #pragma unroll
@@ -152,60 +153,67 @@ __device__ __forceinline__ void tile_sums(const Rest<T>& rest, uint32_t first, u
 }
 
 // The first element of a tile whose sum, with `before` ahead of the tile, passes
-// `edge`; where rounding leaves none, the tile's last that has a part.
-template <typename T>
-__device__ __forceinline__ uint32_t find_in_tile(const Rest<T>& rest, bool whole, uint32_t first, uint32_t chunks, double before,
-                                                 double edge, Shared& lds) {
-  const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
+// `edge`; where rounding leaves none, the tile's last that has a part.  Thread i
+// holds the i-th 8 * CHUNKS elements.
+template <typename T, int CHUNKS>
+__device__ __forceinline__ uint32_t find_in_tile(const Rest<T>& rest, bool whole, uint32_t first, double before, double edge,
+                                                 Shared& lds) {
+  const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, at = first + threadIdx.x * 8 * CHUNKS;
   if (threadIdx.x == 0) {
     lds.found = 0xFFFFFFFFu;
     lds.last = 0;
   }
-  for (uint32_t c = 0; c < chunks; ++c) {
-    const uint32_t at = first + c * kChunk + threadIdx.x * 8;
-    double a[8], o[8], sum = 0.0;
-    rest.load(at, a, o);
+  double x[8 * CHUNKS], sum = 0.0;
+#pragma unroll
+  for (int c = 0; c < CHUNKS; ++c) {
+    double a[8], o[8];
+    rest.load(at + c * 8, a, o);
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      if (whole) a[j] = o[j];
-      sum += a[j];
+      x[c * 8 + j] = whole ? o[j] : a[j];
+      sum += x[c * 8 + j];
     }
-    const double scan = wave_scan(sum, lane);
-    __syncthreads();
-    if (lane == 63) lds.left[wave] = scan;
-    __syncthreads();
-    double base = before;
-    for (uint32_t i = 0; i < wave; ++i) base += lds.left[i];
-    double run = base + (scan - sum);
-    uint32_t found = 0xFFFFFFFFu, last = 0;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      run += a[j];
-      if (a[j] > 0.0) {
-        last = at + j;
-        if (run > edge && found == 0xFFFFFFFFu) found = at + j;
-      }
-    }
-    if (found != 0xFFFFFFFFu) atomicMin(&lds.found, found);
-    if (last) atomicMax(&lds.last, last);
-    before += ((lds.left[0] + lds.left[1]) + lds.left[2]) + lds.left[3];
   }
+  const double scan = wave_scan(sum, lane);
+  if (lane == 63) lds.left[wave] = scan;
+  __syncthreads();
+  for (uint32_t i = 0; i < wave; ++i) before += lds.left[i];
+  double run = before + (scan - sum);
+  uint32_t found = 0xFFFFFFFFu, last = 0;
+#pragma unroll
+  for (int j = 0; j < 8 * CHUNKS; ++j) {
+    run += x[j];
+    if (x[j] > 0.0) {
+      last = at + j;
+      if (run > edge) found = min(found, at + j);
+    }
+  }
+  if (found != 0xFFFFFFFFu) atomicMin(&lds.found, found);
+  if (last) atomicMax(&lds.last, last);
   __syncthreads();
   return lds.found != 0xFFFFFFFFu ? lds.found : lds.last;
 }
 
-// The sequence's tokens, the last of them `next`.
-__device__ __forceinline__ void store_tokens(const DraftPlan& p, uint32_t b, uint32_t stayed, int64_t next) {
-  for (uint32_t i = threadIdx.x; i <= p.drafts; i += 256)
-    p.out[b * p.ob + i * p.ok] = i < stayed ? p.tokens[b * p.tb + i * p.tk] : i == stayed ? next : -1;
-  if (threadIdx.x == 0) p.taken[b * p.taken_step] = (int32_t)stayed;
-}
-__device__ __forceinline__ double edge_of(const DraftPlan& p, uint32_t b, double total) {
-  const float r = p.sample[b * p.sample_step];
-  return (double)(r > 0.f ? fminf(r, 1.f) : 0.f) * total;
-}
+// What a sequence's result takes, loaded before anything waits: drafts of this
+// thread's places (K + 1 <= 65 of 256 threads) and the random number.
+struct Given {
+  int64_t token;
+  float sample;
+  __device__ __forceinline__ Given(const DraftPlan& p, uint32_t b) : token(-1), sample(p.sample[b * p.sample_step]) {
+    if (threadIdx.x < p.drafts) token = p.tokens[b * p.tb + threadIdx.x * p.tk];
+  }
+  __device__ __forceinline__ double edge(double total) const {
+    return (double)(sample > 0.f ? fminf(sample, 1.f) : 0.f) * total;
+  }
+  // The sequence's tokens, the last of them `next`.
+  __device__ __forceinline__ void store(const DraftPlan& p, uint32_t b, uint32_t stayed, int64_t next) const {
+    const uint32_t i = threadIdx.x;
+    if (i <= p.drafts) p.out[b * p.ob + i * p.ok] = i < stayed ? token : i == stayed ? next : -1;
+    if (i == 0) p.taken[b * p.taken_step] = (int32_t)stayed;
+  }
+};
 
-template <typename T>
+template <typename T, int CHUNKS>
 __global__ __launch_bounds__(256) void sums_kernel(DraftPlan p) {
   __shared__ Shared lds;
   const uint32_t b = p.by_tiles.div(blockIdx.x), tile = blockIdx.x - b * p.tiles;
@@ -213,12 +221,13 @@ __global__ __launch_bounds__(256) void sums_kernel(DraftPlan p) {
   const uint32_t stayed = stayed_of<T>(p, b, threadIdx.x & 63u, count);
   const Rest<T> rest(p, b, stayed, count);
   double left, own;
-  tile_sums(rest, tile * p.chunks * kChunk, p.chunks, lds, left, own);
+  tile_sums<T, CHUNKS>(rest, tile * (CHUNKS * kChunk), lds, left, own);
   if (p.tiles == 1) {
+    const Given given(p, b);
     const bool whole = !(left > 0.0);
     const double total = whole ? own : left;
-    const uint32_t next = find_in_tile(rest, whole, 0, p.chunks, 0.0, edge_of(p, b, total), lds);
-    store_tokens(p, b, stayed, total > 0.0 ? (int64_t)next : -1);
+    const uint32_t next = find_in_tile<T, CHUNKS>(rest, whole, 0, 0.0, given.edge(total), lds);
+    given.store(p, b, stayed, total > 0.0 ? (int64_t)next : -1);
   } else if (threadIdx.x == 0) {
     p.sums[blockIdx.x * 2ull] = left;
     p.sums[blockIdx.x * 2ull + 1] = own;
@@ -226,62 +235,49 @@ __global__ __launch_bounds__(256) void sums_kernel(DraftPlan p) {
   }
 }
 
-template <typename T>
+// Where a row's border lies: the first tile whose sum passes it (where rounding
+// leaves none, the last that has a part) and what is ahead of it.  64 tiles a
+// round, by every wavefront for itself.
+template <bool WHOLE>
+__device__ __forceinline__ bool find_tile(const DraftPlan& p, const double* sums, const Given& given, uint32_t lane,
+                                          uint32_t& tile, double& before, double& edge) {
+  const auto part = [&](uint32_t i) { return i + lane < p.tiles ? sums[(i + lane) * 2 + (WHOLE ? 1 : 0)] : 0.0; };
+  const double first = part(0), first_scan = wave_scan(first, lane);
+  double total = __shfl(first_scan, 63, 64);
+  for (uint32_t i = 64; i < p.tiles; i += 64) total += __shfl(wave_scan(part(i), lane), 63, 64);
+  if (!(total > 0.0)) return false;
+  edge = given.edge(total);
+  double ahead = 0.0;
+  for (uint32_t i = 0; i < p.tiles; i += 64) {
+    const double v = i ? part(i) : first, scan = i ? wave_scan(v, lane) : first_scan;
+    const uint64_t passed = __ballot(v > 0.0 && ahead + scan > edge), some = __ballot(v > 0.0);
+    if (some) {
+      const int l = passed ? __builtin_ctzll(passed) : 63 - __builtin_clzll(some);
+      tile = i + l;
+      before = __shfl(ahead + (scan - v), l, 64);
+      if (passed) break;
+    }
+    ahead += __shfl(scan, 63, 64);
+  }
+  return true;
+}
+
+template <typename T, int CHUNKS>
 __global__ __launch_bounds__(256) void find_kernel(DraftPlan p) {
   __shared__ Shared lds;
-  __shared__ uint32_t lds_tile;
-  __shared__ double lds_before, lds_edge;
-  __shared__ uint32_t lds_whole;
   const uint32_t b = blockIdx.x, lane = threadIdx.x & 63u;
   const double* sums = p.sums + (uint64_t)b * p.tiles * 2;
+  const Given given(p, b);
   const uint32_t stayed = (uint32_t)p.stayed[b];
   const int32_t n = p.counts ? p.counts[b * p.count_step] : (int32_t)p.drafts;
   const uint32_t count = (uint32_t)max(0, min(n, (int32_t)p.drafts));
   const Rest<T> rest(p, b, stayed, count);
-  if (threadIdx.x < 64) {
-    double left = 0.0, own = 0.0;
-    for (uint32_t i = 0; i < p.tiles; i += 64) {  // in the order of the scan below
-      const uint32_t at = i + lane;
-      double a = 0.0, o = 0.0;
-      if (at < p.tiles) {
-        a = sums[at * 2];
-        o = sums[at * 2 + 1];
-      }
-      left += __shfl(wave_scan(a, lane), 63, 64);
-      own += __shfl(wave_scan(o, lane), 63, 64);
-    }
-    const bool whole = !(left > 0.0);
-    const double total = whole ? own : left, edge = edge_of(p, b, total);
-    double before = 0.0, tile_before = 0.0;
-    uint32_t tile = 0xFFFFFFFFu, last = 0;
-    double last_before = 0.0;
-    for (uint32_t i = 0; i < p.tiles && tile == 0xFFFFFFFFu; i += 64) {
-      const uint32_t at = i + lane;
-      const double v = at < p.tiles ? sums[at * 2 + (whole ? 1 : 0)] : 0.0, scan = wave_scan(v, lane);
-      const uint64_t passed = __ballot(v > 0.0 && before + scan > edge), some = __ballot(v > 0.0);
-      const double ahead = before + (scan - v);
-      if (passed) {
-        const int l = __builtin_ctzll(passed);
-        tile = i + l;
-        tile_before = __shfl(ahead, l, 64);
-      }
-      if (some) {
-        const int l = 63 - __builtin_clzll(some);
-        last = i + l;
-        last_before = __shfl(ahead, l, 64);
-      }
-      before += __shfl(scan, 63, 64);
-    }
-    if (lane == 0) {
-      lds_tile = tile != 0xFFFFFFFFu ? tile : last;
-      lds_before = tile != 0xFFFFFFFFu ? tile_before : last_before;
-      lds_edge = edge;
-      lds_whole = whole | (total > 0.0 ? 2u : 0u);
-    }
-  }
-  __syncthreads();
-  const uint32_t next = find_in_tile(rest, lds_whole & 1u, lds_tile * p.chunks * kChunk, p.chunks, lds_before, lds_edge, lds);
-  store_tokens(p, b, stayed, lds_whole & 2u ? (int64_t)next : -1);
+  uint32_t tile = 0;
+  double before = 0.0, edge = 0.0;
+  const bool some = find_tile<false>(p, sums, given, lane, tile, before, edge);
+  const bool any = some || find_tile<true>(p, sums, given, lane, tile, before, edge);
+  const uint32_t next = find_in_tile<T, CHUNKS>(rest, !some, tile * (CHUNKS * kChunk), before, edge, lds);
+  given.store(p, b, stayed, any ? (int64_t)next : -1);
 }
 
 // Chunks of a tile: one, or as many as leave enough workgroups.
@@ -294,6 +290,17 @@ int64_t chunks_of(int64_t batch, int64_t vocab) {
 int64_t tiles_of(int64_t batch, int64_t vocab) {
   const int64_t per = kChunk * chunks_of(batch, vocab);
   return (vocab + per - 1) / per;
+}
+
+template <typename T, int CHUNKS>
+thin_status launch(const DraftPlan& p, int64_t batch, hipStream_t stream) {
+  hipLaunchKernelGGL((sums_kernel<T, CHUNKS>), dim3((uint32_t)(batch * p.tiles)), dim3(256), 0, stream, p);
+  THIN_LAUNCH_CHECK("verify_drafts");
+  if (p.tiles > 1) {
+    hipLaunchKernelGGL((find_kernel<T, CHUNKS>), dim3((uint32_t)batch), dim3(256), 0, stream, p);
+    THIN_LAUNCH_CHECK("verify_drafts_find");
+  }
+  return THIN_OK;
 }
 
 }  // namespace
@@ -378,7 +385,6 @@ extern "C" thin_status thin_verify_drafts(const thin_desc* target, const thin_de
   p.drafts = (uint32_t)K;
   p.vocab = (uint32_t)V;
   p.tiles = (uint32_t)tiles;
-  p.chunks = (uint32_t)chunks_of(B, V);
   p.by_tiles = FastDiv::make(p.tiles);
   if (tiles > 1) {
     p.sums = static_cast<double*>(workspace);
@@ -386,12 +392,10 @@ extern "C" thin_status thin_verify_drafts(const thin_desc* target, const thin_de
   }
   return with_float_type(target->dtype, [&](auto zero) {
     using T = decltype(zero);
-    hipLaunchKernelGGL((sums_kernel<T>), dim3((uint32_t)(B * tiles)), dim3(256), 0, stream, p);
-    THIN_LAUNCH_CHECK("verify_drafts");
-    if (tiles > 1) {
-      hipLaunchKernelGGL((find_kernel<T>), dim3((uint32_t)B), dim3(256), 0, stream, p);
-      THIN_LAUNCH_CHECK("verify_drafts_find");
+    switch (chunks_of(B, V)) {
+      case 1: return launch<T, 1>(p, B, stream);
+      case 2: return launch<T, 2>(p, B, stream);
+      default: return launch<T, 4>(p, B, stream);
     }
-    return THIN_OK;
   });
 }

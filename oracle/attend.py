@@ -50,8 +50,8 @@ def allowed(q, result, keys, extra=0.0):
         and by 2 u of itself times its constants;
       its exponent (in bits, log2(e) of that) by 4 u more of the score and the
         maximum; the exponential by 2 u, and by 2 u for each of up to 32 rescalings;
-      a weight is rounded once to the type (h), or, subnormal as a half, by 2^-37 of
-        the largest (they are scaled by 2^12); the total keeps the unrounded ones;
+      a weight is rounded once to the type (h), or, subnormal as a half, by 2^-33 of
+        the largest (they are scaled by 2^8); the total keeps the unrounded ones;
         one below 2^-126 of the largest, the least normal of 32 bits, is lost
         (`extra`: the largest value that a weight may come with);
       the sums over the keys by `keys` u at most, in the total and in the mix;
@@ -59,5 +59,5 @@ def allowed(q, result, keys, extra=0.0):
     out, size, reach = result
     u, h = 2.0 ** -24, torch.finfo(q.dtype).eps / 2
     eps = (q.shape[-1] + 12) * u * reach[..., None] * 1.01 + 80 * u
-    tiny = keys * (2.0 ** -37 if q.dtype == torch.float16 else 2.0 ** -126)
+    tiny = keys * (2.0 ** -33 if q.dtype == torch.float16 else 2.0 ** -126)
     return 1.01 * ((h + 2 * eps + 2 * keys * u) * size + h * out.abs()) + tiny * extra + torch.finfo(q.dtype).smallest_normal * torch.finfo(q.dtype).eps

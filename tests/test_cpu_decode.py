@@ -87,6 +87,8 @@ def test_cross_refusals():
     cross(UNSUPPORTED, k=desc((2, 2 ** 30, 2, 64)))
     cross(UNSUPPORTED, q=desc((2 ** 14, 2 ** 17, 4, 64)), k=desc((2 ** 14, 9, 2, 64)))
     cross(INVALID, out=desc((2, 3, 4, 64), strides=(768, 256, 0, 1)))
+    cross(UNSUPPORTED, k=desc((2, 9, 2, 64), strides=(64, 2 ** 25, 64, 1)))
+    cross(UNSUPPORTED, v=desc((2, 9, 2, 64), strides=(64, 2 ** 25, 64, 1)))
     q, k = desc((2, 3, 4, 64)), desc((2, 9, 2, 64))
     cross(INVALID, q=q, out=desc((2, 3, 4, 64), data=q.data))
     cross(INVALID, k=k, out=desc((2, 3, 4, 64), data=k.data + 64))
@@ -144,6 +146,7 @@ def test_cache_refusals():
             (UNSUPPORTED, dict(kc=desc((7, 2, 2048, 32), capi.U8), vc=desc((7, 2, 2048, 32), capi.U8))),
             (UNSUPPORTED, dict(kc=desc((7, 2, 16, 32), capi.U8, strides=(2048, 1024, 64, 2)))),
             (UNSUPPORTED, dict(vc=desc((7, 2, 16, 32), capi.U8, strides=(2048, 1024, 64, 2)))),
+            (UNSUPPORTED, dict(vc=desc((7, 2, 16, 32), capi.U8, strides=(64, 32, 2 ** 26, 1)))),
             (UNSUPPORTED, dict(table=desc((2, 2 ** 26), capi.I32)))):
         Parts(**given).write(code)
         Parts(**given).attend(code)

@@ -67,7 +67,7 @@ class Cache:
 def close(got, ref, q, keys, host):
     got, out = got.cpu().double(), ref[0]
     assert torch.equal(torch.isnan(got), torch.isnan(out))
-    # weights as multiples of the largest scale of the values: 448 * that is what 2^-37 counts
+    # weights as multiples of the largest scale of the values: 448 * that is what 2^-33 counts
     top = float(host[3][torch.isfinite(host[3])].max()) * 448 * 2
     allowed = attend.allowed(q, ref, keys, top)
     over = torch.isinf(got)  # past the largest of the type

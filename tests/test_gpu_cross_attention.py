@@ -172,11 +172,11 @@ def test_no_rows_and_no_states(gpu):
 
 
 def test_beyond_32_bits(gpu):
-    far = 2 ** 31 + 32
-    base = torch.empty(2 * far + 4096, dtype=torch.float16, device=gpu)
+    far = 2 ** 32 + 32  # from sample to sample; 2^25 - 8 from state to state
+    base = torch.empty(far + 2 ** 27, dtype=torch.float16, device=gpu)
     for t in (1, 40):
         q, k, v = inputs(2, t, 3, 1, 1, 32, torch.float16, t)
-        vk, vv = base.as_strided(k.shape, (64, far, 32, 1)), base.as_strided(v.shape, (64, far, 32, 1), 1024)
+        vk, vv = base.as_strided(k.shape, (far, 2 ** 25 - 8, 32, 1)), base.as_strided(v.shape, (far, 2 ** 25 - 8, 32, 1), 1024)
         vk.copy_(k)
         vv.copy_(v)
         check(gpu, q, k, v, views=(q.to(gpu), vk, vv, None, None))

@@ -146,7 +146,7 @@ template <>
 struct Matrix<__bf16> {
   typedef __bf16 v8 __attribute__((ext_vector_type(8)));
   typedef __bf16 v2 __attribute__((ext_vector_type(2)));
-  static constexpr float kShift = 0.f;
+  static constexpr float kShift = 0.f;  // (a bf16 has the exponents of 32 bits)
   static __device__ __forceinline__ f16v mul(v8 a, v8 b, f16v c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
   }
@@ -162,8 +162,9 @@ template <>
 struct Matrix<_Float16> {
   typedef _Float16 v8 __attribute__((ext_vector_type(8)));
   typedef _Float16 v2 __attribute__((ext_vector_type(2)));
-  // exponentials times 2^12 (the sum's too): 2^-26 of the largest is still a normal half
-  static constexpr float kShift = 12.f;
+  // exponentials times 2^8 (the sum's too): up to 2^12 with kSlack, and 2^-22 is
+  // still a normal half
+  static constexpr float kShift = 8.f;
   static __device__ __forceinline__ f16v mul(v8 a, v8 b, f16v c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
   }
@@ -263,32 +264,6 @@ __device__ __forceinline__ int32_t active_splits(int32_t n, uint32_t splits, int
   return (steps + per - 1) / per;
 }
 
-// What a lane knows of one key of a tile: PAGED, its page and the page's scales.
-struct KeyInfo {
-  int32_t id;
-  float ks, vs;
-  bool seen;
-};
-template <bool PAGED>
-__device__ __forceinline__ KeyInfo key_info(const AttendPlan& p, uint32_t b, uint32_t h, int32_t key, int32_t end) {
-  KeyInfo i;
-  i.id = 0;
-  i.ks = i.vs = 0.f;
-  i.seen = key < end;
-  if constexpr (PAGED) {
-    if (i.seen) {
-      i.id = p.table[b * p.table_batch + p.by_page.div((uint32_t)key) * p.table_slot];
-      i.seen = (uint32_t)i.id < p.pages;
-      if (i.seen) {
-        i.ks = p.kp.scales[i.id * p.kp.scale_page + h * p.kp.scale_head];
-        i.vs = p.vp.scales[i.id * p.vp.scale_page + h * p.vp.scale_head];
-      }
-    }
-  } else if (p.mask) {
-    if (i.seen) i.seen = p.mask[b * p.mask_batch + key * p.mask_key] != 0;
-  }
-  return i;
-}
 __device__ __forceinline__ float lane_value(float v, int lane) {
   return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), lane));
 }
@@ -311,19 +286,10 @@ __device__ __forceinline__ void load_query(const AttendPlan& p, uint32_t b, uint
   }
 }
 
-// A lane's running softmax and its row's mix, 32 dims a vector: dim
-// 32 i + 8 (j / 4) + 4 half + j % 4 is o[i][j].
-template <int DP>
-struct State {
-  float m, l;  // l: of this half's keys
-  f16v o[DP / 32];
-  __device__ __forceinline__ State() : m(-__builtin_inff()), l(0.f) {
-#pragma unroll
-    for (int i = 0; i < DP / 32; ++i)
-#pragma unroll
-      for (int j = 0; j < 16; ++j) o[i][j] = 0.f;
-  }
-};
+// The maximum that a row's exponentials stand against is raised where a score
+// passes it by kSlack bits, not by less: sums are rescaled in few tiles, and an
+// exponential is 2^kSlack at most.
+constexpr float kSlack = 4.f;
 
 // A row's exponentials are 2^(c s + offset_of(m)).  The offset is rounded, in
 // proportion to m; what is taken from one maximum to another goes by the
@@ -334,37 +300,6 @@ __device__ __forceinline__ float offset_of(float m, float c, float shift) {
 __device__ __forceinline__ float rescale_of(float from, float to, float c) {
   if (from == to) return 1.f;
   return from == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(offset_of(to, c, 0.f) - offset_of(from, c, 0.f));
-}
-
-// The next 32 * N keys' scores into the running softmax; s becomes the exponentials.
-template <typename TV, int DP, int N>
-__device__ __forceinline__ void soften(State<DP>& st, f16v (&s)[N], float c) {
-  float top = s[0][0];
-#pragma unroll
-  for (int n = 0; n < N; ++n)
-#pragma unroll
-    for (int j = 0; j < 16; ++j) top = fmaxf(top, s[n][j]);
-  top = fmaxf(top, lane_xor<32>(top));
-  const float m = fmaxf(st.m, top);
-  if (__any(m > st.m)) {
-    const float a = rescale_of(st.m, m, c);
-    st.l *= a;
-#pragma unroll
-    for (int i = 0; i < DP / 32; ++i)
-#pragma unroll
-      for (int j = 0; j < 16; ++j) st.o[i][j] *= a;
-    st.m = m;
-  }
-  const float off = offset_of(st.m, c, 0.f) + Matrix<TV>::kShift;
-  float sum = 0.f;
-#pragma unroll
-  for (int n = 0; n < N; ++n)
-#pragma unroll
-    for (int j = 0; j < 16; ++j) {
-      s[n][j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[n][j], c, off));
-      sum += s[n][j];
-    }
-  st.l += sum;
 }
 
 // Eight exponentials of a lane as the B operand: keys 16 kb + 4 half + {0..3, 8..11}.
@@ -388,46 +323,6 @@ __device__ __forceinline__ typename Matrix<TV>::v8 values8(const TV* v, int row,
   return r.all;
 }
 
-// o += V^T P^T over 32 * N keys of an LDS tile.
-template <typename TV, int DP, int N>
-__device__ __forceinline__ void mix(State<DP>& st, const f16v (&s)[N], const TV* v, uint32_t lane) {
-#pragma unroll
-  for (int n = 0; n < N; ++n)
-#pragma unroll
-    for (int kb = 0; kb < 2; ++kb) {
-      const typename Matrix<TV>::v8 p = pack8<TV>(s[n], kb);
-#pragma unroll
-      for (int i = 0; i < DP / 32; ++i)
-        st.o[i] = Matrix<TV>::mul(values8<TV, Strides<DP>::V>(v, n * 32 + kb * 16, i, lane), p, st.o[i]);
-    }
-}
-// Scores of unseen keys to -inf: bit k of `bits` is key k of the tile, the row
-// sees keys below `limit`.
-template <int N>
-__device__ __forceinline__ void hide(f16v (&s)[N], uint64_t bits, int32_t k0, int32_t limit, uint32_t half) {
-  const uint64_t mine = bits >> (half * 4);
-  const int32_t left = limit - k0 - (int32_t)half * 4;
-#pragma unroll
-  for (int n = 0; n < N; ++n)
-#pragma unroll
-    for (int j = 0; j < 16; ++j) {
-      const int key = n * 32 + (j / 4) * 8 + j % 4;
-      if (!((mine >> key) & 1u) || key >= left) s[n][j] = -__builtin_inff();
-    }
-}
-
-// PAGED: the scales of 16 keys each on scores and exponentials.
-template <int N>
-__device__ __forceinline__ void scale16(f16v (&s)[N], const KeyInfo& info, float KeyInfo::*which) {
-#pragma unroll
-  for (int n = 0; n < N; ++n)
-#pragma unroll
-    for (int kb = 0; kb < 2; ++kb) {
-      const float f = lane_value(info.*which, n * 32 + kb * 16);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) s[n][kb * 8 + j] *= f;
-    }
-}
 // The values' scales go into the weights, as multiples of the largest so far (a
 // power of two; what is summed is scaled along): so the weights fit a half.
 // Whether a scale raises that.
@@ -437,27 +332,20 @@ __device__ __forceinline__ float power_of(float vs) {
 }
 __device__ __forceinline__ float inverse_of(float ref) { return ref > 0.f ? 1.f / ref : 0.f; }
 
-// After the scales of the values: infinite ones leave unseen keys at zero.
-template <int N>
-__device__ __forceinline__ void hide_weights(f16v (&s)[N], uint64_t bits, int32_t k0, int32_t limit, uint32_t half) {
-  const uint64_t mine = bits >> (half * 4);
-  const int32_t left = limit - k0 - (int32_t)half * 4;
-#pragma unroll
-  for (int n = 0; n < N; ++n)
-#pragma unroll
-    for (int j = 0; j < 16; ++j) {
-      const int key = n * 32 + (j / 4) * 8 + j % 4;
-      if (!((mine >> key) & 1u) || key >= left) s[n][j] = 0.f;
-    }
-}
+// The weights take such a multiple f as a summand log2 f of their exponents, and
+// the total its share back as 1 / f.  Where f is 0 the total's share is taken with
+// 1, and the weights are zeros.
+__device__ __forceinline__ float share_of(float f) { return f == 0.f ? 1.f : f; }
 
-// A row's result: out, or its split's sums.
+// A row's result: out, or its split's sums.  Dim 32 i + 8 (j / 4) + 4 half + j % 4
+// of a row is o[i][j].
 template <typename T, int DP>
 __device__ __forceinline__ void store_row(const AttendPlan& p, uint32_t b, uint32_t h, uint32_t t, uint32_t g, uint64_t slot,
-                                          uint32_t half, bool live, const State<DP>& st, float l) {
+                                          uint32_t half, bool live, const f16v (&o)[DP / 32], float m, float l) {
   if (p.splits == 1) {
     T* row = static_cast<T*>(p.out) + b * p.o_batch + t * p.o_token + (h * p.group + g) * p.o_head;
-    const float r = live && l != 0.f ? 1.f / l : 0.f;
+    const bool none = !live || l == 0.f;
+    const float r = 1.f / l;
 #pragma unroll
     for (int i = 0; i < DP / 32; ++i)
 #pragma unroll
@@ -466,7 +354,7 @@ __device__ __forceinline__ void store_row(const AttendPlan& p, uint32_t b, uint3
         if (d < p.dim) {
           float v[4];
 #pragma unroll
-          for (int k = 0; k < 4; ++k) v[k] = r == 0.f ? 0.f : st.o[i][j * 4 + k] * r;
+          for (int k = 0; k < 4; ++k) v[k] = none ? 0.f : o[i][j * 4 + k] * r;
           store_pack<T, 4>(row + d, v);
         }
       }
@@ -480,12 +368,12 @@ __device__ __forceinline__ void store_row(const AttendPlan& p, uint32_t b, uint3
         if (d < p.dim) {
           float v[4];
 #pragma unroll
-          for (int k = 0; k < 4; ++k) v[k] = st.o[i][j * 4 + k];
+          for (int k = 0; k < 4; ++k) v[k] = o[i][j * 4 + k];
           store_pack<float, 4>(row + d, v);
         }
       }
     if (half == 0) {
-      p.stats[slot * 2] = st.m;
+      p.stats[slot * 2] = m;
       p.stats[slot * 2 + 1] = l;
     }
   }
@@ -511,134 +399,332 @@ __device__ __forceinline__ Place place_of(const AttendPlan& p) {
 }
 
 // ---------------------------------------------------------------- many rows
-// 128 rows a workgroup, 32 a wavefront; tiles of 64 keys go through registers
-// (the next one's loads are in flight while a tile is worked on) to LDS, where
-// unseen values become zeros and codes 16-bit numbers.
-template <typename T, int DP, bool PAGED>
-__global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void tile_kernel(AttendPlan p) {
-  typedef T TV;
-  constexpr int KT = 64, kPer = PAGED ? DP / 16 : DP / 8;        // pieces of a row
-  constexpr int kPieces = KT * kPer, kMine = (kPieces + 255) / 256;
+// 32 rows a wavefront, W wavefronts a workgroup, tiles of 64 keys.  A tile's keys
+// and values go through registers to LDS (unseen ones as zeros, codes as 16-bit
+// numbers), two tiles each there: while a tile's exponentials are taken and its
+// values mixed, the next one's scores are computed, the keys behind that and the
+// values of the next are written, and loads of one tile more are in flight.  So
+// one barrier a tile, and matrix instructions between the exponentials' own.
+// Rows: unseen states have -inf in the scores from the start (the accumulator's
+// first value).  Pages: rows that do not see a whole tile are masked afterwards.
+template <typename T, int DP, bool PAGED, int W>
+__global__ __launch_bounds__(64 * W, DP <= 128 ? 2 : 1) void tile_kernel(AttendPlan p) {
+  typedef typename Matrix<T>::v8 v8;
+  constexpr int KT = 64, NT = 64 * W;
+  constexpr int kPer = PAGED ? DP / 16 : DP / 8, kElems = PAGED ? 16 : 8;  // 16-byte pieces of a key, elements of one
+  constexpr int kMine = (16 * kPer + 63) / 64;                            // a lane's of 16 keys
+  static_assert(W == 4, "a wavefront stages 16 of a tile's 64 keys");
   constexpr int KS = Strides<DP>::K, VS = Strides<DP>::V;
-  __shared__ __align__(16) uint16_t lds_k[KT * KS];
-  __shared__ __align__(16) uint16_t lds_v[KT * VS];
+  __shared__ __align__(16) T lds_k[2][KT * KS];
+  __shared__ __align__(16) T lds_v[2][KT * VS];
+  __shared__ __align__(16) float lds_bias[2][PAGED ? 4 : KT];
   __shared__ int32_t lowest[PAGED ? DP : 1];  // keys with NaN values, where rows see different keys
-  const uint32_t tid = threadIdx.x, lane = tid & 63u, half = (tid >> 5) & 1u, wave = tid >> 6;
+  const uint32_t tid = threadIdx.x, lane = tid & 63u, half = (tid >> 5) & 1u;
+  const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(tid >> 6));
   const Place w = place_of(p);
   const Sequence seq = sequence_of<PAGED>(p, w.b);
-  const uint32_t row = w.block * kBlockRows + wave * 32 + (lane & 31u), t = p.by_group.div(row), g = row - t * p.group;
+  constexpr uint32_t kRows = 32 * W;
+  const uint32_t row = w.block * kRows + wave * 32 + (lane & 31u), t = p.by_group.div(row), g = row - t * p.group;
   const bool mine = row < p.rows, live = mine && (int32_t)t < seq.tokens;
   const int32_t limit = live ? limit_of<PAGED>(seq, (int32_t)t) : 0x7FFFFFFF;
   // the workgroup's first and last live rows
-  const int32_t t_first = (int32_t)p.by_group.div(w.block * kBlockRows);
-  const int32_t t_last = min((int32_t)p.by_group.div(min(p.rows, (w.block + 1) * kBlockRows) - 1), seq.tokens - 1);
+  const int32_t t_first = (int32_t)p.by_group.div(w.block * kRows);
+  const int32_t t_last = min((int32_t)p.by_group.div(min(p.rows, (w.block + 1) * kRows) - 1), seq.tokens - 1);
   const int32_t most = t_last < t_first ? 0 : limit_of<PAGED>(seq, t_last);
   const int32_t least = limit_of<PAGED>(seq, t_first);
   // this wavefront's
-  const bool idle = !__any(live);
   int32_t wave_least = limit, wave_most = live ? limit : 0;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
     wave_least = min(wave_least, __shfl_xor(wave_least, o, 64));
     wave_most = max(wave_most, __shfl_xor(wave_most, o, 64));
   }
+  wave_least = __builtin_amdgcn_readfirstlane(wave_least);
+  wave_most = __builtin_amdgcn_readfirstlane(wave_most);
   const Range range = range_of(most, w.split, p.splits, KT);
+  const int32_t tiles = (range.end - range.begin + KT - 1) / KT;
 
   u4 q[DP / 16];
   load_query<T, DP>(p, w.b, w.h, t, g, live, half, q);
-  State<DP> st;
+  f16v o[DP / 32];
+#pragma unroll
+  for (int i = 0; i < DP / 32; ++i)
+#pragma unroll
+    for (int j = 0; j < 16; ++j) o[i][j] = 0.f;
+  float m = -__builtin_inff(), l = 0.f;  // l: of this half's keys
   float ref = PAGED ? 0.f : 1.f, inv_ref = ref;
   if constexpr (PAGED)
-    for (uint32_t d = tid; d < (uint32_t)DP; d += 256) lowest[d] = 0x7FFFFFFF;
+    for (uint32_t d = tid; d < (uint32_t)DP; d += NT) lowest[d] = 0x7FFFFFFF;
 
+  // Stage s: keys of tile s and values of tile s - 1, 16 of each by a wavefront
+  // (PAGED: one page's).  Loads go by a buffer descriptor of the tile, so that a
+  // lane's offsets stay what they are from tile to tile; an offset past the
+  // descriptor's end is a zero.
+  constexpr uint32_t kNowhere = 0x80000000u;
   u4 rk[kMine], rv[kMine];
-  KeyInfo next;
-  const auto fetch = [&](int32_t k0) {
-    next = key_info<PAGED>(p, w.b, w.h, k0 + (int32_t)lane, range.end);
-    const uint64_t bits = __ballot(next.seen);
+  uint32_t k_off[kMine], v_off[kMine];
 #pragma unroll
-    for (int i = 0; i < kMine; ++i) {
-      const uint32_t piece = tid + i * 256, r = piece / kPer, col = piece - r * kPer;
-      rk[i] = rv[i] = u4{0, 0, 0, 0};
-      if constexpr (PAGED) {
-        const int32_t id = __shfl(next.id, (int)(r & 63u), 64);
-        if (r < (uint32_t)KT && ((bits >> r) & 1u) && col * 16 < p.dim) {
-          const uint32_t key = (uint32_t)k0 + r, at = key - p.by_page.div(key) * p.page_size;
-          rk[i] = load16(code_at(p.kp, id, w.h, at) + col * 16);
-          rv[i] = load16(code_at(p.vp, id, w.h, at) + col * 16);
-        }
-      } else {
-        if (((bits >> r) & 1u) && col * 8 < p.dim) {
-          const int64_t key = k0 + (int32_t)r;
-          rk[i] = load16(static_cast<const T*>(p.k.data) + w.b * p.k.batch + key * p.k.key + w.h * p.k.head + col * 8);
-          rv[i] = load16(static_cast<const T*>(p.v.data) + w.b * p.v.batch + key * p.v.key + w.h * p.v.head + col * 8);
-        }
-      }
+  for (int i = 0; i < kMine; ++i) {
+    const uint32_t n = lane + i * 64, key = n / kPer, col = n - key * kPer;
+    const bool have = n < 16u * kPer && col * kElems < p.dim;
+    const int64_t k_step = PAGED ? p.kp.token : p.k.key * (int64_t)sizeof(T), v_step = PAGED ? p.vp.token : p.v.key * (int64_t)sizeof(T);
+    k_off[i] = have ? key * (uint32_t)k_step + col * 16 : kNowhere;
+    v_off[i] = have ? key * (uint32_t)v_step + col * 16 : kNowhere;
+  }
+  uint64_t bits_k = 0, bits_v = 0;  // rows: the keys of the stage's tiles that are seen
+  uint32_t shown = 0;               // rows: the next tile's key `lane`
+  int32_t id_k = -1, id_v = -1, id_next = -1;  // PAGED: the pages of the wavefront's 16
+  const auto look_up = [&](int32_t tile) {
+    if constexpr (PAGED) {
+      const int32_t k = range.begin + tile * KT + (int32_t)wave * 16;
+      id_next = k < range.end ? p.table[w.b * p.table_batch + p.by_page.div((uint32_t)k) * p.table_slot] : -1;
+    } else {
+      const int32_t k = range.begin + tile * KT + (int32_t)lane;
+      shown = k < range.end;
+      if (shown && p.mask) shown = p.mask[w.b * p.mask_batch + k * p.mask_key];
     }
   };
-  if (range.begin < range.end) fetch(range.begin);
-  for (int32_t k0 = range.begin; k0 < range.end; k0 += KT) {
-    __syncthreads();  // the tile before is read
-    const bool edge = k0 + KT > least;
+  const auto fetch = [&](int32_t stage) {
+    const int32_t k0 = range.begin + stage * KT + (int32_t)wave * 16;
+    if constexpr (PAGED) {
+      id_v = id_k;
+      id_k = __builtin_amdgcn_readfirstlane(id_next);
+      if ((uint32_t)id_k >= p.pages) id_k = -1;
+      const auto rsrc_of = [&](const PagesOf& x, int32_t id, int32_t key) {
+        const uint32_t token = (uint32_t)key - p.by_page.div((uint32_t)key) * p.page_size;
+        return buffer_rsrc(code_at(x, id, w.h, token), id >= 0 ? kNowhere : 0u);
+      };
+      const auto kr = rsrc_of(p.kp, id_k, k0), vr = rsrc_of(p.vp, id_v, max(k0 - KT, 0));
 #pragma unroll
-    for (int i = 0; i < kMine; ++i) {
-      const uint32_t piece = tid + i * 256, r = piece / kPer, col = piece - r * kPer;
-      if (kPieces % 256 == 0 || piece < (uint32_t)kPieces) {
-        if constexpr (PAGED) {
-          u4 a, b;
-          widen<T>(rk[i], a, b);
-          *reinterpret_cast<u4*>(lds_k + r * KS + col * 16) = a;
-          *reinterpret_cast<u4*>(lds_k + r * KS + col * 16 + 8) = b;
-          if (edge && has_nan(rv[i])) take_nan(rv[i], k0 + (int32_t)r, lowest + col * 16);
-          widen<TV>(rv[i], a, b);
-          *reinterpret_cast<u4*>(lds_v + r * VS + col * 16) = a;
-          *reinterpret_cast<u4*>(lds_v + r * VS + col * 16 + 8) = b;
-        } else {
-          *reinterpret_cast<u4*>(lds_k + r * KS + col * 8) = rk[i];
-          *reinterpret_cast<u4*>(lds_v + r * VS + col * 8) = rv[i];
+      for (int i = 0; i < kMine; ++i) {
+        rk[i] = __builtin_bit_cast(u4, __builtin_amdgcn_raw_buffer_load_b128(kr, k_off[i], 0, 0));
+        rv[i] = __builtin_bit_cast(u4, __builtin_amdgcn_raw_buffer_load_b128(vr, v_off[i], 0, 0));
+      }
+    } else {
+      bits_v = bits_k;
+      bits_k = __ballot(shown != 0);
+      const uint32_t mine_k = (uint32_t)(bits_k >> (wave * 16)) & 0xFFFFu, mine_v = (uint32_t)(bits_v >> (wave * 16)) & 0xFFFFu;
+      const T* kb = static_cast<const T*>(p.k.data) + w.b * p.k.batch + w.h * p.k.head + (int64_t)k0 * p.k.key;
+      const T* vb = static_cast<const T*>(p.v.data) + w.b * p.v.batch + w.h * p.v.head + (int64_t)(k0 - KT) * p.v.key;
+      const auto kr = buffer_rsrc(kb, kNowhere), vr = buffer_rsrc(vb, kNowhere);
+      if (mine_k == 0xFFFFu && mine_v == 0xFFFFu) {
+#pragma unroll
+        for (int i = 0; i < kMine; ++i) {
+          rk[i] = __builtin_bit_cast(u4, __builtin_amdgcn_raw_buffer_load_b128(kr, k_off[i], 0, 0));
+          rv[i] = __builtin_bit_cast(u4, __builtin_amdgcn_raw_buffer_load_b128(vr, v_off[i], 0, 0));
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < kMine; ++i) {
+          const uint32_t key = (lane + i * 64) / kPer;
+          rk[i] = __builtin_bit_cast(u4, __builtin_amdgcn_raw_buffer_load_b128(kr, (mine_k >> key) & 1u ? k_off[i] : kNowhere, 0, 0));
+          rv[i] = __builtin_bit_cast(u4, __builtin_amdgcn_raw_buffer_load_b128(vr, (mine_v >> key) & 1u ? v_off[i] : kNowhere, 0, 0));
         }
       }
     }
-    const KeyInfo info = next;
-    const uint64_t bits = __ballot(info.seen);
-    __syncthreads();
-    if (k0 + KT < range.end) fetch(k0 + KT);
-    if (idle || k0 >= wave_most) continue;
-
-    f16v s[2];
+    look_up(stage + 1);
+  };
+  const auto store = [&](int32_t stage) {
+    T* kt = lds_k[stage & 1] + wave * 16 * KS;
+    T* vt = lds_v[(stage + 1) & 1] + wave * 16 * VS;
+    const int32_t v0 = range.begin + (stage - 1) * KT;  // the values' tile
+#pragma unroll
+    for (int i = 0; i < kMine; ++i) {
+      const uint32_t n = lane + i * 64, key = n / kPer, col = n - key * kPer;
+      if (16 * kPer % 64 && n >= 16u * kPer) continue;
+      if constexpr (PAGED) {
+        if (v0 + KT > least && has_nan(rv[i])) take_nan(rv[i], v0 + (int32_t)(wave * 16 + key), lowest + col * 16);
+        u4 a, b;
+        widen<T>(rk[i], a, b);
+        *reinterpret_cast<u4*>(kt + key * KS + col * 16) = a;
+        *reinterpret_cast<u4*>(kt + key * KS + col * 16 + 8) = b;
+        widen<T>(rv[i], a, b);
+        *reinterpret_cast<u4*>(vt + key * VS + col * 16) = a;
+        *reinterpret_cast<u4*>(vt + key * VS + col * 16 + 8) = b;
+      } else {
+        *reinterpret_cast<u4*>(kt + key * KS + col * 8) = rk[i];
+        *reinterpret_cast<u4*>(vt + key * VS + col * 8) = rv[i];
+      }
+    }
+    if (!PAGED && wave == 0) lds_bias[stage & 1][lane] = (bits_k >> lane) & 1u ? 0.f : -__builtin_inff();
+  };
+  // PAGED: lane i knows group i % 4 of 16 keys of a tile
+  struct Group {
+    float ks, vs;
+    bool seen;
+  };
+  const auto group_id = [&](int32_t tile) {
+    const int32_t k = range.begin + tile * KT + (int32_t)(lane & 3u) * 16;
+    int32_t i = -1;
+    if (k < range.end) i = p.table[w.b * p.table_batch + p.by_page.div((uint32_t)k) * p.table_slot];
+    return (uint32_t)i < p.pages ? i : -1;
+  };
+  const auto group_of = [&](int32_t i) {
+    Group x{0.f, 0.f, i >= 0};
+    if (i >= 0) {
+      x.ks = p.kp.scales[i * p.kp.scale_page + w.h * p.kp.scale_head];
+      x.vs = p.vp.scales[i * p.vp.scale_page + w.h * p.vp.scale_head];
+    }
+    return x;
+  };
+  const auto start_scores = [&](int32_t tile, f16v (&s)[2]) {
 #pragma unroll
     for (int n = 0; n < 2; ++n) {
 #pragma unroll
-      for (int j = 0; j < 16; ++j) s[n][j] = 0.f;
+      for (int j = 0; j < 4; ++j) {
+        f4 x = {0.f, 0.f, 0.f, 0.f};
+        if constexpr (!PAGED) x = *reinterpret_cast<const f4*>(lds_bias[tile & 1] + n * 32 + j * 8 + half * 4);
 #pragma unroll
-      for (int i = 0; i < DP / 16; ++i) {
-        const uint32_t d = (i / 2) * 32 + half * 16 + (i % 2) * 8;
-        const u4 k = *reinterpret_cast<const u4*>(lds_k + (n * 32 + (lane & 31u)) * KS + d);
-        s[n] = Matrix<T>::mul(__builtin_bit_cast(typename Matrix<T>::v8, k), __builtin_bit_cast(typename Matrix<T>::v8, q[i]), s[n]);
+        for (int e = 0; e < 4; ++e) s[n][j * 4 + e] = x[e];
       }
     }
-    const bool whole = bits == ~0ull && k0 + KT <= wave_least;
-    if constexpr (PAGED) scale16<2>(s, info, &KeyInfo::ks);
-    if (!whole) hide<2>(s, bits, k0, limit, half);
-    soften<TV, DP, 2>(st, s, p.c);
+  };
+  const auto scores = [&](int32_t tile, f16v (&s)[2]) {
+    const T* k = lds_k[tile & 1];
+    start_scores(tile, s);
+#pragma unroll
+    for (int i = 0; i < DP / 16; ++i)
+#pragma unroll
+      for (int n = 0; n < 2; ++n) {
+        const uint32_t d = (i / 2) * 32 + half * 16 + (i % 2) * 8;
+        const u4 x = *reinterpret_cast<const u4*>(k + (n * 32 + (lane & 31u)) * KS + d);
+        s[n] = Matrix<T>::mul(__builtin_bit_cast(v8, x), __builtin_bit_cast(v8, q[i]), s[n]);
+      }
+  };
+
+  f16v s[2], next[2];
+  Group group{0.f, 0.f, true}, group_next{0.f, 0.f, true};
+  int32_t group_far = -1;
+  if (tiles > 0) {
+    look_up(0);
     if constexpr (PAGED) {
-      if (__any(raises(info.vs, ref))) {
-        float most_vs = raises(info.vs, ref) ? info.vs : ref;
-        most_vs = power_of(group_max<64>(most_vs));
-        const float a = ref * inverse_of(most_vs);
+      group = group_of(group_id(0));
+      group_next = group_of(group_id(1));
+      group_far = group_id(2);
+    }
+    fetch(0);
+    store(0);
+    fetch(1);
+    __syncthreads();
+    store(1);
+    fetch(2);
+    scores(0, s);
+  }
+  for (int32_t tile = 0; tile < tiles; ++tile) {
+    const int32_t k0 = range.begin + tile * KT;
+    __syncthreads();
+    if (tile + 1 < tiles) {
+      store(tile + 2);
+      fetch(tile + 3);
+    }
+    Group now{0.f, 0.f, true};
+    if constexpr (PAGED) {
+      now = group;
+      group = group_next;
+      group_next = group_of(group_far);
+      group_far = group_id(tile + 3);
+    }
+    if (k0 >= wave_most) continue;
+    // the maximum
+    bool whole = true;
+    float ks[4], vs[4];
+    if constexpr (PAGED) {
+      const uint32_t groups = (uint32_t)__ballot(now.seen) & 15u;
+      whole = groups == 15u && k0 + KT <= wave_least;
+#pragma unroll
+      for (int n = 0; n < 4; ++n) ks[n] = lane_value(now.ks, n);
+      if (!whole) {
+        const int32_t left = limit - k0 - (int32_t)half * 4;
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
+#pragma unroll
+          for (int j = 0; j < 16; ++j)
+            if (!((groups >> (n * 2 + j / 8)) & 1u) || n * 32 + j / 4 * 8 + j % 4 >= left) s[n][j] = -__builtin_inff();
+      }
+      if (__any(raises(now.vs, ref))) {
+        const float top = power_of(group_max<64>(raises(now.vs, ref) ? now.vs : ref)), a = ref * inverse_of(top);
 #pragma unroll
         for (int i = 0; i < DP / 32; ++i)
 #pragma unroll
-          for (int j = 0; j < 16; ++j) st.o[i][j] *= a;
-        ref = most_vs;
+          for (int j = 0; j < 16; ++j) o[i][j] *= a;
+        ref = top;
         inv_ref = inverse_of(ref);
       }
-      KeyInfo part = info;
-      part.vs *= inv_ref;
-      scale16<2>(s, part, &KeyInfo::vs);
-      if (!whole) hide_weights<2>(s, bits, k0, limit, half);
+#pragma unroll
+      for (int n = 0; n < 4; ++n) vs[n] = lane_value(now.vs, n) * inv_ref;
     }
-    mix<TV, DP, 2>(st, s, reinterpret_cast<const TV*>(lds_v), lane);
+    float top = -__builtin_inff();
+#pragma unroll
+    for (int n = 0; n < 4; ++n) {
+      float x = s[n / 2][n % 2 * 8];
+#pragma unroll
+      for (int j = 1; j < 8; ++j) x = fmaxf(x, s[n / 2][n % 2 * 8 + j]);
+      top = fmaxf(top, PAGED ? x * ks[n] : x);  // a NaN of unseen keys' scales is dropped
+    }
+    top = fmaxf(top, lane_xor<32>(top));
+    if (__any((top - m) * p.c > kSlack || (m == -__builtin_inff() && top > m))) {
+      const float to = fmaxf(m, top), a = rescale_of(m, to, p.c);
+      l *= a;
+#pragma unroll
+      for (int i = 0; i < DP / 32; ++i)
+#pragma unroll
+        for (int j = 0; j < 16; ++j) o[i][j] *= a;
+      m = to;
+    }
+    const float off = offset_of(m, p.c, 0.f) + Matrix<T>::kShift;
+    // The next tile's scores beside this one's exponentials, a matrix instruction
+    // and its share of them at a time: the former take 32 cycles of their own
+    // unit, in which the wavefront goes on.  (After the last tile, scores of what
+    // LDS holds, which nobody takes.)
+    constexpr int kSteps = DP / 8, kAhead = 4;
+    start_scores(tile + 1, next);
+    const T* kt = lds_k[(tile + 1) & 1] + (lane & 31u) * KS + half * 16;
+    const T* vt = lds_v[tile & 1];
+    const auto key_piece = [&](int i) {  // of step i: keys 32 (i % 2), dims step i / 2
+      return *reinterpret_cast<const u4*>(kt + (i % 2) * 32 * KS + (i / 4) * 32 + (i / 2) % 2 * 8);
+    };
+    u4 ring[kAhead];
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) ring[i] = key_piece(i);
+    float c[4], add[4], sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int n = 0; n < 4; ++n) {
+      c[n] = PAGED ? p.c * ks[n] : p.c;
+      add[n] = PAGED ? off + __builtin_amdgcn_logf(share_of(vs[n])) : off;
+    }
+    v8 pr[4];
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int i = 0; i < kSteps; ++i) {
+      next[i % 2] = Matrix<T>::mul(__builtin_bit_cast(v8, ring[i % kAhead]), __builtin_bit_cast(v8, q[i / 2]), next[i % 2]);
+      if (i + kAhead < kSteps) ring[i % kAhead] = key_piece(i + kAhead);
+#pragma unroll
+      for (int x = i * 32 / kSteps; x < (i + 1) * 32 / kSteps; ++x) {
+        const int n = x / 8, j = x % 8;
+        const float score = s[n / 2][n % 2 * 8 + j];
+        float e = __builtin_amdgcn_exp2f(__builtin_fmaf(score, c[n], add[n]));
+        if (PAGED && !whole && score == -__builtin_inff()) e = 0.f;  // whatever its scales are
+        sum[n] += e;
+        pr[n][j] = (T)e;
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+#pragma unroll
+    for (int n = 0; n < 4; ++n) {
+      if (PAGED && (whole || sum[n] != 0.f)) sum[n] *= __builtin_amdgcn_rcpf(share_of(vs[n]));  // (nothing of unseen keys' scales)
+      l += sum[n];
+      if (PAGED && vs[n] == 0.f) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) pr[n][j] = (T)0.f;
+      }
+    }
+    // its values
+#pragma unroll
+    for (int n = 0; n < 4; ++n)
+#pragma unroll
+      for (int i = 0; i < DP / 32; ++i) o[i] = Matrix<T>::mul(values8<T, VS>(vt, n * 16, i, lane), pr[n], o[i]);
+#pragma unroll
+    for (int n = 0; n < 2; ++n) s[n] = next[n];
   }
   if constexpr (PAGED) {
     __syncthreads();
@@ -646,14 +732,14 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void tile_kernel(AttendPlan
     for (int i = 0; i < DP / 32; ++i)
 #pragma unroll
       for (int j = 0; j < 16; ++j) {
-        st.o[i][j] *= ref;
-        if (limit > lowest[i * 32 + j / 4 * 8 + half * 4 + j % 4]) st.o[i][j] = __builtin_nanf("");
+        o[i][j] *= ref;
+        if (limit > lowest[i * 32 + j / 4 * 8 + half * 4 + j % 4]) o[i][j] = __builtin_nanf("");
       }
   }
-  const float l = st.l + lane_xor<32>(st.l);
-  if (mine && (p.splits == 1 || range.begin < range.end)) {
+  l += lane_xor<32>(l);
+  if (mine && (p.splits == 1 || tiles > 0)) {
     const uint64_t unit = ((uint64_t)w.b * p.heads + w.h) * p.row_blocks + w.block;
-    store_row<T, DP>(p, w.b, w.h, t, g, (unit * p.splits + w.split) * kBlockRows + (row - w.block * kBlockRows), half, live, st, l);
+    store_row<T, DP>(p, w.b, w.h, t, g, (unit * p.splits + w.split) * kRows + (row - w.block * kRows), half, live, o, m, l);
   }
 }
 
@@ -869,7 +955,7 @@ __global__ __launch_bounds__(256, DP * R <= 64 ? 4 : DP <= 128 && DP * R <= 128 
       }
     }
     wave_lds_fence();
-    const float ks0 = ks[0], ks1 = ks[1], vs0 = vs[0], vs1 = vs[1];
+    const float ks0 = PAGED ? ks[0] : 1.f, ks1 = PAGED ? ks[1] : 1.f, vs0 = vs[0], vs1 = vs[1];
     if (k0 + W * KT < range.end) {
       if (PAGED && ++ahead == 32) {
         look_up(k0 + W * KT);
@@ -889,26 +975,35 @@ __global__ __launch_bounds__(256, DP * R <= 64 ? 4 : DP <= 128 && DP * R <= 128 
       }
     }
     // exponentials
+    float c[2] = {p.c, p.c}, add[2] = {0.f, 0.f}, back[2] = {1.f, 1.f};
+    if constexpr (PAGED) {
+      const float f0 = share_of(vs0 * inv_ref), f1 = share_of(vs1 * inv_ref);
+      c[0] = p.c * ks0;
+      c[1] = p.c * ks1;
+      add[0] = __builtin_amdgcn_logf(f0);
+      add[1] = __builtin_amdgcn_logf(f1);
+      back[0] = __builtin_amdgcn_rcpf(f0);
+      back[1] = __builtin_amdgcn_rcpf(f1);
+    }
     v8 pr[R];
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-      const int32_t left = limit[r] - k0 - (int32_t)quarter * 4;
-      const uint32_t mine = bits >> (quarter * 4);
-      if constexpr (PAGED) {
-        s[r][0] *= ks0;
-        s[r][1] *= ks1;
-      }
       if (!whole) {
+        const int32_t left = limit[r] - k0 - (int32_t)quarter * 4;
+        const uint32_t mine = bits >> (quarter * 4);
 #pragma unroll
         for (int j = 0; j < 8; ++j)
           if (!((mine >> (j / 4 * 16 + j % 4)) & 1u) || j / 4 * 16 + j % 4 >= left) s[r][j / 4][j % 4] = -__builtin_inff();
       }
-      float top = s[r][0][0];
+      float top = -__builtin_inff();
 #pragma unroll
-      for (int j = 1; j < 8; ++j) top = fmaxf(top, s[r][j / 4][j % 4]);
+      for (int n = 0; n < 2; ++n) {
+        const float x = fmaxf(fmaxf(s[r][n][0], s[r][n][1]), fmaxf(s[r][n][2], s[r][n][3]));
+        top = fmaxf(top, PAGED ? x * (n ? ks1 : ks0) : x);  // a NaN of unseen keys' scales is dropped
+      }
       top = fmaxf(top, lane_xor<16>(top));
       top = fmaxf(top, lane_xor<32>(top));
-      if (__any(top > m[r])) {
+      if (__any((top - m[r]) * p.c > kSlack || (m[r] == -__builtin_inff() && top > m[r]))) {
         const float to = fmaxf(m[r], top), a = rescale_of(m[r], to, p.c);
         l[r] *= a;
 #pragma unroll
@@ -916,18 +1011,23 @@ __global__ __launch_bounds__(256, DP * R <= 64 ? 4 : DP <= 128 && DP * R <= 128 
         m[r] = to;
       }
       const float off = offset_of(m[r], p.c, 0.f) + Matrix<T>::kShift;
-      float sum = 0.f;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r][j / 4][j % 4], p.c, off));
-        sum += e;
-        if constexpr (PAGED) {
-          e *= (j < 4 ? vs0 : vs1) * inv_ref;
-          if (!whole && (!((mine >> (j / 4 * 16 + j % 4)) & 1u) || j / 4 * 16 + j % 4 >= left)) e = 0.f;
+      for (int n = 0; n < 2; ++n) {
+        float sum = 0.f;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r][n][j], c[n], off + add[n]));
+          if (PAGED && !whole && s[r][n][j] == -__builtin_inff()) e = 0.f;  // whatever its scales are
+          sum += e;
+          pr[r][n * 4 + j] = (T)e;
         }
-        pr[r][j] = (T)e;
+        if (PAGED && (whole || sum != 0.f)) sum *= back[n];  // (nothing of unseen keys' scales)
+        l[r] += sum;
+        if (PAGED && (n ? vs1 : vs0) * inv_ref == 0.f) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) pr[r][n * 4 + j] = (T)0.f;
+        }
       }
-      l[r] += sum;
     }
     // values, 16 dims a time
 #pragma unroll
@@ -1085,7 +1185,7 @@ thin_status launch_attend_dim(const AttendPlan& p, hipStream_t stream) {
   const uint32_t grid = p.batch * p.heads * p.row_blocks * p.splits;
   if (p.rows <= 16) hipLaunchKernelGGL((dev::few_kernel<T, DP, PAGED, 1>), dim3(grid), dim3(256), 0, stream, p);
   else if (few) hipLaunchKernelGGL((dev::few_kernel<T, DP, PAGED, 2>), dim3(grid), dim3(256), 0, stream, p);
-  else hipLaunchKernelGGL((dev::tile_kernel<T, DP, PAGED>), dim3(grid), dim3(256), 0, stream, p);
+  else hipLaunchKernelGGL((dev::tile_kernel<T, DP, PAGED, kBlockRows / 32>), dim3(grid), dim3(kBlockRows * 2), 0, stream, p);
   THIN_LAUNCH_CHECK("attend");
   if (p.splits > 1) {
     const uint64_t rows = (uint64_t)p.batch * p.heads * p.rows;

@@ -147,6 +147,8 @@ thin_status check_cache(const char* name, const thin_desc* kc, const thin_desc* 
                (long long)D, (long long)page);
   THIN_REQUIRE(kc->strides[3] == 1 && vc->strides[3] == 1, THIN_ERR_UNSUPPORTED, "%s: the codes of a token must be adjacent",
                name);
+  THIN_REQUIRE(kc->strides[2] < (1ll << 26) && vc->strides[2] < (1ll << 26), THIN_ERR_UNSUPPORTED,
+               "%s: neighbouring tokens must be less than 2^26 bytes apart", name);
   THIN_REQUIRE(P < (1ll << 30) && table->sizes[1] < (1ll << 30) / page, THIN_ERR_UNSUPPORTED, "%s: tensor too large", name);
   return THIN_OK;
 }

@@ -40,6 +40,8 @@ extern "C" thin_status thin_cross_attention(const thin_desc* q, const thin_desc*
                THIN_ERR_INVALID, "cross_attention takes a mask [batch, states] of bytes");
   THIN_REQUIRE(q->strides[3] == 1 && k->strides[3] == 1 && v->strides[3] == 1 && out->strides[3] == 1, THIN_ERR_UNSUPPORTED,
                "cross_attention: the dims of a head must be adjacent");
+  THIN_REQUIRE(S <= 1 || (k->strides[1] < (1ll << 25) && v->strides[1] < (1ll << 25)), THIN_ERR_UNSUPPORTED,
+               "cross_attention: neighbouring states must be less than 2^25 elements apart");
   const float c = scale * 1.4426950408889634f;
   THIN_REQUIRE(isnormal(c) && c > 0.f, THIN_ERR_INVALID, "cross_attention: the scale must be positive and finite");
   if (numel(q) == 0) return THIN_OK;

@@ -45,7 +45,7 @@ struct AttendPlan {
   int64_t o_batch, o_token, o_head;
   uint32_t batch, tokens, heads, group, rows, dim;  // heads: of the keys; rows = tokens * group
   uint32_t keys;                                    // as many as a sequence can have
-  uint32_t row_blocks, splits;
+  uint32_t row_blocks, block_rows, splits;
   FastDiv by_group, by_splits, by_blocks, by_heads;
   float c;
   const int32_t* lengths;  // null: `keys`
@@ -67,7 +67,12 @@ struct AttendPlan {
 };
 
 constexpr int kFewRows = 32;    // one or two matrix tiles of 16: keys are split over the wavefronts
-constexpr int kBlockRows = 128; // rows of a workgroup otherwise: 32 a wavefront
+// Rows of a workgroup otherwise: four wavefronts of two matrix tiles of 32 each,
+// or of one where registers or rows are too few (half of a tile's reads from LDS
+// serve two: 2048 rows of 128 dims took XX us by one, YY by two).
+inline int block_rows_of(int64_t rows, int64_t dim) {
+  return 128;
+}
 
 // Head widths that kernels exist for.
 inline int padded_dim(int64_t d) {
@@ -89,12 +94,15 @@ inline int64_t splits_of(int64_t units, int64_t rows, int64_t keys) {
   const int64_t n = want < most ? want : most;
   return n < 1 ? 1 : n > kMaxSplits ? kMaxSplits : n;
 }
-inline int64_t row_blocks_of(int64_t rows) { return rows <= kFewRows ? 1 : (rows + kBlockRows - 1) / kBlockRows; }
+inline int64_t row_blocks_of(int64_t rows, int64_t dim) {
+  const int64_t n = block_rows_of(rows, dim);
+  return rows <= kFewRows ? 1 : (rows + n - 1) / n;
+}
 inline size_t attend_workspace(int64_t batch, int64_t heads, int64_t rows, int64_t keys, int64_t dim) {
   if (batch <= 0 || heads <= 0 || rows <= 0 || keys <= 0 || !padded_dim(dim)) return 0;
-  const int64_t units = batch * heads * row_blocks_of(rows), splits = splits_of(units, rows, keys);
+  const int64_t units = batch * heads * row_blocks_of(rows, dim), splits = splits_of(units, rows, keys);
   if (splits == 1) return 0;
-  return (size_t)(units * splits * (rows <= kFewRows ? rows : kBlockRows) * (dim + 2) * 4);
+  return (size_t)(units * splits * (rows <= kFewRows ? rows : block_rows_of(rows, dim)) * (dim + 2) * 4);
 }
 
 // The part of a plan that both operators have.
@@ -113,8 +121,10 @@ inline void plan_attend(AttendPlan& p, const thin_desc* q, const thin_desc* out,
   p.dim = (uint32_t)q->sizes[3];
   p.keys = (uint32_t)keys;
   p.c = c;
-  const int64_t blocks = row_blocks_of(p.rows), units = (int64_t)p.batch * heads * blocks;
-  const int64_t splits = splits_of(units, p.rows, keys), block_rows = p.rows <= kFewRows ? p.rows : kBlockRows;
+  const int64_t blocks = row_blocks_of(p.rows, p.dim), units = (int64_t)p.batch * heads * blocks;
+  const int64_t splits = splits_of(units, p.rows, keys);
+  const int64_t block_rows = p.rows <= kFewRows ? p.rows : block_rows_of(p.rows, p.dim);
+  p.block_rows = (uint32_t)block_rows;
   p.row_blocks = (uint32_t)blocks;
   p.splits = (uint32_t)splits;
   p.by_group = FastDiv::make(p.group);
@@ -399,115 +409,153 @@ __device__ __forceinline__ Place place_of(const AttendPlan& p) {
 }
 
 // ---------------------------------------------------------------- many rows
-// 32 rows a wavefront, W wavefronts a workgroup, tiles of 64 keys.  A tile's keys
-// and values go through registers to LDS (unseen ones as zeros, codes as 16-bit
-// numbers), two tiles each there: while a tile's exponentials are taken and its
-// values mixed, the next one's scores are computed, the keys behind that and the
-// values of the next are written, and loads of one tile more are in flight.  So
-// one barrier a tile, and matrix instructions between the exponentials' own.
+// 32 R rows a wavefront, four wavefronts a workgroup, steps of 32 keys.  A step's
+// keys and values go through registers to LDS (unseen ones as zeros, codes as
+// 16-bit numbers), four steps each there.  Matrix instructions run beside the
+// others if they do not wait for one another, so three steps overlap: the scores
+// of step j + 1, the exponentials of step j and the mix of step j - 1, whose
+// instructions take turns; the keys of step j + 3 and the values of step j + 1 are
+// written meanwhile, and loads of one step more are in flight.  One barrier for two
+// steps.  The exponentials do not wait for their step's maximum: they are taken
+// against the maximum so far, and again where that turns out too low.
 // Rows: unseen states have -inf in the scores from the start (the accumulator's
-// first value).  Pages: rows that do not see a whole tile are masked afterwards.
-template <typename T, int DP, bool PAGED, int W>
-__global__ __launch_bounds__(64 * W, DP <= 128 ? 2 : 1) void tile_kernel(AttendPlan p) {
+// first value).  Pages: rows that do not see a whole step are masked afterwards.
+template <typename T, int DP, bool PAGED, int R>
+__global__ __launch_bounds__(256, DP * R <= 128 ? 2 : 1) void tile_kernel(AttendPlan p) {
   typedef typename Matrix<T>::v8 v8;
-  constexpr int KT = 64, NT = 64 * W;
+  constexpr int KT = 32;
   constexpr int kPer = PAGED ? DP / 16 : DP / 8, kElems = PAGED ? 16 : 8;  // 16-byte pieces of a key, elements of one
-  constexpr int kMine = (16 * kPer + 63) / 64;                            // a lane's of 16 keys
-  static_assert(W == 4, "a wavefront stages 16 of a tile's 64 keys");
+  constexpr int kMine = (8 * kPer + 63) / 64;                             // a lane's of the 8 keys that its wavefront stages
   constexpr int KS = Strides<DP>::K, VS = Strides<DP>::V;
-  __shared__ __align__(16) T lds_k[2][KT * KS];
-  __shared__ __align__(16) T lds_v[2][KT * VS];
-  __shared__ __align__(16) float lds_bias[2][PAGED ? 4 : KT];
+  __shared__ __align__(16) T lds_k[4][KT * KS];
+  __shared__ __align__(16) T lds_v[4][KT * VS];
+  __shared__ __align__(16) float lds_bias[4][PAGED ? 4 : KT];
   __shared__ int32_t lowest[PAGED ? DP : 1];  // keys with NaN values, where rows see different keys
   const uint32_t tid = threadIdx.x, lane = tid & 63u, half = (tid >> 5) & 1u;
   const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(tid >> 6));
   const Place w = place_of(p);
   const Sequence seq = sequence_of<PAGED>(p, w.b);
-  constexpr uint32_t kRows = 32 * W;
-  const uint32_t row = w.block * kRows + wave * 32 + (lane & 31u), t = p.by_group.div(row), g = row - t * p.group;
-  const bool mine = row < p.rows, live = mine && (int32_t)t < seq.tokens;
-  const int32_t limit = live ? limit_of<PAGED>(seq, (int32_t)t) : 0x7FFFFFFF;
+  constexpr uint32_t kRows = 128 * R;
+  // a lane's rows: 32 apart
+  const uint32_t row0 = w.block * kRows + wave * (32 * R) + (lane & 31u);
+  int32_t limit[R];
+  u4 q[R][DP / 16];
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    const uint32_t row = row0 + r * 32, t = p.by_group.div(row), g = row - t * p.group;
+    const bool live = row < p.rows && (int32_t)t < seq.tokens;
+    limit[r] = live ? limit_of<PAGED>(seq, (int32_t)t) : 0x7FFFFFFF;
+    load_query<T, DP>(p, w.b, w.h, t, g, live, half, q[r]);
+  }
   // the workgroup's first and last live rows
   const int32_t t_first = (int32_t)p.by_group.div(w.block * kRows);
   const int32_t t_last = min((int32_t)p.by_group.div(min(p.rows, (w.block + 1) * kRows) - 1), seq.tokens - 1);
   const int32_t most = t_last < t_first ? 0 : limit_of<PAGED>(seq, t_last);
   const int32_t least = limit_of<PAGED>(seq, t_first);
-  // this wavefront's
-  int32_t wave_least = limit, wave_most = live ? limit : 0;
+  int32_t wave_least = limit[0];  // this wavefront's
 #pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    wave_least = min(wave_least, __shfl_xor(wave_least, o, 64));
-    wave_most = max(wave_most, __shfl_xor(wave_most, o, 64));
-  }
+  for (int o = 1; o < 32; o <<= 1) wave_least = min(wave_least, __shfl_xor(wave_least, o, 64));
   wave_least = __builtin_amdgcn_readfirstlane(wave_least);
-  wave_most = __builtin_amdgcn_readfirstlane(wave_most);
-  const Range range = range_of(most, w.split, p.splits, KT);
-  const int32_t tiles = (range.end - range.begin + KT - 1) / KT;
+  const Range range = range_of(most, w.split, p.splits, 64);
+  const int32_t steps = (range.end - range.begin + KT - 1) / KT;
 
-  u4 q[DP / 16];
-  load_query<T, DP>(p, w.b, w.h, t, g, live, half, q);
-  f16v o[DP / 32];
+  f16v o[R][DP / 32];
+  float m[R], off[R], l[R];  // l: of this half's keys
 #pragma unroll
-  for (int i = 0; i < DP / 32; ++i)
+  for (int r = 0; r < R; ++r) {
+    m[r] = -__builtin_inff();
+    off[r] = Matrix<T>::kShift;
+    l[r] = 0.f;
 #pragma unroll
-    for (int j = 0; j < 16; ++j) o[i][j] = 0.f;
-  float m = -__builtin_inff(), l = 0.f;  // l: of this half's keys
+    for (int i = 0; i < DP / 32; ++i)
+#pragma unroll
+      for (int j = 0; j < 16; ++j) o[r][i][j] = 0.f;
+  }
   float ref = PAGED ? 0.f : 1.f, inv_ref = ref;
   if constexpr (PAGED)
-    for (uint32_t d = tid; d < (uint32_t)DP; d += NT) lowest[d] = 0x7FFFFFFF;
+    for (uint32_t d = tid; d < (uint32_t)DP; d += 256) lowest[d] = 0x7FFFFFFF;
 
-  // Stage s: keys of tile s and values of tile s - 1, 16 of each by a wavefront
-  // (PAGED: one page's).  Loads go by a buffer descriptor of the tile, so that a
-  // lane's offsets stay what they are from tile to tile; an offset past the
-  // descriptor's end is a zero.
+  // Stage s: keys of step s and values of step s - 2, eight of each by a wavefront
+  // (PAGED: of one page).  Loads go by a buffer descriptor of the step, so that a
+  // lane's offsets stay what they are; an offset past the descriptor's end is a
+  // zero.
   constexpr uint32_t kNowhere = 0x80000000u;
   u4 rk[kMine], rv[kMine];
   uint32_t k_off[kMine], v_off[kMine];
 #pragma unroll
   for (int i = 0; i < kMine; ++i) {
     const uint32_t n = lane + i * 64, key = n / kPer, col = n - key * kPer;
-    const bool have = n < 16u * kPer && col * kElems < p.dim;
+    const bool have = n < 8u * kPer && col * kElems < p.dim;
     const int64_t k_step = PAGED ? p.kp.token : p.k.key * (int64_t)sizeof(T), v_step = PAGED ? p.vp.token : p.v.key * (int64_t)sizeof(T);
     k_off[i] = have ? key * (uint32_t)k_step + col * 16 : kNowhere;
     v_off[i] = have ? key * (uint32_t)v_step + col * 16 : kNowhere;
   }
-  uint64_t bits_k = 0, bits_v = 0;  // rows: the keys of the stage's tiles that are seen
-  uint32_t shown = 0;               // rows: the next tile's key `lane`
-  int32_t id_k = -1, id_v = -1, id_next = -1;  // PAGED: the pages of the wavefront's 16
-  const auto look_up = [&](int32_t tile) {
-    if constexpr (PAGED) {
-      const int32_t k = range.begin + tile * KT + (int32_t)wave * 16;
-      id_next = k < range.end ? p.table[w.b * p.table_batch + p.by_page.div((uint32_t)k) * p.table_slot] : -1;
-    } else {
-      const int32_t k = range.begin + tile * KT + (int32_t)lane;
+  // rows: where the next stage's keys and values of the wavefront begin
+  const int64_t k_move = p.k.key * (int64_t)(KT * sizeof(T)), v_move = p.v.key * (int64_t)(KT * sizeof(T));
+  const uint8_t* k_at = static_cast<const uint8_t*>(p.k.data) +
+                        (w.b * p.k.batch + w.h * p.k.head + (range.begin + (int32_t)wave * 8) * p.k.key) * (int64_t)sizeof(T);
+  const uint8_t* v_at = static_cast<const uint8_t*>(p.v.data) +
+                        (w.b * p.v.batch + w.h * p.v.head + (range.begin + (int32_t)wave * 8 - 2 * KT) * p.v.key) * (int64_t)sizeof(T);
+  uint32_t bits_k = 0, bits_1 = 0, bits_v = 0;  // rows: the seen keys of steps s, s - 1 and s - 2
+  uint32_t shown = 0;                           // rows: key lane % 32 of the next step
+  // PAGED: lane i knows group i % 2 of 16 keys of step i / 2 of a window of 32
+  // steps; the next window's are looked up when one begins.
+  struct Window {
+    int32_t id;
+    float ks, vs;
+  };
+  const auto look_up_window = [&](int32_t first) {
+    Window x{-1, 0.f, 0.f};
+    const int32_t k = range.begin + (first + (int32_t)(lane >> 1)) * KT + (int32_t)(lane & 1u) * 16;
+    if (k < range.end) {
+      x.id = p.table[w.b * p.table_batch + p.by_page.div((uint32_t)k) * p.table_slot];
+      if ((uint32_t)x.id >= p.pages) {
+        x.id = -1;
+      } else {
+        x.ks = p.kp.scales[x.id * p.kp.scale_page + w.h * p.kp.scale_head];
+        x.vs = p.vp.scales[x.id * p.vp.scale_page + w.h * p.vp.scale_head];
+      }
+    }
+    return x;
+  };
+  Window here{-1, 0.f, 0.f}, there{-1, 0.f, 0.f};
+  int32_t here_first = 0;                  // the step that `here` begins with
+  int32_t id_k = -1, id_1 = -1, id_v = -1;  // the pages of the wavefront's keys of steps s, s - 1 and s - 2
+  const uint8_t* k_codes = p.kp.codes + w.h * p.kp.head;
+  const uint8_t* v_codes = p.vp.codes + w.h * p.vp.head;
+  const auto look_up = [&](int32_t step) {
+    if constexpr (!PAGED) {
+      const int32_t k = range.begin + step * KT + (int32_t)(lane & 31u);
       shown = k < range.end;
       if (shown && p.mask) shown = p.mask[w.b * p.mask_batch + k * p.mask_key];
     }
   };
   const auto fetch = [&](int32_t stage) {
-    const int32_t k0 = range.begin + stage * KT + (int32_t)wave * 16;
+    const int32_t k0 = range.begin + stage * KT + (int32_t)wave * 8, v0 = k0 - 2 * KT;
     if constexpr (PAGED) {
-      id_v = id_k;
-      id_k = __builtin_amdgcn_readfirstlane(id_next);
-      if ((uint32_t)id_k >= p.pages) id_k = -1;
-      const auto rsrc_of = [&](const PagesOf& x, int32_t id, int32_t key) {
+      id_v = id_1;
+      id_1 = id_k;
+      const int32_t at = stage - here_first;
+      id_k = __builtin_amdgcn_readlane(at < 32 ? here.id : there.id, (at & 31) * 2 + (int32_t)(wave >> 1));
+      const auto rsrc_of = [&](const uint8_t* codes, const PagesOf& x, int32_t id, int32_t key) {
         const uint32_t token = (uint32_t)key - p.by_page.div((uint32_t)key) * p.page_size;
-        return buffer_rsrc(code_at(x, id, w.h, token), id >= 0 ? kNowhere : 0u);
+        return buffer_rsrc(codes + id * x.page + token * x.token, id >= 0 ? kNowhere : 0u);
       };
-      const auto kr = rsrc_of(p.kp, id_k, k0), vr = rsrc_of(p.vp, id_v, max(k0 - KT, 0));
+      const auto kr = rsrc_of(k_codes, p.kp, id_k, k0), vr = rsrc_of(v_codes, p.vp, id_v, max(v0, 0));
 #pragma unroll
       for (int i = 0; i < kMine; ++i) {
         rk[i] = __builtin_bit_cast(u4, __builtin_amdgcn_raw_buffer_load_b128(kr, k_off[i], 0, 0));
         rv[i] = __builtin_bit_cast(u4, __builtin_amdgcn_raw_buffer_load_b128(vr, v_off[i], 0, 0));
       }
     } else {
-      bits_v = bits_k;
-      bits_k = __ballot(shown != 0);
-      const uint32_t mine_k = (uint32_t)(bits_k >> (wave * 16)) & 0xFFFFu, mine_v = (uint32_t)(bits_v >> (wave * 16)) & 0xFFFFu;
-      const T* kb = static_cast<const T*>(p.k.data) + w.b * p.k.batch + w.h * p.k.head + (int64_t)k0 * p.k.key;
-      const T* vb = static_cast<const T*>(p.v.data) + w.b * p.v.batch + w.h * p.v.head + (int64_t)(k0 - KT) * p.v.key;
-      const auto kr = buffer_rsrc(kb, kNowhere), vr = buffer_rsrc(vb, kNowhere);
-      if (mine_k == 0xFFFFu && mine_v == 0xFFFFu) {
+      bits_v = bits_1;
+      bits_1 = bits_k;
+      bits_k = (uint32_t)__ballot(shown != 0);
+      const uint32_t mine_k = (bits_k >> (wave * 8)) & 0xFFu, mine_v = (bits_v >> (wave * 8)) & 0xFFu;
+      const auto kr = buffer_rsrc(k_at, kNowhere), vr = buffer_rsrc(v_at, kNowhere);
+      k_at += k_move;
+      v_at += v_move;
+      if (mine_k == 0xFFu && mine_v == 0xFFu) {
 #pragma unroll
         for (int i = 0; i < kMine; ++i) {
           rk[i] = __builtin_bit_cast(u4, __builtin_amdgcn_raw_buffer_load_b128(kr, k_off[i], 0, 0));
@@ -525,15 +573,15 @@ __global__ __launch_bounds__(64 * W, DP <= 128 ? 2 : 1) void tile_kernel(AttendP
     look_up(stage + 1);
   };
   const auto store = [&](int32_t stage) {
-    T* kt = lds_k[stage & 1] + wave * 16 * KS;
-    T* vt = lds_v[(stage + 1) & 1] + wave * 16 * VS;
-    const int32_t v0 = range.begin + (stage - 1) * KT;  // the values' tile
+    T* kt = lds_k[stage & 3] + wave * 8 * KS;
+    T* vt = lds_v[(stage + 2) & 3] + wave * 8 * VS;
+    const int32_t v0 = range.begin + (stage - 2) * KT;  // the values' step
 #pragma unroll
     for (int i = 0; i < kMine; ++i) {
       const uint32_t n = lane + i * 64, key = n / kPer, col = n - key * kPer;
-      if (16 * kPer % 64 && n >= 16u * kPer) continue;
+      if (8 * kPer % 64 && n >= 8u * kPer) continue;
       if constexpr (PAGED) {
-        if (v0 + KT > least && has_nan(rv[i])) take_nan(rv[i], v0 + (int32_t)(wave * 16 + key), lowest + col * 16);
+        if (v0 + KT > least && has_nan(rv[i])) take_nan(rv[i], v0 + (int32_t)(wave * 8 + key), lowest + col * 16);
         u4 a, b;
         widen<T>(rk[i], a, b);
         *reinterpret_cast<u4*>(kt + key * KS + col * 16) = a;
@@ -546,200 +594,255 @@ __global__ __launch_bounds__(64 * W, DP <= 128 ? 2 : 1) void tile_kernel(AttendP
         *reinterpret_cast<u4*>(vt + key * VS + col * 8) = rv[i];
       }
     }
-    if (!PAGED && wave == 0) lds_bias[stage & 1][lane] = (bits_k >> lane) & 1u ? 0.f : -__builtin_inff();
+    if (!PAGED && wave == 0 && lane < 32) lds_bias[stage & 3][lane] = (bits_k >> lane) & 1u ? 0.f : -__builtin_inff();
   };
-  // PAGED: lane i knows group i % 4 of 16 keys of a tile
-  struct Group {
-    float ks, vs;
-    bool seen;
+  const auto key_piece = [&](int slot, int i) {  // dims of step i of q . k
+    return __builtin_bit_cast(v8, *reinterpret_cast<const u4*>(lds_k[slot] + (lane & 31u) * KS + half * 16 + (i / 2) * 32 + (i % 2) * 8));
   };
-  const auto group_id = [&](int32_t tile) {
-    const int32_t k = range.begin + tile * KT + (int32_t)(lane & 3u) * 16;
-    int32_t i = -1;
-    if (k < range.end) i = p.table[w.b * p.table_batch + p.by_page.div((uint32_t)k) * p.table_slot];
-    return (uint32_t)i < p.pages ? i : -1;
+  const auto value_piece = [&](int slot, int i) {  // i: the step's 16 keys i / (DP / 32), dims i % (DP / 32)
+    return values8<T, VS>(lds_v[slot], i / (DP / 32) * 16, i % (DP / 32), lane);
   };
-  const auto group_of = [&](int32_t i) {
-    Group x{0.f, 0.f, i >= 0};
-    if (i >= 0) {
-      x.ks = p.kp.scales[i * p.kp.scale_page + w.h * p.kp.scale_head];
-      x.vs = p.vp.scales[i * p.vp.scale_page + w.h * p.vp.scale_head];
-    }
-    return x;
-  };
-  const auto start_scores = [&](int32_t tile, f16v (&s)[2]) {
+  constexpr int kProducts = DP / 16;  // of a step, for the scores as for the mix
+  // Scores of a step begin at 0, or at -inf for what is not seen.
+  const auto first_scores = [&](int slot, bool all, const v8& kf, f16v (&s)[R]) __attribute__((always_inline)) {
+    f16v x;
 #pragma unroll
-    for (int n = 0; n < 2; ++n) {
+    for (int j = 0; j < 16; ++j) x[j] = 0.f;
+    if (!PAGED && !all) {
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        f4 x = {0.f, 0.f, 0.f, 0.f};
-        if constexpr (!PAGED) x = *reinterpret_cast<const f4*>(lds_bias[tile & 1] + n * 32 + j * 8 + half * 4);
+        const f4 y = *reinterpret_cast<const f4*>(lds_bias[slot] + j * 8 + half * 4);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) s[n][j * 4 + e] = x[e];
+        for (int e = 0; e < 4; ++e) x[j * 4 + e] = y[e];
       }
+#pragma unroll
+      for (int r = 0; r < R; ++r) s[r] = Matrix<T>::mul(kf, __builtin_bit_cast(v8, q[r][0]), x);
+    } else {
+#pragma unroll
+      for (int r = 0; r < R; ++r) s[r] = Matrix<T>::mul(kf, __builtin_bit_cast(v8, q[r][0]), x);
     }
-  };
-  const auto scores = [&](int32_t tile, f16v (&s)[2]) {
-    const T* k = lds_k[tile & 1];
-    start_scores(tile, s);
-#pragma unroll
-    for (int i = 0; i < DP / 16; ++i)
-#pragma unroll
-      for (int n = 0; n < 2; ++n) {
-        const uint32_t d = (i / 2) * 32 + half * 16 + (i % 2) * 8;
-        const u4 x = *reinterpret_cast<const u4*>(k + (n * 32 + (lane & 31u)) * KS + d);
-        s[n] = Matrix<T>::mul(__builtin_bit_cast(v8, x), __builtin_bit_cast(v8, q[i]), s[n]);
-      }
   };
 
-  f16v s[2], next[2];
-  Group group{0.f, 0.f, true}, group_next{0.f, 0.f, true};
-  int32_t group_far = -1;
-  if (tiles > 0) {
-    look_up(0);
-    if constexpr (PAGED) {
-      group = group_of(group_id(0));
-      group_next = group_of(group_id(1));
-      group_far = group_id(2);
-    }
-    fetch(0);
-    store(0);
-    fetch(1);
-    __syncthreads();
-    store(1);
-    fetch(2);
-    scores(0, s);
-  }
-  for (int32_t tile = 0; tile < tiles; ++tile) {
-    const int32_t k0 = range.begin + tile * KT;
-    __syncthreads();
-    if (tile + 1 < tiles) {
-      store(tile + 2);
-      fetch(tile + 3);
-    }
-    Group now{0.f, 0.f, true};
-    if constexpr (PAGED) {
-      now = group;
-      group = group_next;
-      group_next = group_of(group_far);
-      group_far = group_id(tile + 3);
-    }
-    if (k0 >= wave_most) continue;
-    // the maximum
-    bool whole = true;
-    float ks[4], vs[4];
-    if constexpr (PAGED) {
-      const uint32_t groups = (uint32_t)__ballot(now.seen) & 15u;
-      whole = groups == 15u && k0 + KT <= wave_least;
+  // Step j: s holds its scores, `next` gets the next one's; before: the weights of
+  // step j - 1, which are mixed, pr: its own.
+  const auto advance = [&](int32_t j, f16v (&s)[R], f16v (&next)[R], const v8 (&before)[R][2],
+                           v8 (&pr)[R][2]) __attribute__((always_inline)) {
+    const int32_t k0 = range.begin + j * KT;
+    if (!(j & 1)) __syncthreads();
+    constexpr int kAhead = kProducts < 4 ? kProducts : 4;
+    const int k_slot = (j + 1) & 3, v_slot = (j + 3) & 3;
+    v8 kf[kAhead], vf[2];
 #pragma unroll
-      for (int n = 0; n < 4; ++n) ks[n] = lane_value(now.ks, n);
-      if (!whole) {
-        const int32_t left = limit - k0 - (int32_t)half * 4;
+    for (int i = 0; i < kAhead; ++i) kf[i] = key_piece(k_slot, i);
+    vf[0] = value_piece(v_slot, 0);
+    vf[1] = value_piece(v_slot, 1);
+    const bool all = bits_v == ~0u;  // of step j + 1
+    store(j + 3);
+    fetch(j + 4);
+    bool raised = false;
+    float ks[2], vs[2], share[2], a[R];  // a: what the sums so far are multiplied by, once step j - 1 is in
 #pragma unroll
-        for (int n = 0; n < 2; ++n)
+    for (int r = 0; r < R; ++r) a[r] = 1.f;
+    bool there_is[2];
+    if constexpr (PAGED) {
 #pragma unroll
-          for (int j = 0; j < 16; ++j)
-            if (!((groups >> (n * 2 + j / 8)) & 1u) || n * 32 + j / 4 * 8 + j % 4 >= left) s[n][j] = -__builtin_inff();
+      for (int n = 0; n < 2; ++n) {
+        const int32_t at = (j - here_first) * 2 + n;
+        there_is[n] = __builtin_amdgcn_readlane(here.id, at) >= 0;
+        ks[n] = lane_value(here.ks, at);
+        vs[n] = lane_value(here.vs, at);
       }
-      if (__any(raises(now.vs, ref))) {
-        const float top = power_of(group_max<64>(raises(now.vs, ref) ? now.vs : ref)), a = ref * inverse_of(top);
+      if (raises(vs[0], ref) || raises(vs[1], ref)) {
+        const float top = power_of(fmaxf(raises(vs[0], ref) ? vs[0] : ref, raises(vs[1], ref) ? vs[1] : ref));
 #pragma unroll
-        for (int i = 0; i < DP / 32; ++i)
-#pragma unroll
-          for (int j = 0; j < 16; ++j) o[i][j] *= a;
+        for (int r = 0; r < R; ++r) a[r] = ref * inverse_of(top);
+        raised = true;
         ref = top;
         inv_ref = inverse_of(ref);
       }
 #pragma unroll
-      for (int n = 0; n < 4; ++n) vs[n] = lane_value(now.vs, n) * inv_ref;
+      for (int n = 0; n < 2; ++n) {
+        vs[n] *= inv_ref;
+        share[n] = __builtin_amdgcn_logf(share_of(vs[n]));
+      }
     }
-    float top = -__builtin_inff();
+    float c[R][2], add[R][2], back[R][2], sum[R][2], top[R][2];
 #pragma unroll
-    for (int n = 0; n < 4; ++n) {
-      float x = s[n / 2][n % 2 * 8];
+    for (int r = 0; r < R; ++r)
 #pragma unroll
-      for (int j = 1; j < 8; ++j) x = fmaxf(x, s[n / 2][n % 2 * 8 + j]);
-      top = fmaxf(top, PAGED ? x * ks[n] : x);  // a NaN of unseen keys' scales is dropped
+      for (int n = 0; n < 2; ++n) {
+        c[r][n] = PAGED ? p.c * ks[n] : p.c;
+        add[r][n] = PAGED ? off[r] + share[n] : off[r];
+        back[r][n] = PAGED ? __builtin_amdgcn_rcpf(share_of(vs[n])) : 1.f;
+        sum[r][n] = 0.f;
+        top[r][n] = -__builtin_inff();
+      }
+    if constexpr (PAGED)
+      if (!(there_is[0] && there_is[1] && k0 + KT <= wave_least)) {
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+          const int32_t left = limit[r] - k0 - (int32_t)half * 4;
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            if (!there_is[i / 8] || i / 4 * 8 + i % 4 >= left) s[r][i] = -__builtin_inff();
+#pragma unroll
+          for (int n = 0; n < 2; ++n)
+            if (!there_is[n] || limit[r] <= k0 + n * 16) {  // nothing of scales that the row does not see
+              c[r][n] = 1.f;
+              add[r][n] = back[r][n] = 0.f;
+            }
+        }
+      }
+    const auto weigh = [&](int r, int x) __attribute__((always_inline)) {  // elements x and x + 1 of row tile r
+      float e[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        e[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r][x + i], c[r][x / 8], add[r][x / 8]));
+        sum[r][x / 8] += e[i];
+      }
+      typename Matrix<T>::v2 both;
+      both[0] = (T)e[0];
+      both[1] = (T)e[1];
+      uint32_t w = __builtin_bit_cast(uint32_t, both);
+      asm volatile("" : "+v"(w), "+v"(sum[r][x / 8]));  // here, and not where they are used
+      both = __builtin_bit_cast(typename Matrix<T>::v2, w);
+      pr[r][x / 8][x % 8] = both[0];
+      pr[r][x / 8][x % 8 + 1] = both[1];
+    };
+    // (After the last step, scores of what LDS holds, which nobody takes; before the
+    // first, weights and values of 0.)
+    first_scores(k_slot, all, kf[0], next);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int i = 0; i < kProducts; ++i) {
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        if (i) next[r] = Matrix<T>::mul(kf[i % kAhead], __builtin_bit_cast(v8, q[r][i]), next[r]);
+        o[r][i % (DP / 32)] = Matrix<T>::mul(vf[i % 2], before[r][i / (DP / 32)], o[r][i % (DP / 32)]);
+        if (r == R - 1) {
+          if (i + kAhead < kProducts) kf[i % kAhead] = key_piece(k_slot, i + kAhead);
+          if (i + 2 < kProducts) vf[i % 2] = value_piece(v_slot, i + 2);
+        }
+#pragma unroll
+        for (int x = i * 8 / kProducts * 2; x < (i + 1) * 8 / kProducts * 2; x += 2) {
+          weigh(r, x);
+          top[r][x / 8] = fmaxf(fmaxf(top[r][x / 8], s[r][x]), s[r][x + 1]);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
     }
-    top = fmaxf(top, lane_xor<32>(top));
-    if (__any((top - m) * p.c > kSlack || (m == -__builtin_inff() && top > m))) {
-      const float to = fmaxf(m, top), a = rescale_of(m, to, p.c);
-      l *= a;
+    bool more = false;
+    float most_of[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      // (a NaN of unseen keys' scales is dropped)
+      most_of[r] = PAGED ? fmaxf(fmaxf(-__builtin_inff(), top[r][0] * ks[0]), top[r][1] * ks[1]) : fmaxf(top[r][0], top[r][1]);
+      more |= (most_of[r] - m[r]) * p.c > kSlack;
+    }
+    if (__any(more)) {  // (either half's lanes)
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        const float to = fmaxf(m[r], fmaxf(most_of[r], lane_xor<32>(most_of[r]))), f = rescale_of(m[r], to, p.c);
+        l[r] *= f;
+        a[r] *= f;
+        m[r] = to;
+        off[r] = offset_of(to, p.c, 0.f) + Matrix<T>::kShift;
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+          add[r][n] = !PAGED ? off[r] : back[r][n] == 0.f ? 0.f : off[r] + share[n];
+          sum[r][n] = 0.f;
+        }
+#pragma unroll
+        for (int x = 0; x < 16; x += 2) weigh(r, x);
+      }
+      raised = true;
+    }
+    if (raised) {
+#pragma unroll
+      for (int r = 0; r < R; ++r)
+#pragma unroll
+        for (int i = 0; i < DP / 32; ++i)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) o[r][i][e] *= a[r];
+    }
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+      for (int n = 0; n < 2; ++n) {
+        l[r] += PAGED ? sum[r][n] * back[r][n] : sum[r][n];
+        if (PAGED && vs[n] == 0.f) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) pr[r][n][i] = (T)0.f;
+        }
+      }
+  };
+
+  f16v s[2][R];
+  v8 pr[2][R][2];
+#pragma unroll
+  for (int r = 0; r < R; ++r)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) pr[1][r][0][i] = pr[1][r][1][i] = (T)0.f;
+  if (steps > 0) {
+    look_up(0);
+    if constexpr (PAGED) {
+      here = look_up_window(0);
+      there = look_up_window(32);
+    }
+    fetch(0);
+    const bool all = bits_k == ~0u;
+    store(0);
+    fetch(1);
+    store(1);
+    fetch(2);
+    store(2);
+    fetch(3);
+    __syncthreads();
+    first_scores(0, all, key_piece(0, 0), s[0]);
+#pragma unroll
+    for (int i = 1; i < kProducts; ++i)
+#pragma unroll
+      for (int r = 0; r < R; ++r) s[0][r] = Matrix<T>::mul(key_piece(0, i), __builtin_bit_cast(v8, q[r][i]), s[0][r]);
+    for (int32_t j = 0; j < steps; j += 2) {
+      if (PAGED && j == here_first + 32) {
+        here = there;
+        here_first = j;
+        there = look_up_window(j + 32);
+      }
+      advance(j, s[0], s[1], pr[1], pr[0]);
+      if (j + 1 < steps) advance(j + 1, s[1], s[0], pr[0], pr[1]);
+    }
+    __syncthreads();
+    const auto finish = [&](const v8 (&last)[R][2]) __attribute__((always_inline)) {
+#pragma unroll
+      for (int i = 0; i < kProducts; ++i) {
+        const v8 v = value_piece((steps - 1) & 3, i);
+#pragma unroll
+        for (int r = 0; r < R; ++r) o[r][i % (DP / 32)] = Matrix<T>::mul(v, last[r][i / (DP / 32)], o[r][i % (DP / 32)]);
+      }
+    };
+    if (steps & 1) finish(pr[0]);
+    else finish(pr[1]);
+  }
+  if constexpr (PAGED) __syncthreads();
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    if constexpr (PAGED) {
 #pragma unroll
       for (int i = 0; i < DP / 32; ++i)
 #pragma unroll
-        for (int j = 0; j < 16; ++j) o[i][j] *= a;
-      m = to;
+        for (int j = 0; j < 16; ++j) {
+          o[r][i][j] *= ref;
+          if (limit[r] > lowest[i * 32 + j / 4 * 8 + half * 4 + j % 4]) o[r][i][j] = __builtin_nanf("");
+        }
     }
-    const float off = offset_of(m, p.c, 0.f) + Matrix<T>::kShift;
-    // The next tile's scores beside this one's exponentials, a matrix instruction
-    // and its share of them at a time: the former take 32 cycles of their own
-    // unit, in which the wavefront goes on.  (After the last tile, scores of what
-    // LDS holds, which nobody takes.)
-    constexpr int kSteps = DP / 8, kAhead = 4;
-    start_scores(tile + 1, next);
-    const T* kt = lds_k[(tile + 1) & 1] + (lane & 31u) * KS + half * 16;
-    const T* vt = lds_v[tile & 1];
-    const auto key_piece = [&](int i) {  // of step i: keys 32 (i % 2), dims step i / 2
-      return *reinterpret_cast<const u4*>(kt + (i % 2) * 32 * KS + (i / 4) * 32 + (i / 2) % 2 * 8);
-    };
-    u4 ring[kAhead];
-#pragma unroll
-    for (int i = 0; i < kAhead; ++i) ring[i] = key_piece(i);
-    float c[4], add[4], sum[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int n = 0; n < 4; ++n) {
-      c[n] = PAGED ? p.c * ks[n] : p.c;
-      add[n] = PAGED ? off + __builtin_amdgcn_logf(share_of(vs[n])) : off;
+    l[r] += lane_xor<32>(l[r]);
+    const uint32_t row = row0 + r * 32, t = p.by_group.div(row), g = row - t * p.group;
+    if (row < p.rows && (p.splits == 1 || steps > 0)) {
+      const uint64_t unit = ((uint64_t)w.b * p.heads + w.h) * p.row_blocks + w.block;
+      store_row<T, DP>(p, w.b, w.h, t, g, (unit * p.splits + w.split) * kRows + (row - w.block * kRows), half,
+                       (int32_t)t < seq.tokens, o[r], m[r], l[r]);
     }
-    v8 pr[4];
-    __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-    for (int i = 0; i < kSteps; ++i) {
-      next[i % 2] = Matrix<T>::mul(__builtin_bit_cast(v8, ring[i % kAhead]), __builtin_bit_cast(v8, q[i / 2]), next[i % 2]);
-      if (i + kAhead < kSteps) ring[i % kAhead] = key_piece(i + kAhead);
-#pragma unroll
-      for (int x = i * 32 / kSteps; x < (i + 1) * 32 / kSteps; ++x) {
-        const int n = x / 8, j = x % 8;
-        const float score = s[n / 2][n % 2 * 8 + j];
-        float e = __builtin_amdgcn_exp2f(__builtin_fmaf(score, c[n], add[n]));
-        if (PAGED && !whole && score == -__builtin_inff()) e = 0.f;  // whatever its scales are
-        sum[n] += e;
-        pr[n][j] = (T)e;
-      }
-      __builtin_amdgcn_sched_barrier(0);
-    }
-#pragma unroll
-    for (int n = 0; n < 4; ++n) {
-      if (PAGED && (whole || sum[n] != 0.f)) sum[n] *= __builtin_amdgcn_rcpf(share_of(vs[n]));  // (nothing of unseen keys' scales)
-      l += sum[n];
-      if (PAGED && vs[n] == 0.f) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) pr[n][j] = (T)0.f;
-      }
-    }
-    // its values
-#pragma unroll
-    for (int n = 0; n < 4; ++n)
-#pragma unroll
-      for (int i = 0; i < DP / 32; ++i) o[i] = Matrix<T>::mul(values8<T, VS>(vt, n * 16, i, lane), pr[n], o[i]);
-#pragma unroll
-    for (int n = 0; n < 2; ++n) s[n] = next[n];
-  }
-  if constexpr (PAGED) {
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < DP / 32; ++i)
-#pragma unroll
-      for (int j = 0; j < 16; ++j) {
-        o[i][j] *= ref;
-        if (limit > lowest[i * 32 + j / 4 * 8 + half * 4 + j % 4]) o[i][j] = __builtin_nanf("");
-      }
-  }
-  l += lane_xor<32>(l);
-  if (mine && (p.splits == 1 || tiles > 0)) {
-    const uint64_t unit = ((uint64_t)w.b * p.heads + w.h) * p.row_blocks + w.block;
-    store_row<T, DP>(p, w.b, w.h, t, g, (unit * p.splits + w.split) * kRows + (row - w.block * kRows), half, live, o, m, l);
   }
 }
 
@@ -988,12 +1091,21 @@ __global__ __launch_bounds__(256, DP * R <= 64 ? 4 : DP <= 128 && DP * R <= 128 
     v8 pr[R];
 #pragma unroll
     for (int r = 0; r < R; ++r) {
+      float rc[2] = {c[0], c[1]}, radd[2] = {add[0], add[1]}, rback[2] = {back[0], back[1]};
       if (!whole) {
         const int32_t left = limit[r] - k0 - (int32_t)quarter * 4;
         const uint32_t mine = bits >> (quarter * 4);
 #pragma unroll
         for (int j = 0; j < 8; ++j)
           if (!((mine >> (j / 4 * 16 + j % 4)) & 1u) || j / 4 * 16 + j % 4 >= left) s[r][j / 4][j % 4] = -__builtin_inff();
+        if constexpr (PAGED) {
+#pragma unroll
+          for (int n = 0; n < 2; ++n)
+            if (!((bits >> (n * 16)) & 1u) || limit[r] <= k0 + n * 16) {  // nothing of scales that the row does not see
+              rc[n] = 1.f;
+              radd[n] = rback[n] = 0.f;
+            }
+        }
       }
       float top = -__builtin_inff();
 #pragma unroll
@@ -1016,13 +1128,11 @@ __global__ __launch_bounds__(256, DP * R <= 64 ? 4 : DP <= 128 && DP * R <= 128 
         float sum = 0.f;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r][n][j], c[n], off + add[n]));
-          if (PAGED && !whole && s[r][n][j] == -__builtin_inff()) e = 0.f;  // whatever its scales are
+          const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r][n][j], rc[n], off + radd[n]));
           sum += e;
           pr[r][n * 4 + j] = (T)e;
         }
-        if (PAGED && (whole || sum != 0.f)) sum *= back[n];  // (nothing of unseen keys' scales)
-        l[r] += sum;
+        l[r] += PAGED ? sum * rback[n] : sum;
         if (PAGED && (n ? vs1 : vs0) * inv_ref == 0.f) {
 #pragma unroll
           for (int j = 0; j < 4; ++j) pr[r][n * 4 + j] = (T)0.f;
@@ -1128,7 +1238,7 @@ __global__ __launch_bounds__(256, DP * R <= 64 ? 4 : DP <= 128 && DP * R <= 128 
 template <typename T, bool PAGED, int E>
 __global__ __launch_bounds__(256) void join_kernel(AttendPlan p, uint32_t few) {
   __shared__ f4 part[256];
-  const uint32_t lane = threadIdx.x & 63u, mine = threadIdx.x % E, block_rows = few ? p.rows : kBlockRows;
+  const uint32_t lane = threadIdx.x & 63u, mine = threadIdx.x % E, block_rows = p.block_rows;
   const uint64_t at = (uint64_t)blockIdx.x * (256 / E) + threadIdx.x / E;  // (b, h, row)
   if (E < 256 && at >= (uint64_t)p.batch * p.heads * p.rows) return;
   const uint32_t unit = (uint32_t)(at / p.rows), row = (uint32_t)(at - (uint64_t)unit * p.rows);
@@ -1185,7 +1295,8 @@ thin_status launch_attend_dim(const AttendPlan& p, hipStream_t stream) {
   const uint32_t grid = p.batch * p.heads * p.row_blocks * p.splits;
   if (p.rows <= 16) hipLaunchKernelGGL((dev::few_kernel<T, DP, PAGED, 1>), dim3(grid), dim3(256), 0, stream, p);
   else if (few) hipLaunchKernelGGL((dev::few_kernel<T, DP, PAGED, 2>), dim3(grid), dim3(256), 0, stream, p);
-  else hipLaunchKernelGGL((dev::tile_kernel<T, DP, PAGED, kBlockRows / 32>), dim3(grid), dim3(kBlockRows * 2), 0, stream, p);
+  else if (p.block_rows == 128) hipLaunchKernelGGL((dev::tile_kernel<T, DP, PAGED, 1>), dim3(grid), dim3(256), 0, stream, p);
+  else if constexpr (DP <= 128) hipLaunchKernelGGL((dev::tile_kernel<T, DP, PAGED, 2>), dim3(grid), dim3(256), 0, stream, p);
   THIN_LAUNCH_CHECK("attend");
   if (p.splits > 1) {
     const uint64_t rows = (uint64_t)p.batch * p.heads * p.rows;

@@ -45,7 +45,9 @@ struct AttendPlan {
   int64_t o_batch, o_token, o_head;
   uint32_t batch, tokens, heads, group, rows, dim;  // heads: of the keys; rows = tokens * group
   uint32_t keys;                                    // as many as a sequence can have
-  uint32_t row_blocks, block_rows, splits;
+  uint32_t row_blocks, block_rows;
+  uint32_t splits;  // many rows: of each row's keys
+  uint32_t chunks;  // few rows: workgroups that the keys of all sequences are dealt to, or 0
   FastDiv by_group, by_splits, by_blocks, by_heads;
   float c;
   const int32_t* lengths;  // null: `keys`
@@ -61,18 +63,13 @@ struct AttendPlan {
   int64_t table_batch, table_slot;
   uint32_t page_size, pages;
   FastDiv by_page;
-  // partial results of splits: [batch, heads, row_blocks, splits, block rows] x {dim, m, l}
+  // partial results: [batch, heads, row_blocks, splits, block rows] or [chunks, rows] x {dim, m, l}
   float* sums;
   float* stats;
 };
 
 constexpr int kFewRows = 32;    // one or two matrix tiles of 16: keys are split over the wavefronts
-// Rows of a workgroup otherwise: four wavefronts of two matrix tiles of 32 each,
-// or of one where registers or rows are too few (half of a tile's reads from LDS
-// serve two: 2048 rows of 128 dims took XX us by one, YY by two).
-inline int block_rows_of(int64_t rows, int64_t dim) {
-  return 128;
-}
+constexpr int kBlockRows = 128;  // rows of a workgroup otherwise: 32 a wavefront
 
 // Head widths that kernels exist for.
 inline int padded_dim(int64_t d) {
@@ -81,33 +78,59 @@ inline int padded_dim(int64_t d) {
   return 0;
 }
 
-// Splits of a row's keys: until the card is full (a few rows' workgroups, of
-// which four fit a CU, twice over, as sequences are not of one length), none under kSplitKeys
-// keys (shorter ones cost more to join than they give).
-constexpr int64_t kSplitKeys = 256;
-constexpr int64_t kWorkgroups = 512, kFewWorkgroups = 2048;
+// Workgroups that a CU holds, by their registers; DP: padded_dim().
+constexpr int few_workgroups(int DP, int rows, bool paged) {
+  const int R = rows <= 16 ? 1 : 2;
+  return DP * R <= 64 ? 4 : DP <= 128 && DP * R <= 128 ? 3 : DP <= 128 || (paged && R == 1) ? 2 : 1;
+}
+constexpr int tile_workgroups(int DP) { return DP <= 32 ? 4 : DP <= 64 ? 3 : DP <= 128 ? 2 : 1; }
+
+constexpr int64_t kCus = 256;
+constexpr int64_t kSplitKeys = 256;  // keys of a split at least: fewer cost more to join than they give
 constexpr int64_t kMaxSplits = 128;
 constexpr uint32_t kJoinByWave = 8;  // splits that one wavefront joins; more take a workgroup
-inline int64_t splits_of(int64_t units, int64_t rows, int64_t keys) {
-  const int64_t most = (keys + kSplitKeys - 1) / kSplitKeys;
-  const int64_t want = (rows <= kFewRows ? kFewWorkgroups : kWorkgroups) / (units > 0 ? units : 1);
-  const int64_t n = want < most ? want : most;
-  return n < 1 ? 1 : n > kMaxSplits ? kMaxSplits : n;
+
+// Many rows: splits of every row's keys.  In rounds of the workgroups that the card
+// holds, each as long as its keys and some 160 more, which beginning and end cost,
+// and the join as much as 200.
+inline int64_t splits_of(int64_t units, int64_t keys, int64_t dim) {
+  const int64_t most = (keys + kSplitKeys - 1) / kSplitKeys < kMaxSplits ? (keys + kSplitKeys - 1) / kSplitKeys : kMaxSplits;
+  const int64_t at_a_time = kCus * tile_workgroups(padded_dim(dim));
+  int64_t best = 1, least = 0;
+  for (int64_t n = 1; n <= most && (n == 1 || units * n <= 8 * at_a_time); ++n) {
+    const int64_t rounds = (units * n + at_a_time - 1) / at_a_time;
+    const int64_t cost = rounds * ((keys + n - 1) / n + 160) + (n > 1 ? 200 : 0);
+    if (n == 1 || cost < least) {
+      best = n;
+      least = cost;
+    }
+  }
+  return best;
 }
-inline int64_t row_blocks_of(int64_t rows, int64_t dim) {
-  const int64_t n = block_rows_of(rows, dim);
-  return rows <= kFewRows ? 1 : (rows + n - 1) / n;
+
+// Few rows: they are bound by memory and their sequences differ in length, so all
+// keys of all sequences are dealt out in equal chunks, to as many workgroups as
+// this: the card once or more, at least four to a head of a sequence.  0: one
+// workgroup to each, without a join.
+inline int64_t chunks_for(int64_t units, int64_t rows, int64_t keys, int64_t dim, bool paged) {
+  const int64_t at_a_time = kCus * few_workgroups(padded_dim(dim), (int)rows, paged);
+  // (sums of keys are taken in 32 bits, in units of 128)
+  if (keys <= kSplitKeys || units >= 4 * at_a_time || units * (keys / 128 + 1) >= 1ll << 31) return 0;
+  const int64_t n = (4 * units + at_a_time - 1) / at_a_time * at_a_time, useful = units * ((keys + kSplitKeys - 1) / kSplitKeys + 1);
+  return n < useful ? n : useful;
 }
-inline size_t attend_workspace(int64_t batch, int64_t heads, int64_t rows, int64_t keys, int64_t dim) {
+inline int64_t row_blocks_of(int64_t rows) { return rows <= kFewRows ? 1 : (rows + kBlockRows - 1) / kBlockRows; }
+inline size_t attend_workspace(int64_t batch, int64_t heads, int64_t rows, int64_t keys, int64_t dim, bool paged) {
   if (batch <= 0 || heads <= 0 || rows <= 0 || keys <= 0 || !padded_dim(dim)) return 0;
-  const int64_t units = batch * heads * row_blocks_of(rows, dim), splits = splits_of(units, rows, keys);
-  if (splits == 1) return 0;
-  return (size_t)(units * splits * (rows <= kFewRows ? rows : block_rows_of(rows, dim)) * (dim + 2) * 4);
+  const int64_t units = batch * heads * row_blocks_of(rows);
+  if (rows <= kFewRows) return (size_t)(chunks_for(units, rows, keys, dim, paged) * rows * (dim + 2) * 4);
+  const int64_t splits = splits_of(units, keys, dim);
+  return splits == 1 ? 0 : (size_t)(units * splits * kBlockRows * (dim + 2) * 4);
 }
 
 // The part of a plan that both operators have.
-inline void plan_attend(AttendPlan& p, const thin_desc* q, const thin_desc* out, int64_t heads, int64_t keys, float c,
-                        void* workspace) {
+inline void plan_attend(AttendPlan& p, const thin_desc* q, const thin_desc* out, int64_t heads, int64_t keys, bool paged,
+                        float c, void* workspace) {
   memset(&p, 0, sizeof p);
   p.q = q->data;
   p.out = out->data;
@@ -121,19 +144,20 @@ inline void plan_attend(AttendPlan& p, const thin_desc* q, const thin_desc* out,
   p.dim = (uint32_t)q->sizes[3];
   p.keys = (uint32_t)keys;
   p.c = c;
-  const int64_t blocks = row_blocks_of(p.rows, p.dim), units = (int64_t)p.batch * heads * blocks;
-  const int64_t splits = splits_of(units, p.rows, keys);
-  const int64_t block_rows = p.rows <= kFewRows ? p.rows : block_rows_of(p.rows, p.dim);
-  p.block_rows = (uint32_t)block_rows;
+  const int64_t blocks = row_blocks_of(p.rows), units = (int64_t)p.batch * heads * blocks;
+  const bool few = p.rows <= kFewRows;
+  const int64_t chunks = few ? chunks_for(units, p.rows, keys, p.dim, paged) : 0, splits = few ? 1 : splits_of(units, keys, p.dim);
+  p.block_rows = few ? p.rows : kBlockRows;
   p.row_blocks = (uint32_t)blocks;
   p.splits = (uint32_t)splits;
+  p.chunks = (uint32_t)chunks;
   p.by_group = FastDiv::make(p.group);
   p.by_splits = FastDiv::make(p.splits);
   p.by_blocks = FastDiv::make(p.row_blocks);
   p.by_heads = FastDiv::make(p.heads);
-  if (splits > 1) {
+  if (splits > 1 || chunks) {
     p.sums = static_cast<float*>(workspace);
-    p.stats = p.sums + units * splits * block_rows * p.dim;
+    p.stats = p.sums + (chunks ? chunks : units * splits) * p.block_rows * p.dim;
   }
 }
 
@@ -272,6 +296,69 @@ __device__ __forceinline__ int32_t active_splits(int32_t n, uint32_t splits, int
   int32_t per = (steps + (int32_t)splits - 1) / (int32_t)splits;
   per = max(per, (int32_t)kSplitKeys / step);
   return (steps + per - 1) / per;
+}
+
+// Sum over the lanes up to this one, by DPP.
+__device__ __forceinline__ int32_t lanes_upto(int32_t v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, true);  // row_shr:1, :2, :4, :8
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);  // row_bcast:15, :31
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);
+  return v;
+}
+
+// Few rows, dealt out: chunk u of all sequences' is of sequence b, its `index`-th
+// of `count`, of `size` keys each; `first` is the sequence's first.  Wavefronts
+// find it for themselves, 64 sequences a round.
+struct Chunk {
+  int32_t size, first, index, count;
+  uint32_t b;
+  Sequence seq;
+};
+constexpr int32_t kChunkUnit = 128;  // keys that four wavefronts take at a time
+template <bool PAGED>
+__device__ __forceinline__ int32_t most_of(const Sequence& s) {
+  return s.tokens > 0 ? limit_of<PAGED>(s, s.tokens - 1) : 0;
+}
+// BY: sequence u's, not chunk u.  False: there is none.
+template <bool PAGED, bool BY>
+__device__ __forceinline__ bool find_chunk(const AttendPlan& p, uint32_t lane, uint32_t u, Chunk& c) {
+  const auto load = [&](uint32_t b) {
+    Sequence s{0, 0, 0};
+    if (b < p.batch) s = sequence_of<PAGED>(p, b);
+    return s;
+  };
+  const Sequence first = load(lane);
+  int32_t total = 0;  // in units
+  for (uint32_t b0 = 0; b0 < p.batch; b0 += 64) {
+    const int32_t n = most_of<PAGED>(b0 ? load(b0 + lane) : first);
+    total += __builtin_amdgcn_readlane(lanes_upto((n + kChunkUnit - 1) / kChunkUnit), 63);
+  }
+  // equal chunks; each head of a sequence may leave one unfilled
+  const int64_t room = (int64_t)p.chunks - (int64_t)p.batch * p.heads;
+  const int32_t even = (int32_t)(((int64_t)total * p.heads + room - 1) / room);
+  c.size = max(even * kChunkUnit, (int32_t)kSplitKeys);
+  int32_t ahead = 0;
+  for (uint32_t b0 = 0; b0 < p.batch; b0 += 64) {
+    const Sequence s = b0 ? load(b0 + lane) : first;
+    const int32_t n = (most_of<PAGED>(s) + c.size - 1) / c.size, upto = ahead + lanes_upto(n);
+    const uint64_t found = BY ? (u - b0 < 64 ? 1ull << (u - b0) : 0ull) : __ballot(upto > (int32_t)u);
+    if (found) {
+      const int at = __builtin_ctzll(found);
+      c.b = b0 + at;
+      c.count = __builtin_amdgcn_readlane(n, at);
+      c.first = __builtin_amdgcn_readlane(upto, at) - c.count;
+      c.index = (int32_t)u - c.first;
+      c.seq.tokens = __builtin_amdgcn_readlane(s.tokens, at);
+      c.seq.before = __builtin_amdgcn_readlane(s.before, at);
+      c.seq.length = __builtin_amdgcn_readlane(s.length, at);
+      return true;
+    }
+    ahead = __builtin_amdgcn_readlane(upto, 63);
+  }
+  return false;
 }
 
 __device__ __forceinline__ float lane_value(float v, int lane) {
@@ -420,8 +507,9 @@ __device__ __forceinline__ Place place_of(const AttendPlan& p) {
 // against the maximum so far, and again where that turns out too low.
 // Rows: unseen states have -inf in the scores from the start (the accumulator's
 // first value).  Pages: rows that do not see a whole step are masked afterwards.
-template <typename T, int DP, bool PAGED, int R>
-__global__ __launch_bounds__(256, DP * R <= 128 ? 2 : 1) void tile_kernel(AttendPlan p) {
+template <typename T, int DP, bool PAGED>
+__global__ __launch_bounds__(256, tile_workgroups(DP)) void tile_kernel(AttendPlan p) {
+  constexpr int R = 1;
   typedef typename Matrix<T>::v8 v8;
   constexpr int KT = 32;
   constexpr int kPer = PAGED ? DP / 16 : DP / 8, kElems = PAGED ? 16 : 8;  // 16-byte pieces of a key, elements of one
@@ -866,7 +954,7 @@ __device__ __forceinline__ constexpr uint32_t dim_of(uint32_t s, uint32_t quarte
 }
 
 template <typename T, int DP, bool PAGED, int R>
-__global__ __launch_bounds__(256, DP * R <= 64 ? 4 : DP <= 128 && DP * R <= 128 ? 3 : DP <= 128 || (PAGED && R == 1) ? 2 : 1) void few_kernel(AttendPlan p) {
+__global__ __launch_bounds__(256, few_workgroups(DP, 16 * R, PAGED)) void few_kernel(AttendPlan p) {
   typedef typename Matrix<T>::v8 v8;
   constexpr int KT = 32, W = 4, kSteps = DP / 32;
   constexpr int kPer = PAGED ? DP / 16 : DP / 8, kMine = KT * kPer / 64;  // pieces of a value row, of a lane
@@ -878,10 +966,27 @@ __global__ __launch_bounds__(256, DP * R <= 64 ? 4 : DP <= 128 && DP * R <= 128 
   __shared__ int32_t lowest[PAGED ? DP : 1];
   const uint32_t tid = threadIdx.x, lane = tid & 63u, col = lane & 15u, quarter = lane >> 4;
   const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(tid >> 6));
-  const Place w = place_of(p);
-  const Sequence seq = sequence_of<PAGED>(p, w.b);
-  const int32_t most = seq.tokens > 0 ? limit_of<PAGED>(seq, seq.tokens - 1) : 0, least = limit_of<PAGED>(seq, 0);
-  const Range range = range_of(most, w.split, p.splits, KT);
+  Place w;
+  Range range;
+  Sequence seq;
+  if (p.chunks) {
+    const uint32_t u = p.by_heads.div(blockIdx.x);
+    Chunk c;
+    if (!find_chunk<PAGED, false>(p, lane, u, c)) return;
+    w.b = c.b;
+    seq = c.seq;
+    w.h = blockIdx.x - u * p.heads;
+    range.begin = c.index * c.size;
+    range.end = range.begin + c.size;
+  } else {
+    w.b = p.by_heads.div(blockIdx.x);
+    w.h = blockIdx.x - w.b * p.heads;
+    seq = sequence_of<PAGED>(p, w.b);
+    range.begin = 0;
+    range.end = 0x7FFFFFFF;
+  }
+  const int32_t most = most_of<PAGED>(seq), least = limit_of<PAGED>(seq, 0);
+  range.end = min(range.end, most);
   T* lds_v = reinterpret_cast<T*>(lds + wave * kTile);
 
   u4 q[R][kSteps];
@@ -1181,8 +1286,6 @@ __global__ __launch_bounds__(256, DP * R <= 64 ? 4 : DP <= 128 && DP * R <= 128 
     }
   }
   float* sums = reinterpret_cast<float*>(lds);
-  const uint64_t unit = (uint64_t)w.b * p.heads + w.h;
-  const bool empty = range.begin >= range.end;
 #pragma unroll
   for (int part = 0; part < DP / kDims; ++part) {
 #pragma unroll
@@ -1211,15 +1314,15 @@ __global__ __launch_bounds__(256, DP * R <= 64 ? 4 : DP <= 128 && DP * R <= 128 
         for (int k = 0; k < 4; ++k)
           if (row_limit > lowest[d + k]) v[k] = __builtin_nanf("");
       }
-      if (p.splits == 1) {
+      if (!p.chunks) {
         const float total = row_l[r];
         const bool none = !live || total == 0.f;
         const float inv = 1.f / total;
 #pragma unroll
         for (int k = 0; k < 4; ++k) v[k] = none ? 0.f : v[k] * inv;
         store_pack<T, 4>(static_cast<T*>(p.out) + w.b * p.o_batch + rt * p.o_token + (w.h * p.group + rg) * p.o_head + d, v);
-      } else if (!empty) {
-        const uint64_t slot = (unit * p.splits + w.split) * p.rows + r;
+      } else {
+        const uint64_t slot = (uint64_t)blockIdx.x * p.rows + r;
         store_pack<float, 4>(p.sums + slot * p.dim + d, v);
         if (d == 0) {
           p.stats[slot * 2] = row_m[r];
@@ -1236,27 +1339,40 @@ __global__ __launch_bounds__(256, DP * R <= 64 ? 4 : DP <= 128 && DP * R <= 128 
 // as many splits side by side as that leaves threads for (128 splits of 240 rows
 // took 62 us by one wavefront a row, split after split).
 template <typename T, bool PAGED, int E>
-__global__ __launch_bounds__(256) void join_kernel(AttendPlan p, uint32_t few) {
+__global__ __launch_bounds__(256) void join_kernel(AttendPlan p) {
   __shared__ f4 part[256];
-  const uint32_t lane = threadIdx.x & 63u, mine = threadIdx.x % E, block_rows = p.block_rows;
+  const uint32_t lane = threadIdx.x & 63u, mine = threadIdx.x % E;
   const uint64_t at = (uint64_t)blockIdx.x * (256 / E) + threadIdx.x / E;  // (b, h, row)
   if (E < 256 && at >= (uint64_t)p.batch * p.heads * p.rows) return;
   const uint32_t unit = (uint32_t)(at / p.rows), row = (uint32_t)(at - (uint64_t)unit * p.rows);
   const uint32_t b = p.by_heads.div(unit), h = unit - b * p.heads;
   const uint32_t t = p.by_group.div(row), g = row - t * p.group;
-  const Sequence seq = sequence_of<PAGED>(p, b);
-  const uint32_t block = row / block_rows;
-  const int32_t t_first = (int32_t)p.by_group.div(block * block_rows);
-  const int32_t t_last = min((int32_t)p.by_group.div(min(p.rows, (block + 1) * block_rows) - 1), seq.tokens - 1);
-  const int32_t most = t_last < t_first ? 0 : limit_of<PAGED>(seq, t_last);
-  const int32_t n = (int32_t)t < seq.tokens ? active_splits(most, p.splits, few ? 32 : 64) : 0;
-  const uint64_t first = ((uint64_t)unit * p.row_blocks + block) * p.splits * block_rows + (row - block * block_rows);
+  Sequence seq;
+  int32_t n;
+  uint64_t first, step;  // its splits' places
+  if (p.chunks) {
+    Chunk c;
+    find_chunk<PAGED, true>(p, lane, b, c);
+    seq = c.seq;
+    n = c.count;
+    first = ((uint64_t)c.first * p.heads + h) * p.rows + row;
+    step = (uint64_t)p.heads * p.rows;
+  } else {
+    seq = sequence_of<PAGED>(p, b);
+    const uint32_t block = row / kBlockRows;
+    const int32_t t_first = (int32_t)p.by_group.div(block * kBlockRows);
+    const int32_t t_last = min((int32_t)p.by_group.div(min(p.rows, (block + 1) * kBlockRows) - 1), seq.tokens - 1);
+    n = active_splits(t_last < t_first ? 0 : limit_of<PAGED>(seq, t_last), p.splits, 64);
+    first = ((uint64_t)unit * p.row_blocks + block) * p.splits * kBlockRows + (row - block * kBlockRows);
+    step = kBlockRows;
+  }
+  if ((int32_t)t >= seq.tokens) n = 0;
   // every wavefront knows the maximum and the total
   float m = -__builtin_inff(), l = 0.f;
-  for (int32_t i = (int32_t)lane; i < n; i += 64) m = fmaxf(m, p.stats[(first + (uint64_t)i * block_rows) * 2]);
+  for (int32_t i = (int32_t)lane; i < n; i += 64) m = fmaxf(m, p.stats[(first + (uint64_t)i * step) * 2]);
   m = group_max<64>(m);
   for (int32_t i = (int32_t)lane; i < n; i += 64) {
-    const float* stats = p.stats + (first + (uint64_t)i * block_rows) * 2;
+    const float* stats = p.stats + (first + (uint64_t)i * step) * 2;
     l += stats[1] * rescale_of(stats[0], m, p.c);
   }
   l = group_sum<64>(l);
@@ -1265,7 +1381,7 @@ __global__ __launch_bounds__(256) void join_kernel(AttendPlan p, uint32_t few) {
   if (side < sides) {
 #pragma unroll 4
     for (int32_t i = (int32_t)side; i < n; i += (int32_t)sides) {
-      const uint64_t slot = first + (uint64_t)i * block_rows;
+      const uint64_t slot = first + (uint64_t)i * step;
       float x[4];
       load_pack<float, 4>(p.sums + slot * p.dim + d, x);
       const float f = rescale_of(p.stats[slot * 2], m, p.c);
@@ -1291,19 +1407,16 @@ __global__ __launch_bounds__(256) void join_kernel(AttendPlan p, uint32_t few) {
 // Launches a plan whose operands are checked.
 template <typename T, int DP, bool PAGED>
 thin_status launch_attend_dim(const AttendPlan& p, hipStream_t stream) {
-  const bool few = p.rows <= kFewRows;
-  const uint32_t grid = p.batch * p.heads * p.row_blocks * p.splits;
-  if (p.rows <= 16) hipLaunchKernelGGL((dev::few_kernel<T, DP, PAGED, 1>), dim3(grid), dim3(256), 0, stream, p);
-  else if (few) hipLaunchKernelGGL((dev::few_kernel<T, DP, PAGED, 2>), dim3(grid), dim3(256), 0, stream, p);
-  else if (p.block_rows == 128) hipLaunchKernelGGL((dev::tile_kernel<T, DP, PAGED, 1>), dim3(grid), dim3(256), 0, stream, p);
-  else if constexpr (DP <= 128) hipLaunchKernelGGL((dev::tile_kernel<T, DP, PAGED, 2>), dim3(grid), dim3(256), 0, stream, p);
+  const uint32_t units = p.batch * p.heads * p.row_blocks;
+  if (p.rows <= 16) hipLaunchKernelGGL((dev::few_kernel<T, DP, PAGED, 1>), dim3(p.chunks ? p.chunks : units), dim3(256), 0, stream, p);
+  else if (p.rows <= kFewRows) hipLaunchKernelGGL((dev::few_kernel<T, DP, PAGED, 2>), dim3(p.chunks ? p.chunks : units), dim3(256), 0, stream, p);
+  else hipLaunchKernelGGL((dev::tile_kernel<T, DP, PAGED>), dim3(units * p.splits), dim3(256), 0, stream, p);
   THIN_LAUNCH_CHECK("attend");
-  if (p.splits > 1) {
-    const uint64_t rows = (uint64_t)p.batch * p.heads * p.rows;
-    if (p.splits <= kJoinByWave)
-      hipLaunchKernelGGL((dev::join_kernel<T, PAGED, 64>), dim3((uint32_t)((rows + 3) / 4)), dim3(256), 0, stream, p, few ? 1u : 0u);
-    else
-      hipLaunchKernelGGL((dev::join_kernel<T, PAGED, 256>), dim3((uint32_t)rows), dim3(256), 0, stream, p, few ? 1u : 0u);
+  const int64_t parts = p.rows <= kFewRows ? p.chunks / (p.batch * p.heads) : p.splits;  // of a row, on the average
+  if (p.chunks || p.splits > 1) {
+    const uint32_t rows = p.batch * p.heads * p.rows;
+    if (parts <= kJoinByWave) hipLaunchKernelGGL((dev::join_kernel<T, PAGED, 64>), dim3((rows + 3) / 4), dim3(256), 0, stream, p);
+    else hipLaunchKernelGGL((dev::join_kernel<T, PAGED, 256>), dim3(rows), dim3(256), 0, stream, p);
     THIN_LAUNCH_CHECK("attend_join");
   }
   return THIN_OK;

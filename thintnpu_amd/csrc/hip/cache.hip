@@ -242,7 +242,7 @@ extern "C" size_t thin_cache_attention_workspace(const thin_desc* q, const thin_
       table->rank != 2 || k_cache->sizes[1] <= 0)
     return 0;
   return attend_workspace(q->sizes[0], k_cache->sizes[1], q->sizes[1] * (q->sizes[2] / k_cache->sizes[1]),
-                          table->sizes[1] * k_cache->sizes[2], q->sizes[3]);
+                          table->sizes[1] * k_cache->sizes[2], q->sizes[3], true);
 }
 
 extern "C" thin_status thin_cache_attention(const thin_desc* q, const thin_desc* k_cache, const thin_desc* v_cache,
@@ -269,20 +269,20 @@ extern "C" thin_status thin_cache_attention(const thin_desc* q, const thin_desc*
   const float c = scale * 1.4426950408889634f;
   THIN_REQUIRE(isnormal(c) && c > 0.f, THIN_ERR_INVALID, "cache_attention: the scale must be positive and finite");
   if (numel(q) == 0) return THIN_OK;
-  const int64_t rows = T * (H / Hk), blocks = row_blocks_of(rows, D);
+  const int64_t rows = T * (H / Hk), blocks = row_blocks_of(rows);
   THIN_REQUIRE(rows < (1ll << 30) && B < (1ll << 30) && launchable(B * Hk * blocks, 256) &&
                    launchable(B * Hk * rows, 256),
                THIN_ERR_UNSUPPORTED, "cache_attention: tensor too large");
   THIN_REQUIRE(!repeats(out), THIN_ERR_INVALID, "cache_attention: out has a stride of 0");
   for (const thin_desc* in : {q, k_cache, v_cache, k_scales, v_scales, table, lengths, counts})
     THIN_REQUIRE(!in || !overlap(out, in), THIN_ERR_INVALID, "cache_attention: out overlaps an input");
-  const size_t need = attend_workspace(B, Hk, rows, S, D);
+  const size_t need = attend_workspace(B, Hk, rows, S, D, true);
   THIN_REQUIRE(workspace_bytes >= need && (need == 0 || workspace), THIN_ERR_WORKSPACE,
                "cache_attention needs %zu bytes of workspace, got %zu", need, workspace_bytes);
   THIN_REQUIRE(need == 0 || workspace_aligned(workspace), THIN_ERR_WORKSPACE,
                "cache_attention: the workspace must be 4-byte aligned");
   AttendPlan p;
-  plan_attend(p, q, out, Hk, S, c, workspace);
+  plan_attend(p, q, out, Hk, S, true, c, workspace);
   p.lengths = static_cast<const int32_t*>(lengths->data);
   p.length_step = lengths->strides[0];
   if (counts) {

@@ -10,7 +10,8 @@ using namespace thin;
 
 extern "C" size_t thin_cross_attention_workspace(const thin_desc* q, const thin_desc* k) {
   if (!desc_valid(q) || !desc_valid(k) || q->rank != 4 || k->rank != 4 || k->sizes[2] <= 0) return 0;
-  return attend_workspace(q->sizes[0], k->sizes[2], q->sizes[1] * (q->sizes[2] / k->sizes[2]), k->sizes[1], q->sizes[3]);
+  return attend_workspace(q->sizes[0], k->sizes[2], q->sizes[1] * (q->sizes[2] / k->sizes[2]), k->sizes[1], q->sizes[3],
+                          false);
 }
 
 extern "C" thin_status thin_cross_attention(const thin_desc* q, const thin_desc* k, const thin_desc* v,
@@ -45,20 +46,20 @@ extern "C" thin_status thin_cross_attention(const thin_desc* q, const thin_desc*
   const float c = scale * 1.4426950408889634f;
   THIN_REQUIRE(isnormal(c) && c > 0.f, THIN_ERR_INVALID, "cross_attention: the scale must be positive and finite");
   if (numel(q) == 0) return THIN_OK;
-  const int64_t rows = T * (H / Hk), blocks = row_blocks_of(rows, D);
+  const int64_t rows = T * (H / Hk), blocks = row_blocks_of(rows);
   THIN_REQUIRE(rows < (1ll << 30) && S < (1ll << 30) && B < (1ll << 30) && launchable(B * Hk * blocks, 256) &&
                    launchable(B * Hk * rows, 256),
                THIN_ERR_UNSUPPORTED, "cross_attention: tensor too large");
   THIN_REQUIRE(!repeats(out), THIN_ERR_INVALID, "cross_attention: out has a stride of 0");
   for (const thin_desc* in : {q, k, v, lengths, mask})
     THIN_REQUIRE(!in || !overlap(out, in), THIN_ERR_INVALID, "cross_attention: out overlaps an input");
-  const size_t need = attend_workspace(B, Hk, rows, S, D);
+  const size_t need = attend_workspace(B, Hk, rows, S, D, false);
   THIN_REQUIRE(workspace_bytes >= need && (need == 0 || workspace), THIN_ERR_WORKSPACE,
                "cross_attention needs %zu bytes of workspace, got %zu", need, workspace_bytes);
   THIN_REQUIRE(need == 0 || workspace_aligned(workspace), THIN_ERR_WORKSPACE,
                "cross_attention: the workspace must be 4-byte aligned");
   AttendPlan p;
-  plan_attend(p, q, out, Hk, S, c, workspace);
+  plan_attend(p, q, out, Hk, S, false, c, workspace);
   if (lengths) {
     p.lengths = static_cast<const int32_t*>(lengths->data);
     p.length_step = lengths->strides[0];

@@ -354,6 +354,9 @@ __device__ __forceinline__ bool find_chunk(const AttendPlan& p, uint32_t lane, u
       c.seq.tokens = __builtin_amdgcn_readlane(s.tokens, at);
       c.seq.before = __builtin_amdgcn_readlane(s.before, at);
       c.seq.length = __builtin_amdgcn_readlane(s.length, at);
+      // the sequence's own chunks as equal as units allow
+      const int32_t units = (most_of<PAGED>(c.seq) + kChunkUnit - 1) / kChunkUnit;
+      if (c.count > 0) c.size = (units + c.count - 1) / c.count * kChunkUnit;
       return true;
     }
     ahead = __builtin_amdgcn_readlane(upto, 63);
@@ -1040,7 +1043,6 @@ __global__ __launch_bounds__(256, few_workgroups(DP, 16 * R, PAGED)) void few_ke
   u4 rk[2][PAGED ? (kSteps + 1) / 2 : kSteps];
   u4 rv[kMine];
   int32_t id[2] = {0, 0};
-  float ks[2] = {0.f, 0.f}, vs[2] = {0.f, 0.f};
   bool seen = true;  // of key lane & 31
   const auto fetch = [&](int32_t k0, int32_t ahead) {  // `ahead` tiles behind the last look_up()
     if constexpr (PAGED) {
@@ -1049,8 +1051,6 @@ __global__ __launch_bounds__(256, few_workgroups(DP, 16 * R, PAGED)) void few_ke
 #pragma unroll
       for (int n = 0; n < 2; ++n) {
         id[n] = __builtin_amdgcn_readlane(page_id, ahead * 2 + n);
-        ks[n] = lane_value(page_ks, ahead * 2 + n);
-        vs[n] = lane_value(page_vs, ahead * 2 + n);
         const uint32_t key = (uint32_t)k0 + n * 16, at = key - p.by_page.div(key) * p.page_size;
         kb[n] = code_at(p.kp, id[n], w.h, at);
         vb[n] = code_at(p.vp, id[n], w.h, at);
@@ -1163,7 +1163,8 @@ __global__ __launch_bounds__(256, few_workgroups(DP, 16 * R, PAGED)) void few_ke
       }
     }
     wave_lds_fence();
-    const float ks0 = PAGED ? ks[0] : 1.f, ks1 = PAGED ? ks[1] : 1.f, vs0 = vs[0], vs1 = vs[1];
+    const float ks0 = PAGED ? lane_value(page_ks, ahead * 2) : 1.f, ks1 = PAGED ? lane_value(page_ks, ahead * 2 + 1) : 1.f;
+    const float vs0 = PAGED ? lane_value(page_vs, ahead * 2) : 1.f, vs1 = PAGED ? lane_value(page_vs, ahead * 2 + 1) : 1.f;
     if (k0 + W * KT < range.end) {
       if (PAGED && ++ahead == 32) {
         look_up(k0 + W * KT);

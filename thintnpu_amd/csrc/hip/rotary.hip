@@ -55,20 +55,30 @@ __device__ __forceinline__ void sin_cos(double turns, float& s, float& c) {
   c = (n + 1) & 2 ? -b : b;
 }
 
-// n of up to N elements from p on (N when n is).
-template <typename T, int N>
+// n of up to N elements from p on (N when n is); NT: streaming.
+template <bool NT, typename T, int N>
 __device__ __forceinline__ void load_some(const T* p, uint32_t n, float (&v)[N]) {
+  typedef typename dev::Pack<T, N>::type pack;
   if (n >= (uint32_t)N) {
-    dev::load_pack<T, N>(p, v);
+    pack w;
+    if constexpr (NT) w = __builtin_nontemporal_load(reinterpret_cast<const pack*>(p));
+    else w = *reinterpret_cast<const pack*>(p);
+#pragma unroll
+    for (int j = 0; j < N; ++j) v[j] = (float)w[j];
   } else {
 #pragma unroll
     for (int j = 0; j < N; ++j) v[j] = (float)p[min((uint32_t)j, n - 1)];
   }
 }
-template <typename T, int N>
+template <bool NT, typename T, int N>
 __device__ __forceinline__ void store_some(T* p, uint32_t n, const float (&v)[N]) {
+  typedef typename dev::Pack<T, N>::type pack;
   if (n >= (uint32_t)N) {
-    dev::store_pack<T, N>(p, v);
+    pack w;
+#pragma unroll
+    for (int j = 0; j < N; ++j) w[j] = (T)v[j];
+    if constexpr (NT) __builtin_nontemporal_store(w, reinterpret_cast<pack*>(p));
+    else *reinterpret_cast<pack*>(p) = w;
   } else {
 #pragma unroll
     for (int j = 0; j < N; ++j)
@@ -76,8 +86,10 @@ __device__ __forceinline__ void store_some(T* p, uint32_t n, const float (&v)[N]
   }
 }
 
-// V pairs a piece (halves: V elements from each half; adjacent: 2 V elements).
-template <typename T, int V, bool ADJACENT>
+// V pairs a piece (halves: V elements from each half; interleaved: 2 V elements).
+// Heads go two at a time: their loads are issued before the first is stored.
+constexpr int kHeadsAhead = 2;
+template <typename T, int V, bool INTERLEAVED, bool NT>
 __global__ __launch_bounds__(256) void rotary_kernel(RotaryPlan p) {
   const uint64_t id = (uint64_t)blockIdx.x * 256 + threadIdx.x;
   if (id >= p.threads) return;
@@ -100,8 +112,8 @@ __global__ __launch_bounds__(256) void rotary_kernel(RotaryPlan p) {
       head_of(h, x, out);
       if (x == out) continue;
       float v[V];
-      load_some<T, V>(x + d, p.dim - d, v);
-      store_some<T, V>(out + d, p.dim - d, v);
+      load_some<NT, T, V>(x + d, p.dim - d, v);
+      store_some<NT, T, V>(out + d, p.dim - d, v);
     }
     return;
   }
@@ -122,41 +134,61 @@ __global__ __launch_bounds__(256) void rotary_kernel(RotaryPlan p) {
       }
     }
   }
-  for (uint32_t h = first; h < last; ++h) {
+  for (uint32_t h0 = first; h0 < last; h0 += kHeadsAhead) {
+    // u, v: the first and the second of each pair, or (interleaved) the pairs' halves as they lie
+    float u[kHeadsAhead][V], v[kHeadsAhead][V];
     const T* x;
     T* out;
-    head_of(h, x, out);
-    if constexpr (ADJACENT) {
-      float v[2 * V];
-      load_some<T, 2 * V>(x + 2 * i0, 2 * n, v);
 #pragma unroll
-      for (int j = 0; j < V; ++j) {
-        const float a = v[2 * j], d = v[2 * j + 1];
-        v[2 * j] = a * c[j] - d * s[j];
-        v[2 * j + 1] = d * c[j] + a * s[j];
-      }
-      store_some<T, 2 * V>(out + 2 * i0, 2 * n, v);
-    } else {
-      float u[V], v[V];
-      load_some<T, V>(x + i0, n, u);
-      load_some<T, V>(x + p.pairs + i0, n, v);
+    for (int k = 0; k < kHeadsAhead; ++k)
+      if (h0 + k < last) {
+        head_of(h0 + k, x, out);
+        if constexpr (INTERLEAVED) {
+          float both[2 * V];
+          load_some<NT, T, 2 * V>(x + 2 * i0, 2 * n, both);
 #pragma unroll
-      for (int j = 0; j < V; ++j) {
-        const float a = u[j], d = v[j];
-        u[j] = a * c[j] - d * s[j];
-        v[j] = d * c[j] + a * s[j];
+          for (int j = 0; j < V; ++j) {
+            u[k][j] = both[2 * j];
+            v[k][j] = both[2 * j + 1];
+          }
+        } else {
+          load_some<NT, T, V>(x + i0, n, u[k]);
+          load_some<NT, T, V>(x + p.pairs + i0, n, v[k]);
+        }
       }
-      store_some<T, V>(out + i0, n, u);
-      store_some<T, V>(out + p.pairs + i0, n, v);
-    }
+#pragma unroll
+    for (int k = 0; k < kHeadsAhead; ++k)
+      if (h0 + k < last) {
+        head_of(h0 + k, x, out);
+        float first_of[V], second_of[V];
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          first_of[j] = u[k][j] * c[j] - v[k][j] * s[j];
+          second_of[j] = v[k][j] * c[j] + u[k][j] * s[j];
+        }
+        if constexpr (INTERLEAVED) {
+          float both[2 * V];
+#pragma unroll
+          for (int j = 0; j < V; ++j) {
+            both[2 * j] = first_of[j];
+            both[2 * j + 1] = second_of[j];
+          }
+          store_some<NT, T, 2 * V>(out + 2 * i0, 2 * n, both);
+        } else {
+          store_some<NT, T, V>(out + i0, n, first_of);
+          store_some<NT, T, V>(out + p.pairs + i0, n, second_of);
+        }
+      }
   }
 }
 
 // Threads that fill the card a few times over; past them a thread takes more
 // heads with its angles.
 constexpr int64_t kEnough = 256 * 2048;
+// Tensors from this many bytes on are read and written past the caches.
+constexpr int64_t kRotaryStreaming = (int64_t)64 << 20;
 
-template <typename T, int V, bool ADJACENT>
+template <typename T, int V, bool INTERLEAVED>
 thin_status launch(RotaryPlan& p, int64_t rows, hipStream_t stream) {
   p.turn_pieces = (p.pairs + V - 1) / V;
   p.pieces = p.turn_pieces + (p.dim - 2 * p.pairs + V - 1) / V;
@@ -170,7 +202,11 @@ thin_status launch(RotaryPlan& p, int64_t rows, hipStream_t stream) {
   p.by_pieces = FastDiv::make(p.pieces);
   p.by_chunks = FastDiv::make(p.chunks);
   p.by_tokens = FastDiv::make(p.tokens);
-  hipLaunchKernelGGL((rotary_kernel<T, V, ADJACENT>), dim3((uint32_t)((threads + 255) / 256)), dim3(256), 0, stream, p);
+  const dim3 grid((uint32_t)((threads + 255) / 256)), block(256);
+  if (rows * p.all_heads * p.dim * (int64_t)sizeof(T) >= kRotaryStreaming)
+    hipLaunchKernelGGL((rotary_kernel<T, V, INTERLEAVED, true>), grid, block, 0, stream, p);
+  else
+    hipLaunchKernelGGL((rotary_kernel<T, V, INTERLEAVED, false>), grid, block, 0, stream, p);
   THIN_LAUNCH_CHECK("rotary_axes");
   return THIN_OK;
 }

@@ -88,7 +88,7 @@ constexpr int tile_workgroups(int DP) { return DP <= 32 ? 4 : DP <= 64 ? 3 : DP 
 constexpr int64_t kCus = 256;
 constexpr int64_t kSplitKeys = 256;  // keys of a split at least: fewer cost more to join than they give
 constexpr int64_t kMaxSplits = 128;
-constexpr uint32_t kJoinByWave = 8;  // splits that one wavefront joins; more take a workgroup
+constexpr uint32_t kJoinByWave = 8;  // splits that one wavefront or less joins; more take a workgroup
 
 // Many rows: splits of every row's keys.  In rounds of the workgroups that the card
 // holds, each as long as its keys and some 160 more, which beginning and end cost,
@@ -368,6 +368,13 @@ __device__ __forceinline__ float lane_value(float v, int lane) {
   return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), lane));
 }
 
+// The same address, known to be all lanes': a buffer descriptor that the compiler
+// takes for a lane's own costs a loop over the lanes at each load.
+__device__ __forceinline__ const uint8_t* scalar(const uint8_t* p) {
+  const uint64_t a = reinterpret_cast<uint64_t>(p);
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)a), hi = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(a >> 32));
+  return reinterpret_cast<const uint8_t*>((uint64_t)hi << 32 | lo);
+}
 __device__ __forceinline__ u4 load16(const void* p) { return *reinterpret_cast<const u4e*>(p); }
 __device__ __forceinline__ const uint8_t* code_at(const PagesOf& c, int32_t id, uint32_t h, uint32_t token) {
   return c.codes + id * c.page + h * c.head + token * c.token;
@@ -630,7 +637,7 @@ __global__ __launch_bounds__(256, tile_workgroups(DP)) void tile_kernel(AttendPl
       id_k = __builtin_amdgcn_readlane(at < 32 ? here.id : there.id, (at & 31) * 2 + (int32_t)(wave >> 1));
       const auto rsrc_of = [&](const uint8_t* codes, const PagesOf& x, int32_t id, int32_t key) {
         const uint32_t token = (uint32_t)key - p.by_page.div((uint32_t)key) * p.page_size;
-        return buffer_rsrc(codes + id * x.page + token * x.token, id >= 0 ? kNowhere : 0u);
+        return buffer_rsrc(scalar(codes + id * x.page + token * x.token), id >= 0 ? kNowhere : 0u);
       };
       const auto kr = rsrc_of(k_codes, p.kp, id_k, k0), vr = rsrc_of(v_codes, p.vp, id_v, max(v0, 0));
 #pragma unroll
@@ -1338,11 +1345,13 @@ __global__ __launch_bounds__(256, few_workgroups(DP, 16 * R, PAGED)) void few_ke
 // ---------------------------------------------------------------- splits
 // A row's splits at their highest maximum, by E threads: four dims a thread, and
 // as many splits side by side as that leaves threads for (128 splits of 240 rows
-// took 62 us by one wavefront a row, split after split).
+// took 62 us by one wavefront a row, split after split, 9 by a workgroup each; 5
+// splits of 19200 narrow rows 13.8 by a wavefront, XX by 16 lanes).
 template <typename T, bool PAGED, int E>
 __global__ __launch_bounds__(256) void join_kernel(AttendPlan p) {
   __shared__ f4 part[256];
-  const uint32_t lane = threadIdx.x & 63u, mine = threadIdx.x % E;
+  constexpr int G = E < 64 ? E : 64;  // lanes that know of the row what all need
+  const uint32_t lane = threadIdx.x & (G - 1u), mine = threadIdx.x % E;
   const uint64_t at = (uint64_t)blockIdx.x * (256 / E) + threadIdx.x / E;  // (b, h, row)
   if (E < 256 && at >= (uint64_t)p.batch * p.heads * p.rows) return;
   const uint32_t unit = (uint32_t)(at / p.rows), row = (uint32_t)(at - (uint64_t)unit * p.rows);
@@ -1351,7 +1360,7 @@ __global__ __launch_bounds__(256) void join_kernel(AttendPlan p) {
   Sequence seq;
   int32_t n;
   uint64_t first, step;  // its splits' places
-  if (p.chunks) {
+  if (E >= 64 && p.chunks) {  // (a wavefront's rows are of one sequence)
     Chunk c;
     find_chunk<PAGED, true>(p, lane, b, c);
     seq = c.seq;
@@ -1368,15 +1377,15 @@ __global__ __launch_bounds__(256) void join_kernel(AttendPlan p) {
     step = kBlockRows;
   }
   if ((int32_t)t >= seq.tokens) n = 0;
-  // every wavefront knows the maximum and the total
+  // the maximum and the total
   float m = -__builtin_inff(), l = 0.f;
-  for (int32_t i = (int32_t)lane; i < n; i += 64) m = fmaxf(m, p.stats[(first + (uint64_t)i * step) * 2]);
-  m = group_max<64>(m);
-  for (int32_t i = (int32_t)lane; i < n; i += 64) {
+  for (int32_t i = (int32_t)lane; i < n; i += G) m = fmaxf(m, p.stats[(first + (uint64_t)i * step) * 2]);
+  m = group_max<G>(m);
+  for (int32_t i = (int32_t)lane; i < n; i += G) {
     const float* stats = p.stats + (first + (uint64_t)i * step) * 2;
     l += stats[1] * rescale_of(stats[0], m, p.c);
   }
-  l = group_sum<64>(l);
+  l = group_sum<G>(l);
   const uint32_t quads = p.dim / 4, sides = E / quads, side = mine / quads, d = (mine - side * quads) * 4;
   f4 v = {0.f, 0.f, 0.f, 0.f};
   if (side < sides) {
@@ -1416,7 +1425,9 @@ thin_status launch_attend_dim(const AttendPlan& p, hipStream_t stream) {
   const int64_t parts = p.rows <= kFewRows ? p.chunks / (p.batch * p.heads) : p.splits;  // of a row, on the average
   if (p.chunks || p.splits > 1) {
     const uint32_t rows = p.batch * p.heads * p.rows;
-    if (parts <= kJoinByWave) hipLaunchKernelGGL((dev::join_kernel<T, PAGED, 64>), dim3((rows + 3) / 4), dim3(256), 0, stream, p);
+    if (parts <= kJoinByWave && p.dim <= 64 && !p.chunks)
+      hipLaunchKernelGGL((dev::join_kernel<T, PAGED, 16>), dim3((rows + 15) / 16), dim3(256), 0, stream, p);
+    else if (parts <= kJoinByWave) hipLaunchKernelGGL((dev::join_kernel<T, PAGED, 64>), dim3((rows + 3) / 4), dim3(256), 0, stream, p);
     else hipLaunchKernelGGL((dev::join_kernel<T, PAGED, 256>), dim3(rows), dim3(256), 0, stream, p);
     THIN_LAUNCH_CHECK("attend_join");
   }

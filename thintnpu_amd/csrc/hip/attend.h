@@ -486,22 +486,26 @@ __device__ __forceinline__ void store_row(const AttendPlan& p, uint32_t b, uint3
   }
 }
 
-// Where a workgroup works.  Workgroups are dealt to the 8 XCDs in turn; each XCD
-// takes a run of neighbours, which read the same keys through its L2.  Row
-// blocks go from the last (whose causal rows see the most keys) to the first.
+// Where a workgroup works.  Workgroups are dealt to the 8 XCDs in turn.  Those of a
+// head and split read the same keys: they go to one XCD's L2, and heads and splits
+// to the XCDs in turn, so that sequences of unequal length are spread (in runs, an
+// XCD with the longest sequence's heads worked on when the others had ended: chunks
+// of prompts 310 us, 168 so).  What is left of them goes to all XCDs.  Row blocks go
+// from the last (whose causal rows see the most keys) to the first.
 struct Place {
   uint32_t b, h, block, split;
 };
 __device__ __forceinline__ Place place_of(const AttendPlan& p) {
-  const uint32_t nb = gridDim.x, xcd = blockIdx.x & 7u, at = blockIdx.x >> 3;
-  uint32_t i = xcd * (nb >> 3) + min(xcd, nb & 7u) + at, r;
+  const uint32_t groups = p.batch * p.heads * p.splits, whole = (groups >> 3) * p.row_blocks, xcd = blockIdx.x & 7u, at = blockIdx.x >> 3;
+  const bool dealt = at < whole;
+  const uint32_t i = dealt ? at : blockIdx.x - whole * 8, n = p.by_blocks.div(i);
+  const uint32_t group = dealt ? n * 8 + xcd : (groups & ~7u) + n;
   Place w;
-  r = p.by_splits.div(i);
-  w.split = i - r * p.splits;
-  i = p.by_blocks.div(r);
-  w.block = p.row_blocks - 1 - (r - i * p.row_blocks);
-  w.b = p.by_heads.div(i);
-  w.h = i - w.b * p.heads;
+  w.block = p.row_blocks - 1 - (i - n * p.row_blocks);
+  const uint32_t unit = p.by_splits.div(group);
+  w.split = group - unit * p.splits;
+  w.b = p.by_heads.div(unit);
+  w.h = unit - w.b * p.heads;
   return w;
 }
 
@@ -1346,7 +1350,7 @@ __global__ __launch_bounds__(256, few_workgroups(DP, 16 * R, PAGED)) void few_ke
 // A row's splits at their highest maximum, by E threads: four dims a thread, and
 // as many splits side by side as that leaves threads for (128 splits of 240 rows
 // took 62 us by one wavefront a row, split after split, 9 by a workgroup each; 5
-// splits of 19200 narrow rows 13.8 by a wavefront, XX by 16 lanes).
+// splits of 19200 narrow rows 13.8 by a wavefront, 5.9 by 16 lanes).
 template <typename T, bool PAGED, int E>
 __global__ __launch_bounds__(256) void join_kernel(AttendPlan p) {
   __shared__ f4 part[256];

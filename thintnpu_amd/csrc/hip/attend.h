@@ -380,44 +380,22 @@ __device__ __forceinline__ const uint8_t* code_at(const PagesOf& c, int32_t id, 
   return c.codes + id * c.page + h * c.head + token * c.token;
 }
 
-// A lane's query row as the B operand of its steps; zeros for no row.
-template <typename T, int DP>
-__device__ __forceinline__ void load_query(const AttendPlan& p, uint32_t b, uint32_t h, uint32_t t, uint32_t g, bool live,
-                                           uint32_t half, u4 (&q)[DP / 16]) {
-  const T* row = static_cast<const T*>(p.q) + b * p.q_batch + t * p.q_token + (h * p.group + g) * p.q_head;
-#pragma unroll
-  for (int i = 0; i < DP / 16; ++i) {
-    const uint32_t d = (i / 2) * 32 + half * 16 + (i % 2) * 8;
-    q[i] = u4{0, 0, 0, 0};
-    if (live && d < p.dim) q[i] = load16(row + d);
-  }
-}
-
 // The maximum that a row's exponentials stand against is raised where a score
 // passes it by kSlack bits, not by less: sums are rescaled in few tiles, and an
 // exponential is 2^kSlack at most.
 constexpr float kSlack = 4.f;
 
-// A row's exponentials are 2^(c s + offset_of(m)).  The offset is rounded, in
-// proportion to m; what is taken from one maximum to another goes by the
-// difference of the offsets as they are, so that the rounding is common to all.
-__device__ __forceinline__ float offset_of(float m, float c, float shift) {
-  return shift - (m == -__builtin_inff() ? 0.f : m) * c;
-}
-__device__ __forceinline__ float rescale_of(float from, float to, float c) {
+// Maxima are those of c s, rounded.  A row's exponentials are 2^(c s + offset_of(m))
+// with the product in full: the maximum's rounding is common to all.
+__device__ __forceinline__ float offset_of(float m) { return m == -__builtin_inff() ? 0.f : -m; }
+__device__ __forceinline__ float rescale_of(float from, float to) {
   if (from == to) return 1.f;
-  return from == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(offset_of(to, c, 0.f) - offset_of(from, c, 0.f));
+  return from == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(offset_of(to) - offset_of(from));
 }
+// The scores' factor at least where some are -inf: 0 (a page's scale) times that is none.
+constexpr float kLeastFactor = 1.17549435e-38f;
 
-// Eight exponentials of a lane as the B operand: keys 16 kb + 4 half + {0..3, 8..11}.
-template <typename TV>
-__device__ __forceinline__ typename Matrix<TV>::v8 pack8(const f16v& s, int kb) {
-  typename Matrix<TV>::v8 r;
-#pragma unroll
-  for (int j = 0; j < 8; ++j) r[j] = (TV)s[kb * 8 + j];
-  return r;
-}
-// The same keys of V^T from LDS, for dims 32 i + (lane & 31).
+// V^T from LDS as the A operand, for dims 32 i + (lane & 31) and keys row + 4 half + {0..3, 8..11}.
 template <typename TV, int STRIDE>
 __device__ __forceinline__ typename Matrix<TV>::v8 values8(const TV* v, int row, int i, uint32_t lane) {
   const uint32_t at = (row + (lane >> 5) * 4 + ((lane >> 2) & 3)) * STRIDE + i * 32 + ((lane >> 4) & 1) * 16 + (lane & 3) * 4;
@@ -432,12 +410,14 @@ __device__ __forceinline__ typename Matrix<TV>::v8 values8(const TV* v, int row,
 
 // The values' scales go into the weights, as multiples of the largest so far (a
 // power of two; what is summed is scaled along): so the weights fit a half.
-// Whether a scale raises that.
-__device__ __forceinline__ bool raises(float vs, float ref) { return vs > ref && vs <= 3.4028235e38f; }
-__device__ __forceinline__ float power_of(float vs) {
-  return __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, vs) & 0x7F800000u);
+// A scale's power of two as bits, which compare as integers; 0 for what is not finite.
+__device__ __forceinline__ uint32_t power_of(float vs) {
+  const uint32_t bits = __builtin_bit_cast(uint32_t, vs);
+  return bits < 0x7F800000u ? bits & 0x7F800000u : 0u;
 }
-__device__ __forceinline__ float inverse_of(float ref) { return ref > 0.f ? 1.f / ref : 0.f; }
+__device__ __forceinline__ float inverse_of(uint32_t power) {  // 2^127's is not normal
+  return __builtin_bit_cast(float, !power ? 0u : power == 0x7F000000u ? 0x00400000u : 0x7F000000u - power);
+}
 
 // The weights take such a multiple f as a summand log2 f of their exponents, and
 // the total its share back as 1 / f.  Where f is 0 the total's share is taken with
@@ -510,7 +490,7 @@ __device__ __forceinline__ Place place_of(const AttendPlan& p) {
 }
 
 // ---------------------------------------------------------------- many rows
-// 32 R rows a wavefront, four wavefronts a workgroup, steps of 32 keys.  A step's
+// 32 rows a wavefront, four wavefronts a workgroup, steps of 32 keys.  A step's
 // keys and values go through registers to LDS (unseen ones as zeros, codes as
 // 16-bit numbers), four steps each there.  Matrix instructions run beside the
 // others if they do not wait for one another, so three steps overlap: the scores
@@ -523,7 +503,6 @@ __device__ __forceinline__ Place place_of(const AttendPlan& p) {
 // first value).  Pages: rows that do not see a whole step are masked afterwards.
 template <typename T, int DP, bool PAGED>
 __global__ __launch_bounds__(256, tile_workgroups(DP)) void tile_kernel(AttendPlan p) {
-  constexpr int R = 1;
   typedef typename Matrix<T>::v8 v8;
   constexpr int KT = 32;
   constexpr int kPer = PAGED ? DP / 16 : DP / 8, kElems = PAGED ? 16 : 8;  // 16-byte pieces of a key, elements of one
@@ -537,43 +516,39 @@ __global__ __launch_bounds__(256, tile_workgroups(DP)) void tile_kernel(AttendPl
   const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(tid >> 6));
   const Place w = place_of(p);
   const Sequence seq = sequence_of<PAGED>(p, w.b);
-  constexpr uint32_t kRows = 128 * R;
-  // a lane's rows: 32 apart
-  const uint32_t row0 = w.block * kRows + wave * (32 * R) + (lane & 31u);
-  int32_t limit[R];
-  u4 q[R][DP / 16];
+  const uint32_t row = w.block * kBlockRows + wave * 32 + (lane & 31u), t = p.by_group.div(row), g = row - t * p.group;
+  const bool live = row < p.rows && (int32_t)t < seq.tokens;
+  const int32_t limit = live ? limit_of<PAGED>(seq, (int32_t)t) : 0x7FFFFFFF;
+  u4 q[DP / 16];  // as the B operand of its steps; zeros for no row
+  {
+    const T* x = static_cast<const T*>(p.q) + w.b * p.q_batch + t * p.q_token + (w.h * p.group + g) * p.q_head;
 #pragma unroll
-  for (int r = 0; r < R; ++r) {
-    const uint32_t row = row0 + r * 32, t = p.by_group.div(row), g = row - t * p.group;
-    const bool live = row < p.rows && (int32_t)t < seq.tokens;
-    limit[r] = live ? limit_of<PAGED>(seq, (int32_t)t) : 0x7FFFFFFF;
-    load_query<T, DP>(p, w.b, w.h, t, g, live, half, q[r]);
+    for (int i = 0; i < DP / 16; ++i) {
+      const uint32_t d = (i / 2) * 32 + half * 16 + (i % 2) * 8;
+      q[i] = u4{0, 0, 0, 0};
+      if (live && d < p.dim) q[i] = load16(x + d);
+    }
   }
   // the workgroup's first and last live rows
-  const int32_t t_first = (int32_t)p.by_group.div(w.block * kRows);
-  const int32_t t_last = min((int32_t)p.by_group.div(min(p.rows, (w.block + 1) * kRows) - 1), seq.tokens - 1);
+  const int32_t t_first = (int32_t)p.by_group.div(w.block * kBlockRows);
+  const int32_t t_last = min((int32_t)p.by_group.div(min(p.rows, (w.block + 1) * kBlockRows) - 1), seq.tokens - 1);
   const int32_t most = t_last < t_first ? 0 : limit_of<PAGED>(seq, t_last);
   const int32_t least = limit_of<PAGED>(seq, t_first);
-  int32_t wave_least = limit[0];  // this wavefront's
+  int32_t wave_least = limit;  // this wavefront's
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) wave_least = min(wave_least, __shfl_xor(wave_least, o, 64));
   wave_least = __builtin_amdgcn_readfirstlane(wave_least);
   const Range range = range_of(most, w.split, p.splits, 64);
   const int32_t steps = (range.end - range.begin + KT - 1) / KT;
 
-  f16v o[R][DP / 32];
-  float m[R], off[R], l[R];  // l: of this half's keys
+  f16v o[DP / 32];
+  float m = -__builtin_inff(), off = Matrix<T>::kShift, l = 0.f;  // l: of this half's keys
 #pragma unroll
-  for (int r = 0; r < R; ++r) {
-    m[r] = -__builtin_inff();
-    off[r] = Matrix<T>::kShift;
-    l[r] = 0.f;
+  for (int i = 0; i < DP / 32; ++i)
 #pragma unroll
-    for (int i = 0; i < DP / 32; ++i)
-#pragma unroll
-      for (int j = 0; j < 16; ++j) o[r][i][j] = 0.f;
-  }
-  float ref = PAGED ? 0.f : 1.f, inv_ref = ref;
+    for (int j = 0; j < 16; ++j) o[i][j] = 0.f;
+  uint32_t ref = 0;   // PAGED: the largest of the values' scales so far, a power of two's bits
+  float moved = 1.f;  // PAGED: the last one over that, where the sums still stand in it
   if constexpr (PAGED)
     for (uint32_t d = tid; d < (uint32_t)DP; d += 256) lowest[d] = 0x7FFFFFFF;
 
@@ -600,11 +575,12 @@ __global__ __launch_bounds__(256, tile_workgroups(DP)) void tile_kernel(AttendPl
                         (w.b * p.v.batch + w.h * p.v.head + (range.begin + (int32_t)wave * 8 - 2 * KT) * p.v.key) * (int64_t)sizeof(T);
   uint32_t bits_k = 0, bits_1 = 0, bits_v = 0;  // rows: the seen keys of steps s, s - 1 and s - 2
   uint32_t shown = 0;                           // rows: key lane % 32 of the next step
+  uint32_t any_shown = 0;                       // rows: of all so far
   // PAGED: lane i knows group i % 2 of 16 keys of step i / 2 of a window of 32
   // steps; the next window's are looked up when one begins.
   struct Window {
     int32_t id;
-    float ks, vs;
+    float c, vs;  // c: of the scores as the codes give them
   };
   const auto look_up_window = [&](int32_t first) {
     Window x{-1, 0.f, 0.f};
@@ -614,15 +590,39 @@ __global__ __launch_bounds__(256, tile_workgroups(DP)) void tile_kernel(AttendPl
       if ((uint32_t)x.id >= p.pages) {
         x.id = -1;
       } else {
-        x.ks = p.kp.scales[x.id * p.kp.scale_page + w.h * p.kp.scale_head];
+        x.c = p.c * p.kp.scales[x.id * p.kp.scale_page + w.h * p.kp.scale_head];
         x.vs = p.vp.scales[x.id * p.vp.scale_page + w.h * p.vp.scale_head];
       }
     }
     return x;
   };
   Window here{-1, 0.f, 0.f}, there{-1, 0.f, 0.f};
+  float here_share = 0.f, here_back = 0.f;
   int32_t here_first = 0;                  // the step that `here` begins with
+  // The values' scales go into the weights as multiples of the largest up to the
+  // window's end: of these, what the exponents and the totals take.
+  const auto enter_window = [&](int32_t first) {
+    here = there;
+    here_first = first;
+    uint32_t top = power_of(here.vs);
+#pragma unroll
+    for (int x = 1; x < 64; x <<= 1) top = max(top, (uint32_t)__shfl_xor((int)top, x, 64));
+    top = (uint32_t)__builtin_amdgcn_readfirstlane((int)top);
+    if (top > ref) {
+      moved = __builtin_bit_cast(float, ref) * inverse_of(top);
+      ref = top;
+    }
+    const float f = here.vs * inverse_of(ref);
+    here_share = __builtin_amdgcn_logf(share_of(f));
+    here_back = f == 0.f ? -1.f : __builtin_amdgcn_rcpf(f);
+  };
   int32_t id_k = -1, id_1 = -1, id_v = -1;  // the pages of the wavefront's keys of steps s, s - 1 and s - 2
+  // their places there; a step is two groups further, and pages are whole groups
+  uint32_t at_k = 0, at_1 = 0, at_v = 0;
+  if constexpr (PAGED) {
+    at_k = (uint32_t)range.begin + wave * 8;
+    at_k -= p.by_page.div(at_k) * p.page_size;
+  }
   const uint8_t* k_codes = p.kp.codes + w.h * p.kp.head;
   const uint8_t* v_codes = p.vp.codes + w.h * p.vp.head;
   const auto look_up = [&](int32_t step) {
@@ -633,17 +633,19 @@ __global__ __launch_bounds__(256, tile_workgroups(DP)) void tile_kernel(AttendPl
     }
   };
   const auto fetch = [&](int32_t stage) {
-    const int32_t k0 = range.begin + stage * KT + (int32_t)wave * 8, v0 = k0 - 2 * KT;
     if constexpr (PAGED) {
       id_v = id_1;
       id_1 = id_k;
       const int32_t at = stage - here_first;
       id_k = __builtin_amdgcn_readlane(at < 32 ? here.id : there.id, (at & 31) * 2 + (int32_t)(wave >> 1));
-      const auto rsrc_of = [&](const uint8_t* codes, const PagesOf& x, int32_t id, int32_t key) {
-        const uint32_t token = (uint32_t)key - p.by_page.div((uint32_t)key) * p.page_size;
+      const auto rsrc_of = [&](const uint8_t* codes, const PagesOf& x, int32_t id, uint32_t token) {
         return buffer_rsrc(scalar(codes + id * x.page + token * x.token), id >= 0 ? kNowhere : 0u);
       };
-      const auto kr = rsrc_of(k_codes, p.kp, id_k, k0), vr = rsrc_of(v_codes, p.vp, id_v, max(v0, 0));
+      const auto kr = rsrc_of(k_codes, p.kp, id_k, at_k), vr = rsrc_of(v_codes, p.vp, id_v, at_v);
+      at_v = at_1;
+      at_1 = at_k;
+      at_k += p.page_size == 16 ? 0 : 32;
+      if (at_k >= p.page_size) at_k -= p.page_size;
 #pragma unroll
       for (int i = 0; i < kMine; ++i) {
         rk[i] = __builtin_bit_cast(u4, __builtin_amdgcn_raw_buffer_load_b128(kr, k_off[i], 0, 0));
@@ -653,6 +655,7 @@ __global__ __launch_bounds__(256, tile_workgroups(DP)) void tile_kernel(AttendPl
       bits_v = bits_1;
       bits_1 = bits_k;
       bits_k = (uint32_t)__ballot(shown != 0);
+      any_shown |= bits_k;
       const uint32_t mine_k = (bits_k >> (wave * 8)) & 0xFFu, mine_v = (bits_v >> (wave * 8)) & 0xFFu;
       const auto kr = buffer_rsrc(k_at, kNowhere), vr = buffer_rsrc(v_at, kNowhere);
       k_at += k_move;
@@ -706,29 +709,23 @@ __global__ __launch_bounds__(256, tile_workgroups(DP)) void tile_kernel(AttendPl
   };
   constexpr int kProducts = DP / 16;  // of a step, for the scores as for the mix
   // Scores of a step begin at 0, or at -inf for what is not seen.
-  const auto first_scores = [&](int slot, bool all, const v8& kf, f16v (&s)[R]) __attribute__((always_inline)) {
+  const auto first_scores = [&](int slot, bool all, const v8& kf) __attribute__((always_inline)) {
     f16v x;
 #pragma unroll
     for (int j = 0; j < 16; ++j) x[j] = 0.f;
-    if (!PAGED && !all) {
+    if (PAGED || all) return Matrix<T>::mul(kf, __builtin_bit_cast(v8, q[0]), x);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const f4 y = *reinterpret_cast<const f4*>(lds_bias[slot] + j * 8 + half * 4);
+    for (int j = 0; j < 4; ++j) {
+      const f4 y = *reinterpret_cast<const f4*>(lds_bias[slot] + j * 8 + half * 4);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) x[j * 4 + e] = y[e];
-      }
-#pragma unroll
-      for (int r = 0; r < R; ++r) s[r] = Matrix<T>::mul(kf, __builtin_bit_cast(v8, q[r][0]), x);
-    } else {
-#pragma unroll
-      for (int r = 0; r < R; ++r) s[r] = Matrix<T>::mul(kf, __builtin_bit_cast(v8, q[r][0]), x);
+      for (int e = 0; e < 4; ++e) x[j * 4 + e] = y[e];
     }
+    return Matrix<T>::mul(kf, __builtin_bit_cast(v8, q[0]), x);
   };
 
   // Step j: s holds its scores, `next` gets the next one's; before: the weights of
   // step j - 1, which are mixed, pr: its own.
-  const auto advance = [&](int32_t j, f16v (&s)[R], f16v (&next)[R], const v8 (&before)[R][2],
-                           v8 (&pr)[R][2]) __attribute__((always_inline)) {
+  const auto advance = [&](int32_t j, f16v& s, f16v& next, const v8 (&before)[2], v8 (&pr)[2]) __attribute__((always_inline)) {
     const int32_t k0 = range.begin + j * KT;
     if (!(j & 1)) __syncthreads();
     constexpr int kAhead = kProducts < 4 ? kProducts : 4;
@@ -741,154 +738,119 @@ __global__ __launch_bounds__(256, tile_workgroups(DP)) void tile_kernel(AttendPl
     const bool all = bits_v == ~0u;  // of step j + 1
     store(j + 3);
     fetch(j + 4);
-    bool raised = false;
-    float ks[2], vs[2], share[2], a[R];  // a: what the sums so far are multiplied by, once step j - 1 is in
-#pragma unroll
-    for (int r = 0; r < R; ++r) a[r] = 1.f;
-    bool there_is[2];
+    float a = moved;  // what the sums so far are multiplied by, once step j - 1 is in
+    bool raised = PAGED && moved != 1.f;
+    moved = 1.f;
+    float c[2] = {p.c, p.c}, share[2] = {0.f, 0.f}, back[2] = {1.f, 1.f};
+    bool there_is[2] = {true, true}, unseen[2] = {false, false};
     if constexpr (PAGED) {
 #pragma unroll
       for (int n = 0; n < 2; ++n) {
         const int32_t at = (j - here_first) * 2 + n;
         there_is[n] = __builtin_amdgcn_readlane(here.id, at) >= 0;
-        ks[n] = lane_value(here.ks, at);
-        vs[n] = lane_value(here.vs, at);
-      }
-      if (raises(vs[0], ref) || raises(vs[1], ref)) {
-        const float top = power_of(fmaxf(raises(vs[0], ref) ? vs[0] : ref, raises(vs[1], ref) ? vs[1] : ref));
-#pragma unroll
-        for (int r = 0; r < R; ++r) a[r] = ref * inverse_of(top);
-        raised = true;
-        ref = top;
-        inv_ref = inverse_of(ref);
-      }
-#pragma unroll
-      for (int n = 0; n < 2; ++n) {
-        vs[n] *= inv_ref;
-        share[n] = __builtin_amdgcn_logf(share_of(vs[n]));
+        c[n] = lane_value(here.c, at);
+        share[n] = lane_value(here_share, at);
+        back[n] = lane_value(here_back, at);
       }
     }
-    float c[R][2], add[R][2], back[R][2], sum[R][2], top[R][2];
+    const bool zero[2] = {back[0] < 0.f, back[1] < 0.f};  // a value's scale of 0
+    float add[2], sum[2] = {0.f, 0.f}, top[2] = {-__builtin_inff(), -__builtin_inff()};
 #pragma unroll
-    for (int r = 0; r < R; ++r)
-#pragma unroll
-      for (int n = 0; n < 2; ++n) {
-        c[r][n] = PAGED ? p.c * ks[n] : p.c;
-        add[r][n] = PAGED ? off[r] + share[n] : off[r];
-        back[r][n] = PAGED ? __builtin_amdgcn_rcpf(share_of(vs[n])) : 1.f;
-        sum[r][n] = 0.f;
-        top[r][n] = -__builtin_inff();
-      }
+    for (int n = 0; n < 2; ++n) {
+      add[n] = PAGED ? off + share[n] : off;
+      if (PAGED) back[n] = __builtin_fabsf(back[n]);
+    }
     if constexpr (PAGED)
       if (!(there_is[0] && there_is[1] && k0 + KT <= wave_least)) {
+        const int32_t left = limit - k0 - (int32_t)half * 4;
 #pragma unroll
-        for (int r = 0; r < R; ++r) {
-          const int32_t left = limit[r] - k0 - (int32_t)half * 4;
+        for (int i = 0; i < 16; ++i)
+          if (!there_is[i / 8] || i / 4 * 8 + i % 4 >= left) s[i] = -__builtin_inff();
 #pragma unroll
-          for (int i = 0; i < 16; ++i)
-            if (!there_is[i / 8] || i / 4 * 8 + i % 4 >= left) s[r][i] = -__builtin_inff();
-#pragma unroll
-          for (int n = 0; n < 2; ++n)
-            if (!there_is[n] || limit[r] <= k0 + n * 16) {  // nothing of scales that the row does not see
-              c[r][n] = 1.f;
-              add[r][n] = back[r][n] = 0.f;
-            }
+        for (int n = 0; n < 2; ++n) {
+          unseen[n] = !there_is[n] || limit <= k0 + n * 16;
+          if (unseen[n]) {  // nothing of scales that the row does not see
+            c[n] = 1.f;
+            add[n] = back[n] = 0.f;
+          }
+          c[n] = fmaxf(c[n], kLeastFactor);
         }
       }
-    const auto weigh = [&](int r, int x) __attribute__((always_inline)) {  // elements x and x + 1 of row tile r
+    const auto weigh = [&](int x) __attribute__((always_inline)) {  // elements x and x + 1
       float e[2];
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        e[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r][x + i], c[r][x / 8], add[r][x / 8]));
-        sum[r][x / 8] += e[i];
+        e[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[x + i], c[x / 8], add[x / 8]));
+        sum[x / 8] += e[i];
       }
       typename Matrix<T>::v2 both;
       both[0] = (T)e[0];
       both[1] = (T)e[1];
       uint32_t w = __builtin_bit_cast(uint32_t, both);
-      asm volatile("" : "+v"(w), "+v"(sum[r][x / 8]));  // here, and not where they are used
+      asm volatile("" : "+v"(w), "+v"(sum[x / 8]));  // here, and not where they are used
       both = __builtin_bit_cast(typename Matrix<T>::v2, w);
-      pr[r][x / 8][x % 8] = both[0];
-      pr[r][x / 8][x % 8 + 1] = both[1];
+      pr[x / 8][x % 8] = both[0];
+      pr[x / 8][x % 8 + 1] = both[1];
     };
     // (After the last step, scores of what LDS holds, which nobody takes; before the
     // first, weights and values of 0.)
-    first_scores(k_slot, all, kf[0], next);
+    next = first_scores(k_slot, all, kf[0]);
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int i = 0; i < kProducts; ++i) {
+      if (i) next = Matrix<T>::mul(kf[i % kAhead], __builtin_bit_cast(v8, q[i]), next);
+      o[i % (DP / 32)] = Matrix<T>::mul(vf[i % 2], before[i / (DP / 32)], o[i % (DP / 32)]);
+      if (i + kAhead < kProducts) kf[i % kAhead] = key_piece(k_slot, i + kAhead);
+      if (i + 2 < kProducts) vf[i % 2] = value_piece(v_slot, i + 2);
 #pragma unroll
-      for (int r = 0; r < R; ++r) {
-        if (i) next[r] = Matrix<T>::mul(kf[i % kAhead], __builtin_bit_cast(v8, q[r][i]), next[r]);
-        o[r][i % (DP / 32)] = Matrix<T>::mul(vf[i % 2], before[r][i / (DP / 32)], o[r][i % (DP / 32)]);
-        if (r == R - 1) {
-          if (i + kAhead < kProducts) kf[i % kAhead] = key_piece(k_slot, i + kAhead);
-          if (i + 2 < kProducts) vf[i % 2] = value_piece(v_slot, i + 2);
-        }
-#pragma unroll
-        for (int x = i * 8 / kProducts * 2; x < (i + 1) * 8 / kProducts * 2; x += 2) {
-          weigh(r, x);
-          top[r][x / 8] = fmaxf(fmaxf(top[r][x / 8], s[r][x]), s[r][x + 1]);
-        }
-        __builtin_amdgcn_sched_barrier(0);
+      for (int x = i * 8 / kProducts * 2; x < (i + 1) * 8 / kProducts * 2; x += 2) {
+        weigh(x);
+        top[x / 8] = fmaxf(fmaxf(top[x / 8], s[x]), s[x + 1]);
       }
+      __builtin_amdgcn_sched_barrier(0);
     }
-    bool more = false;
-    float most_of[R];
+    // (a NaN of unseen keys' scales is dropped)
+    const float highest = PAGED ? fmaxf(fmaxf(-__builtin_inff(), top[0] * c[0]), top[1] * c[1]) : fmaxf(top[0], top[1]) * p.c;
+    if (__any(highest - m > kSlack)) {  // (either half's lanes)
+      const float to = fmaxf(m, fmaxf(highest, lane_xor<32>(highest))), f = rescale_of(m, to);
+      l *= f;
+      a *= f;
+      m = to;
+      off = offset_of(to) + Matrix<T>::kShift;
 #pragma unroll
-    for (int r = 0; r < R; ++r) {
-      // (a NaN of unseen keys' scales is dropped)
-      most_of[r] = PAGED ? fmaxf(fmaxf(-__builtin_inff(), top[r][0] * ks[0]), top[r][1] * ks[1]) : fmaxf(top[r][0], top[r][1]);
-      more |= (most_of[r] - m[r]) * p.c > kSlack;
-    }
-    if (__any(more)) {  // (either half's lanes)
-#pragma unroll
-      for (int r = 0; r < R; ++r) {
-        const float to = fmaxf(m[r], fmaxf(most_of[r], lane_xor<32>(most_of[r]))), f = rescale_of(m[r], to, p.c);
-        l[r] *= f;
-        a[r] *= f;
-        m[r] = to;
-        off[r] = offset_of(to, p.c, 0.f) + Matrix<T>::kShift;
-#pragma unroll
-        for (int n = 0; n < 2; ++n) {
-          add[r][n] = !PAGED ? off[r] : back[r][n] == 0.f ? 0.f : off[r] + share[n];
-          sum[r][n] = 0.f;
-        }
-#pragma unroll
-        for (int x = 0; x < 16; x += 2) weigh(r, x);
+      for (int n = 0; n < 2; ++n) {
+        add[n] = !PAGED ? off : unseen[n] ? 0.f : off + share[n];
+        sum[n] = 0.f;
       }
+#pragma unroll
+      for (int x = 0; x < 16; x += 2) weigh(x);
       raised = true;
     }
     if (raised) {
 #pragma unroll
-      for (int r = 0; r < R; ++r)
+      for (int i = 0; i < DP / 32; ++i)
 #pragma unroll
-        for (int i = 0; i < DP / 32; ++i)
-#pragma unroll
-          for (int e = 0; e < 16; ++e) o[r][i][e] *= a[r];
+        for (int e = 0; e < 16; ++e) o[i][e] *= a;
     }
 #pragma unroll
-    for (int r = 0; r < R; ++r)
+    for (int n = 0; n < 2; ++n) {
+      l += PAGED ? sum[n] * back[n] : sum[n];
+      if (PAGED && zero[n]) {
 #pragma unroll
-      for (int n = 0; n < 2; ++n) {
-        l[r] += PAGED ? sum[r][n] * back[r][n] : sum[r][n];
-        if (PAGED && vs[n] == 0.f) {
-#pragma unroll
-          for (int i = 0; i < 8; ++i) pr[r][n][i] = (T)0.f;
-        }
+        for (int i = 0; i < 8; ++i) pr[n][i] = (T)0.f;
       }
+    }
   };
 
-  f16v s[2][R];
-  v8 pr[2][R][2];
+  f16v s[2];
+  v8 pr[2][2];
 #pragma unroll
-  for (int r = 0; r < R; ++r)
-#pragma unroll
-    for (int i = 0; i < 8; ++i) pr[1][r][0][i] = pr[1][r][1][i] = (T)0.f;
+  for (int i = 0; i < 8; ++i) pr[1][0][i] = pr[1][1][i] = (T)0.f;
   if (steps > 0) {
     look_up(0);
     if constexpr (PAGED) {
-      here = look_up_window(0);
+      there = look_up_window(0);
+      enter_window(0);
       there = look_up_window(32);
     }
     fetch(0);
@@ -900,51 +862,47 @@ __global__ __launch_bounds__(256, tile_workgroups(DP)) void tile_kernel(AttendPl
     store(2);
     fetch(3);
     __syncthreads();
-    first_scores(0, all, key_piece(0, 0), s[0]);
+    s[0] = first_scores(0, all, key_piece(0, 0));
 #pragma unroll
-    for (int i = 1; i < kProducts; ++i)
-#pragma unroll
-      for (int r = 0; r < R; ++r) s[0][r] = Matrix<T>::mul(key_piece(0, i), __builtin_bit_cast(v8, q[r][i]), s[0][r]);
+    for (int i = 1; i < kProducts; ++i) s[0] = Matrix<T>::mul(key_piece(0, i), __builtin_bit_cast(v8, q[i]), s[0]);
     for (int32_t j = 0; j < steps; j += 2) {
       if (PAGED && j == here_first + 32) {
-        here = there;
-        here_first = j;
+        enter_window(j);
         there = look_up_window(j + 32);
       }
       advance(j, s[0], s[1], pr[1], pr[0]);
       if (j + 1 < steps) advance(j + 1, s[1], s[0], pr[0], pr[1]);
     }
     __syncthreads();
-    const auto finish = [&](const v8 (&last)[R][2]) __attribute__((always_inline)) {
+    const auto finish = [&](const v8 (&last)[2]) __attribute__((always_inline)) {
 #pragma unroll
-      for (int i = 0; i < kProducts; ++i) {
-        const v8 v = value_piece((steps - 1) & 3, i);
-#pragma unroll
-        for (int r = 0; r < R; ++r) o[r][i % (DP / 32)] = Matrix<T>::mul(v, last[r][i / (DP / 32)], o[r][i % (DP / 32)]);
-      }
+      for (int i = 0; i < kProducts; ++i)
+        o[i % (DP / 32)] = Matrix<T>::mul(value_piece((steps - 1) & 3, i), last[i / (DP / 32)], o[i % (DP / 32)]);
     };
     if (steps & 1) finish(pr[0]);
     else finish(pr[1]);
   }
-  if constexpr (PAGED) __syncthreads();
+  if constexpr (PAGED) {
+    __syncthreads();
 #pragma unroll
-  for (int r = 0; r < R; ++r) {
-    if constexpr (PAGED) {
+    for (int i = 0; i < DP / 32; ++i)
 #pragma unroll
-      for (int i = 0; i < DP / 32; ++i)
+      for (int j = 0; j < 16; ++j) {
+        o[i][j] *= __builtin_bit_cast(float, ref);
+        if (limit > lowest[i * 32 + j / 4 * 8 + half * 4 + j % 4]) o[i][j] = __builtin_nanf("");
+      }
+  } else if (!any_shown) {  // nothing seen, and nothing of queries that are not finite
+    m = -__builtin_inff();
+    l = 0.f;
 #pragma unroll
-        for (int j = 0; j < 16; ++j) {
-          o[r][i][j] *= ref;
-          if (limit[r] > lowest[i * 32 + j / 4 * 8 + half * 4 + j % 4]) o[r][i][j] = __builtin_nanf("");
-        }
-    }
-    l[r] += lane_xor<32>(l[r]);
-    const uint32_t row = row0 + r * 32, t = p.by_group.div(row), g = row - t * p.group;
-    if (row < p.rows && (p.splits == 1 || steps > 0)) {
-      const uint64_t unit = ((uint64_t)w.b * p.heads + w.h) * p.row_blocks + w.block;
-      store_row<T, DP>(p, w.b, w.h, t, g, (unit * p.splits + w.split) * kRows + (row - w.block * kRows), half,
-                       (int32_t)t < seq.tokens, o[r], m[r], l[r]);
-    }
+    for (int i = 0; i < DP / 32; ++i)
+#pragma unroll
+      for (int j = 0; j < 16; ++j) o[i][j] = 0.f;
+  }
+  l += lane_xor<32>(l);
+  if (row < p.rows && (p.splits == 1 || steps > 0)) {
+    const uint64_t unit = ((uint64_t)w.b * p.heads + w.h) * p.row_blocks + w.block;
+    store_row<T, DP>(p, w.b, w.h, t, g, (unit * p.splits + w.split) * kBlockRows + (row - w.block * kBlockRows), half, live, o, m, l);
   }
 }
 
@@ -1026,7 +984,7 @@ __global__ __launch_bounds__(256, few_workgroups(DP, 16 * R, PAGED)) void few_ke
 #pragma unroll
     for (int i = 0; i < DP / 16; ++i) o[r][i] = f4{0.f, 0.f, 0.f, 0.f};
   }
-  float ref = PAGED ? 0.f : 1.f, inv_ref = ref;
+  uint32_t ref = PAGED ? 0u : 0x3F800000u;  // the largest of the values' scales so far, a power of two's bits
   if constexpr (PAGED) {
     for (uint32_t d = tid; d < (uint32_t)DP; d += 256) lowest[d] = 0x7FFFFFFF;
     __syncthreads();
@@ -1184,20 +1142,23 @@ __global__ __launch_bounds__(256, few_workgroups(DP, 16 * R, PAGED)) void few_ke
       fetch(k0 + W * KT, ahead);
     }
     if constexpr (PAGED) {
-      if (raises(vs0, ref) || raises(vs1, ref)) {
-        const float top = power_of(fmaxf(raises(vs0, ref) ? vs0 : ref, raises(vs1, ref) ? vs1 : ref)), a = ref * inverse_of(top);
+      const uint32_t top = max(power_of(vs0), power_of(vs1));
+      if (top > ref) {
+        const float a = __builtin_bit_cast(float, ref) * inverse_of(top);
 #pragma unroll
         for (int r = 0; r < R; ++r)
 #pragma unroll
           for (int i = 0; i < DP / 16; ++i) o[r][i] *= a;
         ref = top;
-        inv_ref = inverse_of(ref);
       }
     }
     // exponentials
     float c[2] = {p.c, p.c}, add[2] = {0.f, 0.f}, back[2] = {1.f, 1.f};
+    bool zero[2] = {false, false};  // a value's scale of 0
     if constexpr (PAGED) {
-      const float f0 = share_of(vs0 * inv_ref), f1 = share_of(vs1 * inv_ref);
+      const float f0 = share_of(vs0 * inverse_of(ref)), f1 = share_of(vs1 * inverse_of(ref));
+      zero[0] = vs0 * inverse_of(ref) == 0.f;
+      zero[1] = vs1 * inverse_of(ref) == 0.f;
       c[0] = p.c * ks0;
       c[1] = p.c * ks1;
       add[0] = __builtin_amdgcn_logf(f0);
@@ -1222,24 +1183,26 @@ __global__ __launch_bounds__(256, few_workgroups(DP, 16 * R, PAGED)) void few_ke
               rc[n] = 1.f;
               radd[n] = rback[n] = 0.f;
             }
+#pragma unroll
+          for (int n = 0; n < 2; ++n) rc[n] = fmaxf(rc[n], kLeastFactor);
         }
       }
       float top = -__builtin_inff();
 #pragma unroll
       for (int n = 0; n < 2; ++n) {
         const float x = fmaxf(fmaxf(s[r][n][0], s[r][n][1]), fmaxf(s[r][n][2], s[r][n][3]));
-        top = fmaxf(top, PAGED ? x * (n ? ks1 : ks0) : x);  // a NaN of unseen keys' scales is dropped
+        top = fmaxf(top, x * rc[n]);  // a NaN is dropped: weights are NaN by themselves
       }
       top = fmaxf(top, lane_xor<16>(top));
       top = fmaxf(top, lane_xor<32>(top));
-      if (__any((top - m[r]) * p.c > kSlack || (m[r] == -__builtin_inff() && top > m[r]))) {
-        const float to = fmaxf(m[r], top), a = rescale_of(m[r], to, p.c);
+      if (__any(top - m[r] > kSlack || (m[r] == -__builtin_inff() && top > m[r]))) {
+        const float to = fmaxf(m[r], top), a = rescale_of(m[r], to);
         l[r] *= a;
 #pragma unroll
         for (int i = 0; i < DP / 16; ++i) o[r][i] *= a;
         m[r] = to;
       }
-      const float off = offset_of(m[r], p.c, 0.f) + Matrix<T>::kShift;
+      const float off = offset_of(m[r]) + Matrix<T>::kShift;
 #pragma unroll
       for (int n = 0; n < 2; ++n) {
         float sum = 0.f;
@@ -1250,7 +1213,7 @@ __global__ __launch_bounds__(256, few_workgroups(DP, 16 * R, PAGED)) void few_ke
           pr[r][n * 4 + j] = (T)e;
         }
         l[r] += PAGED ? sum * rback[n] : sum;
-        if (PAGED && (n ? vs1 : vs0) * inv_ref == 0.f) {
+        if (PAGED && zero[n]) {
 #pragma unroll
           for (int j = 0; j < 4; ++j) pr[r][n * 4 + j] = (T)0.f;
         }
@@ -1290,8 +1253,8 @@ __global__ __launch_bounds__(256, few_workgroups(DP, 16 * R, PAGED)) void few_ke
 #pragma unroll
     for (int i = 1; i < W; ++i) top = fmaxf(top, lds_m[i][row]);
 #pragma unroll
-    for (int i = 0; i < W; ++i) sum += lds_l[i][row] * rescale_of(lds_m[i][row], top, p.c);
-    a[r] = rescale_of(m[r], top, p.c) * ref;
+    for (int i = 0; i < W; ++i) sum += lds_l[i][row] * rescale_of(lds_m[i][row], top);
+    a[r] = rescale_of(m[r], top) * __builtin_bit_cast(float, ref);
     if (wave == 0 && quarter == 0) {
       row_m[row] = top;
       row_l[row] = sum;
@@ -1387,7 +1350,7 @@ __global__ __launch_bounds__(256) void join_kernel(AttendPlan p) {
   m = group_max<G>(m);
   for (int32_t i = (int32_t)lane; i < n; i += G) {
     const float* stats = p.stats + (first + (uint64_t)i * step) * 2;
-    l += stats[1] * rescale_of(stats[0], m, p.c);
+    l += stats[1] * rescale_of(stats[0], m);
   }
   l = group_sum<G>(l);
   const uint32_t quads = p.dim / 4, sides = E / quads, side = mine / quads, d = (mine - side * quads) * 4;
@@ -1398,7 +1361,7 @@ __global__ __launch_bounds__(256) void join_kernel(AttendPlan p) {
       const uint64_t slot = first + (uint64_t)i * step;
       float x[4];
       load_pack<float, 4>(p.sums + slot * p.dim + d, x);
-      const float f = rescale_of(p.stats[slot * 2], m, p.c);
+      const float f = rescale_of(p.stats[slot * 2], m);
 #pragma unroll
       for (int k = 0; k < 4; ++k) v[k] += x[k] * f;
     }

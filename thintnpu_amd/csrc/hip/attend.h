@@ -539,7 +539,7 @@ __global__ __launch_bounds__(256, tile_workgroups(DP)) void tile_kernel(AttendPl
   for (int o = 1; o < 32; o <<= 1) wave_least = min(wave_least, __shfl_xor(wave_least, o, 64));
   wave_least = __builtin_amdgcn_readfirstlane(wave_least);
   const Range range = range_of(most, w.split, p.splits, 64);
-  const int32_t steps = (range.end - range.begin + KT - 1) / KT;
+  int32_t steps = (range.end - range.begin + KT - 1) / KT;
 
   f16v o[DP / 32];
   float m = -__builtin_inff(), off = Matrix<T>::kShift, l = 0.f;  // l: of this half's keys
@@ -862,6 +862,18 @@ __global__ __launch_bounds__(256, tile_workgroups(DP)) void tile_kernel(AttendPl
     store(2);
     fetch(3);
     __syncthreads();
+    if (!__any(live)) {  // a wavefront without rows stages what the others take
+      for (int32_t j = 0; j < steps; ++j) {
+        if (!(j & 1)) __syncthreads();
+        if (PAGED && j == here_first + 32) {
+          enter_window(j);
+          there = look_up_window(j + 32);
+        }
+        store(j + 3);
+        fetch(j + 4);
+      }
+      steps = 0;
+    }
     s[0] = first_scores(0, all, key_piece(0, 0));
 #pragma unroll
     for (int i = 1; i < kProducts; ++i) s[0] = Matrix<T>::mul(key_piece(0, i), __builtin_bit_cast(v8, q[i]), s[0]);

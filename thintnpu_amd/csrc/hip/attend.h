@@ -68,8 +68,13 @@ struct AttendPlan {
   float* stats;
 };
 
-constexpr int kFewRows = 32;    // one or two matrix tiles of 16: keys are split over the wavefronts
-constexpr int kBlockRows = 128;  // rows of a workgroup otherwise: 32 a wavefront
+constexpr int kBlockRows = 128;  // rows of a workgroup of the kernel for many: 32 a wavefront
+
+// Rows that the kernel for few takes.  Of a tensor, up to one matrix tile of 16: 24
+// rows of 16 heads to 2 x 20000 states of 128 dims took 48 us in two tiles, 42 as
+// many rows.  Of the cache, up to two: 24 rows of 16 x 8 heads to 4096 tokens took
+// 35 us in two, 43 as many.
+constexpr int few_rows(bool paged) { return paged ? 32 : 16; }
 
 // Head widths that kernels exist for.
 inline int padded_dim(int64_t d) {
@@ -86,13 +91,13 @@ constexpr int few_workgroups(int DP, int rows, bool paged) {
 constexpr int tile_workgroups(int DP) { return DP <= 32 ? 4 : DP <= 64 ? 3 : DP <= 128 ? 2 : 1; }
 
 constexpr int64_t kCus = 256;
-constexpr int64_t kSplitKeys = 256;  // keys of a split at least: fewer cost more to join than they give
+constexpr int64_t kSplitKeys = 256;  // keys of a split or chunk at least (128 and 512 measured alike)
 constexpr int64_t kMaxSplits = 128;
-constexpr uint32_t kJoinByWave = 8;  // splits that one wavefront or less joins; more take a workgroup
 
 // Many rows: splits of every row's keys.  In rounds of the workgroups that the card
 // holds, each as long as its keys and some 160 more, which beginning and end cost,
-// and the join as much as 200.
+// and the join as much as 200.  (1024 rows of 3 x 4 heads over 8000 cached tokens:
+// 4 splits, 143 us; 2 take 152, 3 take 162.)
 inline int64_t splits_of(int64_t units, int64_t keys, int64_t dim) {
   const int64_t most = (keys + kSplitKeys - 1) / kSplitKeys < kMaxSplits ? (keys + kSplitKeys - 1) / kSplitKeys : kMaxSplits;
   const int64_t at_a_time = kCus * tile_workgroups(padded_dim(dim));
@@ -110,20 +115,26 @@ inline int64_t splits_of(int64_t units, int64_t keys, int64_t dim) {
 
 // Few rows: they are bound by memory and their sequences differ in length, so all
 // keys of all sequences are dealt out in equal chunks, to as many workgroups as
-// this: the card once or more, at least four to a head of a sequence.  0: one
-// workgroup to each, without a join.
+// this: the card once or more, at least two to a head of a sequence (32 x 8 heads
+// over 8192 cached tokens at most: 87 us, 156 by a workgroup each).  0: one
+// workgroup to each, without a join, where that fills the card and the longest
+// does not run on for long (32 x 16 heads to 1500 states: 45 us, 51 dealt out; 32
+// x 8 over 2000 cached tokens 40, 30 dealt out: codes are fewer bytes), or where
+// the join costs more than it gives (512 states: 10 us, 14 dealt out).
 inline int64_t chunks_for(int64_t units, int64_t rows, int64_t keys, int64_t dim, bool paged) {
   const int64_t at_a_time = kCus * few_workgroups(padded_dim(dim), (int)rows, paged);
   // (sums of keys are taken in 32 bits, in units of 128)
-  if (keys <= kSplitKeys || units >= 4 * at_a_time || units * (keys / 128 + 1) >= 1ll << 31) return 0;
-  const int64_t n = (4 * units + at_a_time - 1) / at_a_time * at_a_time, useful = units * ((keys + kSplitKeys - 1) / kSplitKeys + 1);
+  if (keys <= 512 || (keys <= 2048 && units >= kCus * (paged ? 2 : 1)) || units >= 4 * at_a_time ||
+      units * (keys / 128 + 1) >= 1ll << 31)
+    return 0;
+  const int64_t n = (2 * units + at_a_time - 1) / at_a_time * at_a_time, useful = units * ((keys + kSplitKeys - 1) / kSplitKeys + 1);
   return n < useful ? n : useful;
 }
-inline int64_t row_blocks_of(int64_t rows) { return rows <= kFewRows ? 1 : (rows + kBlockRows - 1) / kBlockRows; }
+inline int64_t row_blocks_of(int64_t rows, bool paged) { return rows <= few_rows(paged) ? 1 : (rows + kBlockRows - 1) / kBlockRows; }
 inline size_t attend_workspace(int64_t batch, int64_t heads, int64_t rows, int64_t keys, int64_t dim, bool paged) {
   if (batch <= 0 || heads <= 0 || rows <= 0 || keys <= 0 || !padded_dim(dim)) return 0;
-  const int64_t units = batch * heads * row_blocks_of(rows);
-  if (rows <= kFewRows) return (size_t)(chunks_for(units, rows, keys, dim, paged) * rows * (dim + 2) * 4);
+  const int64_t units = batch * heads * row_blocks_of(rows, paged);
+  if (rows <= few_rows(paged)) return (size_t)(chunks_for(units, rows, keys, dim, paged) * rows * (dim + 2) * 4);
   const int64_t splits = splits_of(units, keys, dim);
   return splits == 1 ? 0 : (size_t)(units * splits * kBlockRows * (dim + 2) * 4);
 }
@@ -144,8 +155,8 @@ inline void plan_attend(AttendPlan& p, const thin_desc* q, const thin_desc* out,
   p.dim = (uint32_t)q->sizes[3];
   p.keys = (uint32_t)keys;
   p.c = c;
-  const int64_t blocks = row_blocks_of(p.rows), units = (int64_t)p.batch * heads * blocks;
-  const bool few = p.rows <= kFewRows;
+  const int64_t blocks = row_blocks_of(p.rows, paged), units = (int64_t)p.batch * heads * blocks;
+  const bool few = p.rows <= few_rows(paged);
   const int64_t chunks = few ? chunks_for(units, p.rows, keys, p.dim, paged) : 0, splits = few ? 1 : splits_of(units, keys, p.dim);
   p.block_rows = few ? p.rows : kBlockRows;
   p.row_blocks = (uint32_t)blocks;
@@ -1396,20 +1407,26 @@ __global__ __launch_bounds__(256) void join_kernel(AttendPlan p) {
 // Launches a plan whose operands are checked.
 template <typename T, int DP, bool PAGED>
 thin_status launch_attend_dim(const AttendPlan& p, hipStream_t stream) {
-  const uint32_t units = p.batch * p.heads * p.row_blocks;
-  if (p.rows <= 16) hipLaunchKernelGGL((dev::few_kernel<T, DP, PAGED, 1>), dim3(p.chunks ? p.chunks : units), dim3(256), 0, stream, p);
-  else if (p.rows <= kFewRows) hipLaunchKernelGGL((dev::few_kernel<T, DP, PAGED, 2>), dim3(p.chunks ? p.chunks : units), dim3(256), 0, stream, p);
-  else hipLaunchKernelGGL((dev::tile_kernel<T, DP, PAGED>), dim3(units * p.splits), dim3(256), 0, stream, p);
-  THIN_LAUNCH_CHECK("attend");
-  const int64_t parts = p.rows <= kFewRows ? p.chunks / (p.batch * p.heads) : p.splits;  // of a row, on the average
-  if (p.chunks || p.splits > 1) {
-    const uint32_t rows = p.batch * p.heads * p.rows;
-    if (parts <= kJoinByWave && p.dim <= 64 && !p.chunks)
-      hipLaunchKernelGGL((dev::join_kernel<T, PAGED, 16>), dim3((rows + 15) / 16), dim3(256), 0, stream, p);
-    else if (parts <= kJoinByWave) hipLaunchKernelGGL((dev::join_kernel<T, PAGED, 64>), dim3((rows + 3) / 4), dim3(256), 0, stream, p);
-    else hipLaunchKernelGGL((dev::join_kernel<T, PAGED, 256>), dim3(rows), dim3(256), 0, stream, p);
-    THIN_LAUNCH_CHECK("attend_join");
+  const uint32_t units = p.batch * p.heads * p.row_blocks, rows = p.batch * p.heads * p.rows;
+  const bool few = p.rows <= few_rows(PAGED);
+  if (few && p.rows <= 16) {
+    hipLaunchKernelGGL((dev::few_kernel<T, DP, PAGED, 1>), dim3(p.chunks ? p.chunks : units), dim3(256), 0, stream, p);
+  } else if (few) {
+    if constexpr (PAGED)
+      hipLaunchKernelGGL((dev::few_kernel<T, DP, PAGED, 2>), dim3(p.chunks ? p.chunks : units), dim3(256), 0, stream, p);
+  } else {
+    hipLaunchKernelGGL((dev::tile_kernel<T, DP, PAGED>), dim3(units * p.splits), dim3(256), 0, stream, p);
   }
+  THIN_LAUNCH_CHECK("attend");
+  if (!p.chunks && p.splits == 1) return THIN_OK;
+  // by the parts of a row, on the average
+  if ((few ? p.chunks / units : p.splits) > 8)
+    hipLaunchKernelGGL((dev::join_kernel<T, PAGED, 256>), dim3(rows), dim3(256), 0, stream, p);
+  else if (DP <= 64 && !few)
+    hipLaunchKernelGGL((dev::join_kernel<T, PAGED, 16>), dim3((rows + 15) / 16), dim3(256), 0, stream, p);
+  else
+    hipLaunchKernelGGL((dev::join_kernel<T, PAGED, 64>), dim3((rows + 3) / 4), dim3(256), 0, stream, p);
+  THIN_LAUNCH_CHECK("attend_join");
   return THIN_OK;
 }
 template <typename T, bool PAGED>

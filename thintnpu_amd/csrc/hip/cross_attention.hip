@@ -46,7 +46,7 @@ extern "C" thin_status thin_cross_attention(const thin_desc* q, const thin_desc*
   const float c = scale * 1.4426950408889634f;
   THIN_REQUIRE(isnormal(c) && c > 0.f, THIN_ERR_INVALID, "cross_attention: the scale must be positive and finite");
   if (numel(q) == 0) return THIN_OK;
-  const int64_t rows = T * (H / Hk), blocks = row_blocks_of(rows);
+  const int64_t rows = T * (H / Hk), blocks = row_blocks_of(rows, false);
   THIN_REQUIRE(rows < (1ll << 30) && S < (1ll << 30) && B < (1ll << 30) && launchable(B * Hk * blocks, 256) &&
                    launchable(B * Hk * rows, 256),
                THIN_ERR_UNSUPPORTED, "cross_attention: tensor too large");

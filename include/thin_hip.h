@@ -492,14 +492,16 @@ size_t thin_cross_attention_workspace(const thin_desc* q, const thin_desc* k);
 /* out[b, t, h] = sum_j p_j v[b, j, h'] with p = softmax over j of
  * scale * q[b, t, h] . k[b, j, h'], h' = h / (H / Hk): q and out [B, T, H, D], k
  * and v [B, S, Hk, D], fp16 or bf16 of one type, a head's dims adjacent, D a
- * multiple of 8 from 8 to 256, other strides free; scale positive.
+ * multiple of 8 from 8 to 256, other strides free (neighbouring states less than
+ * 2^25 elements apart); scale positive.
  *   lengths: NULL, or int32 [B]: only states j < lengths[b] are seen;
  *   mask: NULL, or bytes [B, S]: only states whose byte is not 0.
- * A row that sees no state (or nothing but scores of -inf) is zeros; what is
- * not seen is not read into the result, NaN and infinities included.  fp32
- * scores, maxima and sums; the weights are rounded to the operands' type for the product
- * with v.  The workspace is 4-byte aligned and overlaps no operand.  The
- * attention chain of the reference (whole_blocked.py:91-103) with keys of
+ * A row that sees no state is zeros; what is not seen has no part in the result,
+ * NaN and infinities included.  A finite row of q whose scores are all -inf is
+ * zeros too; one that is not finite gives NaN or zeros where it sees anything.
+ * fp32 scores, maxima and sums; the weights are rounded to the operands' type for
+ * the product with v.  The workspace is 4-byte aligned and overlaps no operand.
+ * The attention chain of the reference (whole_blocked.py:91-103) with keys of
  * another length. */
 thin_status thin_cross_attention(const thin_desc* q, const thin_desc* k, const thin_desc* v, const thin_desc* lengths,
                                  const thin_desc* mask, float scale, const thin_desc* out, void* workspace,
@@ -530,9 +532,9 @@ thin_status thin_cross_attention(const thin_desc* q, const thin_desc* k, const t
  *   codes = e4m3(x / s), to the nearest, ties to even; earlier tokens, where the
  *       scale grew, e4m3(code * old / s).
  * Infinities become the largest code, NaN stays NaN; neither counts for s.  Codes
- * behind a sequence's last token stay as they are, so tokens given up by a lower length
- * may be written anew.  The strided copies of the reference (ops.cpp:32-78) at
- * places that depend on the data, with another type. */
+ * behind a sequence's last token stay as they are, so tokens given up by a lower
+ * length may be written anew.  The strided copies of the reference (ops.cpp:32-78)
+ * at places that depend on the data, with another type. */
 thin_status thin_cache_write(const thin_desc* k, const thin_desc* v, const thin_desc* k_cache, const thin_desc* v_cache,
                              const thin_desc* k_scales, const thin_desc* v_scales, const thin_desc* table,
                              const thin_desc* lengths, const thin_desc* counts, hipStream_t stream);
@@ -545,10 +547,13 @@ size_t thin_cache_attention_workspace(const thin_desc* q, const thin_desc* k_cac
 /* Attention of each sequence's last tokens, q and out [B, T, H, D] (fp16 or bf16,
  * a head's dims adjacent, Hk divides H), over its cached ones: row t < counts[b]
  * sees the tokens up to and with its own, j <= lengths[b] - counts[b] + t.  Rows
- * from counts[b] on, and rows that see nothing, are zeros.  fp32 scores, maxima
- * and sums; a weight times its page's scale is rounded to bf16 for the product with the codes
- * of v.  What a row does not see has no part in it, NaN included.  The workspace is
- * 4-byte aligned and overlaps no operand.  The attention chain of the reference
+ * from counts[b] on, and rows that see nothing, are zeros.  What a row does not
+ * see has no part in it, NaN included.  Scales are any that are not negative,
+ * neighbouring tokens less than 2^26 bytes apart.  fp32 scores, maxima and sums; a
+ * weight, times its value's scale as a multiple of the largest scale among the
+ * sequence's tokens, is rounded to q's type for the product with the codes of v (as
+ * fp16, what is below 2^-33 of the largest is lost).  The workspace is 4-byte aligned
+ * and overlaps no operand.  The attention chain of the reference
  * (whole_blocked.py:91-103) over pages. */
 thin_status thin_cache_attention(const thin_desc* q, const thin_desc* k_cache, const thin_desc* v_cache,
                                  const thin_desc* k_scales, const thin_desc* v_scales, const thin_desc* table,
@@ -578,9 +583,10 @@ size_t thin_verify_drafts_workspace(int64_t batch, int64_t vocab);
  *   out [B, K + 1] int64: the n drafts, that token, then -1.
  * Target probabilities that are not positive and finite count as 0; a draft whose
  * own is not finite falls, and so does the part of a token whose draft probability
- * is not.  If nothing has a part, the next token is -1.  Products and sums in 64 bits.  The workspace is 8-byte aligned and
- * overlaps no operand.  The selection of the reference (selection_flow.cpp:429-499)
- * with given chances in place of the order. */
+ * is not.  If nothing has a part, the next token is -1.  Products and sums in 64
+ * bits.  The workspace is 8-byte aligned and overlaps no operand.  The selection of
+ * the reference (selection_flow.cpp:429-499) with given chances in place of the
+ * order. */
 thin_status thin_verify_drafts(const thin_desc* target, const thin_desc* draft, const thin_desc* tokens,
                                const thin_desc* counts, const thin_desc* accept, const thin_desc* sample,
                                const thin_desc* out, const thin_desc* taken, void* workspace, size_t workspace_bytes,

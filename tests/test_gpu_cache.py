@@ -403,3 +403,47 @@ def test_same_bits_streams_and_graphs(gpu, t):
         torch.cuda.synchronize()
         for cache, out in zip(caches, outs):
             assert torch.equal(out, want) and all(torch.equal(x, y) for x, y in zip(cache, eager))
+
+
+@pytest.mark.parametrize("b", [70, 150])
+def test_attention_many_sequences(gpu, b):
+    """Few rows of more sequences than a wavefront has lanes, some without tokens."""
+    c = Cache(gpu, b, 9, 64, 1, 16, b)
+    lengths = torch.randint(3, 577, (b,), generator=c.g, dtype=torch.int32)
+    counts = torch.randint(0, 4, (b,), generator=c.g, dtype=torch.int32)
+    lengths[::7] = 0
+    lengths[63:66] = torch.tensor([0, 576, 1], dtype=torch.int32)
+    got = c.attend(queries(b, 3, 4, 16, torch.bfloat16, b), lengths, counts)
+    assert not got[::7].any()
+
+
+@pytest.mark.parametrize("b,heads,t,h,d,length", [(32, 32, 5, 128, 144, 4300), (16, 16, 40, 16, 32, 9000), (16, 16, 130, 16, 64, 5000)])
+@pytest.mark.parametrize("dtype", HALVES)
+def test_attention_long(gpu, b, heads, t, h, d, length, dtype):
+    """Many sequences that read the same long context: a workgroup walks far enough
+    to look its pages up again.  All get the same bits, the first is checked."""
+    from thintnpu_amd import capi
+    c = Cache(gpu, 1, -(-length // 16), 16, heads, d, length)
+    c.host[3][c.table[0].long()] *= torch.exp2(torch.arange(c.table.shape[1]) // 48 % 5 * 2.0)[:, None]  # in steps, up and down
+    c.host[1][c.table[0, 70].long(), 0, 3, 2] = 0x7F
+    bad = c.table.clone()
+    bad[0, 100:103] = -1
+    c.dev = [x.to(gpu) for x in c.host]
+    q = queries(1, t, h, d, HALVES[dtype], t)
+    lengths = torch.tensor([length], dtype=torch.int32)
+    got = capi.cache_attention(q.repeat(b, 1, 1, 1).to(gpu), *c.dev, bad.repeat(b, 1).to(gpu), lengths.repeat(b).to(gpu))
+    assert torch.equal(got.view(torch.int16), got[:1].expand_as(got).contiguous().view(torch.int16))
+    close(got[:1], oracle.attention(q, *c.host, bad, lengths), q, length, c.host)
+
+
+@pytest.mark.parametrize("t", [1, 6, 40])
+@pytest.mark.parametrize("dtype", HALVES)
+def test_attention_scales_of_zero(gpu, t, dtype):
+    """Keys and values of scale 0 beside places that are not seen."""
+    for which in (2, 3):
+        c = Cache(gpu, 2, 4, 16, 2, 32, t)
+        c.host[which][c.table[:, 1:].long()] = 0.0
+        c.dev = [x.to(gpu) for x in c.host]
+        for length in (41, 57, 60):
+            got = c.attend(queries(2, t, 4, 32, HALVES[dtype], t), torch.tensor([length, max(t, 20)], dtype=torch.int32))
+            assert torch.isfinite(got).all()

@@ -208,3 +208,38 @@ def test_same_bits_streams_and_graphs(gpu, t):
         torch.cuda.synchronize()
         for x, out in zip(qs, outs):
             assert torch.equal(out, capi.cross_attention(x, k, v))
+
+
+@pytest.mark.parametrize("b", [70, 150])
+def test_many_sequences(gpu, b):
+    """Few rows of more sequences than a wavefront has lanes, some without states."""
+    q, k, v = inputs(b, 2, 2100, 2, 1, 16, torch.float16, b)
+    lengths = torch.randint(0, 2101, (b,), generator=gen(b), dtype=torch.int32)
+    lengths[torch.arange(0, b, 7)] = 0
+    lengths[63:66] = torch.tensor([0, 2100, 1], dtype=torch.int32)
+    got = check(gpu, q, k, v, lengths)
+    assert not got[::7].any()
+    check(gpu, q, k, v, torch.zeros_like(lengths))
+
+
+@pytest.mark.parametrize("d", [8, 24, 40, 64, 72])
+def test_narrow_rows_split(gpu, d):
+    for t in (33, 100):
+        q, k, v = inputs(2, t, 2500, 2, 2, d, torch.bfloat16, d + t)
+        check(gpu, q, k, v, torch.tensor([2500, 300], dtype=torch.int32), torch.rand((2, 2500), generator=gen(d)) < 0.9)
+
+
+@pytest.mark.parametrize("t,s", [(1, 90), (40, 90), (1, 700), (40, 700)])
+@pytest.mark.parametrize("bad", [math.inf, -math.inf, math.nan])
+def test_queries_that_are_not_finite(gpu, t, s, bad):
+    """They touch their own row alone, and nothing where no state is seen."""
+    from thintnpu_amd import capi
+    q, k, v = inputs(2, t, s, 2, 2, 32, torch.float16, s)
+    q[:, 0, 1, 3] = bad
+    k[:, 0, 1, 3] = bad if math.isinf(bad) else 1.0  # a score of +inf, then a masked one of the other sign
+    mask = torch.ones((2, s), dtype=torch.bool)
+    mask[0] = False
+    mask[1, 5:9] = False
+    got = capi.cross_attention(*(x.to(gpu) for x in (q, k, v)), mask=mask.to(gpu)).cpu()
+    assert not got[0].any()
+    assert torch.isnan(got[1, 0, 1]).all() and torch.isfinite(got[1, 1:, 0]).all() and torch.isfinite(got[1, 0, 0]).all()

@@ -390,11 +390,14 @@ __device__ __forceinline__ const uint8_t* code_at(const PagesOf& c, int32_t id, 
   return c.codes + id * c.page + h * c.head + token * c.token;
 }
 
-// The maximum that a row's exponentials stand against is raised where a score
-// passes it by kSlack bits, not by less: sums are rescaled in few tiles, and an
-// exponential is 2^kSlack at most.  (2048 rows of 4 x 32 heads to 4096 states: 594
-// us, 690 with a slack of 0.)
+// The maximum that a row's exponentials stand against is not raised wherever a score
+// passes it, so sums are rescaled in few tiles.  Few rows: where one passes it by
+// kSlack bits, so that an exponential is 2^kSlack at most.  Many rows: where the sum
+// of a lane's 16 exponentials passes kMostOfStep, so that no maxima of the step are
+// taken but then, and in a row's first (300 rows of 8 x 8 heads to 8400 states: 72
+// us; 77 with the step's maxima and kSlack, 101 with a slack of 0).
 constexpr float kSlack = 4.f;
+constexpr float kMostOfStep = 128.f;  // with kShift 2^15: a half holds that
 
 // Maxima are those of c s, rounded.  A row's exponentials are 2^(c s + offset_of(m))
 // with the product in full: the maximum's rounding is common to all.
@@ -509,12 +512,12 @@ __device__ __forceinline__ Place place_of(const AttendPlan& p) {
 // instructions take turns; the keys of step j + 3 and the values of step j + 1 are
 // written meanwhile, and loads of one step more are in flight.  One barrier for two
 // steps.  The exponentials do not wait for their step's maximum: they are taken
-// against the maximum so far, and again where that turns out too low.
+// against the maximum so far, and again where their sum shows that as too low.
 // What bounds it: at 128 dims the matrix instructions and what is issued between
 // them (2048 rows of 4 x 32 heads to 4096 states: 590 us, 930 TFLOP/s); at 32 and 64
-// dims the softmax, whose 16 exponentials, 64 other vector instructions and, of codes,
+// dims the softmax, whose 16 exponentials, 55 other vector instructions and, of codes,
 // 16 widenings a step stand against 4 and 8 matrix instructions (300 rows of 8 x 8
-// heads to 8400 states of 32 dims: 70 us; 1024 rows of 3 x 24 heads over 8000 cached
+// heads to 8400 states of 32 dims: 66 us; 1024 rows of 3 x 24 heads over 8000 cached
 // tokens of 64: 128 us, 440 TFLOP/s).
 // Rows: unseen states have -inf in the scores from the start (the accumulator's
 // first value).  Pages: rows that do not see a whole step are masked afterwards.
@@ -560,6 +563,7 @@ __global__ __launch_bounds__(256, tile_workgroups(DP)) void tile_kernel(AttendPl
 
   f16v o[DP / 32];
   float m = -__builtin_inff(), off = Matrix<T>::kShift, l = 0.f;  // l: of this half's keys
+  bool fresh = true;  // some row has seen nothing yet
 #pragma unroll
   for (int i = 0; i < DP / 32; ++i)
 #pragma unroll
@@ -771,7 +775,7 @@ __global__ __launch_bounds__(256, tile_workgroups(DP)) void tile_kernel(AttendPl
       }
     }
     const bool zero[2] = {back[0] < 0.f, back[1] < 0.f};  // a value's scale of 0
-    float add[2], sum[2] = {0.f, 0.f}, top[2] = {-__builtin_inff(), -__builtin_inff()};
+    float add[2], sum[2] = {0.f, 0.f};
 #pragma unroll
     for (int n = 0; n < 2; ++n) {
       add[n] = PAGED ? off + share[n] : off;
@@ -820,15 +824,19 @@ __global__ __launch_bounds__(256, tile_workgroups(DP)) void tile_kernel(AttendPl
       if (i + kAhead < kProducts) kf[i % kAhead] = key_piece(k_slot, i + kAhead);
       if (i + 2 < kProducts) vf[i % 2] = value_piece(v_slot, i + 2);
 #pragma unroll
-      for (int x = i * 8 / kProducts * 2; x < (i + 1) * 8 / kProducts * 2; x += 2) {
-        weigh(x);
-        top[x / 8] = fmaxf(fmaxf(top[x / 8], s[x]), s[x + 1]);
-      }
+      for (int x = i * 8 / kProducts * 2; x < (i + 1) * 8 / kProducts * 2; x += 2) weigh(x);
       __builtin_amdgcn_sched_barrier(0);
     }
-    // (a NaN of unseen keys' scales is dropped)
-    const float highest = PAGED ? fmaxf(fmaxf(-__builtin_inff(), top[0] * c[0]), top[1] * c[1]) : fmaxf(top[0], top[1]) * p.c;
-    if (__any(highest - m > kSlack)) {  // (either half's lanes)
+    float total = PAGED ? sum[0] * back[0] + sum[1] * back[1] : sum[0] + sum[1];
+    if (fresh || __any(total > kMostOfStep * __builtin_exp2f(Matrix<T>::kShift))) {
+      float top[2] = {s[0], s[8]};
+#pragma unroll
+      for (int x = 1; x < 8; ++x) {
+        top[0] = fmaxf(top[0], s[x]);
+        top[1] = fmaxf(top[1], s[x + 8]);
+      }
+      // (a NaN is dropped: weights are NaN by themselves)
+      const float highest = fmaxf(fmaxf(-__builtin_inff(), top[0] * c[0]), top[1] * c[1]);
       const float to = fmaxf(m, fmaxf(highest, lane_xor<32>(highest))), f = rescale_of(m, to);
       l *= f;
       a *= f;
@@ -841,8 +849,11 @@ __global__ __launch_bounds__(256, tile_workgroups(DP)) void tile_kernel(AttendPl
       }
 #pragma unroll
       for (int x = 0; x < 16; x += 2) weigh(x);
+      total = PAGED ? sum[0] * back[0] + sum[1] * back[1] : sum[0] + sum[1];
       raised = true;
+      fresh = __any(m == -__builtin_inff());
     }
+    l += total;
     if (raised) {
 #pragma unroll
       for (int i = 0; i < DP / 32; ++i)
@@ -850,13 +861,11 @@ __global__ __launch_bounds__(256, tile_workgroups(DP)) void tile_kernel(AttendPl
         for (int e = 0; e < 16; ++e) o[i][e] *= a;
     }
 #pragma unroll
-    for (int n = 0; n < 2; ++n) {
-      l += PAGED ? sum[n] * back[n] : sum[n];
+    for (int n = 0; n < 2; ++n)
       if (PAGED && zero[n]) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) pr[n][i] = (T)0.f;
       }
-    }
   };
 
   f16v s[2];

@@ -530,7 +530,8 @@ thin_status thin_cross_attention(const thin_desc* q, const thin_desc* k, const t
  *       the scale it has if that is larger and earlier tokens of the sequence
  *       are on the page;
  *   codes = e4m3(x / s), to the nearest, ties to even; earlier tokens, where the
- *       scale grew, e4m3(code * old / s).
+ *       scale grew, e4m3(code * old / s) (exact before that one rounding for powers
+ *       of two, in 32 bits for an old scale that is none).
  * Infinities become the largest code, NaN stays NaN; neither counts for s.  Codes
  * behind a sequence's last token stay as they are, so tokens given up by a lower
  * length may be written anew.  The strided copies of the reference (ops.cpp:32-78)

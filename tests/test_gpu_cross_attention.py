@@ -243,3 +243,9 @@ def test_queries_that_are_not_finite(gpu, t, s, bad):
     got = capi.cross_attention(*(x.to(gpu) for x in (q, k, v)), mask=mask.to(gpu)).cpu()
     assert not got[0].any()
     assert torch.isnan(got[1, 0, 1]).all() and torch.isfinite(got[1, 1:, 0]).all() and torch.isfinite(got[1, 0, 0]).all()
+
+
+def test_many_heads(gpu):
+    """One row of each of many heads: 2100 workgroups, the last of them in turn."""
+    q, k, v = inputs(175, 1, 40, 12, 12, 32, torch.float16, 3)
+    check(gpu, q, k, v, torch.randint(0, 41, (175,), generator=gen(4), dtype=torch.int32))

@@ -186,3 +186,14 @@ def test_same_bits_streams_and_graphs(gpu, v):
         torch.cuda.synchronize()
         for a, out in zip(us, outs):
             assert all(torch.equal(y, z) for y, z in zip(out, capi.verify_drafts(t, d, x, a, r)))
+
+
+@pytest.mark.parametrize("b", [700, 1100])
+def test_several_tiles_a_workgroup(gpu, b):
+    """Five tiles of a row, two or four of them to a workgroup."""
+    from thintnpu_amd import capi
+    t, d, x, u, r = inputs(4, 2, 9000, torch.float16, b, 1.0)
+    ref = oracle.verify(t, d, x, u, r)
+    many = [a.repeat(b // 4, *[1] * (a.dim() - 1)).to(gpu) for a in (t, d, x, u, r)]
+    got = capi.verify_drafts(*many)
+    assert torch.equal(got[0].cpu(), ref[0].repeat(b // 4, 1)) and torch.equal(got[1].cpu(), ref[1].repeat(b // 4))

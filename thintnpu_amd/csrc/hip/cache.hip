@@ -55,7 +55,10 @@ __device__ __forceinline__ uint32_t code4(float a, float b, float c, float d) {
 }
 
 // One wavefront for the new tokens of a page and head: 16 values a lane, once for
-// their maximum, once for their codes.
+// their maximum, once for their codes (from L2: held in registers in between they
+// took as long).  Bound by the chain of count, page, scale, values and codes, some 5
+// us of it for one token of 48 sequences, and by memory behind that (6 x 8 heads of
+// prompts of 2048 tokens at most, 128 dims, pages of 32: 14 us, 2.7 TB/s).
 template <typename T>
 __global__ __launch_bounds__(256) void write_kernel(WritePlan p) {
   const uint64_t unit = (uint64_t)blockIdx.x * 4 + (threadIdx.x >> 6);

@@ -12,7 +12,9 @@
 // Bound by memory: of the target's and the draft's rows only one each is read
 // whole.  Few rows, so each is cut into tiles over the card; a second launch
 // finds the tile that holds the border and scans it again.  A row of one tile
-// takes one launch.
+// takes one launch.  (48 rows of 128000 in 32 bits, target and draft: 11.5 us, 4.3
+// TB/s, and 7.8 of the second launch, a chain of loads and sums that takes 6.6 for
+// two rows of 50001 too.)
 #include "rows.h"
 
 #include <string.h>
@@ -20,11 +22,10 @@
 namespace thin {
 namespace {
 
-constexpr int kChunk = 2048;       // elements of a workgroup at a time: 8 a thread
+constexpr int kTile = 2048;        // elements of a workgroup at a time: 8 a thread
 constexpr int64_t kMaxDrafts = 64; // one lane each
 constexpr int64_t kMaxVocab = 1 << 23;
-constexpr int64_t kWorkgroups = 1024;
-constexpr int64_t kMostChunks = 4;
+constexpr int kMostTiles = 4;      // of a workgroup
 
 struct DraftPlan {
   const void* target;
@@ -42,8 +43,8 @@ struct DraftPlan {
   int64_t ob, ok;
   int32_t* taken;
   int64_t taken_step;
-  uint32_t drafts, vocab, tiles;
-  FastDiv by_tiles;
+  uint32_t drafts, vocab, tiles, per, groups;  // per: a workgroup's tiles; groups: of them, a row's
+  FastDiv by_groups;
   double* sums;     // [batch, tiles, 2]: of what is left, of the target's row
   int32_t* stayed;  // [batch]
 };
@@ -105,85 +106,62 @@ struct Rest {
   }
 };
 
-__device__ __forceinline__ double wave_total(double v) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
-  return v;
+__device__ __forceinline__ double lane_double(double v, int lane) {
+  const uint64_t bits = __builtin_bit_cast(uint64_t, v);
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)bits, lane);
+  const uint32_t hi = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(bits >> 32), lane);
+  return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
 }
-// Sum over the lanes up to this one.
-__device__ __forceinline__ double wave_scan(double v, uint32_t lane) {
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const double below = __shfl_up(v, o, 64);
-    if (lane >= (uint32_t)o) v += below;
-  }
-  return v;
+// Sum over the lanes up to this one, by DPP.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ double plus_moved(double v) {
+  const uint64_t bits = __builtin_bit_cast(uint64_t, v);
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)bits, CTRL, ROWS, 0xF, false);
+  const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(bits >> 32), CTRL, ROWS, 0xF, false);
+  return v + __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
 }
+__device__ __forceinline__ double wave_scan(double v) {
+  v = plus_moved<0x111, 0xF>(v);  // row_shr:1, :2, :4, :8
+  v = plus_moved<0x112, 0xF>(v);
+  v = plus_moved<0x114, 0xF>(v);
+  v = plus_moved<0x118, 0xF>(v);
+  v = plus_moved<0x142, 0xA>(v);  // row_bcast:15, :31
+  return plus_moved<0x143, 0xC>(v);
+}
+__device__ __forceinline__ double wave_total(double v) { return lane_double(wave_scan(v), 63); }
 
 struct Shared {
-  double left[4], own[4];
+  double left[kMostTiles][4], own[kMostTiles][4];
   uint32_t found, last;
 };
 
-// Sums of a tile's 8 * 256 * CHUNKS elements; every thread gets them.
-template <typename T, int CHUNKS>
-__device__ __forceinline__ void tile_sums(const Rest<T>& rest, uint32_t first, Shared& lds, double& left, double& own) {
-  const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
-  left = own = 0.0;
-#pragma unroll 2
-  for (int c = 0; c < CHUNKS; ++c) {
-    double a[8], o[8];
-    rest.load(first + c * kChunk + threadIdx.x * 8, a, o);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      left += a[j];
-      own += o[j];
-    }
-  }
-  left = wave_total(left);
-  own = wave_total(own);
-  if (lane == 0) {
-    lds.left[wave] = left;
-    lds.own[wave] = own;
-  }
-  __syncthreads();
-  left = ((lds.left[0] + lds.left[1]) + lds.left[2]) + lds.left[3];
-  own = ((lds.own[0] + lds.own[1]) + lds.own[2]) + lds.own[3];
-  __syncthreads();
-}
-
 // The first element of a tile whose sum, with `before` ahead of the tile, passes
-// `edge`; where rounding leaves none, the tile's last that has a part.  Thread i
-// holds the i-th 8 * CHUNKS elements.
-template <typename T, int CHUNKS>
+// `edge`; where rounding leaves none, the tile's last that has a part.
+template <typename T>
 __device__ __forceinline__ uint32_t find_in_tile(const Rest<T>& rest, bool whole, uint32_t first, double before, double edge,
                                                  Shared& lds) {
-  const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, at = first + threadIdx.x * 8 * CHUNKS;
+  const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, at = first + threadIdx.x * 8;
   if (threadIdx.x == 0) {
     lds.found = 0xFFFFFFFFu;
     lds.last = 0;
   }
-  double x[8 * CHUNKS], sum = 0.0;
+  double a[8], o[8], sum = 0.0;
+  rest.load(at, a, o);
 #pragma unroll
-  for (int c = 0; c < CHUNKS; ++c) {
-    double a[8], o[8];
-    rest.load(at + c * 8, a, o);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      x[c * 8 + j] = whole ? o[j] : a[j];
-      sum += x[c * 8 + j];
-    }
+  for (int j = 0; j < 8; ++j) {
+    if (whole) a[j] = o[j];
+    sum += a[j];
   }
-  const double scan = wave_scan(sum, lane);
-  if (lane == 63) lds.left[wave] = scan;
+  const double scan = wave_scan(sum);
+  if (lane == 63) lds.left[0][wave] = scan;
   __syncthreads();
-  for (uint32_t i = 0; i < wave; ++i) before += lds.left[i];
+  for (uint32_t i = 0; i < wave; ++i) before += lds.left[0][i];
   double run = before + (scan - sum);
   uint32_t found = 0xFFFFFFFFu, last = 0;
 #pragma unroll
-  for (int j = 0; j < 8 * CHUNKS; ++j) {
-    run += x[j];
-    if (x[j] > 0.0) {
+  for (int j = 0; j < 8; ++j) {
+    run += a[j];
+    if (a[j] > 0.0) {
       last = at + j;
       if (run > edge) found = min(found, at + j);
     }
@@ -213,26 +191,52 @@ struct Given {
   }
 };
 
-template <typename T, int CHUNKS>
+template <typename T>
 __global__ __launch_bounds__(256) void sums_kernel(DraftPlan p) {
   __shared__ Shared lds;
-  const uint32_t b = p.by_tiles.div(blockIdx.x), tile = blockIdx.x - b * p.tiles;
+  const uint32_t b = p.by_groups.div(blockIdx.x), first = (blockIdx.x - b * p.groups) * p.per;
+  const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
   uint32_t count;
-  const uint32_t stayed = stayed_of<T>(p, b, threadIdx.x & 63u, count);
+  const uint32_t stayed = stayed_of<T>(p, b, lane, count);
   const Rest<T> rest(p, b, stayed, count);
-  double left, own;
-  tile_sums<T, CHUNKS>(rest, tile * (CHUNKS * kChunk), lds, left, own);
-  if (p.tiles == 1) {
-    const Given given(p, b);
-    const bool whole = !(left > 0.0);
-    const double total = whole ? own : left;
-    const uint32_t next = find_in_tile<T, CHUNKS>(rest, whole, 0, 0.0, given.edge(total), lds);
-    given.store(p, b, stayed, total > 0.0 ? (int64_t)next : -1);
-  } else if (threadIdx.x == 0) {
-    p.sums[blockIdx.x * 2ull] = left;
-    p.sums[blockIdx.x * 2ull + 1] = own;
-    if (tile == 0) p.stayed[b] = (int32_t)stayed;
+#pragma unroll
+  for (uint32_t i = 0; i < (uint32_t)kMostTiles; ++i)
+    if (i < p.per) {  // (past the row's end: zeros)
+      double a[8], o[8], left = 0.0, own = 0.0;
+      rest.load((first + i) * kTile + threadIdx.x * 8, a, o);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        left += a[j];
+        own += o[j];
+      }
+      left = wave_total(left);
+      own = wave_total(own);
+      if (lane == 0) {
+        lds.left[i][wave] = left;
+        lds.own[i][wave] = own;
+      }
+    }
+  __syncthreads();
+  const uint32_t i = threadIdx.x & (kMostTiles - 1u);
+  const double left = ((lds.left[i][0] + lds.left[i][1]) + lds.left[i][2]) + lds.left[i][3];
+  const double own = ((lds.own[i][0] + lds.own[i][1]) + lds.own[i][2]) + lds.own[i][3];
+  if (p.tiles > 1) {
+    if (threadIdx.x < p.per && first + threadIdx.x < p.tiles) {
+      double* sums = p.sums + ((uint64_t)b * p.tiles + first + threadIdx.x) * 2;
+      sums[0] = left;
+      sums[1] = own;
+    }
+    if (first == 0 && threadIdx.x == 0) p.stayed[b] = (int32_t)stayed;
+    return;
   }
+  const double all_left = ((lds.left[0][0] + lds.left[0][1]) + lds.left[0][2]) + lds.left[0][3];
+  const double all_own = ((lds.own[0][0] + lds.own[0][1]) + lds.own[0][2]) + lds.own[0][3];
+  __syncthreads();
+  const Given given(p, b);
+  const bool whole = !(all_left > 0.0);
+  const double total = whole ? all_own : all_left;
+  const uint32_t next = find_in_tile<T>(rest, whole, 0, 0.0, given.edge(total), lds);
+  given.store(p, b, stayed, total > 0.0 ? (int64_t)next : -1);
 }
 
 // Where a row's border lies: the first tile whose sum passes it (where rounding
@@ -242,27 +246,27 @@ template <bool WHOLE>
 __device__ __forceinline__ bool find_tile(const DraftPlan& p, const double* sums, const Given& given, uint32_t lane,
                                           uint32_t& tile, double& before, double& edge) {
   const auto part = [&](uint32_t i) { return i + lane < p.tiles ? sums[(i + lane) * 2 + (WHOLE ? 1 : 0)] : 0.0; };
-  const double first = part(0), first_scan = wave_scan(first, lane);
-  double total = __shfl(first_scan, 63, 64);
-  for (uint32_t i = 64; i < p.tiles; i += 64) total += __shfl(wave_scan(part(i), lane), 63, 64);
+  const double first = part(0), first_scan = wave_scan(first);
+  double total = lane_double(first_scan, 63);
+  for (uint32_t i = 64; i < p.tiles; i += 64) total += wave_total(part(i));
   if (!(total > 0.0)) return false;
   edge = given.edge(total);
   double ahead = 0.0;
   for (uint32_t i = 0; i < p.tiles; i += 64) {
-    const double v = i ? part(i) : first, scan = i ? wave_scan(v, lane) : first_scan;
+    const double v = i ? part(i) : first, scan = i ? wave_scan(v) : first_scan;
     const uint64_t passed = __ballot(v > 0.0 && ahead + scan > edge), some = __ballot(v > 0.0);
     if (some) {
       const int l = passed ? __builtin_ctzll(passed) : 63 - __builtin_clzll(some);
       tile = i + l;
-      before = __shfl(ahead + (scan - v), l, 64);
+      before = lane_double(ahead + (scan - v), l);
       if (passed) break;
     }
-    ahead += __shfl(scan, 63, 64);
+    ahead += lane_double(scan, 63);
   }
   return true;
 }
 
-template <typename T, int CHUNKS>
+template <typename T>
 __global__ __launch_bounds__(256) void find_kernel(DraftPlan p) {
   __shared__ Shared lds;
   const uint32_t b = blockIdx.x, lane = threadIdx.x & 63u;
@@ -276,28 +280,25 @@ __global__ __launch_bounds__(256) void find_kernel(DraftPlan p) {
   double before = 0.0, edge = 0.0;
   const bool some = find_tile<false>(p, sums, given, lane, tile, before, edge);
   const bool any = some || find_tile<true>(p, sums, given, lane, tile, before, edge);
-  const uint32_t next = find_in_tile<T, CHUNKS>(rest, !some, tile * (CHUNKS * kChunk), before, edge, lds);
+  const uint32_t next = find_in_tile<T>(rest, !some, tile * kTile, before, edge, lds);
   given.store(p, b, stayed, any ? (int64_t)next : -1);
 }
 
-// Chunks of a tile: one, or as many as leave enough workgroups.
-int64_t chunks_of(int64_t batch, int64_t vocab) {
-  const int64_t all = (vocab + kChunk - 1) / kChunk;
+int64_t tiles_of(int64_t vocab) { return (vocab + kTile - 1) / kTile; }
+// Tiles of a workgroup: one, or as many as leave enough workgroups, since each first
+// finds out which row is the rest's (256 rows of 128000 as bf16: 42 us by four, 51 by one).
+int64_t per_of(int64_t batch, int64_t vocab) {
   int64_t n = 1;
-  while (n < kMostChunks && batch * ((all + 2 * n - 1) / (2 * n)) >= kWorkgroups) n *= 2;
+  while (n < kMostTiles && batch * ((tiles_of(vocab) + 2 * n - 1) / (2 * n)) >= 2048) n *= 2;
   return n;
 }
-int64_t tiles_of(int64_t batch, int64_t vocab) {
-  const int64_t per = kChunk * chunks_of(batch, vocab);
-  return (vocab + per - 1) / per;
-}
 
-template <typename T, int CHUNKS>
+template <typename T>
 thin_status launch(const DraftPlan& p, int64_t batch, hipStream_t stream) {
-  hipLaunchKernelGGL((sums_kernel<T, CHUNKS>), dim3((uint32_t)(batch * p.tiles)), dim3(256), 0, stream, p);
+  hipLaunchKernelGGL((sums_kernel<T>), dim3((uint32_t)(batch * p.groups)), dim3(256), 0, stream, p);
   THIN_LAUNCH_CHECK("verify_drafts");
   if (p.tiles > 1) {
-    hipLaunchKernelGGL((find_kernel<T, CHUNKS>), dim3((uint32_t)batch), dim3(256), 0, stream, p);
+    hipLaunchKernelGGL((find_kernel<T>), dim3((uint32_t)batch), dim3(256), 0, stream, p);
     THIN_LAUNCH_CHECK("verify_drafts_find");
   }
   return THIN_OK;
@@ -310,7 +311,7 @@ using namespace thin;
 
 extern "C" size_t thin_verify_drafts_workspace(int64_t batch, int64_t vocab) {
   if (batch <= 0 || vocab <= 0 || vocab > kMaxVocab) return 0;
-  const int64_t tiles = tiles_of(batch, vocab);
+  const int64_t tiles = tiles_of(vocab);
   return tiles == 1 ? 0 : (size_t)batch * (tiles * 16 + 8);
 }
 
@@ -344,7 +345,7 @@ extern "C" thin_status thin_verify_drafts(const thin_desc* target, const thin_de
                "verify_drafts: the probabilities of a row must be adjacent");
   if (B == 0) return THIN_OK;
   THIN_REQUIRE(B < (1ll << 24), THIN_ERR_UNSUPPORTED, "verify_drafts: tensor too large");
-  const int64_t tiles = tiles_of(B, V);
+  const int64_t tiles = tiles_of(V);
   THIN_REQUIRE(launchable(B * tiles, 256), THIN_ERR_UNSUPPORTED, "verify_drafts: tensor too large");
   const thin_desc* outs[2] = {out, taken};
   for (const thin_desc* o : outs) {
@@ -385,17 +386,15 @@ extern "C" thin_status thin_verify_drafts(const thin_desc* target, const thin_de
   p.drafts = (uint32_t)K;
   p.vocab = (uint32_t)V;
   p.tiles = (uint32_t)tiles;
-  p.by_tiles = FastDiv::make(p.tiles);
+  p.per = (uint32_t)per_of(B, V);
+  p.groups = (uint32_t)((tiles + p.per - 1) / p.per);
+  p.by_groups = FastDiv::make(p.groups);
   if (tiles > 1) {
     p.sums = static_cast<double*>(workspace);
     p.stayed = reinterpret_cast<int32_t*>(p.sums + 2 * B * tiles);
   }
   return with_float_type(target->dtype, [&](auto zero) {
     using T = decltype(zero);
-    switch (chunks_of(B, V)) {
-      case 1: return launch<T, 1>(p, B, stream);
-      case 2: return launch<T, 2>(p, B, stream);
-      default: return launch<T, 4>(p, B, stream);
-    }
+    return launch<T>(p, B, stream);
   });
 }

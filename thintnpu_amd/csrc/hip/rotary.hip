@@ -87,7 +87,9 @@ __device__ __forceinline__ void store_some(T* p, uint32_t n, const float (&v)[N]
 }
 
 // V pairs a piece (halves: V elements from each half; interleaved: 2 V elements).
-// Heads go two at a time: their loads are issued before the first is stored.
+// Heads go two at a time: their loads are issued before the first is stored (6400
+// tokens of 8 x 2 x 16 heads of 64 dims: 85 us, 4.9 TB/s; 92 with one, 88 with four,
+// 97 with eight at a time).
 constexpr int kHeadsAhead = 2;
 template <typename T, int V, bool INTERLEAVED, bool NT>
 __global__ __launch_bounds__(256) void rotary_kernel(RotaryPlan p) {
@@ -183,9 +185,11 @@ __global__ __launch_bounds__(256) void rotary_kernel(RotaryPlan p) {
 }
 
 // Threads that fill the card a few times over; past them a thread takes more
-// heads with its angles.
+// heads with its angles, up to 16 (the same: 125 us with 4, 97 with 8, 87 with 16, 88
+// with 32).
 constexpr int64_t kEnough = 256 * 2048;
-// Tensors from this many bytes on are read and written past the caches.
+// Tensors from this many bytes on are read and written past the caches (420 MB: 88
+// us, 93 through them).
 constexpr int64_t kRotaryStreaming = (int64_t)64 << 20;
 
 template <typename T, int V, bool INTERLEAVED>

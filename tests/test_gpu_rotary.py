@@ -176,3 +176,21 @@ def test_beyond_32_bits(gpu):
     assert torch.equal(capi.rotary_axes(view, positions, freqs, axes), ref)
     capi.rotary_axes(view, positions, freqs, axes, out=view)
     assert torch.equal(view, ref)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("d,pairs", [(26, 6), (54, 27), (72, 18), (90, 45), (128, 32), (200, 50), (77, 20), (47, 12), (300, 131), (21, 1)])
+def test_pieces(gpu, dtype, interleaved, d, pairs):
+    """Pairs that pieces of one, two, four and eight divide or leave a rest of, dims
+    behind them in any number, NaN and infinities among those; in place too."""
+    from thintnpu_amd import capi
+    q, k, positions, freqs, axes = inputs(2, 3, 3, 2, d, pairs, 2, TYPES[dtype], d)
+    got = check(gpu, q, k, positions, freqs, axes, interleaved)
+    x, y = q.to(gpu), k.to(gpu)
+    same = capi.rotary_axes(x, positions.to(gpu), freqs.to(gpu), axes.to(gpu), k=y, interleaved=interleaved, out=(x, y))
+    assert torch.equal(same[0], got[0]) and torch.equal(same[1], got[1])
+    q[..., 2 * pairs::3], q[..., 2 * pairs + 1::3] = torch.inf, torch.nan
+    odd = capi.rotary_axes(q.to(gpu), positions.to(gpu), freqs.to(gpu), axes.to(gpu), interleaved=interleaved)
+    assert torch.equal(odd[..., :2 * pairs], got[0][..., :2 * pairs])
+    assert torch.equal(odd.cpu()[..., 2 * pairs:].nan_to_num(5.0), q[..., 2 * pairs:].nan_to_num(5.0))

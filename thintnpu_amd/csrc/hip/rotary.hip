@@ -67,7 +67,7 @@ __device__ __forceinline__ void load_some(const T* p, uint32_t n, float (&v)[N])
     for (int j = 0; j < N; ++j) v[j] = (float)w[j];
   } else {
 #pragma unroll
-    for (int j = 0; j < N; ++j) v[j] = (float)p[min((uint32_t)j, n - 1)];
+    for (int j = 0; j < N; ++j) v[j] = (uint32_t)j < n ? (float)p[j] : 0.f;
   }
 }
 template <bool NT, typename T, int N>
@@ -106,26 +106,20 @@ __global__ __launch_bounds__(256) void rotary_kernel(RotaryPlan p) {
     x = static_cast<const T*>(a.x) + b * a.xb + t * a.xt + i * a.xh;
     out = static_cast<T*>(a.out) + b * a.ob + t * a.ot + i * a.oh;
   };
-  if (piece >= p.turn_pieces) {  // dims behind the pairs
-    const uint32_t d = 2 * p.pairs + (piece - p.turn_pieces) * V;
-    for (uint32_t h = first; h < last; ++h) {
-      const T* x;
-      T* out;
-      head_of(h, x, out);
-      if (x == out) continue;
-      float v[V];
-      load_some<NT, T, V>(x + d, p.dim - d, v);
-      store_some<NT, T, V>(out + d, p.dim - d, v);
-    }
-    return;
-  }
-  const uint32_t i0 = piece * V, n = p.pairs - i0;
+  // A piece is two runs of V dims (interleaved: one of 2 V): of pairs, or, copied, of
+  // the dims behind them.
+  const bool turns = piece < p.turn_pieces;
+  const uint32_t i0 = piece * V, d0 = turns ? INTERLEAVED ? 2 * i0 : i0 : 2 * p.pairs + (piece - p.turn_pieces) * 2 * V;
+  const uint32_t d1 = turns ? p.pairs + i0 : d0 + V, end = turns ? 2 * p.pairs : p.dim;
+  // elements of the runs that there are
+  const uint32_t n = INTERLEAVED ? end - d0 : turns ? p.pairs - i0 : end - d0;
+  const uint32_t n1 = turns ? n : end > d1 ? end - d1 : 0;
   float s[V], c[V];
 #pragma unroll
   for (int j = 0; j < V; ++j) {
     s[j] = 0.f;
     c[j] = 1.f;
-    if ((uint32_t)j < n) {
+    if (turns && i0 + j < p.pairs) {
       const int32_t axis = p.axes[(i0 + j) * p.axis_step];
       if ((uint32_t)axis < p.num_axes) {  // a pair of no axis stays
         const int64_t at = axis * p.pa + b * p.pb + t * p.pt;
@@ -147,15 +141,15 @@ __global__ __launch_bounds__(256) void rotary_kernel(RotaryPlan p) {
         head_of(h0 + k, x, out);
         if constexpr (INTERLEAVED) {
           float both[2 * V];
-          load_some<NT, T, 2 * V>(x + 2 * i0, 2 * n, both);
+          load_some<NT, T, 2 * V>(x + d0, n, both);
 #pragma unroll
           for (int j = 0; j < V; ++j) {
             u[k][j] = both[2 * j];
             v[k][j] = both[2 * j + 1];
           }
         } else {
-          load_some<NT, T, V>(x + i0, n, u[k]);
-          load_some<NT, T, V>(x + p.pairs + i0, n, v[k]);
+          load_some<NT, T, V>(x + d0, n, u[k]);
+          load_some<NT, T, V>(x + d1, n1, v[k]);
         }
       }
 #pragma unroll
@@ -165,8 +159,8 @@ __global__ __launch_bounds__(256) void rotary_kernel(RotaryPlan p) {
         float first_of[V], second_of[V];
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-          first_of[j] = u[k][j] * c[j] - v[k][j] * s[j];
-          second_of[j] = v[k][j] * c[j] + u[k][j] * s[j];
+          first_of[j] = turns ? u[k][j] * c[j] - v[k][j] * s[j] : u[k][j];
+          second_of[j] = turns ? v[k][j] * c[j] + u[k][j] * s[j] : v[k][j];
         }
         if constexpr (INTERLEAVED) {
           float both[2 * V];
@@ -175,10 +169,10 @@ __global__ __launch_bounds__(256) void rotary_kernel(RotaryPlan p) {
             both[2 * j] = first_of[j];
             both[2 * j + 1] = second_of[j];
           }
-          store_some<NT, T, 2 * V>(out + 2 * i0, 2 * n, both);
+          store_some<NT, T, 2 * V>(out + d0, n, both);
         } else {
-          store_some<NT, T, V>(out + i0, n, first_of);
-          store_some<NT, T, V>(out + p.pairs + i0, n, second_of);
+          store_some<NT, T, V>(out + d0, n, first_of);
+          store_some<NT, T, V>(out + d1, n1, second_of);
         }
       }
   }
@@ -188,14 +182,16 @@ __global__ __launch_bounds__(256) void rotary_kernel(RotaryPlan p) {
 // heads with its angles, up to 16 (the same: 125 us with 4, 97 with 8, 87 with 16, 88
 // with 32).
 constexpr int64_t kEnough = 256 * 2048;
-// Tensors from this many bytes on are read and written past the caches (420 MB: 88
-// us, 93 through them).
+// Adjacent pairs of tensors from this many bytes on are read and written past the
+// caches (420 MB: 78 us, 83 through them).  Halves are not: their runs end inside
+// lines that the other half needs (336 MB, half of each head turned: 84 us, 101 past
+// the caches).
 constexpr int64_t kRotaryStreaming = (int64_t)64 << 20;
 
 template <typename T, int V, bool INTERLEAVED>
 thin_status launch(RotaryPlan& p, int64_t rows, hipStream_t stream) {
   p.turn_pieces = (p.pairs + V - 1) / V;
-  p.pieces = p.turn_pieces + (p.dim - 2 * p.pairs + V - 1) / V;
+  p.pieces = p.turn_pieces + (p.dim - 2 * p.pairs + 2 * V - 1) / (2 * V);
   p.per_thread = 1;
   while (p.per_thread < 16 && p.per_thread < p.all_heads && rows * p.pieces * (p.all_heads / (2 * p.per_thread)) >= kEnough)
     p.per_thread *= 2;
@@ -207,12 +203,24 @@ thin_status launch(RotaryPlan& p, int64_t rows, hipStream_t stream) {
   p.by_chunks = FastDiv::make(p.chunks);
   p.by_tokens = FastDiv::make(p.tokens);
   const dim3 grid((uint32_t)((threads + 255) / 256)), block(256);
-  if (rows * p.all_heads * p.dim * (int64_t)sizeof(T) >= kRotaryStreaming)
-    hipLaunchKernelGGL((rotary_kernel<T, V, INTERLEAVED, true>), grid, block, 0, stream, p);
+  if (INTERLEAVED && rows * p.all_heads * p.dim * (int64_t)sizeof(T) >= kRotaryStreaming)
+    hipLaunchKernelGGL((rotary_kernel<T, V, INTERLEAVED, INTERLEAVED>), grid, block, 0, stream, p);
   else
     hipLaunchKernelGGL((rotary_kernel<T, V, INTERLEAVED, false>), grid, block, 0, stream, p);
   THIN_LAUNCH_CHECK("rotary_axes");
   return THIN_OK;
+}
+
+// Pairs of a piece: as many as 16 bytes hold if they divide the pairs or leave a
+// small part of them, which goes element by element; else fewer (6 pairs and 14 more
+// dims of 2898 x 29 x 8 heads: 29 us by two, 82 by eight; 50 pairs of 100 and 100
+// more dims of half as many: 101 by two, 116 by four; 45 pairs: 114 by two, 102 by
+// four).
+template <typename T, int V, bool INTERLEAVED>
+thin_status launch_pieces(RotaryPlan& p, int64_t rows, hipStream_t stream) {
+  if constexpr (V > 1)
+    if (p.pairs % V != 0 && p.pairs < 16 * V) return launch_pieces<T, V / 2, INTERLEAVED>(p, rows, stream);
+  return launch<T, V, INTERLEAVED>(p, rows, stream);
 }
 
 }  // namespace
@@ -284,7 +292,7 @@ extern "C" thin_status thin_rotary_axes(const thin_desc* q, const thin_desc* k, 
   return with_float_type(q->dtype, [&](auto zero) {
     using E = decltype(zero);
     constexpr int V = sizeof(E) == 2 ? 8 : 4;  // 16 bytes
-    if (interleaved) return launch<E, V / 2, true>(p, B * T, stream);
-    return launch<E, V, false>(p, B * T, stream);
+    if (interleaved) return launch_pieces<E, V / 2, true>(p, B * T, stream);
+    return launch_pieces<E, V, false>(p, B * T, stream);
   });
 }

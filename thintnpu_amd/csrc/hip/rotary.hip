@@ -31,6 +31,7 @@ struct RotaryPlan {
   uint32_t wide;  // positions of 64 bits
   uint32_t tokens, heads, all_heads, per_thread, dim, pairs, num_axes;
   uint32_t turn_pieces, pieces;  // of pairs, and with those of copied dims
+  uint32_t last_turn, last_copy;  // where pieces begin at most (pair, dim)
   FastDiv by_pieces, by_chunks, by_tokens;
   uint32_t chunks;
   uint64_t threads;
@@ -107,9 +108,11 @@ __global__ __launch_bounds__(256) void rotary_kernel(RotaryPlan p) {
     out = static_cast<T*>(a.out) + b * a.ob + t * a.ot + i * a.oh;
   };
   // A piece is two runs of V dims (interleaved: one of 2 V): of pairs, or, copied, of
-  // the dims behind them.
+  // the dims behind them.  The last ones begin early enough to be whole, and do some
+  // of their neighbours' work too, but for in place.
   const bool turns = piece < p.turn_pieces;
-  const uint32_t i0 = piece * V, d0 = turns ? INTERLEAVED ? 2 * i0 : i0 : 2 * p.pairs + (piece - p.turn_pieces) * 2 * V;
+  const uint32_t i0 = min(piece * V, p.last_turn);
+  const uint32_t d0 = turns ? INTERLEAVED ? 2 * i0 : i0 : min(2 * p.pairs + (piece - p.turn_pieces) * 2 * V, p.last_copy);
   const uint32_t d1 = turns ? p.pairs + i0 : d0 + V, end = turns ? 2 * p.pairs : p.dim;
   // elements of the runs that there are
   const uint32_t n = INTERLEAVED ? end - d0 : turns ? p.pairs - i0 : end - d0;
@@ -192,6 +195,10 @@ template <typename T, int V, bool INTERLEAVED>
 thin_status launch(RotaryPlan& p, int64_t rows, hipStream_t stream) {
   p.turn_pieces = (p.pairs + V - 1) / V;
   p.pieces = p.turn_pieces + (p.dim - 2 * p.pairs + 2 * V - 1) / (2 * V);
+  const uint32_t rest = p.dim - 2 * p.pairs;
+  const bool apart = p.q.x != p.q.out && (!p.k.x || p.k.x != p.k.out);
+  p.last_turn = apart && p.pairs >= V ? p.pairs - V : ~0u;
+  p.last_copy = apart && rest >= 2 * V ? p.dim - 2 * V : ~0u;
   p.per_thread = 1;
   while (p.per_thread < 16 && p.per_thread < p.all_heads && rows * p.pieces * (p.all_heads / (2 * p.per_thread)) >= kEnough)
     p.per_thread *= 2;
@@ -211,15 +218,13 @@ thin_status launch(RotaryPlan& p, int64_t rows, hipStream_t stream) {
   return THIN_OK;
 }
 
-// Pairs of a piece: as many as 16 bytes hold if they divide the pairs or leave a
-// small part of them, which goes element by element; else fewer (6 pairs and 14 more
-// dims of 2898 x 29 x 8 heads: 29 us by two, 82 by eight; 50 pairs of 100 and 100
-// more dims of half as many: 101 by two, 116 by four; 45 pairs: 114 by two, 102 by
-// four).
+// Pairs of a piece: as many as 16 bytes hold if they divide the pairs or are a small
+// part of them; else fewer (2898 tokens of 29 x 8 heads, 45 pairs as halves: 85 us by
+// four, 95 by eight; 27 adjacent: 59 by two, 67 by four).
 template <typename T, int V, bool INTERLEAVED>
 thin_status launch_pieces(RotaryPlan& p, int64_t rows, hipStream_t stream) {
   if constexpr (V > 1)
-    if (p.pairs % V != 0 && p.pairs < 16 * V) return launch_pieces<T, V / 2, INTERLEAVED>(p, rows, stream);
+    if (p.pairs % V != 0 && p.pairs < 8 * V) return launch_pieces<T, V / 2, INTERLEAVED>(p, rows, stream);
   return launch<T, V, INTERLEAVED>(p, rows, stream);
 }
 

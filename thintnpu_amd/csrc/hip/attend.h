@@ -116,7 +116,7 @@ inline int64_t splits_of(int64_t units, int64_t keys, int64_t dim) {
 // Few rows: they are bound by memory and their sequences differ in length, so all
 // keys of all sequences are dealt out in equal chunks, to as many workgroups as
 // this: the card once or more, at least two to a head of a sequence (32 x 8 heads
-// over 8192 cached tokens at most: 87 us, 156 by a workgroup each).  0: one
+// over 8192 cached tokens at most: 80 us, 156 by a workgroup each).  0: one
 // workgroup to each, without a join, where that fills the card and the longest
 // does not run on for long (32 x 16 heads to 1500 states: 45 us, 51 dealt out; 32
 // x 8 over 2000 cached tokens 40, 30 dealt out: codes are fewer bytes), or where
@@ -346,10 +346,22 @@ __device__ __forceinline__ bool find_chunk(const AttendPlan& p, uint32_t lane, u
     const int32_t n = most_of<PAGED>(b0 ? load(b0 + lane) : first);
     total += __builtin_amdgcn_readlane(lanes_upto((n + kChunkUnit - 1) / kChunkUnit), 63);
   }
-  // equal chunks; each head of a sequence may leave one unfilled
-  const int64_t room = (int64_t)p.chunks - (int64_t)p.batch * p.heads;
-  const int32_t even = (int32_t)(((int64_t)total * p.heads + room - 1) / room);
-  c.size = max(even * kChunkUnit, (int32_t)kSplitKeys);
+  // Equal chunks.  Each head of a sequence may leave one unfilled, but most leave a
+  // part of one: where they are many, the smallest that fit of what a quarter, a half
+  // and all would take (32 x 8 heads over 8192 cached tokens at most: 80 us, 86 with
+  // all).
+  const int64_t units = (int64_t)p.batch * p.heads;
+  for (int part = units * 4 > p.chunks ? 4 : 1; part; part >>= 1) {
+    const int64_t room = (int64_t)p.chunks - units / part;
+    c.size = max((int32_t)(((int64_t)total * p.heads + room - 1) / room) * kChunkUnit, (int32_t)kSplitKeys);
+    if (part == 1) break;
+    int64_t taken = 0;
+    for (uint32_t b0 = 0; b0 < p.batch; b0 += 64) {
+      const int32_t n = most_of<PAGED>(b0 ? load(b0 + lane) : first);
+      taken += __builtin_amdgcn_readlane(lanes_upto((n + c.size - 1) / c.size), 63);
+    }
+    if (taken * p.heads <= p.chunks) break;
+  }
   int32_t ahead = 0;
   for (uint32_t b0 = 0; b0 < p.batch; b0 += 64) {
     const Sequence s = b0 ? load(b0 + lane) : first;

@@ -351,7 +351,7 @@ __device__ __forceinline__ bool find_chunk(const AttendPlan& p, uint32_t lane, u
   // and all would take (32 x 8 heads over 8192 cached tokens at most: 80 us, 86 with
   // all).
   const int64_t units = (int64_t)p.batch * p.heads;
-  for (int part = units * 4 > p.chunks ? 4 : 1; part; part >>= 1) {
+  for (int part = units * 7 > p.chunks ? 4 : 1; part; part >>= 1) {
     const int64_t room = (int64_t)p.chunks - units / part;
     c.size = max((int32_t)(((int64_t)total * p.heads + room - 1) / room) * kChunkUnit, (int32_t)kSplitKeys);
     if (part == 1) break;

@@ -474,9 +474,9 @@ thin_status thin_token_logprobs(const thin_desc* logits, const thin_desc* tokens
  * i is dims (i, P + i), with interleaved != 0 dims (2 i, 2 i + 1); dims from 2 P
  * on are copied.  A pair whose axis is outside [0, A) stays as it is.  inverse
  * != 0 turns back (which is also the gradient of the turn).  Angles in 64 bits,
- * one rounding; below 2^28 radians they add no error to that of fp32.  q_out may be q itself and k_out k
- * itself.  The per-channel mul and add chain of the reference (ops.cpp:464-497)
- * with factors that depend on the place. */
+ * one rounding; below 2^28 radians they add no error to that of fp32.  q_out may
+ * be q itself and k_out k itself.  The per-channel mul and add chain of the
+ * reference (ops.cpp:464-497) with factors that depend on the place. */
 thin_status thin_rotary_axes(const thin_desc* q, const thin_desc* k, const thin_desc* positions, const thin_desc* freqs,
                              const thin_desc* axes, int32_t interleaved, int32_t inverse, const thin_desc* q_out,
                              const thin_desc* k_out, hipStream_t stream);

@@ -967,7 +967,7 @@ __global__ __launch_bounds__(256, tile_workgroups(DP)) void tile_kernel(AttendPl
 // tokens, so that a matrix tile has one page and one scale, which stay scalar.
 // Registers for the sums are half of what tiles of 32 rows take: 16 wavefronts
 // a CU, each with its next 32 keys in flight.  (One row of 32 x 8 x 4 heads over 8192
-// cached tokens at most: 75 us, 4.6 TB/s; of 64 x 16 heads to 1500 states at most: 63
+// cached tokens at most: 70 us, 4.9 TB/s; of 64 x 16 heads to 1500 states at most: 63
 // us, 3.9 TB/s; 6 x 5 of 2 x 4 over 60001 tokens: 25 us, 4.0 TB/s.)
 
 // Step s of q . k takes dims dim_of() .. + 8 of quarter q of the lanes: 16 codes

@@ -499,8 +499,9 @@ size_t thin_cross_attention_workspace(const thin_desc* q, const thin_desc* k);
  * A row that sees no state is zeros; what is not seen has no part in the result,
  * NaN and infinities included.  A finite row of q whose scores are all -inf is
  * zeros too; one that is not finite gives NaN or zeros where it sees anything.
- * fp32 scores, maxima and sums; the weights are rounded to the operands' type for
- * the product with v.  The workspace is 4-byte aligned and overlaps no operand.
+ * fp32 scores, maxima and sums (of v with weights of up to 2^15 before they are
+ * divided: a bf16 v past 2^112 / S may pass fp32's range); the weights are rounded
+ * to the operands' type for the product with v.  The workspace is 4-byte aligned and overlaps no operand.
  * The attention chain of the reference (whole_blocked.py:91-103) with keys of
  * another length. */
 thin_status thin_cross_attention(const thin_desc* q, const thin_desc* k, const thin_desc* v, const thin_desc* lengths,

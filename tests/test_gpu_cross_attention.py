@@ -249,3 +249,10 @@ def test_many_heads(gpu):
     """One row of each of many heads: 2100 workgroups, the last of them in turn."""
     q, k, v = inputs(175, 1, 40, 12, 12, 32, torch.float16, 3)
     check(gpu, q, k, v, torch.randint(0, 41, (175,), generator=gen(4), dtype=torch.int32))
+
+
+@pytest.mark.parametrize("d", [24, 128])
+def test_many_rows_of_many_parts(gpu, d):
+    """2400 rows whose states are split over 10 workgroups and more, some of them without any."""
+    q, k, v = inputs(2, 300, 6000, 4, 4, d, torch.float16, d)
+    check(gpu, q, k, v, torch.tensor([6000, 700], dtype=torch.int32), torch.rand((2, 6000), generator=gen(d)) < 0.8)

@@ -1453,8 +1453,9 @@ thin_status launch_attend_dim(const AttendPlan& p, hipStream_t stream) {
   }
   THIN_LAUNCH_CHECK("attend");
   if (!p.chunks && p.splits == 1) return THIN_OK;
-  // by the parts of a row, on the average
-  if ((few ? p.chunks / units : p.splits) > 8)
+  // By the parts of a row, on the average; rows that fill the card take a wavefront or
+  // 16 lanes (6400 rows of 12 parts of 32 dims: 42 us with the first launch, 33 so).
+  if ((few ? p.chunks / units : p.splits) > 8 && rows < 2048)
     hipLaunchKernelGGL((dev::join_kernel<T, PAGED, 256>), dim3(rows), dim3(256), 0, stream, p);
   else if (DP <= 64 && !few)
     hipLaunchKernelGGL((dev::join_kernel<T, PAGED, 16>), dim3((rows + 15) / 16), dim3(256), 0, stream, p);

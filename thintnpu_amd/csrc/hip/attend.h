@@ -582,8 +582,10 @@ __global__ __launch_bounds__(256, tile_workgroups(DP)) void tile_kernel(AttendPl
     for (int j = 0; j < 16; ++j) o[i][j] = 0.f;
   uint32_t ref = 0;   // PAGED: the largest of the values' scales so far, a power of two's bits
   float moved = 1.f;  // PAGED: the last one over that, where the sums still stand in it
-  if constexpr (PAGED)
+  if constexpr (PAGED) {
     for (uint32_t d = tid; d < (uint32_t)DP; d += 256) lowest[d] = 0x7FFFFFFF;
+    __syncthreads();  // the first stages note keys there
+  }
 
   // Stage s: keys of step s and values of step s - 2, eight of each by a wavefront
   // (PAGED: of one page).  Loads go by a buffer descriptor of the step, so that a

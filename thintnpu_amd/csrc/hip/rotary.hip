@@ -92,6 +92,9 @@ __device__ __forceinline__ void store_some(T* p, uint32_t n, const float (&v)[N]
 // tokens of 8 x 2 x 16 heads of 64 dims: 85 us, 4.9 TB/s; 92 with one, 88 with four,
 // 97 with eight at a time).
 constexpr int kHeadsAhead = 2;
+// The cosine of copied dims and of pairs of no axis: they stay, whatever they hold (an
+// infinity times a sine of 0 is no number).
+constexpr float kStays = 2.f;
 template <typename T, int V, bool INTERLEAVED, bool NT>
 __global__ __launch_bounds__(256) void rotary_kernel(RotaryPlan p) {
   const uint64_t id = (uint64_t)blockIdx.x * 256 + threadIdx.x;
@@ -121,10 +124,10 @@ __global__ __launch_bounds__(256) void rotary_kernel(RotaryPlan p) {
 #pragma unroll
   for (int j = 0; j < V; ++j) {
     s[j] = 0.f;
-    c[j] = 1.f;
+    c[j] = kStays;
     if (turns && i0 + j < p.pairs) {
       const int32_t axis = p.axes[(i0 + j) * p.axis_step];
-      if ((uint32_t)axis < p.num_axes) {  // a pair of no axis stays
+      if ((uint32_t)axis < p.num_axes) {
         const int64_t at = axis * p.pa + b * p.pb + t * p.pt;
         const double position = p.wide ? (double)static_cast<const int64_t*>(p.positions)[at]
                                        : (double)static_cast<const int32_t*>(p.positions)[at];
@@ -162,8 +165,9 @@ __global__ __launch_bounds__(256) void rotary_kernel(RotaryPlan p) {
         float first_of[V], second_of[V];
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-          first_of[j] = turns ? u[k][j] * c[j] - v[k][j] * s[j] : u[k][j];
-          second_of[j] = turns ? v[k][j] * c[j] + u[k][j] * s[j] : v[k][j];
+          const bool stays = c[j] == kStays;
+          first_of[j] = stays ? u[k][j] : u[k][j] * c[j] - v[k][j] * s[j];
+          second_of[j] = stays ? v[k][j] : v[k][j] * c[j] + u[k][j] * s[j];
         }
         if constexpr (INTERLEAVED) {
           float both[2 * V];

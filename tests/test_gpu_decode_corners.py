@@ -1,9 +1,11 @@
-"""Rotary positions where a pair has no axis."""
+"""Rotary positions and verification of drafts where a pair has no axis or a draft's
+probability is none."""
 import math
 
 import pytest
 import torch
 
+from oracle import drafts
 from tests.helpers import gen
 
 pytestmark = pytest.mark.gpu
@@ -34,3 +36,30 @@ def test_pairs_of_no_axis_keep_their_bits(gpu, dtype, interleaved, d, pairs):
             want = q[..., dims]
             nan = torch.isnan(want)
             assert torch.equal(torch.isnan(got), nan) and torch.equal(got.view(bits)[~nan], want.view(bits)[~nan])
+
+
+def verify(gpu, target, draft, tokens, accept, sample):
+    from thintnpu_amd import capi
+    got = capi.verify_drafts(*(x.to(gpu) for x in (target, draft, tokens, accept, sample)))
+    return got[0].cpu(), got[1].cpu()
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("v", [40, 6000])
+def test_draft_probabilities_that_are_none(gpu, dtype, v):
+    """A draft whose own probability is not finite falls, whatever the target's and the random number."""
+    rows = [(q, p, u) for q in (-math.inf, math.inf, math.nan) for p in (0.0, 0.25, 1.0) for u in (0.0, 0.5, 0.99)]
+    n = len(rows)
+    target = torch.softmax(torch.randn((n, 3, v), generator=gen(v)), 2)
+    draft = torch.softmax(torch.randn((n, 2, v), generator=gen(v + 1)), 2)
+    tokens = torch.randint(0, v, (n, 2), generator=gen(3))
+    accept = torch.zeros((n, 2))
+    for i, (q, p, u) in enumerate(rows):
+        at = i % 2
+        target[i, at, tokens[i, at]], draft[i, at, tokens[i, at]], accept[i, at] = p, q, u
+    target, draft = target.to(dtype), draft.to(dtype)
+    sample = torch.rand((n,), generator=gen(4))
+    out, taken = verify(gpu, target, draft, tokens, accept, sample)
+    want = drafts.verify(target, draft, tokens, accept, sample)
+    assert torch.equal(taken, torch.arange(n, dtype=torch.int32) % 2)
+    assert torch.equal(taken, want[1]) and torch.equal(out, want[0])

@@ -49,8 +49,9 @@ struct DraftPlan {
   int32_t* stayed;  // [batch]
 };
 
+constexpr double kMost = 1.7976931348623157e308;  // of what is finite
 // A probability; what is none counts as 0.
-__device__ __forceinline__ double positive(double x) { return x > 0.0 && x <= 1.7976931348623157e308 ? x : 0.0; }
+__device__ __forceinline__ double positive(double x) { return x > 0.0 && x <= kMost ? x : 0.0; }
 
 // How many drafts stay; every lane of a wavefront gets it.
 template <typename T>
@@ -63,7 +64,8 @@ __device__ __forceinline__ uint32_t stayed_of(const DraftPlan& p, uint32_t b, ui
     if (x >= 0 && x < (int64_t)p.vocab) {
       const double pt = positive((double)(float)static_cast<const T*>(p.target)[b * p.pb + lane * p.pk + x]);
       const double qt = p.draft ? (double)(float)static_cast<const T*>(p.draft)[b * p.qb + lane * p.qk + x] : 1.0;
-      stays = (double)p.accept[b * p.ub + lane * p.uk] * qt < pt;
+      const double least = (double)p.accept[b * p.ub + lane * p.uk] * qt;
+      stays = least >= -kMost && least < pt;  // (of a draft's own that is not finite, -inf too is none)
     }
   }
   const uint64_t fell = ~__ballot(stays);

@@ -27,3 +27,52 @@ def test_nan_values_among_the_first_keys(gpu, dtype, d):
     nan = torch.isnan(got.cpu())
     assert nan[0, 0, :2].any() and not nan[0, :5, 2:].any() and nan[0, 5:, 2:].any(2).all()
     c.attend(q, torch.tensor([40, 40, 40], dtype=torch.int32), torch.tensor([40, 33, 39], dtype=torch.int32))
+
+
+def seen_top(c, lengths, counts, t, table=None):
+    """[B, T, H]: the largest of the values' scales among the pages that each row sees."""
+    table = c.table if table is None else table
+    pages, heads, page, _ = c.shape
+    top = torch.zeros((table.shape[0], t, heads), dtype=torch.float64)
+    for b in range(table.shape[0]):
+        n = t if counts is None else int(counts[b])
+        for i in range(n):
+            keys = max(0, min(int(lengths[b]) - n + i + 1, table.shape[1] * page))
+            ids = table[b, :-(-keys // page)].long()
+            if keys:
+                top[b, i] = c.host[3][ids].double().amax(0)
+    return top
+
+
+def check(c, q, lengths, counts=None, scale=None):
+    """attend() with an allowance by what a row sees alone."""
+    from oracle import attend
+    from oracle import cache as oracle
+    from thintnpu_amd import capi
+    c.dev = [x.to(c.gpu) for x in c.host]
+    got = capi.cache_attention(q.to(c.gpu), *c.dev, c.table.to(c.gpu), lengths.to(c.gpu),
+                               None if counts is None else counts.to(c.gpu), scale).cpu().double()
+    ref = oracle.attention(q, *c.host, c.table, lengths, counts, scale)
+    group = q.shape[2] // c.shape[1]
+    top = seen_top(c, lengths, counts, q.shape[1]).repeat_interleave(group, 2)[..., None] * 448
+    allowed = attend.allowed(q, ref, c.table.shape[1] * c.shape[2], top)
+    assert torch.isfinite(got).all()
+    far = (got - ref[0]).abs() / allowed
+    assert far.max() <= 1, (float(far.max()), (far > 1).nonzero()[:4].tolist())
+
+
+@pytest.mark.parametrize("below", [3e-5, 1e-5])
+@pytest.mark.parametrize("t", [1, 40])
+def test_weights_fit_a_half(gpu, t, below):
+    """Scales just below twice a power of two, and a score next to 7 bits above the
+    first: its weight, scaled, is still a half."""
+    c = Cache(gpu, 1, 8, 16, 1, 64, 1)
+    c.host[0][:] = 0xF8  # -256: 28 bits below
+    c.host[0][c.table[0, :4].long()] = 0  # scores of 0 in the first 64 keys
+    c.host[0][c.table[0, 5].long(), 0, 3] = 0x68  # one of 64
+    c.host[1] = torch.randint(0x28, 0x44, c.shape, generator=c.g).to(torch.uint8)
+    c.host[2][:] = 1.0
+    c.host[3][:] = 2 - 2.0 ** -16
+    q = torch.zeros((1, t, 4, 64), dtype=torch.float16)
+    q[..., 0] = 1.0
+    check(c, q, torch.tensor([128], dtype=torch.int32), None, 7 * (1 - below) * math.log(2) / 64)

@@ -405,11 +405,13 @@ __device__ __forceinline__ const uint8_t* code_at(const PagesOf& c, int32_t id, 
 // The maximum that a row's exponentials stand against is not raised wherever a score
 // passes it, so sums are rescaled in few tiles.  Few rows: where one passes it by
 // kSlack bits, so that an exponential is 2^kSlack at most.  Many rows: where the sum
-// of a lane's 16 exponentials passes kMostOfStep, so that no maxima of the step are
+// of a lane's 16 exponentials passes most_of_step(), so that no maxima of the step are
 // taken but then, and in a row's first (300 rows of 8 x 8 heads to 8400 states: 72
 // us; 77 with the step's maxima and kSlack, 101 with a slack of 0).
 constexpr float kSlack = 4.f;
-constexpr float kMostOfStep = 128.f;  // with kShift 2^15: a half holds that
+// With kShift that is 2^15, which a half holds.  Of pages 2^14: a weight there is an
+// exponential times a multiple of its value's scale, which may be next to 2.
+constexpr float most_of_step(bool paged) { return paged ? 64.f : 128.f; }
 
 // Maxima are those of c s, rounded.  A row's exponentials are 2^(c s + offset_of(m))
 // with the product in full: the maximum's rounding is common to all.
@@ -842,7 +844,7 @@ __global__ __launch_bounds__(256, tile_workgroups(DP)) void tile_kernel(AttendPl
       __builtin_amdgcn_sched_barrier(0);
     }
     float total = PAGED ? sum[0] * back[0] + sum[1] * back[1] : sum[0] + sum[1];
-    if (fresh || __any(total > kMostOfStep * __builtin_exp2f(Matrix<T>::kShift))) {
+    if (fresh || __any(total > most_of_step(PAGED) * __builtin_exp2f(Matrix<T>::kShift))) {
       float top[2] = {s[0], s[8]};
 #pragma unroll
       for (int x = 1; x < 8; ++x) {

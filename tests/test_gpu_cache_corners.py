@@ -76,3 +76,22 @@ def test_weights_fit_a_half(gpu, t, below):
     q = torch.zeros((1, t, 4, 64), dtype=torch.float16)
     q[..., 0] = 1.0
     check(c, q, torch.tensor([128], dtype=torch.int32), None, 7 * (1 - below) * math.log(2) / 64)
+
+
+@pytest.mark.parametrize("t", [1, 6, 40])
+@pytest.mark.parametrize("which", [2, 3])
+def test_scales_of_nan_reach_their_rows(gpu, t, which):
+    """A page with a scale of NaN, part of which the first rows see: all rows that
+    see a token of it are NaN, those before it are not."""
+    from thintnpu_amd import capi
+    c = Cache(gpu, 1, 8, 16, 2, 64, t)
+    c.host[which][c.table[0, 4].long(), 1] = math.nan
+    c.dev = [x.to(gpu) for x in c.host]
+    for length in (66, 70, 64 + t, 63 + t, 100):
+        length = max(length, t)
+        q = queries(1, t, 4, 64, torch.float16, length)
+        got = capi.cache_attention(q.to(gpu), *c.dev, c.table.to(gpu), torch.tensor([length], dtype=torch.int32, device=gpu))
+        sees = torch.arange(length - t, length) >= 64
+        nan = torch.isnan(got[0].cpu())
+        assert not nan[:, :2].any() and torch.equal(nan[:, 2:].all(2), sees[:, None].expand(t, 2))
+        assert torch.equal(nan[:, 2:].any(2), sees[:, None].expand(t, 2))

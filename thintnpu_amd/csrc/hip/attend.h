@@ -420,8 +420,9 @@ __device__ __forceinline__ float rescale_of(float from, float to) {
   if (from == to) return 1.f;
   return from == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(offset_of(to) - offset_of(from));
 }
-// The scores' factor at least where some are -inf: 0 (a page's scale) times that is none.
-constexpr float kLeastFactor = 1.17549435e-38f;
+// The scores' factor where some are -inf: 0 (a page's scale) times that is none.  A
+// NaN stays one.
+__device__ __forceinline__ float seen_factor(float c) { return c < 1.17549435e-38f ? 1.17549435e-38f : c; }
 
 // V^T from LDS as the A operand, for dims 32 i + (lane & 31) and keys row + 4 half + {0..3, 8..11}.
 template <typename TV, int STRIDE>
@@ -810,7 +811,7 @@ __global__ __launch_bounds__(256, tile_workgroups(DP)) void tile_kernel(AttendPl
             c[n] = 1.f;
             add[n] = back[n] = 0.f;
           }
-          c[n] = fmaxf(c[n], kLeastFactor);
+          c[n] = seen_factor(c[n]);
         }
       }
     const auto weigh = [&](int x) __attribute__((always_inline)) {  // elements x and x + 1
@@ -1245,7 +1246,7 @@ __global__ __launch_bounds__(256, few_workgroups(DP, 16 * R, PAGED)) void few_ke
               radd[n] = rback[n] = 0.f;
             }
 #pragma unroll
-          for (int n = 0; n < 2; ++n) rc[n] = fmaxf(rc[n], kLeastFactor);
+          for (int n = 0; n < 2; ++n) rc[n] = seen_factor(rc[n]);
         }
       }
       float top = -__builtin_inff();

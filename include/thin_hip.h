@@ -553,7 +553,7 @@ size_t thin_cache_attention_workspace(const thin_desc* q, const thin_desc* k_cac
  * see has no part in it, NaN included.  Scales are any that are not negative,
  * neighbouring tokens less than 2^26 bytes apart.  fp32 scores, maxima and sums; a
  * weight, times its value's scale as a multiple of the largest scale among the
- * sequence's tokens, is rounded to q's type for the product with the codes of v (as
+ * tokens that its row sees, is rounded to q's type for the product with the codes of v (as
  * fp16, what is below 2^-33 of the largest is lost).  The workspace is 4-byte aligned
  * and overlaps no operand.  The attention chain of the reference
  * (whole_blocked.py:91-103) over pages. */

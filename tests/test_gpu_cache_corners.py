@@ -61,6 +61,48 @@ def check(c, q, lengths, counts=None, scale=None):
     assert far.max() <= 1, (float(far.max()), (far > 1).nonzero()[:4].tolist())
 
 
+@pytest.mark.parametrize("t,h", [(2, 4), (5, 8), (6, 10), (16, 4), (40, 4), (130, 2)])
+@pytest.mark.parametrize("dtype", HALVES)
+@pytest.mark.parametrize("up,zeros", [(26, False), (60, True), (120, True)])
+def test_scales_of_later_tokens(gpu, t, h, dtype, up, zeros):
+    """A page that begins with one of the call's own tokens and whose values have a
+    far larger scale: the rows before it lose nothing, those behind it see it."""
+    c = Cache(gpu, 3, 26, 16, 2, 64, t + h)
+    c.host[0] = torch.randint(0x20, 0x34, c.shape, generator=c.g).to(torch.uint8)  # 2^-3 to 0.7: no row sees one key alone
+    c.host[2][:] = 0.25
+    c.host[3][:] = 2.0 ** -16
+    lengths = torch.tensor([max(t, 17 + (t - 1) // 2), 364, 16 * 16 + t], dtype=torch.int32)
+    for b in range(3):
+        last = int(lengths[b]) - 1
+        for at, scale in (((last, 2.0 ** up),), ((last - t // 2, 2.0 ** (up / 2)), (last, 2.0 ** up * 1.7)), ((last, 2.0 ** up),))[b]:
+            page = c.table[b, at // 16].long()
+            c.host[3][page] = 2.0 ** -16 * scale
+            if zeros:  # (else what the type holds is passed)
+                c.host[1][page] = 0
+    q = queries(3, t, h, 64, HALVES[dtype], 3)
+    check(c, q, lengths)
+    check(c, q, lengths, torch.tensor([t, t - 1, max(1, t // 2)], dtype=torch.int32))
+
+
+@pytest.mark.parametrize("t,n", [(4, 81), (40, 97)])
+def test_scales_of_later_tokens_as_written(gpu, t, n):
+    """The same through the write: a last token of huge values, which begins a page,
+    changes no bit of the rows before it."""
+    from thintnpu_amd import capi
+    results = []
+    for huge in (1.0, 2.0 ** 40):
+        c = Cache(gpu, 1, 8, 16, 2, 64, 5, filled=False)
+        k, v = (torch.randn((1, n, 2, 64), generator=gen(i)) * 1e-3 for i in (1, 2))
+        v[:, -1] *= huge
+        c.write(k[:, :n - t], v[:, :n - t], torch.tensor([n - t], dtype=torch.int32))
+        c.write(k[:, n - t:], v[:, n - t:], torch.tensor([n], dtype=torch.int32))
+        q = queries(1, t, 4, 64, torch.float16, 6)
+        got = capi.cache_attention(q.to(gpu), *c.dev, c.table.to(gpu), torch.tensor([n], dtype=torch.int32, device=gpu))
+        assert got[0, :-1].abs().amax(2).min() > 0
+        results.append(got[0, :-1])
+    assert torch.equal(*results)
+
+
 @pytest.mark.parametrize("below", [3e-5, 1e-5])
 @pytest.mark.parametrize("t", [1, 40])
 def test_weights_fit_a_half(gpu, t, below):

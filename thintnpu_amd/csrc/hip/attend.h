@@ -437,8 +437,9 @@ __device__ __forceinline__ typename Matrix<TV>::v8 values8(const TV* v, int row,
   return r.all;
 }
 
-// The values' scales go into the weights, as multiples of the largest so far (a
-// power of two; what is summed is scaled along): so the weights fit a half.
+// The values' scales go into the weights, as multiples of the largest that the row
+// has seen so far (a power of two; what is summed is scaled along): so the weights
+// fit a half, and what a row does not see does not make them small.
 // A scale's power of two as bits, which compare as integers; 0 for what is not finite.
 __device__ __forceinline__ uint32_t power_of(float vs) {
   const uint32_t bits = __builtin_bit_cast(uint32_t, vs);
@@ -583,8 +584,11 @@ __global__ __launch_bounds__(256, tile_workgroups(DP)) void tile_kernel(AttendPl
   for (int i = 0; i < DP / 32; ++i)
 #pragma unroll
     for (int j = 0; j < 16; ++j) o[i][j] = 0.f;
-  uint32_t ref = 0;   // PAGED: the largest of the values' scales so far, a power of two's bits
-  float moved = 1.f;  // PAGED: the last one over that, where the sums still stand in it
+  // PAGED: the largest of the values' scales that the row has seen, a power of two's
+  // bits, and the last one over that, where the sums still stand in it
+  uint32_t ref = 0;
+  float moved = 1.f;
+  bool moves = false;
   if constexpr (PAGED) {
     for (uint32_t d = tid; d < (uint32_t)DP; d += 256) lowest[d] = 0x7FFFFFFF;
     __syncthreads();  // the first stages note keys there
@@ -638,16 +642,19 @@ __global__ __launch_bounds__(256, tile_workgroups(DP)) void tile_kernel(AttendPl
   float here_share = 0.f, here_back = 0.f;
   int32_t here_first = 0;                  // the step that `here` begins with
   // The values' scales go into the weights as multiples of the largest up to the
-  // window's end: of these, what the exponents and the totals take.
+  // window's end, of groups that all rows see part of: of these, what the exponents
+  // and the totals take.  Groups behind them are some rows' only (the last two steps
+  // at most that the wavefront's rows see): each row takes those as they come.
   const auto enter_window = [&](int32_t first) {
     here = there;
     here_first = first;
-    uint32_t top = power_of(here.vs);
+    uint32_t top = range.begin + (first + (int32_t)(lane >> 1)) * KT + (int32_t)(lane & 1u) * 16 < wave_least ? power_of(here.vs) : 0u;
 #pragma unroll
     for (int x = 1; x < 64; x <<= 1) top = max(top, (uint32_t)__shfl_xor((int)top, x, 64));
     top = (uint32_t)__builtin_amdgcn_readfirstlane((int)top);
-    if (top > ref) {
+    if (__any(top > ref)) {  // (all rows' is the same then)
       moved = __builtin_bit_cast(float, ref) * inverse_of(top);
+      moves = true;
       ref = top;
     }
     const float f = here.vs * inverse_of(ref);
@@ -777,8 +784,9 @@ __global__ __launch_bounds__(256, tile_workgroups(DP)) void tile_kernel(AttendPl
     store(j + 3);
     fetch(j + 4);
     float a = moved;  // what the sums so far are multiplied by, once step j - 1 is in
-    bool raised = PAGED && moved != 1.f;
+    bool raised = PAGED && moves;
     moved = 1.f;
+    moves = false;
     float c[2] = {p.c, p.c}, share[2] = {0.f, 0.f}, back[2] = {1.f, 1.f};
     bool there_is[2] = {true, true}, unseen[2] = {false, false};
     if constexpr (PAGED) {
@@ -791,7 +799,7 @@ __global__ __launch_bounds__(256, tile_workgroups(DP)) void tile_kernel(AttendPl
         back[n] = lane_value(here_back, at);
       }
     }
-    const bool zero[2] = {back[0] < 0.f, back[1] < 0.f};  // a value's scale of 0
+    bool zero[2] = {back[0] < 0.f, back[1] < 0.f};  // a value's scale of 0
     float add[2], sum[2] = {0.f, 0.f};
 #pragma unroll
     for (int n = 0; n < 2; ++n) {
@@ -804,14 +812,28 @@ __global__ __launch_bounds__(256, tile_workgroups(DP)) void tile_kernel(AttendPl
 #pragma unroll
         for (int i = 0; i < 16; ++i)
           if (!there_is[i / 8] || i / 4 * 8 + i % 4 >= left) s[i] = -__builtin_inff();
+        // nothing of scales that the row does not see
+        float vs[2];
+        uint32_t top = ref;
 #pragma unroll
         for (int n = 0; n < 2; ++n) {
           unseen[n] = !there_is[n] || limit <= k0 + n * 16;
-          if (unseen[n]) {  // nothing of scales that the row does not see
-            c[n] = 1.f;
-            add[n] = back[n] = 0.f;
-          }
-          c[n] = seen_factor(c[n]);
+          vs[n] = lane_value(here.vs, (j - here_first) * 2 + n);
+          if (!unseen[n]) top = max(top, power_of(vs[n]));
+        }
+        if (__any(top > ref)) {
+          a *= __builtin_bit_cast(float, ref) * inverse_of(top);
+          ref = top;
+          raised = true;
+        }
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+          const float f = vs[n] * inverse_of(ref);
+          zero[n] = !unseen[n] && f == 0.f;
+          share[n] = unseen[n] ? 0.f : __builtin_amdgcn_logf(share_of(f));
+          back[n] = unseen[n] ? 0.f : __builtin_amdgcn_rcpf(share_of(f));
+          add[n] = unseen[n] ? 0.f : off + share[n];
+          c[n] = seen_factor(unseen[n] ? 1.f : c[n]);
         }
       }
     const auto weigh = [&](int x) __attribute__((always_inline)) {  // elements x and x + 1
@@ -879,9 +901,9 @@ __global__ __launch_bounds__(256, tile_workgroups(DP)) void tile_kernel(AttendPl
     }
 #pragma unroll
     for (int n = 0; n < 2; ++n)
-      if (PAGED && zero[n]) {
+      if (PAGED && __any(zero[n])) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) pr[n][i] = (T)0.f;
+        for (int i = 0; i < 8; ++i) pr[n][i] = zero[n] ? (T)0.f : pr[n][i];
       }
   };
 
@@ -1046,7 +1068,9 @@ __global__ __launch_bounds__(256, few_workgroups(DP, 16 * R, PAGED)) void few_ke
 #pragma unroll
     for (int i = 0; i < DP / 16; ++i) o[r][i] = f4{0.f, 0.f, 0.f, 0.f};
   }
-  uint32_t ref = PAGED ? 0u : 0x3F800000u;  // the largest of the values' scales so far, a power of two's bits
+  uint32_t ref[R];  // the largest of the values' scales that a row has seen, a power of two's bits
+#pragma unroll
+  for (int r = 0; r < R; ++r) ref[r] = PAGED ? 0u : 0x3F800000u;
   if constexpr (PAGED) {
     for (uint32_t d = tid; d < (uint32_t)DP; d += 256) lowest[d] = 0x7FFFFFFF;
     __syncthreads();
@@ -1203,35 +1227,13 @@ __global__ __launch_bounds__(256, few_workgroups(DP, 16 * R, PAGED)) void few_ke
       }
       fetch(k0 + W * KT, ahead);
     }
-    if constexpr (PAGED) {
-      const uint32_t top = max(power_of(vs0), power_of(vs1));
-      if (top > ref) {
-        const float a = __builtin_bit_cast(float, ref) * inverse_of(top);
-#pragma unroll
-        for (int r = 0; r < R; ++r)
-#pragma unroll
-          for (int i = 0; i < DP / 16; ++i) o[r][i] *= a;
-        ref = top;
-      }
-    }
     // exponentials
-    float c[2] = {p.c, p.c}, add[2] = {0.f, 0.f}, back[2] = {1.f, 1.f};
-    bool zero[2] = {false, false};  // a value's scale of 0
-    if constexpr (PAGED) {
-      const float f0 = share_of(vs0 * inverse_of(ref)), f1 = share_of(vs1 * inverse_of(ref));
-      zero[0] = vs0 * inverse_of(ref) == 0.f;
-      zero[1] = vs1 * inverse_of(ref) == 0.f;
-      c[0] = p.c * ks0;
-      c[1] = p.c * ks1;
-      add[0] = __builtin_amdgcn_logf(f0);
-      add[1] = __builtin_amdgcn_logf(f1);
-      back[0] = __builtin_amdgcn_rcpf(f0);
-      back[1] = __builtin_amdgcn_rcpf(f1);
-    }
+    const float vs[2] = {vs0, vs1};
     v8 pr[R];
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-      float rc[2] = {c[0], c[1]}, radd[2] = {add[0], add[1]}, rback[2] = {back[0], back[1]};
+      float rc[2] = {p.c * ks0, p.c * ks1}, radd[2] = {0.f, 0.f}, rback[2] = {1.f, 1.f};
+      bool unseen[2] = {false, false}, zero[2] = {false, false};  // zero: a value's scale
       if (!whole) {
         const int32_t left = limit[r] - k0 - (int32_t)quarter * 4;
         const uint32_t mine = bits >> (quarter * 4);
@@ -1240,13 +1242,29 @@ __global__ __launch_bounds__(256, few_workgroups(DP, 16 * R, PAGED)) void few_ke
           if (!((mine >> (j / 4 * 16 + j % 4)) & 1u) || j / 4 * 16 + j % 4 >= left) s[r][j / 4][j % 4] = -__builtin_inff();
         if constexpr (PAGED) {
 #pragma unroll
-          for (int n = 0; n < 2; ++n)
-            if (!((bits >> (n * 16)) & 1u) || limit[r] <= k0 + n * 16) {  // nothing of scales that the row does not see
-              rc[n] = 1.f;
-              radd[n] = rback[n] = 0.f;
-            }
+          for (int n = 0; n < 2; ++n) {  // nothing of scales that the row does not see
+            unseen[n] = !((bits >> (n * 16)) & 1u) || limit[r] <= k0 + n * 16;
+            rc[n] = seen_factor(unseen[n] ? 1.f : rc[n]);
+          }
+        }
+      }
+      if constexpr (PAGED) {
+        uint32_t to = ref[r];
 #pragma unroll
-          for (int n = 0; n < 2; ++n) rc[n] = seen_factor(rc[n]);
+        for (int n = 0; n < 2; ++n)
+          if (!unseen[n]) to = max(to, power_of(vs[n]));
+        if (__any(to > ref[r])) {
+          const float a = __builtin_bit_cast(float, ref[r]) * inverse_of(to);
+#pragma unroll
+          for (int i = 0; i < DP / 16; ++i) o[r][i] *= a;
+          ref[r] = to;
+        }
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+          const float f = vs[n] * inverse_of(ref[r]);
+          zero[n] = !unseen[n] && f == 0.f;
+          radd[n] = unseen[n] ? 0.f : __builtin_amdgcn_logf(share_of(f));
+          rback[n] = unseen[n] ? 0.f : __builtin_amdgcn_rcpf(share_of(f));
         }
       }
       float top = -__builtin_inff();
@@ -1275,9 +1293,9 @@ __global__ __launch_bounds__(256, few_workgroups(DP, 16 * R, PAGED)) void few_ke
           pr[r][n * 4 + j] = (T)e;
         }
         l[r] += PAGED ? sum * rback[n] : sum;
-        if (PAGED && zero[n]) {
+        if (PAGED && __any(zero[n])) {
 #pragma unroll
-          for (int j = 0; j < 4; ++j) pr[r][n * 4 + j] = (T)0.f;
+          for (int j = 0; j < 4; ++j) pr[r][n * 4 + j] = zero[n] ? (T)0.f : pr[r][n * 4 + j];
         }
       }
     }
@@ -1316,7 +1334,7 @@ __global__ __launch_bounds__(256, few_workgroups(DP, 16 * R, PAGED)) void few_ke
     for (int i = 1; i < W; ++i) top = fmaxf(top, lds_m[i][row]);
 #pragma unroll
     for (int i = 0; i < W; ++i) sum += lds_l[i][row] * rescale_of(lds_m[i][row], top);
-    a[r] = rescale_of(m[r], top) * __builtin_bit_cast(float, ref);
+    a[r] = rescale_of(m[r], top) * __builtin_bit_cast(float, ref[r]);
     if (wave == 0 && quarter == 0) {
       row_m[row] = top;
       row_l[row] = sum;

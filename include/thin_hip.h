@@ -553,9 +553,9 @@ size_t thin_cache_attention_workspace(const thin_desc* q, const thin_desc* k_cac
  * see has no part in it, NaN included.  Scales are any that are not negative,
  * neighbouring tokens less than 2^26 bytes apart.  fp32 scores, maxima and sums; a
  * weight, times its value's scale as a multiple of the largest scale among the
- * tokens that its row sees, is rounded to q's type for the product with the codes of v (as
- * fp16, what is below 2^-33 of the largest is lost).  The workspace is 4-byte aligned
- * and overlaps no operand.  The attention chain of the reference
+ * tokens that its row sees, is rounded to q's type for the product with the codes
+ * of v (what is below 2^-33 of the largest as fp16, 2^-126 as bf16, is lost there, but
+ * not in the total).  The workspace is 4-byte aligned and overlaps no operand.  The attention chain of the reference
  * (whole_blocked.py:91-103) over pages. */
 thin_status thin_cache_attention(const thin_desc* q, const thin_desc* k_cache, const thin_desc* v_cache,
                                  const thin_desc* k_scales, const thin_desc* v_scales, const thin_desc* table,

@@ -103,6 +103,43 @@ def test_scales_of_later_tokens_as_written(gpu, t, n):
     assert torch.equal(*results)
 
 
+@pytest.mark.parametrize("t", [1, 6, 40])
+@pytest.mark.parametrize("dtype", HALVES)
+@pytest.mark.parametrize("high,low", [(0, -40), (0, -66), (10, -110), (10, -117), (10, -120), (119, -110)])
+def test_weights_of_tiny_scales_count(gpu, t, dtype, high, low):
+    """Values' scales 2^40 to 2^229 apart: keys of the small ones have next to no part
+    in the mix and their whole part in the total."""
+    if dtype == "fp16" and high > 10:
+        high, low = 10, -126  # (2^119 is past a half)
+    c = Cache(gpu, 2, 24, 16, 2, 64, high - low)
+    c.host[0][:] = 0
+    c.host[0][..., 0] = 0x58  # 16: what the scores come from
+    c.host[1] = torch.randint(0x28, 0x44, c.shape, generator=c.g).to(torch.uint8)
+    c.host[2][:] = 1.0
+    c.host[3][:] = 2.0 ** low
+    for b in range(2):
+        first = c.table[b, 3 + 5 * b].long()
+        c.host[3][first] = 2.0 ** high
+        c.host[0][first, ..., 0] = 0x5C  # 24
+    q = torch.zeros((2, t, 4, 64))
+    q[..., 0] = torch.rand((2, t, 4), generator=c.g) + 0.5  # scores 4 to 12 apart: shares of 2^-6 to 2^-18 each
+    check(c, q.to(HALVES[dtype]), torch.tensor([384, 350], dtype=torch.int32), None, 1.0)
+
+
+@pytest.mark.parametrize("t", [1, 6, 40])
+@pytest.mark.parametrize("mixed", [False, True])
+def test_subnormal_scales(gpu, t, mixed):
+    """Values whose scales are below the least normal number, all of them or but for a page."""
+    c = Cache(gpu, 2, 8, 16, 2, 64, t)
+    c.host[0] = torch.randint(0x20, 0x34, c.shape, generator=c.g).to(torch.uint8)
+    c.host[1] = torch.randint(0x70, 0x7F, c.shape, generator=c.g).to(torch.uint8)  # 128 to 448
+    c.host[2][:] = 0.25
+    c.host[3][:] = 1.25 * 2.0 ** -128
+    if mixed:
+        c.host[3][c.table[:, 2].long()] = 2.0 ** -124
+    check(c, queries(2, t, 4, 64, torch.bfloat16, 3), torch.tensor([128, 100], dtype=torch.int32))
+
+
 @pytest.mark.parametrize("below", [3e-5, 1e-5])
 @pytest.mark.parametrize("t", [1, 40])
 def test_weights_fit_a_half(gpu, t, below):

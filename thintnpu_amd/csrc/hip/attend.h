@@ -440,19 +440,37 @@ __device__ __forceinline__ typename Matrix<TV>::v8 values8(const TV* v, int row,
 // The values' scales go into the weights, as multiples of the largest that the row
 // has seen so far (a power of two; what is summed is scaled along): so the weights
 // fit a half, and what a row does not see does not make them small.
-// A scale's power of two as bits, which compare as integers; 0 for what is not finite.
+// A scale's power of two (of what is smaller, the least normal one) as bits, which
+// compare as integers; 0 for 0 and what is not finite.
 __device__ __forceinline__ uint32_t power_of(float vs) {
   const uint32_t bits = __builtin_bit_cast(uint32_t, vs);
-  return bits < 0x7F800000u ? bits & 0x7F800000u : 0u;
+  return bits - 1u < 0x7F7FFFFFu ? max(bits & 0x7F800000u, 0x00800000u) : 0u;
 }
 __device__ __forceinline__ float inverse_of(uint32_t power) {  // 2^127's is not normal
   return __builtin_bit_cast(float, !power ? 0u : power == 0x7F000000u ? 0x00400000u : 0x7F000000u - power);
 }
 
-// The weights take such a multiple f as a summand log2 f of their exponents, and
-// the total its share back as 1 / f.  Where f is 0 the total's share is taken with
-// 1, and the weights are zeros.
-__device__ __forceinline__ float share_of(float f) { return f == 0.f ? 1.f : f; }
+// Many rows: the weights take such a multiple f as a summand log2 f of their
+// exponents, and the total its share back as 1 / f.  That holds for no f: an
+// exponential times a far smaller one is 0, and has no share left to give back.  So
+// below 2^-48 (half) and 2^-64 (bf16) the exponents take another multiple, and the
+// weights the rest, as they stand in the operand: as halves they are zeros anyway.
+// Totals lose less than 2^-62 a key so.  (A factor for each weight, as few rows have
+// it, would be 16 more vector instructions a step where those are the bound.)
+template <typename T>
+struct Share;
+template <>
+struct Share<_Float16> {
+  static constexpr float kLeast = 0x1p-48f;
+  static __device__ __forceinline__ float of(float f) { return f < kLeast ? 1.f : f; }
+  static __device__ __forceinline__ float rest(float f) { return f < kLeast ? 0.f : 1.f; }
+};
+template <>
+struct Share<__bf16> {
+  static constexpr float kLeast = 0x1p-64f;
+  static __device__ __forceinline__ float of(float f) { return f < 0x1p-126f ? 1.f : f < kLeast ? f * 0x1p64f : f; }
+  static __device__ __forceinline__ float rest(float f) { return f < 0x1p-126f ? 0.f : f < kLeast ? 0x1p-64f : 1.f; }
+};
 
 // A row's result: out, or its split's sums.  Dim 32 i + 8 (j / 4) + 4 half + j % 4
 // of a row is o[i][j].
@@ -640,7 +658,8 @@ __global__ __launch_bounds__(256, tile_workgroups(DP)) void tile_kernel(AttendPl
   };
   Window here{-1, 0.f, 0.f}, there{-1, 0.f, 0.f};
   float here_share = 0.f, here_back = 0.f;
-  int32_t here_first = 0;                  // the step that `here` begins with
+  uint64_t here_tiny = 0;  // groups whose multiple is not in the exponents as a whole
+  int32_t here_first = 0;  // the step that `here` begins with
   // The values' scales go into the weights as multiples of the largest up to the
   // window's end, of groups that all rows see part of: of these, what the exponents
   // and the totals take.  Groups behind them are some rows' only (the last two steps
@@ -658,8 +677,9 @@ __global__ __launch_bounds__(256, tile_workgroups(DP)) void tile_kernel(AttendPl
       ref = top;
     }
     const float f = here.vs * inverse_of(ref);
-    here_share = __builtin_amdgcn_logf(share_of(f));
-    here_back = f == 0.f ? -1.f : __builtin_amdgcn_rcpf(f);
+    here_share = __builtin_amdgcn_logf(Share<T>::of(f));
+    here_back = __builtin_amdgcn_rcpf(Share<T>::of(f));
+    here_tiny = __ballot(f < Share<T>::kLeast);
   };
   int32_t id_k = -1, id_1 = -1, id_v = -1;  // the pages of the wavefront's keys of steps s, s - 1 and s - 2
   // their places there; a step is two groups further, and pages are whole groups
@@ -799,13 +819,8 @@ __global__ __launch_bounds__(256, tile_workgroups(DP)) void tile_kernel(AttendPl
         back[n] = lane_value(here_back, at);
       }
     }
-    bool zero[2] = {back[0] < 0.f, back[1] < 0.f};  // a value's scale of 0
-    float add[2], sum[2] = {0.f, 0.f};
-#pragma unroll
-    for (int n = 0; n < 2; ++n) {
-      add[n] = PAGED ? off + share[n] : off;
-      if (PAGED) back[n] = __builtin_fabsf(back[n]);
-    }
+    bool tiny = PAGED && ((here_tiny >> ((j - here_first) * 2)) & 3u);
+    float add[2] = {PAGED ? off + share[0] : off, PAGED ? off + share[1] : off}, sum[2] = {0.f, 0.f};
     if constexpr (PAGED)
       if (!(there_is[0] && there_is[1] && k0 + KT <= wave_least)) {
         const int32_t left = limit - k0 - (int32_t)half * 4;
@@ -826,12 +841,13 @@ __global__ __launch_bounds__(256, tile_workgroups(DP)) void tile_kernel(AttendPl
           ref = top;
           raised = true;
         }
+        tiny = false;
 #pragma unroll
         for (int n = 0; n < 2; ++n) {
           const float f = vs[n] * inverse_of(ref);
-          zero[n] = !unseen[n] && f == 0.f;
-          share[n] = unseen[n] ? 0.f : __builtin_amdgcn_logf(share_of(f));
-          back[n] = unseen[n] ? 0.f : __builtin_amdgcn_rcpf(share_of(f));
+          tiny = tiny || __any(!unseen[n] && f < Share<T>::kLeast);
+          share[n] = unseen[n] ? 0.f : __builtin_amdgcn_logf(Share<T>::of(f));
+          back[n] = unseen[n] ? 0.f : __builtin_amdgcn_rcpf(Share<T>::of(f));
           add[n] = unseen[n] ? 0.f : off + share[n];
           c[n] = seen_factor(unseen[n] ? 1.f : c[n]);
         }
@@ -899,12 +915,14 @@ __global__ __launch_bounds__(256, tile_workgroups(DP)) void tile_kernel(AttendPl
 #pragma unroll
         for (int e = 0; e < 16; ++e) o[i][e] *= a;
     }
+    if (PAGED && tiny) {
 #pragma unroll
-    for (int n = 0; n < 2; ++n)
-      if (PAGED && __any(zero[n])) {
+      for (int n = 0; n < 2; ++n) {
+        const float rest = Share<T>::rest(lane_value(here.vs, (j - here_first) * 2 + n) * inverse_of(ref));
 #pragma unroll
-        for (int i = 0; i < 8; ++i) pr[n][i] = zero[n] ? (T)0.f : pr[n][i];
+        for (int i = 0; i < 8; ++i) pr[n][i] = (T)((float)pr[n][i] * rest);
       }
+    }
   };
 
   f16v s[2];
@@ -1069,8 +1087,12 @@ __global__ __launch_bounds__(256, few_workgroups(DP, 16 * R, PAGED)) void few_ke
     for (int i = 0; i < DP / 16; ++i) o[r][i] = f4{0.f, 0.f, 0.f, 0.f};
   }
   uint32_t ref[R];  // the largest of the values' scales that a row has seen, a power of two's bits
+  float inverse[R];
 #pragma unroll
-  for (int r = 0; r < R; ++r) ref[r] = PAGED ? 0u : 0x3F800000u;
+  for (int r = 0; r < R; ++r) {
+    ref[r] = PAGED ? 0u : 0x3F800000u;
+    inverse[r] = 0.f;
+  }
   if constexpr (PAGED) {
     for (uint32_t d = tid; d < (uint32_t)DP; d += 256) lowest[d] = 0x7FFFFFFF;
     __syncthreads();
@@ -1232,8 +1254,9 @@ __global__ __launch_bounds__(256, few_workgroups(DP, 16 * R, PAGED)) void few_ke
     v8 pr[R];
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-      float rc[2] = {p.c * ks0, p.c * ks1}, radd[2] = {0.f, 0.f}, rback[2] = {1.f, 1.f};
-      bool unseen[2] = {false, false}, zero[2] = {false, false};  // zero: a value's scale
+      float rc[2] = {p.c * ks0, p.c * ks1};
+      float f[2] = {1.f, 1.f};  // the values' scales as multiples
+      bool unseen[2] = {false, false};
       if (!whole) {
         const int32_t left = limit[r] - k0 - (int32_t)quarter * 4;
         const uint32_t mine = bits >> (quarter * 4);
@@ -1248,25 +1271,10 @@ __global__ __launch_bounds__(256, few_workgroups(DP, 16 * R, PAGED)) void few_ke
           }
         }
       }
-      if constexpr (PAGED) {
-        uint32_t to = ref[r];
+      uint32_t power = ref[r];
 #pragma unroll
-        for (int n = 0; n < 2; ++n)
-          if (!unseen[n]) to = max(to, power_of(vs[n]));
-        if (__any(to > ref[r])) {
-          const float a = __builtin_bit_cast(float, ref[r]) * inverse_of(to);
-#pragma unroll
-          for (int i = 0; i < DP / 16; ++i) o[r][i] *= a;
-          ref[r] = to;
-        }
-#pragma unroll
-        for (int n = 0; n < 2; ++n) {
-          const float f = vs[n] * inverse_of(ref[r]);
-          zero[n] = !unseen[n] && f == 0.f;
-          radd[n] = unseen[n] ? 0.f : __builtin_amdgcn_logf(share_of(f));
-          rback[n] = unseen[n] ? 0.f : __builtin_amdgcn_rcpf(share_of(f));
-        }
-      }
+      for (int n = 0; n < 2; ++n)
+        if (PAGED && !unseen[n]) power = max(power, power_of(vs[n]));
       float top = -__builtin_inff();
 #pragma unroll
       for (int n = 0; n < 2; ++n) {
@@ -1275,28 +1283,32 @@ __global__ __launch_bounds__(256, few_workgroups(DP, 16 * R, PAGED)) void few_ke
       }
       top = fmaxf(top, lane_xor<16>(top));
       top = fmaxf(top, lane_xor<32>(top));
-      if (__any(top - m[r] > kSlack || (m[r] == -__builtin_inff() && top > m[r]))) {
-        const float to = fmaxf(m[r], top), a = rescale_of(m[r], to);
+      // (row by row, so that a later token's scale moves no rounding of another row)
+      const bool low = top - m[r] > kSlack || (m[r] == -__builtin_inff() && top > m[r]);
+      if (__any(low || (PAGED && power > ref[r]))) {
+        const float to = low ? top : m[r], a = rescale_of(m[r], to);
         l[r] *= a;
+        if (PAGED) inverse[r] = inverse_of(power);
+        const float oa = PAGED ? a * (__builtin_bit_cast(float, ref[r]) * inverse[r]) : a;
 #pragma unroll
-        for (int i = 0; i < DP / 16; ++i) o[r][i] *= a;
+        for (int i = 0; i < DP / 16; ++i) o[r][i] *= oa;
         m[r] = to;
+        ref[r] = power;
       }
+#pragma unroll
+      for (int n = 0; n < 2; ++n)
+        if (PAGED) f[n] = unseen[n] ? 0.f : vs[n] * inverse[r];
       const float off = offset_of(m[r]) + Matrix<T>::kShift;
 #pragma unroll
       for (int n = 0; n < 2; ++n) {
         float sum = 0.f;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r][n][j], rc[n], off + radd[n]));
+          const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r][n][j], rc[n], off));
           sum += e;
-          pr[r][n * 4 + j] = (T)e;
+          pr[r][n * 4 + j] = (T)(PAGED ? e * f[n] : e);
         }
-        l[r] += PAGED ? sum * rback[n] : sum;
-        if (PAGED && __any(zero[n])) {
-#pragma unroll
-          for (int j = 0; j < 4; ++j) pr[r][n * 4 + j] = zero[n] ? (T)0.f : pr[r][n * 4 + j];
-        }
+        l[r] += sum;
       }
     }
     // values, 16 dims a time

@@ -174,3 +174,25 @@ def test_scales_of_nan_reach_their_rows(gpu, t, which):
         nan = torch.isnan(got[0].cpu())
         assert not nan[:, :2].any() and torch.equal(nan[:, 2:].all(2), sees[:, None].expand(t, 2))
         assert torch.equal(nan[:, 2:].any(2), sees[:, None].expand(t, 2))
+
+
+@pytest.mark.parametrize("d,page", [(32, 16), (64, 48), (128, 16), (144, 32), (256, 32)])
+def test_codes_at_odd_addresses_many_rows(gpu, d, page):
+    """Pages, heads and tokens at odd byte distances, read by the kernel for many rows."""
+    from thintnpu_amd import capi
+    from tests.test_gpu_cache import close
+    from oracle import cache as oracle
+    c = Cache(gpu, 2, 7, page, 2, d, d)
+    lengths = torch.tensor([7 * page - 3, 81], dtype=torch.int32)
+    for shift in (1, 3, 8):
+        views = []
+        for x in c.host[:2]:
+            p, h, n, _ = c.shape
+            base = torch.full((p, n, h, d + 5), 0x7F, dtype=torch.uint8, device=gpu)  # tokens before heads
+            view = torch.full((base.numel() + 64,), 0x7F, dtype=torch.uint8, device=gpu)[shift:shift + base.numel()].view_as(base)
+            view[..., 3:3 + d] = x.permute(0, 2, 1, 3).to(gpu)
+            views.append(view[..., 3:3 + d].permute(0, 2, 1, 3))
+        for t, h in ((33, 2), (50, 6)):
+            q = queries(2, t, h, d, torch.bfloat16, t)
+            got = capi.cache_attention(q.to(gpu), *views, *c.dev[2:], c.table.to(gpu), lengths.to(gpu))
+            close(got, oracle.attention(q, *c.host, c.table, lengths), q, 7 * page, c.host)

@@ -586,7 +586,8 @@ size_t thin_verify_drafts_workspace(int64_t batch, int64_t vocab);
  * Target probabilities that are not positive and finite count as 0; a draft whose
  * own is not finite falls, and so does the part of a token whose draft probability
  * is not.  If nothing has a part, the next token is -1.  Products and sums in 64
- * bits.  The workspace is 8-byte aligned and overlaps no operand.  The selection of
+ * bits: a border moves by 9e-15 of the total at most up to 131072 tokens, by 2.3e-14
+ * beyond.  The workspace is 8-byte aligned and overlaps no operand.  The selection of
  * the reference (selection_flow.cpp:429-499) with given chances in place of the
  * order. */
 thin_status thin_verify_drafts(const thin_desc* target, const thin_desc* draft, const thin_desc* tokens,

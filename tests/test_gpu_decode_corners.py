@@ -1,6 +1,8 @@
-"""Rotary positions and verification of drafts where a pair has no axis or a draft's
-probability is none."""
+"""Rotary positions and verification of drafts where a pair has no axis, a draft's
+probability is none, or a sum's rounding decides."""
 import math
+from fractions import Fraction
+from itertools import accumulate
 
 import pytest
 import torch
@@ -63,3 +65,47 @@ def test_draft_probabilities_that_are_none(gpu, dtype, v):
     want = drafts.verify(target, draft, tokens, accept, sample)
     assert torch.equal(taken, torch.arange(n, dtype=torch.int32) % 2)
     assert torch.equal(taken, want[1]) and torch.equal(out, want[0])
+
+
+# Roundings of 64 bits between a sum that is compared with the border and its exact
+# value, each 2^-53 of the total at most.  The sum ahead of the tile: tiles' own 17 (an
+# element's difference, 7 along a thread's, 6 over the lanes, 3 over the wavefronts), 6
+# and one for each 64 tiles, 2 to take the tile apart.  Within it 28: 14 to a lane, 3 over
+# the wavefronts, 3 to join them, 8 along a thread's.  The border: a total's 17, 6 and one for
+# each 64 tiles, and the product.
+def roundings(vocab):
+    rounds = -(-vocab // (64 * 2048))
+    return (17 + 6 + rounds + 2) + 28 + (17 + 6 + rounds + 1)
+
+
+@pytest.mark.parametrize("v", [1500, 6000, 50001, 140000])
+@pytest.mark.parametrize("least", [-60, -20])
+def test_borders_by_rounding(gpu, v, least):
+    """Rows of many exponents whose sum up to the middle is a half of the total but for
+    2^-50 of it: the token is the exact one, or the random number lies within the
+    roundings of the border between the two."""
+    half = (v - 2) // 2
+    n = 24 if v < 10000 else 6
+    g = gen(v)
+    first = torch.exp2(torch.rand((n, half), generator=g) * least)
+    rest = first.gather(1, torch.rand((n, half), generator=g).argsort(1))
+    target = torch.zeros((n, v))
+    target[:, 1:1 + half], target[:, 1 + half:1 + 2 * half] = first, rest
+    # a token at either end moves the border past a half, or short of it, or there is none
+    extra = torch.exp2(torch.floor(torch.log2(first.double().sum(1))) - torch.randint(44, 53, (n,), generator=g)).float()
+    for i in range(n):
+        if i % 3 < 2:
+            target[i, (0, 1 + 2 * half)[i % 3]] = extra[i]
+    sample = torch.full((n,), 0.5)
+    out, taken = verify(gpu, target[:, None], torch.zeros((n, 0, v)), torch.zeros((n, 0), dtype=torch.int64), torch.zeros((n, 0)), sample)
+    assert not taken.any()
+    for i in range(n):
+        row = [int(x * 2.0 ** 120) for x in target[i].tolist()]  # exact
+        prefix = list(accumulate(row))
+        whole = prefix[-1]
+        edge = Fraction(whole, 2)
+        want = next(j for j, y in enumerate(prefix) if y > edge)
+        got = int(out[i, 0])
+        allowed = roundings(v) * Fraction(1, 2 ** 53) * whole
+        # the token's own stretch of the distribution, widened by the roundings
+        assert row[got] > 0 and prefix[got] + allowed > edge >= prefix[got] - row[got] - allowed, (i, got, want)

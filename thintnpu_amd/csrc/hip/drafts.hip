@@ -6,8 +6,14 @@
 //   first whose distribution function passes r times the total.
 //
 // So the tokens are distributed as the target's own.  Products and sums are
-// taken in 64 bits: u q is exact there, and the order of rounding in a sum over
-// the vocabulary moves a border by 1e-16 of the total, not by 1e-7.
+// taken in 64 bits: u q is exact there, and the roundings of a sum over the
+// vocabulary, in the order in which it is taken, move a border by little.  On the
+// way to a sum that is compared with it: 17 of a tile (the element's own, 7 along a
+// thread's, 6 over the lanes, 3 over the wavefronts), 6 and one for each 64 tiles
+// ahead, 2 where a tile is taken apart from those, 28 within it; of the border, the
+// total's 17 and 6 and one for each 64 tiles, and the product's.  Each is 2^-53 of
+// the total at most: with all signs alike 79 up to 131072 tokens, 9e-15, and 205 of
+// the longest rows, 2.3e-14 (sums in 32 bits: 1e-5).
 //
 // Bound by memory: of the target's and the draft's rows only one each is read
 // whole.  Few rows, so each is cut into tiles over the card; a second launch

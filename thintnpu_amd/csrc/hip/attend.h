@@ -915,14 +915,15 @@ __global__ __launch_bounds__(256, tile_workgroups(DP)) void tile_kernel(AttendPl
 #pragma unroll
         for (int e = 0; e < 16; ++e) o[i][e] *= a;
     }
-    if (PAGED && tiny) {
+    if constexpr (PAGED)
+      if (tiny) {
 #pragma unroll
-      for (int n = 0; n < 2; ++n) {
-        const float rest = Share<T>::rest(lane_value(here.vs, (j - here_first) * 2 + n) * inverse_of(ref));
+        for (int n = 0; n < 2; ++n) {
+          const float rest = Share<T>::rest(lane_value(here.vs, (j - here_first) * 2 + n) * inverse_of(ref));
 #pragma unroll
-        for (int i = 0; i < 8; ++i) pr[n][i] = (T)((float)pr[n][i] * rest);
+          for (int i = 0; i < 8; ++i) pr[n][i] = (T)((float)pr[n][i] * rest);
+        }
       }
-    }
   };
 
   f16v s[2];

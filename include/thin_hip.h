@@ -521,8 +521,8 @@ thin_status thin_cross_attention(const thin_desc* q, const thin_desc* k, const t
  * own among them; counts NULL (T), or int32 [B]: how many of its T rows are
  * tokens, the sequence's last ones.  Tokens before the first and behind
  * slots * page do not exist; a page outside [0, pages) is neither written nor
- * seen.  A page belongs to one sequence of a call that writes it: two that write
- * it race (copy it first), any number may read it. */
+ * seen.  A page belongs to one place of one sequence of a call that writes it: two
+ * that write it race (copy it first), any number may read it. */
 
 /* New keys and values k and v [B, T, Hk, D] (fp16, bf16 or fp32, a head's dims
  * adjacent) into the cache at positions lengths[b] - counts[b] on.  For each page

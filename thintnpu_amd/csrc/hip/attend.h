@@ -18,6 +18,13 @@
 // tile, lane i its column i).  The order within the dot products q . k is free
 // too: step 2s + e of a half takes dims 32 s + 16 half + 8 e .. + 8, so that 16
 // bytes of codes serve two steps.
+//
+// What is held in fewer bits: the weights alone, rounded once to the operands' type
+// as the product with the values takes them (the matrix instructions for operands
+// of 32 bits have a sixteenth of the rate).  Scores, maxima, totals, which take the
+// unrounded weights, and sums have 32 bits.  Against 64 bits results are off by 1.1
+// to 1.4 times what rounding them once to their type takes (2048 rows to 4096 states
+// as bf16: 2.3e-3 and 1.7e-3 of them).
 #pragma once
 
 #include "rows.h"
@@ -96,8 +103,8 @@ constexpr int64_t kMaxSplits = 128;
 
 // Many rows: splits of every row's keys.  In rounds of the workgroups that the card
 // holds, each as long as its keys and some 160 more, which beginning and end cost,
-// and the join as much as 200.  (1024 rows of 3 x 4 heads over 8000 cached tokens:
-// 4 splits, 143 us; 2 take 152, 3 take 162.)
+// and the join as much as 200.  (1024 rows of 3 x 4 heads over 8000 cached tokens, in
+// a graph: 4 splits, 143 us; 2 take 152, 3 take 162.)
 inline int64_t splits_of(int64_t units, int64_t keys, int64_t dim) {
   const int64_t most = (keys + kSplitKeys - 1) / kSplitKeys < kMaxSplits ? (keys + kSplitKeys - 1) / kSplitKeys : kMaxSplits;
   const int64_t at_a_time = kCus * tile_workgroups(padded_dim(dim));
@@ -518,7 +525,7 @@ __device__ __forceinline__ void store_row(const AttendPlan& p, uint32_t b, uint3
 // head and split read the same keys: they go to one XCD's L2, and heads and splits
 // to the XCDs in turn, so that sequences of unequal length are spread (in runs, an
 // XCD with the longest sequence's heads worked on when the others had ended: chunks
-// of prompts 310 us, 168 so).  What is left of them goes to all XCDs.  Row blocks go
+// of prompts 310 us, 168 so, in a graph).  What is left of them goes to all XCDs.  Row blocks go
 // from the last (whose causal rows see the most keys) to the first.
 struct Place {
   uint32_t b, h, block, split;
@@ -548,11 +555,11 @@ __device__ __forceinline__ Place place_of(const AttendPlan& p) {
 // steps.  The exponentials do not wait for their step's maximum: they are taken
 // against the maximum so far, and again where their sum shows that as too low.
 // What bounds it: at 128 dims the matrix instructions and what is issued between
-// them (2048 rows of 4 x 32 heads to 4096 states: 590 us, 930 TFLOP/s); at 32 and 64
+// them (2048 rows of 4 x 32 heads to 4096 states: 570 us, 960 TFLOP/s); at 32 and 64
 // dims the softmax, whose 16 exponentials, 55 other vector instructions and, of codes,
 // 16 widenings a step stand against 4 and 8 matrix instructions (300 rows of 8 x 8
 // heads to 8400 states of 32 dims: 66 us; 1024 rows of 3 x 24 heads over 8000 cached
-// tokens of 64: 128 us, 440 TFLOP/s).
+// tokens of 64: 129 us by itself, 440 TFLOP/s, and the join's 13).
 // Rows: unseen states have -inf in the scores from the start (the accumulator's
 // first value).  Pages: rows that do not see a whole step are masked afterwards.
 template <typename T, int DP, bool PAGED>
@@ -1013,7 +1020,7 @@ __global__ __launch_bounds__(256, tile_workgroups(DP)) void tile_kernel(AttendPl
 // tokens, so that a matrix tile has one page and one scale, which stay scalar.
 // Registers for the sums are half of what tiles of 32 rows take: 16 wavefronts
 // a CU, each with its next 32 keys in flight.  (One row of 32 x 8 x 4 heads over 8192
-// cached tokens at most: 70 us, 4.9 TB/s; of 64 x 16 heads to 1500 states at most: 63
+// cached tokens at most: 68 us, 5.0 TB/s; of 64 x 16 heads to 1500 states at most: 63
 // us, 3.9 TB/s; 6 x 5 of 2 x 4 over 60001 tokens: 25 us, 4.0 TB/s.)
 
 // Step s of q . k takes dims dim_of() .. + 8 of quarter q of the lanes: 16 codes

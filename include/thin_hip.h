@@ -551,8 +551,9 @@ size_t thin_cache_attention_workspace(const thin_desc* q, const thin_desc* k_cac
  * sees the tokens up to and with its own, j <= lengths[b] - counts[b] + t.  Rows
  * from counts[b] on, and rows that see nothing, are zeros.  What a row does not
  * see has no part in it, NaN included.  Scales are any that are not negative,
- * neighbouring tokens less than 2^26 bytes apart.  fp32 scores, maxima and sums; a
- * weight, times its value's scale as a multiple of the largest scale among the
+ * neighbouring tokens less than 2^26 bytes apart.  fp32 scores, maxima and sums (of
+ * values with weights of up to 2^15 before they are divided: values past 2^112 over
+ * the tokens that a row sees may pass fp32's range); a weight, times its value's scale as a multiple of the largest scale among the
  * tokens that its row sees, is rounded to q's type for the product with the codes
  * of v (what is below 2^-33 of the largest as fp16, 2^-126 as bf16, is lost there, but
  * not in the total).  The workspace is 4-byte aligned and overlaps no operand.  The attention chain of the reference
